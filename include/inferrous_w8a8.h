@@ -483,6 +483,88 @@ int w8a8_linear_argmax_noalloc(void *stream, const int8_t *q, const float *asc,
                                uint32_t k, uint32_t *token, void *logits,
                                int logits_dtype);
 
+/* ------------------------------------------------------------ routed layers
+ * Layers that give a row weights of its own beside the shared projections: a
+ * router, the routed experts' SwiGLU MLP, and low-rank adapters beside a
+ * projection.  No counterpart in the reference, whose layers are dense and
+ * serve one set of weights.  Outputs of W8A8_OUT_F32 hold BF16 values, as the
+ * projections' do.
+ *
+ * w8a8_route_experts: logits[m, n_experts] (F32 or BF16) to the top_k experts
+ * of each row, ids[m, top_k], and their weights[m, top_k]:
+ *   s = softmax(logits) or 1 / (1 + exp(-logits));  c = s + bias (bias[E] or
+ *   NULL: it counts in the choice only);
+ *   an expert whose logit is -inf or NaN, or whose c is NaN or -inf, is out;
+ *   groups > 1: the experts form that many groups of neighbours; a group's
+ *   score is its largest c (group_top 1) or the sum of its two largest
+ *   (group_top 2), of its live experts; all but the top_groups best groups
+ *   (equal ones: the lowest index first) are out;
+ *   the top_k largest c are chosen, equal ones lowest index first; a slot
+ *   left without an expert gets id -1 and weight 0;
+ *   weight = s of the chosen, divided by the chosen ones' sum if renorm (0
+ *   where that sum is 0), times scale.
+ * Everything is held in f32.  Several +inf logits share a softmax row.
+ * 1 <= n_experts <= 1024, groups <= 64 divides n_experts, top_k <= 64 and at
+ * most top_groups * n_experts / groups. */
+#define W8A8_ROUTE_SOFTMAX 0
+#define W8A8_ROUTE_SIGMOID 1
+int w8a8_route_experts(void *stream, const void *logits, int logits_dtype,
+                       size_t m, uint32_t n_experts, int score,
+                       const float *bias, uint32_t groups, uint32_t top_groups,
+                       uint32_t group_top, uint32_t top_k, int renorm,
+                       float scale, int32_t *ids, float *weights);
+
+/* The routed experts' SwiGLU MLP on quantized rows q[m, hidden], asc[m]: for
+ * slot j of row t with expert e = ids[t, j] (outside [0, n_experts): skipped)
+ *   gate = RN(RN(f32(q . w_gate[e]) * asc) * ws_gate[e]), up likewise;
+ *   act = gate / (1 + exp(-gate)) * up, in f32;
+ *   codes of act, one scale s to each 128 columns (the last group of inter %
+ *   128): s = max(1e-8, max |act|) / 127, NaN ignored, code =
+ *   round(act / s), half to even, NaN -> 0;
+ *   y = ws_down[e] * sum over the groups of s * f32(codes . w_down[e]);
+ *   out[t] = bf16(residual[t] + sum over j of weights[t, j] * y)
+ * (residual: f32 [m, hidden] or NULL).  w_gate, w_up: int8 [n_experts, inter,
+ * hidden], w_down [n_experts, hidden, inter], scales [n_experts, inter] and
+ * [n_experts, hidden].  A sum over slots is added in a fixed order: the same
+ * call gives the same bits.  hidden and inter: multiples of 16 up to 65536;
+ * q, the weights, residual and out 16-byte aligned; m * top_k <= 2^24.  The workspace
+ * (256-byte aligned, at least w8a8_experts_mlp_workspace_bytes) is written
+ * before it is read; calls sharing one must not overlap.  out must not
+ * overlap an input. */
+size_t w8a8_experts_mlp_workspace_bytes(size_t m, uint32_t top_k,
+                                        uint32_t n_experts, uint32_t hidden,
+                                        uint32_t inter);
+int w8a8_experts_mlp(void *stream, const int8_t *q, const float *asc, size_t m,
+                     uint32_t hidden, const int32_t *ids, const float *weights,
+                     uint32_t top_k, uint32_t n_experts, const int8_t *w_gate,
+                     const float *ws_gate, const int8_t *w_up,
+                     const float *ws_up, const int8_t *w_down,
+                     const float *ws_down, uint32_t inter,
+                     const float *residual, void *out, int out_dtype,
+                     void *workspace, size_t workspace_bytes);
+
+/* w8a8_linear with a low-rank adapter per row: for row r with a = ids[r]
+ *   out[r] = bf16(residual[r] + f32(q[r] . w) * asc[r] * ws
+ *                 + scaling[a] * B[a] (A[a] bf16(x[r])))
+ * without the last term where ids[r] is outside [0, n_adapters).  x[m, k] is
+ * the rows before their quantization, F32 (rounded to BF16: exact for the
+ * BF16 values that the other operators write) or BF16; a: BF16 [n_adapters,
+ * rank, k], b: BF16 [n_adapters, n, rank]; residual: f32 [m, n] or NULL.
+ * Products and sums are held in f32, the projection's in exact i32.  rank: a
+ * multiple of 8 up to 256 (pad a smaller one with zeros); x, a, b 16-byte
+ * aligned; q, w, k as for w8a8_linear.  Workspace as for w8a8_experts_mlp.
+ * out must not overlap an input. */
+size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k,
+                                            uint32_t rank, uint32_t n_adapters);
+int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
+                         size_t m, const int8_t *w, const float *ws, size_t n,
+                         uint32_t k, const void *x, int x_dtype,
+                         const int32_t *ids, const uint16_t *a,
+                         const uint16_t *b, const float *scaling,
+                         uint32_t rank, uint32_t n_adapters,
+                         const float *residual, void *out, int out_dtype,
+                         void *workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ synthetic
  * Seeded generators for benches and tests (no reference counterpart; the
  * reference loads exported bundles, src/model.rs:46-165).  Pure functions of

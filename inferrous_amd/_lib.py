@@ -16,6 +16,7 @@ OUT_F32, OUT_BF16, OUT_I32 = 0, 1, 2
 PATH_AUTO, PATH_DOT4, PATH_MFMA = 0, 1, 2
 NOALLOC_MAX_ROWS = 262144  # W8A8_NOALLOC_MAX_ROWS
 SEQ_SELECT = 1  # W8A8_SEQ_SELECT
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
 
 class SeqEntry(ctypes.Structure):
@@ -95,6 +96,11 @@ SIGNATURES: dict[str, tuple] = {
     "w8a8_linear_sequence": (I, [P, P, S, P, P, S, U32]),
     "w8a8_linear_sequence_status": (I, [P]),
     "w8a8_linear_sequence_reset": (I, []),
+    "w8a8_route_experts": (I, [P, P, I, S, U32, I, P, U32, U32, U32, U32, I, F, P, P]),
+    "w8a8_experts_mlp_workspace_bytes": (S, [S, U32, U32, U32, U32]),
+    "w8a8_experts_mlp": (I, [P, P, P, S, U32, P, P, U32, U32, P, P, P, P, P, P, U32, P, P, I, P, S]),
+    "w8a8_linear_adapters_workspace_bytes": (S, [S, S, U32, U32, U32]),
+    "w8a8_linear_adapters": (I, [P, P, P, S, P, P, S, U32, P, I, P, P, P, P, U32, U32, P, P, I, P, S]),
     "w8a8_synth_i8": (I, [P, P, S, U64, U64]),
     "w8a8_synth_f32": (I, [P, P, S, U64, U64, F, F]),
 }

@@ -21,7 +21,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libinferrous_w8a8.so"
-SOURCES = ["abi.hip", "quantize.hip", "gemv.hip", "gemm.hip", "head.hip", "synth.hip", "sequence.hip"]
+SOURCES = ["abi.hip", "quantize.hip", "gemv.hip", "gemm.hip", "head.hip", "synth.hip", "sequence.hip",
+           "route.hip", "experts.hip", "adapters.hip"]
 ARCH = "gfx950"
 
 

@@ -1352,4 +1352,151 @@ int w8a8_linear_sequence_reset(void) {
   return W8A8_OK;
 }
 
+// ------------------------------------------------------------ routed layers
+int w8a8_route_experts(void* stream, const void* logits, int logits_dtype, size_t m, uint32_t n_experts, int score,
+                       const float* bias, uint32_t groups, uint32_t top_groups, uint32_t group_top, uint32_t top_k,
+                       int renorm, float scale, int32_t* ids, float* weights) {
+  if (logits_dtype != W8A8_OUT_F32 && logits_dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  if (score != W8A8_ROUTE_SOFTMAX && score != W8A8_ROUTE_SIGMOID) return W8A8_EARG;
+  if (group_top != 1 && group_top != 2) return W8A8_EARG;
+  if (n_experts == 0 || n_experts > kMaxExperts || m > kU32Max / kMaxExperts) return W8A8_ESHAPE;
+  if (groups == 0 || groups > kMaxRouteGroups || n_experts % groups != 0) return W8A8_ESHAPE;
+  if (top_groups == 0 || top_groups > groups) return W8A8_ESHAPE;
+  if (top_k == 0 || top_k > kMaxTopK || top_k > top_groups * (n_experts / groups)) return W8A8_ESHAPE;
+  if (m == 0) return W8A8_OK;
+  if (!logits || !ids || !weights) return W8A8_ENULL;
+  if (!al(logits, out_align(logits_dtype)) || !al(bias, 4) || !al(ids, 4) || !al(weights, 4)) return W8A8_EALIGN;
+  if (!ready()) return W8A8_EINIT;
+  RouteArgs a{};
+  a.logits = logits;
+  a.bf16 = logits_dtype == W8A8_OUT_BF16;
+  a.sigmoid = score == W8A8_ROUTE_SIGMOID;
+  a.renorm = renorm != 0;
+  a.m = (uint32_t)m;
+  a.experts = n_experts;
+  a.groups = groups;
+  a.top_groups = top_groups;
+  a.group_top = group_top;
+  a.k = top_k;
+  a.bias = bias;
+  a.scale = scale;
+  a.ids = ids;
+  a.weights = weights;
+  return hip_status(launch_route((hipStream_t)stream, a));
+}
+
+static int check_experts_shape(size_t m, uint32_t top_k, uint32_t n_experts, uint32_t hidden, uint32_t inter) {
+  if (n_experts == 0 || n_experts > kMaxExperts || top_k == 0 || top_k > kMaxTopK) return W8A8_ESHAPE;
+  if (hidden == 0 || inter == 0 || hidden % 16 != 0 || inter % 16 != 0) return W8A8_ESHAPE;
+  if (hidden > kMaxExpertWidth || inter > kMaxExpertWidth || m > kMaxExpertSlots / top_k) return W8A8_ESHAPE;
+  return W8A8_OK;
+}
+
+size_t w8a8_experts_mlp_workspace_bytes(size_t m, uint32_t top_k, uint32_t n_experts, uint32_t hidden,
+                                        uint32_t inter) {
+  if (m == 0 || check_experts_shape(m, top_k, n_experts, hidden, inter) != W8A8_OK) return 0;
+  return experts_workspace_bytes((uint32_t)m, top_k, n_experts, hidden, inter);
+}
+
+int w8a8_experts_mlp(void* stream, const int8_t* q, const float* asc, size_t m, uint32_t hidden, const int32_t* ids,
+                     const float* weights, uint32_t top_k, uint32_t n_experts, const int8_t* w_gate,
+                     const float* ws_gate, const int8_t* w_up, const float* ws_up, const int8_t* w_down,
+                     const float* ws_down, uint32_t inter, const float* residual, void* out, int out_dtype,
+                     void* workspace, size_t workspace_bytes) {
+  if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  const int s = check_experts_shape(m, top_k, n_experts, hidden, inter);
+  if (s != W8A8_OK || m == 0) return s;
+  if (!q || !asc || !ids || !weights || !w_gate || !ws_gate || !w_up || !ws_up || !w_down || !ws_down || !out)
+    return W8A8_ENULL;
+  if (!al(q, 16) || !al(w_gate, 16) || !al(w_up, 16) || !al(w_down, 16) || !al(residual, 16) || !al(out, 16) ||
+      !al(asc, 4) || !al(ids, 4) || !al(weights, 4) || !al(ws_gate, 4) || !al(ws_up, 4) || !al(ws_down, 4))
+    return W8A8_EALIGN;
+  if (!workspace || workspace_bytes < w8a8_experts_mlp_workspace_bytes(m, top_k, n_experts, hidden, inter))
+    return W8A8_EWORKSPACE;
+  if (!al(workspace, 256)) return W8A8_EALIGN;
+  if (!ready()) return W8A8_EINIT;
+  ExpertsArgs a{};
+  a.q = q;
+  a.asc = asc;
+  a.m = (uint32_t)m;
+  a.k = top_k;
+  a.experts = n_experts;
+  a.hidden = hidden;
+  a.inter = inter;
+  a.ids = ids;
+  a.weights = weights;
+  a.w_gate = w_gate;
+  a.ws_gate = ws_gate;
+  a.w_up = w_up;
+  a.ws_up = ws_up;
+  a.w_down = w_down;
+  a.ws_down = ws_down;
+  a.residual = residual;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  return hip_status(launch_experts((hipStream_t)stream, a, workspace));
+}
+
+static int check_adapters_shape(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters) {
+  if (m > kU32Max || n > kU32Max || k == 0 || k % 16 != 0 || (m > 0 && m * (size_t)k / k != m)) return W8A8_ESHAPE;
+  if (rank == 0 || rank % 8 != 0 || rank > kMaxRank || n_adapters == 0 || n_adapters > kMaxAdapters)
+    return W8A8_ESHAPE;
+  return W8A8_OK;
+}
+
+// The workspace: accumulators [m, n], the adapters' first product [m, rank], the
+// projection's own.
+static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters) {
+  if (m == 0 || n == 0 || check_adapters_shape(m, n, k, rank, n_adapters) != W8A8_OK) return 0;
+  return up256(m * n * 4) + up256(m * rank * 4) + w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO);
+}
+
+int w8a8_linear_adapters(void* stream, const int8_t* q, const float* asc, size_t m, const int8_t* w, const float* ws,
+                         size_t n, uint32_t k, const void* x, int x_dtype, const int32_t* ids, const uint16_t* a,
+                         const uint16_t* b, const float* scaling, uint32_t rank, uint32_t n_adapters,
+                         const float* residual, void* out, int out_dtype, void* workspace, size_t workspace_bytes) {
+  if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  if (x_dtype != W8A8_OUT_F32 && x_dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  int s = check_adapters_shape(m, n, k, rank, n_adapters);
+  if (s != W8A8_OK || m == 0 || n == 0) return s;
+  s = check_linear(q, asc, m, w, ws, n, k, out, out_dtype);
+  if (s != W8A8_OK) return s;
+  if (!x || !ids || !a || !b || !scaling) return W8A8_ENULL;
+  if (!al(x, 16) || !al(a, 16) || !al(b, 16) || !al(ids, 4) || !al(scaling, 4) || !al(residual, 4)) return W8A8_EALIGN;
+  if (!workspace || workspace_bytes < w8a8_linear_adapters_workspace_bytes(m, n, k, rank, n_adapters))
+    return W8A8_EWORKSPACE;
+  if (!al(workspace, 256)) return W8A8_EALIGN;
+  if (!ready()) return W8A8_EINIT;
+  AdapterArgs t{};
+  t.x = x;
+  t.x_bf16 = x_dtype == W8A8_OUT_BF16;
+  t.m = (uint32_t)m;
+  t.n = (uint32_t)n;
+  t.width = k;
+  t.rank = rank;
+  t.adapters = n_adapters;
+  t.asc = asc;
+  t.ws = ws;
+  t.ids = ids;
+  t.a = a;
+  t.b = b;
+  t.scaling = scaling;
+  t.residual = residual;
+  t.out = out;
+  t.out_dtype = out_dtype;
+  char* p = (char*)workspace;
+  int32_t* const acc = (int32_t*)p;
+  float* const h = (float*)(p += up256(m * n * 4));
+  p += up256(m * rank * 4);
+  hipStream_t st = (hipStream_t)stream;
+  hipError_t e = launch_adapters_shrink(st, t, h);
+  if (e != hipSuccess) return hip_status(e);
+  s = run_linear(st, q, asc, m, w, ws, n, k, acc, W8A8_OUT_I32, W8A8_PATH_AUTO, nullptr, nullptr, p,
+                 w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO));
+  if (s != W8A8_OK) return s;
+  return hip_status(launch_adapters_expand(st, t, acc, h));
+}
+
 }  // extern "C"

@@ -221,6 +221,61 @@ uint32_t seq_max_rows(uint32_t grid);
 hipError_t launch_sequence(hipStream_t st, const SeqEntry* tab, uint32_t count, uint32_t base, uint32_t* ctl,
                            uint64_t* keys, uint32_t* token, uint64_t spin, uint32_t grid);
 
+// The router of a layer of experts (route.hip).
+struct RouteArgs {
+  const void* logits;  // [m, experts], f32 or BF16
+  int bf16, sigmoid, renorm;
+  uint32_t m, experts, groups, top_groups, group_top, k;
+  const float* bias;   // [experts], optional
+  float scale;
+  int32_t* ids;        // [m, k]
+  float* weights;      // [m, k]
+};
+constexpr uint32_t kMaxExperts = 1024, kMaxRouteGroups = 64, kMaxTopK = 64;
+constexpr uint32_t kMaxExpertWidth = 65536, kMaxExpertSlots = 1u << 24;  // of experts_mlp
+constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1u << 16;              // of linear_adapters
+hipError_t launch_route(hipStream_t st, const RouteArgs& a);
+
+// The routed experts' SwiGLU products and their weighted sum (experts.hip).
+struct ExpertsArgs {
+  const int8_t* q;     // [m, hidden]
+  const float* asc;    // [m]
+  uint32_t m, k, experts, hidden, inter;
+  const int32_t* ids;  // [m, k]
+  const float* weights;
+  const int8_t* w_gate;  // [experts, inter, hidden]
+  const float* ws_gate;  // [experts, inter]
+  const int8_t* w_up;
+  const float* ws_up;
+  const int8_t* w_down;  // [experts, hidden, inter]
+  const float* ws_down;  // [experts, hidden]
+  const float* residual;  // [m, hidden], optional
+  void* out;              // [m, hidden]
+  int out_dtype;          // F32 or BF16
+};
+size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);
+hipError_t launch_experts(hipStream_t st, const ExpertsArgs& a, void* workspace);
+
+// Low-rank adapters beside a shared projection (adapters.hip): the adapters'
+// first product h[m, rank], then the outputs from the projection's
+// accumulators.
+struct AdapterArgs {
+  const void* x;       // [m, width], f32 or BF16
+  int x_bf16;
+  uint32_t m, n, width, rank, adapters;
+  const float* asc;    // [m]
+  const float* ws;     // [n]
+  const int32_t* ids;  // [m]
+  const uint16_t* a;   // [adapters, rank, width] BF16
+  const uint16_t* b;   // [adapters, n, rank] BF16
+  const float* scaling;   // [adapters]
+  const float* residual;  // [m, n], optional
+  void* out;              // [m, n]
+  int out_dtype;          // F32 or BF16
+};
+hipError_t launch_adapters_shrink(hipStream_t st, const AdapterArgs& a, float* h);
+hipError_t launch_adapters_expand(hipStream_t st, const AdapterArgs& a, const int32_t* acc, const float* h);
+
 hipError_t launch_synth_i8(hipStream_t st, int8_t* out, size_t n, uint64_t seed, uint64_t stream_id);
 hipError_t launch_synth_f32(hipStream_t st, float* out, size_t n, uint64_t seed, uint64_t stream_id,
                             float lo, float hi);

@@ -1,0 +1,40 @@
+// routed_common.hpp -- device helpers of the routed layers (route.hip,
+// experts.hip, adapters.hip).
+#pragma once
+#include "device_common.hpp"
+
+namespace w8a8 {
+
+// Wave sums, returned wave-uniform; every lane of the wave must be active.  The
+// additions' order is fixed: the DPP steps of wave_max_u32 inside the 16-lane
+// rows, then the four rows in pairs.
+__device__ __forceinline__ float wave_sum_f32(float v) {
+  v += __uint_as_float(dpp_u32<0xB1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<0x4E>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<0x141>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<0x140>(__float_as_uint(v)));
+  const int u = __float_as_int(v);
+  return (__int_as_float(__builtin_amdgcn_readlane(u, 0)) + __int_as_float(__builtin_amdgcn_readlane(u, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(u, 32)) + __int_as_float(__builtin_amdgcn_readlane(u, 48)));
+}
+
+__device__ __forceinline__ int wave_sum_i32(int v) {
+  v += (int)dpp_u32<0xB1>((uint32_t)v);
+  v += (int)dpp_u32<0x4E>((uint32_t)v);
+  v += (int)dpp_u32<0x141>((uint32_t)v);
+  v += (int)dpp_u32<0x140>((uint32_t)v);
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+// A BF16-valued output in its buffer's type.
+__device__ __forceinline__ void store_routed(void* out, int out_dtype, size_t o, float v) {
+  v = bf16_rne(v);
+  if (out_dtype == W8A8_OUT_F32) ((float*)out)[o] = v;
+  else ((uint16_t*)out)[o] = (uint16_t)(__float_as_uint(v) >> 16);
+}
+
+}  // namespace w8a8

@@ -31,6 +31,7 @@ from .runtime import CudaContext, CudaStream, DeviceBuffer, is_capturing
 
 _OUT = {np.dtype(np.float32): _lib.OUT_F32, np.dtype(np.uint16): _lib.OUT_BF16,
         np.dtype(np.int32): _lib.OUT_I32}
+_SCORES = {"softmax": _lib.ROUTE_SOFTMAX, "sigmoid": _lib.ROUTE_SIGMOID}
 
 
 def _h(stream: CudaStream | None):
@@ -658,6 +659,125 @@ class LoadedModule:
 
     def sequence_reset(self) -> None:
         check(lib().w8a8_linear_sequence_reset(), "linear_sequence_reset")
+
+    # ------------------------------------------------------------ routed layers
+    def _routed_workspace(self, stream, nbytes: int):
+        """The stream's workspace (the split-K one: calls on a stream follow
+        each other), at least nbytes."""
+        cur = self._gemm_ws.get(_key(stream))
+        if cur is None or cur.nbytes < nbytes:
+            self.reserve_workspace(nbytes, stream)
+            cur = self._gemm_ws[_key(stream)]
+        return cur.ptr, cur.nbytes
+
+    def route_experts(self, stream, logits: DeviceBuffer, n_experts: int, ids: DeviceBuffer,
+                      weights: DeviceBuffer, score: str = "softmax", bias: DeviceBuffer | None = None,
+                      groups: int = 1, top_groups: int = 1, group_top: int = 1, renorm: bool = True,
+                      scale: float = 1.0) -> None:
+        """The router of a layer of experts (w8a8_route_experts; no
+        counterpart in the reference): ``logits`` (float32, or uint16 BF16,
+        [M, n_experts]) to each row's ``ids`` (int32 [M, K]) and ``weights``
+        (float32 [M, K]); ``score`` is "softmax" or "sigmoid", ``bias``
+        (float32 [n_experts]) counts in the choice only, and ``groups`` /
+        ``top_groups`` / ``group_top`` limit the choice to the best groups."""
+        m = len(logits) // n_experts if n_experts > 0 else 0
+        if n_experts <= 0 or m * n_experts != len(logits):
+            raise ValueError("route_experts: logits must hold M rows of n_experts")
+        if len(ids) != len(weights) or (m and len(ids) % m) or (m and not len(ids)):
+            raise ValueError("route_experts: ids and weights must both hold M rows of K")
+        if score not in _SCORES:
+            raise ValueError(f"score {score!r}: one of {sorted(_SCORES)}")
+        if logits.dtype not in (np.float32, np.uint16):
+            raise TypeError(f"logits dtype {logits.dtype} not supported (float32/uint16)")
+        _expect(ids, np.int32, "ids")
+        _expect(weights, np.float32, "weights")
+        if bias is not None:
+            _expect(bias, np.float32, "bias")
+            _check_len(bias, n_experts, "bias")
+        if m == 0:
+            return
+        check(lib().w8a8_route_experts(_h(stream), logits.ptr, _OUT[logits.dtype], m, n_experts, _SCORES[score],
+                                       None if bias is None else bias.ptr, groups, top_groups, group_top,
+                                       len(ids) // m, int(renorm), scale, ids.ptr, weights.ptr), "route_experts")
+
+    def experts_mlp(self, stream, q, asc, width: int, ids: DeviceBuffer, weights: DeviceBuffer, w0, s0, w1, s1, wd,
+                    sd, n_experts: int, out, residual=None) -> None:
+        """The routed experts' SwiGLU MLP and its weighted sum
+        (w8a8_experts_mlp; no counterpart in the reference): rows ``q`` /
+        ``asc`` (as ``quantize`` writes them), ``ids`` / ``weights`` (as
+        ``route_experts`` writes them, id -1 for a slot without an expert),
+        gate ``w0`` / ``s0`` and up ``w1`` / ``s1`` (int8 [n_experts, I,
+        width], float32 [n_experts, I]), down ``wd`` / ``sd`` (int8
+        [n_experts, width, I], float32 [n_experts, width]), into ``out``
+        (float32 or uint16 BF16, [M, width]), with ``residual`` (float32)
+        added.  The scratch space is the stream's workspace;
+        ``reserve_workspace`` it before capturing a graph."""
+        m, width, n_experts = len(asc), int(width), int(n_experts)
+        if n_experts <= 0 or width <= 0 or len(s0) % n_experts or len(s1) != len(s0):
+            raise ValueError("experts_mlp: s_gate and s_up must hold n_experts rows of I")
+        inter = len(s0) // n_experts
+        if len(out) != m * width or len(ids) != len(weights) or (m and len(ids) % m):
+            raise ValueError("experts_mlp: out must hold M*width values, ids and weights M rows of K")
+        for b, dt, nm in ((q, np.int8, "q"), (asc, np.float32, "asc"), (ids, np.int32, "ids"),
+                          (weights, np.float32, "weights"), (w0, np.int8, "w_gate"), (s0, np.float32, "s_gate"),
+                          (w1, np.int8, "w_up"), (s1, np.float32, "s_up"), (wd, np.int8, "w_down"),
+                          (sd, np.float32, "s_down")):
+            _expect(b, dt, nm)
+        _check_len(q, m * width, "q")
+        for b, need, nm in ((w0, n_experts * inter * width, "w_gate"), (w1, n_experts * inter * width, "w_up"),
+                            (wd, n_experts * inter * width, "w_down"), (sd, n_experts * width, "s_down")):
+            _check_len(b, need, nm)
+        if residual is not None:
+            _expect(residual, np.float32, "residual")
+            if len(residual) != m * width:
+                raise ValueError("residual must hold M*width values")
+        if m == 0:
+            return
+        k = len(ids) // m
+        wp, wb = self._routed_workspace(stream, lib().w8a8_experts_mlp_workspace_bytes(m, k, n_experts, width, inter))
+        check(lib().w8a8_experts_mlp(_h(stream), q.ptr, asc.ptr, m, width, ids.ptr, weights.ptr, k, n_experts, w0.ptr,
+                                     s0.ptr, w1.ptr, s1.ptr, wd.ptr, sd.ptr, inter,
+                                     None if residual is None else residual.ptr, out.ptr, _dtype_code(out), wp, wb),
+              "experts_mlp")
+
+    def linear_adapters(self, stream, q, asc, w, ws, width: int, x, ids: DeviceBuffer, a, b, scaling, out,
+                        residual=None) -> None:
+        """``linear`` with a low-rank BF16 adapter per row
+        (w8a8_linear_adapters; no counterpart in the reference): ``x`` is the
+        rows before quantization (float32 or uint16 BF16), ``ids`` (int32
+        [M]) each row's adapter, outside [0, len(scaling)) for none, ``a``
+        (uint16 BF16 [adapters, rank, width]), ``b`` (uint16 BF16 [adapters,
+        N, rank]) and ``scaling`` (float32 [adapters]); ``residual``
+        (float32) is added before the one rounding.  The scratch space is the
+        stream's workspace; ``reserve_workspace`` it before capturing a
+        graph."""
+        m, n, k = _shape(asc, ws, out, width)
+        count = len(scaling)
+        if k <= 0 or count == 0 or len(a) % (count * k):
+            raise ValueError("linear_adapters: a must hold len(scaling) adapters of rank rows of width")
+        rank = len(a) // (count * k)
+        for buf, dt, nm in ((q, np.int8, "q"), (asc, np.float32, "asc"), (w, np.int8, "w"), (ws, np.float32, "ws"),
+                            (ids, np.int32, "ids"), (a, np.uint16, "a"), (b, np.uint16, "b"),
+                            (scaling, np.float32, "scaling")):
+            _expect(buf, dt, nm)
+        if x.dtype not in (np.float32, np.uint16):
+            raise TypeError(f"x dtype {x.dtype} not supported (float32/uint16)")
+        _check_len(q, m * k, "q")
+        _check_len(w, n * k, "w")
+        _check_len(x, m * k, "x")
+        _check_len(ids, m, "ids")
+        _check_len(b, count * n * rank, "b")
+        if residual is not None:
+            _expect(residual, np.float32, "residual")
+            if len(residual) != m * n:
+                raise ValueError("residual must hold M*N values")
+        if m == 0 or n == 0:
+            return
+        wp, wb = self._routed_workspace(stream, lib().w8a8_linear_adapters_workspace_bytes(m, n, k, rank, count))
+        check(lib().w8a8_linear_adapters(_h(stream), q.ptr, asc.ptr, m, w.ptr, ws.ptr, n, k, x.ptr, _OUT[x.dtype],
+                                         ids.ptr, a.ptr, b.ptr, scaling.ptr, rank, count,
+                                         None if residual is None else residual.ptr, out.ptr, _dtype_code(out), wp,
+                                         wb), "linear_adapters")
 
     # ------------------------------------------------------------ synthetic
     def synth_i8(self, stream, out: DeviceBuffer, seed: int, stream_id: int) -> None:
