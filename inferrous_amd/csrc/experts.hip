@@ -10,16 +10,9 @@
 //   out = bf16(residual + sum over the slots of weight * y).
 // One scale to 128 columns, not one to a row: the codes of 128 columns are known
 // once their own sums are, so no pass waits for a row's maximum.
-#include "internal.hpp"
-#include "routed_common.hpp"
+#include "experts.hpp"
 
 namespace w8a8 {
-
-// act of two projections, kept in f32 up to its codes.
-__device__ __forceinline__ float act_f32(int32_t g, int32_t u, float asc, float wg, float wu) {
-  const float gate = (float)g * asc * wg, up = (float)u * asc * wu;
-  return gate / (1.0f + expf(-gate)) * up;
-}
 
 // ------------------------------------------------------------ slot by slot
 // act[slot, I]: a wave holds COLS columns (gate and up row each) of one slot.
@@ -148,12 +141,18 @@ __global__ __launch_bounds__(256) void experts_down_slot(ExpertsArgs a, const in
 
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t, uint32_t, uint32_t inter) {
+// Slot by slot every slot reads its expert's weights; expert by expert they are
+// read once, in more launches.
+static bool by_slot(uint32_t m) { return m <= 4; }
+
+size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
+  if (!by_slot(m)) return experts_tiles_workspace_bytes(m, k, experts, hidden, inter);
   const size_t slots = (size_t)m * k;
   return up256(slots * inter * 4) + up256(slots * inter) + up256(slots * ((inter + 127) / 128) * 4);
 }
 
 hipError_t launch_experts(hipStream_t st, const ExpertsArgs& a, void* workspace) {
+  if (!by_slot(a.m)) return launch_experts_tiles(st, a, workspace);
   const uint32_t slots = a.m * a.k;
   char* p = (char*)workspace;
   float* const act = (float*)p;

@@ -1,0 +1,40 @@
+// experts.hpp -- what the two forms of the routed experts' MLP share: slot by
+// slot (experts.hip) and expert by expert (experts_tiles.hip).
+#pragma once
+#include "internal.hpp"
+#include "routed_common.hpp"
+
+namespace w8a8 {
+
+// The slots sorted by expert: position p of the sorted order holds slot order[p],
+// slot i stands at pos[i] (-1: it has no expert).  A tile is up to BT sorted
+// positions of one expert.
+struct ExpertsTile {
+  uint32_t expert, first, rows, pad;
+};
+struct ExpertsPlan {
+  uint32_t* order;
+  int32_t* pos;
+  ExpertsTile* tiles;
+  uint32_t* n_tiles;
+};
+
+// exp(x) as 2^(x log2 e) on v_exp_f32: the product's rounding error, which
+// grows with |x|, is put back to first order.
+__device__ __forceinline__ float exp_fast(float x) {
+  const float t = x * 1.44269502f;
+  const float lo = __builtin_fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;  // log2 e in two parts
+  const float e = __builtin_amdgcn_exp2f(t);
+  return e < __builtin_inff() && lo == lo ? __builtin_fmaf(e, lo * 0.693147182f, e) : e;  // infinite x: lo is NaN
+}
+
+// act of two projections, kept in f32 up to its codes.
+__device__ __forceinline__ float act_f32(int32_t g, int32_t u, float asc, float wg, float wu) {
+  const float gate = (float)g * asc * wg, up = (float)u * asc * wu;
+  return gate * __builtin_amdgcn_rcpf(1.0f + exp_fast(-gate)) * up;
+}
+
+size_t experts_tiles_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);
+hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* workspace);
+
+}  // namespace w8a8

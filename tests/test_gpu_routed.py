@@ -284,7 +284,7 @@ class Experts:
     (1, 1, 1, 16, 16), (1, 8, 64, 256, 128), (1, 3, 5, 4096, 256), (2, 2, 4, 144, 400), (3, 8, 8, 128, 2064),
     (4, 6, 16, 1040, 240), (7, 2, 3, 272, 144), (16, 8, 32, 512, 192), (33, 2, 4, 2000, 720), (64, 4, 128, 256, 384),
     (65, 1, 2, 512, 256), (130, 3, 5, 784, 272), (300, 2, 3, 384, 640), (600, 4, 6, 256, 128), (1100, 2, 2, 144, 272),
-    (257, 1, 1, 640, 1024)])
+    (257, 1, 1, 640, 1024), (40, 7, 1000, 32, 48), (1000, 6, 1024, 48, 16)])
 def test_experts(env, m, k, e, h, f):
     Experts(m, k, e, h, f, seed=m + e).check(env)
 
