@@ -22,7 +22,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libinferrous_w8a8.so"
 SOURCES = ["abi.hip", "quantize.hip", "gemv.hip", "gemm.hip", "head.hip", "synth.hip", "sequence.hip",
-           "route.hip", "experts.hip", "experts_tiles.hip", "adapters.hip"]
+           "route.hip", "experts.hip", "experts_tiles.hip", "adapters.hip", "adapters_tiles.hip"]
 ARCH = "gfx950"
 
 

@@ -1438,19 +1438,27 @@ int w8a8_experts_mlp(void* stream, const int8_t* q, const float* asc, size_t m, 
 }
 
 static int check_adapters_shape(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters) {
-  if (m > kU32Max || n > kU32Max || k == 0 || k % 16 != 0 || (m > 0 && m * (size_t)k / k != m)) return W8A8_ESHAPE;
+  if (m > kMaxAdapterRows || n > kU32Max || k == 0 || k % 16 != 0) return W8A8_ESHAPE;
   if (rank == 0 || rank % 8 != 0 || rank > kMaxRank || n_adapters == 0 || n_adapters > kMaxAdapters)
     return W8A8_ESHAPE;
   return W8A8_OK;
 }
 
-// The workspace: accumulators [m, n], the adapters' first product [m, rank], the
-// projection's own.
+// The workspace: the adapters' part, then, unless they run with the projection in
+// one kernel, the projection's sums [m, n] and its own workspace.
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters) {
   if (m == 0 || n == 0 || check_adapters_shape(m, n, k, rank, n_adapters) != W8A8_OK) return 0;
-  return up256(m * n * 4) + up256(m * rank * 4) + w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO);
+  AdapterArgs a{};
+  a.m = (uint32_t)m;
+  a.n = (uint32_t)n;
+  a.width = k;
+  a.rank = rank;
+  a.adapters = n_adapters;
+  const size_t part = up256(adapters_workspace_bytes(a));
+  return adapters_fused(a) ? part
+                           : part + up256(m * n * 4) + w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO);
 }
 
 int w8a8_linear_adapters(void* stream, const int8_t* q, const float* asc, size_t m, const int8_t* w, const float* ws,
@@ -1486,17 +1494,37 @@ int w8a8_linear_adapters(void* stream, const int8_t* q, const float* asc, size_t
   t.residual = residual;
   t.out = out;
   t.out_dtype = out_dtype;
-  char* p = (char*)workspace;
-  int32_t* const acc = (int32_t*)p;
-  float* const h = (float*)(p += up256(m * n * 4));
-  p += up256(m * rank * 4);
+  t.q = q;
+  t.w = w;
   hipStream_t st = (hipStream_t)stream;
-  hipError_t e = launch_adapters_shrink(st, t, h);
-  if (e != hipSuccess) return hip_status(e);
-  s = run_linear(st, q, asc, m, w, ws, n, k, acc, W8A8_OUT_I32, W8A8_PATH_AUTO, nullptr, nullptr, p,
-                 w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO));
+  const hipError_t e = launch_adapters_before(st, t, workspace);
+  if (e != hipSuccess || adapters_fused(t)) return hip_status(e);
+  int32_t* acc = (int32_t*)((char*)workspace + up256(adapters_workspace_bytes(t)));
+  char* const slab_space = (char*)acc + up256(m * n * 4);
+  const size_t slab_bytes = w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO);
+  uint32_t slabs = 1;
+  if (slab_bytes && auto_path(m, n, k, slab_bytes) == W8A8_PATH_MFMA) {
+    // a split-K route leaves its slabs to the kernel that reads them
+    GemmArgs g{};
+    g.q = q;
+    g.asc = asc;
+    g.m = (uint32_t)m;
+    g.w = w;
+    g.ws = ws;
+    g.n = (uint32_t)n;
+    g.k = k;
+    g.out_dtype = W8A8_OUT_I32;
+    g.partials = (int32_t*)slab_space;
+    g.partial_bytes = slab_bytes;
+    slabs = gemm_route(g).splits;
+    if (slabs > 1) acc = g.partials;
+    else g.out = acc;
+    s = hip_status(launch_gemm(st, g));
+  } else {
+    s = run_linear(st, q, asc, m, w, ws, n, k, acc, W8A8_OUT_I32, W8A8_PATH_AUTO, nullptr, nullptr);
+  }
   if (s != W8A8_OK) return s;
-  return hip_status(launch_adapters_expand(st, t, acc, h));
+  return hip_status(launch_adapters_after(st, t, acc, slabs, workspace));
 }
 
 }  // extern "C"

@@ -3,19 +3,16 @@
 #pragma once
 #include "internal.hpp"
 #include "routed_common.hpp"
+#include "row_sort.hpp"
 
 namespace w8a8 {
 
 // The slots sorted by expert: position p of the sorted order holds slot order[p],
-// slot i stands at pos[i] (-1: it has no expert).  A tile is up to BT sorted
-// positions of one expert.
-struct ExpertsTile {
-  uint32_t expert, first, rows, pad;
-};
+// slot i stands at pos[i] (-1: it has no expert); tiles of one expert's positions.
 struct ExpertsPlan {
   uint32_t* order;
   int32_t* pos;
-  ExpertsTile* tiles;
+  RowTile* tiles;
   uint32_t* n_tiles;
 };
 

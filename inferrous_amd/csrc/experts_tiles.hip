@@ -13,146 +13,32 @@
 // y goes through memory as 16-bit fixed point against the largest magnitude of
 // 64 columns of its row: half the bytes of f32, which would be the pass's largest
 // stream, at an error below 2^-16 of that magnitude, 2^-8 of what BF16 would add.
-#include <algorithm>
-
 #include "experts.hpp"
 #include "tile_stream.hpp"
 
 namespace w8a8 {
 
 // ------------------------------------------------------------------ plan
-constexpr int kPlanWaves = 16;
-constexpr uint32_t kPlanBlock = 4096;   // slots that one workgroup sorts alone
-constexpr uint32_t kPlanBlocks = 256;   // workgroups of a larger sort, at most
-
-// Entries [begin, end) of each wave: the workgroup's slots in kPlanWaves runs of
-// whole 64s.
-__device__ __forceinline__ void plan_run(uint32_t slots, uint32_t per_block, int wave, uint32_t& begin, uint32_t& end) {
-  const uint32_t b0 = min(blockIdx.x * per_block, slots), b1 = min(b0 + per_block, slots);
-  const uint32_t run = ((b1 - b0 + 64 * kPlanWaves - 1) / (64 * kPlanWaves)) * 64;
-  begin = min(b0 + wave * run, b1);
-  end = min(begin + run, b1);
-}
-
-__device__ __forceinline__ void plan_count(const int32_t* ids, uint32_t experts, uint32_t begin, uint32_t end,
-                                           uint32_t* hist, int lane) {
-  for (uint32_t e = lane; e < experts; e += 64) hist[e] = 0;
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  for (uint32_t i = begin + lane; i < end; i += 64) {
-    const uint32_t e = (uint32_t)ids[i];
-    if (e < experts) atomicAdd(&hist[e], 1u);  // a count: any order gives it
-  }
-}
-
-// counts[block][e] of a sort over several workgroups.
-__global__ __launch_bounds__(64 * kPlanWaves) void experts_plan_counts(const int32_t* ids, uint32_t slots,
-                                                                       uint32_t per_block, uint32_t experts,
-                                                                       uint32_t* counts) {
-  extern __shared__ uint32_t hist[];  // [kPlanWaves][experts]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t begin, end;
-  plan_run(slots, per_block, wave, begin, end);
-  plan_count(ids, experts, begin, end, hist + wave * experts, lane);
-  __syncthreads();
-  for (uint32_t e = threadIdx.x; e < experts; e += 64 * kPlanWaves) {
-    uint32_t n = 0;
-    for (int w = 0; w < kPlanWaves; ++w) n += hist[w * experts + e];
-    counts[(size_t)blockIdx.x * experts + e] = n;
-  }
-}
-
-// Exclusive sums of v over the workgroup's threads; *all receives the total.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* part, uint32_t* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t t = (uint32_t)__shfl_up((int)s, o, kWave);
-    if (lane >= o) s += t;
-  }
-  if (lane == 63) part[wave] = s;
-  __syncthreads();
-  uint32_t before = 0, total = 0;
-  for (int w = 0; w < kPlanWaves; ++w) {
-    if (w < wave) before += part[w];
-    total += part[w];
-  }
-  __syncthreads();
-  *all = total;
-  return before + s - v;
-}
-
-__global__ __launch_bounds__(64 * kPlanWaves) void experts_plan(const int32_t* ids, uint32_t slots, uint32_t per_block,
-                                                                uint32_t experts, const uint32_t* counts, int bt,
+__global__ __launch_bounds__(64 * kSortWaves) void experts_plan(const int32_t* ids, uint32_t slots, uint32_t per_block,
+                                                                uint32_t experts, const uint32_t* counts, uint32_t bt,
                                                                 ExpertsPlan plan) {
-  extern __shared__ uint32_t hist[];  // [kPlanWaves][experts]: counts, then each wave's next position
-  __shared__ uint32_t part[kPlanWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t e = threadIdx.x;  // experts <= 64 * kPlanWaves
-  uint32_t begin, end;
-  plan_run(slots, per_block, wave, begin, end);
-  plan_count(ids, experts, begin, end, hist + wave * experts, lane);
-  __syncthreads();
-  uint32_t total = 0, before = 0;  // of expert e: all its slots, those of earlier workgroups
-  if (e < experts) {
-    if (gridDim.x == 1) {
-      for (int w = 0; w < kPlanWaves; ++w) total += hist[w * experts + e];
-    } else {
-      for (uint32_t b = 0; b < gridDim.x; ++b) {
-        const uint32_t n = counts[(size_t)b * experts + e];
-        if (b < blockIdx.x) before += n;
-        total += n;
-      }
-    }
-  }
-  uint32_t live, tiles;
-  const uint32_t first = block_prefix(total, part, &live);
-  if (e < experts) {
-    uint32_t p = first + before;
-    for (int w = 0; w < kPlanWaves; ++w) {
-      const uint32_t n = hist[w * experts + e];
-      hist[w * experts + e] = p;
-      p += n;
-    }
-  }
-  if (blockIdx.x == 0) {
-    const uint32_t mine = (total + bt - 1) / bt;
-    const uint32_t at = block_prefix(mine, part, &tiles);
-    for (uint32_t i = 0; i < mine; ++i)
-      plan.tiles[at + i] = ExpertsTile{e, first + i * bt, min((uint32_t)bt, total - i * bt), 0};
-    if (threadIdx.x == 0) *plan.n_tiles = tiles;
-  }
-  __syncthreads();
-  // Each wave walks its run in order.  Lanes of one expert find each other by
-  // ballots over the bits of its number; their order is their lanes'.
-  uint32_t* const next = hist + wave * experts;
-  for (uint32_t i0 = begin; i0 < end; i0 += 64) {
-    const uint32_t i = i0 + lane;
-    const uint32_t id = i < end ? (uint32_t)ids[i] : ~0u;
-    const bool on = id < experts;
-    uint64_t peers = __ballot(on);
-#pragma unroll
-    for (int b = 0; b < 10; ++b) {
-      const uint64_t set = __ballot((id >> b) & 1);
-      peers &= ((id >> b) & 1) ? set : ~set;
-    }
-    uint32_t p = 0;
-    if (on) p = next[id] + (uint32_t)__popcll(peers & ((1ull << lane) - 1));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (on && (peers >> lane) == 1) next[id] = p + 1;  // the last of its peers
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (i < end) plan.pos[i] = on ? (int32_t)p : -1;
-    if (on) plan.order[p] = i;
-  }
+  extern __shared__ uint32_t hist[];
+  __shared__ uint32_t part[kSortWaves];
+  sort_items<false>(
+      ids, slots, per_block, experts, counts, hist, part,
+      [&](uint32_t first, uint32_t total) {
+        if (blockIdx.x == 0) list_tiles(first, total, bt, part, plan.tiles, plan.n_tiles);
+      },
+      [&](uint32_t slot, int32_t p) {
+        plan.pos[slot] = p;
+        if (p >= 0) plan.order[p] = slot;
+      });
 }
 
 // The token tile and column tile of a workgroup, or false past the last one.
 // Each XCD takes a contiguous run of the live tiles, a token tile's columns next
 // to each other.
-__device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t cols, ExpertsTile& t, uint32_t& col) {
+__device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t cols, RowTile& t, uint32_t& col) {
   const uint32_t live = *plan.n_tiles * cols, per = (live + 7) / 8;
   const uint32_t at = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per || at >= live) return false;
@@ -172,12 +58,12 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_gate_u
   constexpr int MAXES = T::WAVES_N * T::BT * 4;
   static_assert(T::BN == 256 && MAXES + T::BT * CSTRIDE <= T::LDS, "the epilogue reuses the rings");
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
-  ExpertsTile t;
+  RowTile t;
   uint32_t group;
   if (!own_tile(plan, (a.inter + 127) / 128, t, group)) return;
   const uint32_t H = a.hidden, I = a.inter, c0 = group * 128, slots = a.m * a.k;
-  const int8_t* const wg = a.w_gate + (size_t)t.expert * I * H;
-  const int8_t* const wu = a.w_up + (size_t)t.expert * I * H;
+  const int8_t* const wg = a.w_gate + (size_t)t.of * I * H;
+  const int8_t* const wu = a.w_up + (size_t)t.of * I * H;
   T s;
   s.run(
       lds, H,
@@ -199,7 +85,7 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_gate_u
 #pragma unroll
     for (int v = 0; v < 8; v += 4) {
       const uint32_t c = c0 + (wn * T::FN + j) * 16 + 4 * half + 2 * v;
-      const size_t n = (size_t)t.expert * I + (c < I ? c : c0);
+      const size_t n = (size_t)t.of * I + (c < I ? c : c0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) gs[j][v + i] = a.ws_gate[n + i], us[j][v + i] = a.ws_up[n + i];
     }
@@ -283,11 +169,11 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_down(E
   constexpr int STRIDE = 144;  // bytes of a row of 64 codes in LDS, padded
   static_assert(T::WN == 64 && T::GROUPED && T::NW * T::WT * STRIDE <= T::LDS, "the epilogue reuses the rings");
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
-  ExpertsTile t;
+  RowTile t;
   uint32_t col;
   if (!own_tile(plan, (a.hidden + T::BN - 1) / T::BN, t, col)) return;
   const uint32_t H = a.hidden, I = a.inter, c0 = col * T::BN, slots = a.m * a.k;
-  const int8_t* const w = a.w_down + (size_t)t.expert * H * I;
+  const int8_t* const w = a.w_down + (size_t)t.of * H * I;
   T s;
   s.run(
       lds, I, [&](int r) { return codes + (size_t)(t.first + ((uint32_t)r < t.rows ? r : 0)) * I; },
@@ -304,7 +190,7 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_down(E
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       const uint32_t c = cw + 32 * j + 4 * half + 8 * (v >> 2) + (v & 3);
-      ws[j][v] = a.ws_down[(size_t)t.expert * H + (c < H ? c : H - 1)];
+      ws[j][v] = a.ws_down[(size_t)t.of * H + (c < H ? c : H - 1)];
     }
   __syncthreads();  // every wave is done with the rings
   int8_t* const mine = lds + wave * T::WT * STRIDE;
@@ -402,22 +288,13 @@ static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Rows of a token tile: the smallest that holds an expert's mean share, so that
 // few tiles are half empty and few experts take two where one would do.
-static int tile_rows(uint32_t slots, uint32_t experts) {
+static uint32_t tile_rows(uint32_t slots, uint32_t experts) {
   const uint32_t mean = slots / std::min(slots, experts);
   return mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
 }
 
-static uint32_t most_tiles(uint32_t slots, uint32_t experts, int bt) {
+static uint32_t most_tiles(uint32_t slots, uint32_t experts, uint32_t bt) {
   return slots / bt + std::min(slots, experts);
-}
-
-static uint32_t plan_blocks(uint32_t slots, uint32_t& per_block) {
-  if (slots <= kPlanBlock) {
-    per_block = slots;
-    return 1;
-  }
-  per_block = std::max<uint32_t>(1024, (slots + kPlanBlocks - 1) / kPlanBlocks);
-  return (slots + per_block - 1) / per_block;
 }
 
 namespace {
@@ -426,8 +303,7 @@ struct Layout {
 };
 Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
   const size_t slots = (size_t)m * k;
-  uint32_t per;
-  const uint32_t blocks = plan_blocks((uint32_t)slots, per);
+  const uint32_t blocks = sort_blocks((uint32_t)slots);
   Layout l{};
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -437,7 +313,7 @@ Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_
   };
   l.order = take(slots * 4);
   l.pos = take(slots * 4);
-  l.tiles = take((size_t)most_tiles((uint32_t)slots, experts, tile_rows((uint32_t)slots, experts)) * sizeof(ExpertsTile));
+  l.tiles = take((size_t)most_tiles((uint32_t)slots, experts, tile_rows((uint32_t)slots, experts)) * sizeof(RowTile));
   l.n_tiles = take(4);
   l.counts = take(blocks > 1 ? (size_t)blocks * experts * 4 : 0);
   l.codes = take(slots * inter);
@@ -481,21 +357,20 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
   const uint32_t slots = a.m * a.k;
   const Layout l = layout(a.m, a.k, a.experts, a.hidden, a.inter);
   char* const p = (char*)workspace;
-  const ExpertsPlan plan{(uint32_t*)(p + l.order), (int32_t*)(p + l.pos), (ExpertsTile*)(p + l.tiles),
+  const ExpertsPlan plan{(uint32_t*)(p + l.order), (int32_t*)(p + l.pos), (RowTile*)(p + l.tiles),
                          (uint32_t*)(p + l.n_tiles)};
   int8_t* const codes = (int8_t*)(p + l.codes);
   float* const scales = (float*)(p + l.scales);
   int16_t* const y = (int16_t*)(p + l.y);
   float* const yscale = (float*)(p + l.yscale);
   uint32_t* const counts = (uint32_t*)(p + l.counts);
-  const int bt = tile_rows(slots, a.experts);
+  const uint32_t bt = tile_rows(slots, a.experts);
   const uint32_t tiles = most_tiles(slots, a.experts, bt);
-  uint32_t per;
-  const uint32_t blocks = plan_blocks(slots, per), lds = kPlanWaves * a.experts * 4;
+  const uint32_t blocks = sort_blocks(slots), per = sort_per_block(slots), lds = kSortWaves * a.experts * 4;
   if (blocks > 1)
-    hipLaunchKernelGGL(experts_plan_counts, dim3(blocks), dim3(64 * kPlanWaves), lds, st, a.ids, slots, per, a.experts,
+    hipLaunchKernelGGL(sort_counts<false>, dim3(blocks), dim3(64 * kSortWaves), lds, st, a.ids, slots, per, a.experts,
                        counts);
-  hipLaunchKernelGGL(experts_plan, dim3(blocks), dim3(64 * kPlanWaves), lds, st, a.ids, slots, per, a.experts, counts,
+  hipLaunchKernelGGL(experts_plan, dim3(blocks), dim3(64 * kSortWaves), lds, st, a.ids, slots, per, a.experts, counts,
                      bt, plan);
   if (bt == 32) gate_up_as<32, 32, 64, 4, 4>(st, a, plan, tiles, codes, scales);
   else if (bt == 64) gate_up_as<64, 64, 32, 4, 4>(st, a, plan, tiles, codes, scales);

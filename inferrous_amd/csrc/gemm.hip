@@ -1421,7 +1421,7 @@ static hipError_t launch_slabs(hipStream_t st, const GemmArgs& a, uint32_t split
   if (nt) gemm(std::integral_constant<int, EP_SLAB>{}, p);
   else gemm(std::integral_constant<int, EP_I32>{}, p);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || (!a.out && a.out_dtype == W8A8_OUT_I32)) return e;
   return nt ? launch_splitk_epilogue<true>(st, a, splits) : launch_splitk_epilogue<false>(st, a, splits);
 }
 

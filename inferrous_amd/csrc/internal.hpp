@@ -192,6 +192,8 @@ hipError_t launch_select(hipStream_t st, const float* x, size_t n, uint64_t* key
 // u64 keys the fused selection of an n-row lm_head writes (an upper bound)
 size_t argmax_keys_bound(size_t n);
 
+// a.out null with W8A8_OUT_I32 on a split-K route: the slabs, i32 [splits][m][n]
+// in a.partials, are left for the caller to add.
 hipError_t launch_gemm(hipStream_t st, const GemmArgs& a);
 // The route of a grouped call (r.bn: columns per tile; kRouteNone where one
 // launch per matrix is the route), and the launch (a: q, asc, m, k,
@@ -233,7 +235,7 @@ struct RouteArgs {
 };
 constexpr uint32_t kMaxExperts = 1024, kMaxRouteGroups = 64, kMaxTopK = 64;
 constexpr uint32_t kMaxExpertWidth = 65536, kMaxExpertSlots = 1u << 24;  // of experts_mlp
-constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1u << 16;              // of linear_adapters
+constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1023, kMaxAdapterRows = 65535 * 32;  // of linear_adapters
 hipError_t launch_route(hipStream_t st, const RouteArgs& a);
 
 // The routed experts' SwiGLU products and their weighted sum (experts.hip).
@@ -256,10 +258,10 @@ struct ExpertsArgs {
 size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);
 hipError_t launch_experts(hipStream_t st, const ExpertsArgs& a, void* workspace);
 
-// Low-rank adapters beside a shared projection (adapters.hip): the adapters'
-// first product h[m, rank], then the outputs from the projection's
-// accumulators.
+// Low-rank adapters beside a shared projection (adapters.hip).
 struct AdapterArgs {
+  const int8_t* q;     // [m, width]
+  const int8_t* w;     // [n, width]
   const void* x;       // [m, width], f32 or BF16
   int x_bf16;
   uint32_t m, n, width, rank, adapters;
@@ -273,8 +275,13 @@ struct AdapterArgs {
   void* out;              // [m, n]
   int out_dtype;          // F32 or BF16
 };
-hipError_t launch_adapters_shrink(hipStream_t st, const AdapterArgs& a, float* h);
-hipError_t launch_adapters_expand(hipStream_t st, const AdapterArgs& a, const int32_t* acc, const float* h);
+size_t adapters_workspace_bytes(const AdapterArgs& a);  // of its m, n, width, rank, adapters
+// The whole call (adapters_fused), or what comes before the projection; then,
+// from the projection's i32 sums acc[m, n] (`slabs` partial ones), the outputs.
+bool adapters_fused(const AdapterArgs& a);
+hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* workspace);
+hipError_t launch_adapters_after(hipStream_t st, const AdapterArgs& a, const int32_t* acc, uint32_t slabs,
+                                 const void* workspace);
 
 hipError_t launch_synth_i8(hipStream_t st, int8_t* out, size_t n, uint64_t seed, uint64_t stream_id);
 hipError_t launch_synth_f32(hipStream_t st, float* out, size_t n, uint64_t seed, uint64_t stream_id,

@@ -1,0 +1,177 @@
+// row_sort.hpp -- a counting sort of items by a small class number that keeps
+// the items' order, shared by the routed experts (slots by expert) and the
+// adapters (rows by adapter).
+//
+// Classes are 0 .. classes - 1, classes <= kSortClasses; an item of any other
+// number is of class `classes` where REST is set, and of none otherwise.  A
+// workgroup of kSortWaves waves sorts up to kSortBlock items alone; more are
+// sorted by several workgroups, whose counts a launch before theirs has taken.
+// The order is a function of the items alone: positions come from counts and
+// ballots, never from the order in which atomics return.
+#pragma once
+#include <algorithm>
+
+#include "device_common.hpp"
+
+namespace w8a8 {
+
+constexpr int kSortWaves = 16;
+constexpr uint32_t kSortClasses = 1024;
+constexpr uint32_t kSortBlock = 4096;
+constexpr uint32_t kSortBlocks = 256;  // workgroups at most
+
+// Items of a workgroup: all of them, or runs of at least 1024.
+static inline uint32_t sort_per_block(uint32_t items) {
+  return items <= kSortBlock ? items : std::max<uint32_t>(1024, (items + kSortBlocks - 1) / kSortBlocks);
+}
+static inline uint32_t sort_blocks(uint32_t items) {
+  const uint32_t per = sort_per_block(items);
+  return per ? (items + per - 1) / per : 0;
+}
+
+template <bool REST>
+__device__ __forceinline__ uint32_t sort_class(int32_t id, uint32_t classes) {
+  return (uint32_t)id < classes ? (uint32_t)id : REST ? classes : ~0u;
+}
+
+// Items [begin, end) of a wave: the workgroup's in kSortWaves runs of whole 64s.
+__device__ __forceinline__ void sort_run(uint32_t items, uint32_t per_block, int wave, uint32_t& begin, uint32_t& end) {
+  const uint32_t b0 = min(blockIdx.x * per_block, items), b1 = min(b0 + per_block, items);
+  const uint32_t run = ((b1 - b0 + 64 * kSortWaves - 1) / (64 * kSortWaves)) * 64;
+  begin = min(b0 + wave * run, b1);
+  end = min(begin + run, b1);
+}
+
+template <bool REST>
+__device__ __forceinline__ void sort_count(const int32_t* ids, uint32_t classes, uint32_t begin, uint32_t end,
+                                           uint32_t* hist, int lane) {
+  const uint32_t n = classes + REST;
+  for (uint32_t e = lane; e < n; e += 64) hist[e] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (uint32_t i = begin + lane; i < end; i += 64) {
+    const uint32_t e = sort_class<REST>(ids[i], classes);
+    if (e < n) atomicAdd(&hist[e], 1u);  // a count: any order gives it
+  }
+}
+
+// counts[workgroup][class] of a sort over several workgroups.
+template <bool REST>
+__global__ __launch_bounds__(64 * kSortWaves) void sort_counts(const int32_t* ids, uint32_t items, uint32_t per_block,
+                                                               uint32_t classes, uint32_t* counts) {
+  extern __shared__ uint32_t hist[];  // [kSortWaves][classes]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t n = classes + REST;
+  uint32_t begin, end;
+  sort_run(items, per_block, wave, begin, end);
+  sort_count<REST>(ids, classes, begin, end, hist + wave * n, lane);
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < n; e += 64 * kSortWaves) {
+    uint32_t sum = 0;
+    for (int w = 0; w < kSortWaves; ++w) sum += hist[w * n + e];
+    counts[(size_t)blockIdx.x * n + e] = sum;
+  }
+}
+
+// Exclusive sums of v over the workgroup's threads; *all receives the total.
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* part, uint32_t* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = (uint32_t)__shfl_up((int)s, o, kWave);
+    if (lane >= o) s += t;
+  }
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+  for (int w = 0; w < kSortWaves; ++w) {
+    if (w < wave) before += part[w];
+    total += part[w];
+  }
+  __syncthreads();
+  *all = total;
+  return before + s - v;
+}
+
+// Up to `rows` sorted positions of one class.
+struct RowTile {
+  uint32_t of, first, rows, pad;
+};
+
+// The table of the classes' tiles of up to bt positions, by every thread of one
+// workgroup: thread e lists class e's.
+__device__ __forceinline__ void list_tiles(uint32_t first, uint32_t total, uint32_t bt, uint32_t* part, RowTile* table,
+                                           uint32_t* n_tiles) {
+  uint32_t tiles;
+  const uint32_t mine = (total + bt - 1) / bt, at = block_prefix(mine, part, &tiles);
+  for (uint32_t i = 0; i < mine; ++i)
+    table[at + i] = RowTile{(uint32_t)threadIdx.x, first + i * bt, (uint32_t)min(bt, total - i * bt), 0u};
+  if (threadIdx.x == 0) *n_tiles = tiles;
+}
+
+// The sort's positions.  hist: [kSortWaves][classes + REST] words, part:
+// [kSortWaves] of LDS; counts as sort_counts wrote them (unused by one
+// workgroup).  firsts(first, total) is called once by every thread of the
+// workgroup with its class's first position and item count (thread e: class e;
+// 0 items past the last class), place(item, position) by each item's lane, with
+// -1 for an item of no class.
+template <bool REST, class Firsts, class Place>
+__device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, uint32_t per_block, uint32_t classes,
+                                           const uint32_t* counts, uint32_t* hist, uint32_t* part, Firsts firsts,
+                                           Place place) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t e = threadIdx.x, n = classes + REST;
+  uint32_t begin, end;
+  sort_run(items, per_block, wave, begin, end);
+  sort_count<REST>(ids, classes, begin, end, hist + wave * n, lane);
+  __syncthreads();
+  uint32_t total = 0, before = 0;  // of class e: all its items, those of earlier workgroups
+  if (e < n) {
+    if (gridDim.x == 1) {
+      for (int w = 0; w < kSortWaves; ++w) total += hist[w * n + e];
+    } else {
+      for (uint32_t b = 0; b < gridDim.x; ++b) {
+        const uint32_t c = counts[(size_t)b * n + e];
+        if (b < blockIdx.x) before += c;
+        total += c;
+      }
+    }
+  }
+  uint32_t all;
+  const uint32_t first = block_prefix(total, part, &all);
+  if (e < n) {
+    uint32_t p = first + before;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = hist[w * n + e];
+      hist[w * n + e] = p;
+      p += c;
+    }
+  }
+  firsts(first, total);
+  __syncthreads();
+  // Each wave walks its run in order.  Lanes of one class find each other by
+  // ballots over the bits of its number; their order is their lanes'.
+  uint32_t* const next = hist + wave * n;
+  for (uint32_t i0 = begin; i0 < end; i0 += 64) {
+    const uint32_t i = i0 + lane;
+    const uint32_t c = i < end ? sort_class<REST>(ids[i], classes) : ~0u;
+    const bool on = c < n;
+    uint64_t peers = __ballot(on);
+#pragma unroll
+    for (int b = 0; b < 10; ++b) {
+      const uint64_t set = __ballot((c >> b) & 1);
+      peers &= ((c >> b) & 1) ? set : ~set;
+    }
+    uint32_t p = 0;
+    if (on) p = next[c] + (uint32_t)__popcll(peers & ((1ull << lane) - 1));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (on && (peers >> lane) == 1) next[c] = p + 1;  // the last of its peers
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (i < end) place(i, on ? (int32_t)p : -1);
+  }
+}
+
+}  // namespace w8a8

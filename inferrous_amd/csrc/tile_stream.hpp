@@ -23,9 +23,15 @@
 // i32 sums are scaled into f32 accumulators when the stage is done.  The scales
 // (f32, one per token row of the wave) ride as one more load of the token ring.
 //
-// TAIL (K % 128 != 0): in the last stage a lane whose chunk lies past K reads
-// zeros for the token and its weight row's first chunk: nothing outside the
-// operands is read, and the sums are exact.
+// The op (OP) is the int8 one above or v_mfma_f32_32x32x16_bf16, whose fragments
+// are 16 bytes a lane too and whose result has the same layout.  K is then the
+// weight row's bytes, 2 a value.  OP_BF16_F32's token rows are f32, twice the
+// bytes: a stage takes 256 of them, in two LDS sections of 128 a row, and a
+// fragment is rounded to BF16 as it is read.
+//
+// TAIL (K need not be a multiple of 128): in the last stage a lane whose chunk
+// lies past K reads zeros, for both operands (a BF16 weight may be infinite):
+// nothing outside the operands is read, and the sums are unchanged.
 #pragma once
 #include <type_traits>
 
@@ -47,22 +53,41 @@ __device__ __forceinline__ void await_loads() {
 
 __device__ const v4i kZeros16 = {0, 0, 0, 0};
 
-template <int BT_, int BN_, int WT_, int WN_, int SA_, int SB_, bool GROUPED_, bool TAIL_>
+enum { OP_I8 = 0, OP_BF16 = 1, OP_BF16_F32 = 2 };
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ v16f mfma_bf16(v4i a, v4i b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16i mfma_op(v4i a, v4i b, v16i c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma_op(v4i a, v4i b, v16f c) { return mfma_bf16(a, b, c); }
+
+// Two f32 values as BF16, rounded to nearest even.
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  return (__float_as_uint(bf16_rne(a)) >> 16) | (__float_as_uint(bf16_rne(b)) & 0xffff0000u);
+}
+
+template <int BT_, int BN_, int WT_, int WN_, int SA_, int SB_, bool GROUPED_, bool TAIL_, int OP_ = OP_I8>
 struct TileStream {
+  static constexpr int OP = OP_, TS = OP == OP_BF16_F32 ? 2 : 1;  // sections of a token row's stage
+  using Acc = std::conditional_t<OP == OP_I8, v16i, v16f>;
   static constexpr int BT = BT_, BN = BN_, WT = WT_, WN = WN_, SA = SA_, SB = SB_;
   static constexpr bool GROUPED = GROUPED_, TAIL = TAIL_;
   static constexpr int WAVES_N = BN / WN, NW = (BT / WT) * WAVES_N;
   static constexpr int FT = WT / 32, FN = WN / 32;
-  static constexpr int LT = BT / 8 / NW, LN = BN / 8 / NW;  // row loads per wave per stage
+  static constexpr int LT = TS * BT / 8 / NW, LN = BN / 8 / NW;  // row loads per wave per stage
   static constexpr int LA = LT + (GROUPED ? 1 : 0), L = LA + LN;
-  static constexpr int ASL = BT * 128, BSL = BN * 128, SCL = GROUPED ? 256 : 0;
+  static constexpr int ASL = TS * BT * 128, BSL = BN * 128, SCL = GROUPED ? 256 : 0;
   static constexpr int RINGS = SA * ASL + SB * BSL;
   static constexpr int LDS = RINGS + NW * SA * SCL;
+  static_assert(!GROUPED || OP == OP_I8, "scaled groups are of int8 sums");
   static_assert(LT >= 1 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads");
   static_assert(SA >= 2 && SB >= SA && SB <= 8 && (SA - 1) * LA + (SB - 1) * LN < 64, "ring depths");
   static_assert(LDS <= 160 * 1024, "LDS");
 
-  v16i acc[FT][FN];
+  Acc acc[FT][FN];
   v16f sum[GROUPED ? FT : 1][GROUPED ? FN : 1];
 
   // token_row(r) / weight_row(r): the first byte of tile row r (any row of the
@@ -74,7 +99,7 @@ struct TileStream {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wt0 = (wave / WAVES_N) * WT, wn0 = (wave % WAVES_N) * WN;
-    const uint32_t KT = TAIL ? K / 128 + 1 : K / 128;
+    const uint32_t KT = TAIL ? (K + 127) / 128 : K / 128;
     int8_t* const lds_t = lds;
     int8_t* const lds_n = lds + SA * ASL;
     int8_t* const lds_s = lds + RINGS + wave * SA * SCL;
@@ -82,7 +107,10 @@ struct TileStream {
     auto chunk = [&](int g) { return (uint32_t)((lane & 7) ^ ((lds_row(g) >> 1) & 7)) * 16; };
     const int8_t *pt[LT], *pn[LN];
 #pragma unroll
-    for (int j = 0; j < LT; ++j) pt[j] = token_row(lds_row(wave * LT + j)) + (TAIL ? 0 : chunk(wave * LT + j));
+    for (int j = 0; j < LT; ++j) {  // LDS row BT + r is the second section of token row r
+      const int r = lds_row(wave * LT + j);
+      pt[j] = token_row(TS == 2 && r >= BT ? r - BT : r) + (r >= BT ? 128 : 0) + (TAIL ? 0 : chunk(wave * LT + j));
+    }
 #pragma unroll
     for (int j = 0; j < LN; ++j) pn[j] = weight_row(lds_row(wave * LN + j)) + (TAIL ? 0 : chunk(wave * LN + j));
     const float* ps = nullptr;
@@ -93,10 +121,10 @@ struct TileStream {
                                          W8A8_LDS(lds_s + (kt % SA) * SCL), 4, 0, 0);
         return;
       }
-      const int8_t* p = pt[j] + (size_t)kt * 128;
+      const int8_t* p = pt[j] + (size_t)kt * (128 * TS);
       if constexpr (TAIL) {
-        const uint32_t c = chunk(wave * LT + j);
-        p = kt * 128 + c < K ? p + c : (const int8_t*)&kZeros16;
+        const uint32_t c = chunk(wave * LT + j), sec = lds_row(wave * LT + j) >= BT ? 128 : 0;
+        p = kt * (128 * TS) + sec + c < K * TS ? p + c : (const int8_t*)&kZeros16;
       }
       __builtin_amdgcn_global_load_lds((const void*)p,
                                        W8A8_LDS(lds_t + (kt % SA) * ASL + (wave * LT + j) * 1024), 16, 0, 0);
@@ -105,7 +133,7 @@ struct TileStream {
       const int8_t* p = pn[j] + (size_t)kt * 128;
       if constexpr (TAIL) {
         const uint32_t c = chunk(wave * LN + j);
-        p = kt * 128 + c < K ? p + c : pn[j];
+        p = kt * 128 + c < K ? p + c : (const int8_t*)&kZeros16;
       }
       __builtin_amdgcn_global_load_lds((const void*)p,
                                        W8A8_LDS(lds_n + (kt % SB) * BSL + (wave * LN + j) * 1024), 16, 0, 0);
@@ -118,14 +146,24 @@ struct TileStream {
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        acc[f][j] = v16i{};
+        acc[f][j] = Acc{};
         if constexpr (GROUPED) sum[f][j] = v16f{};
       }
     auto rd = [&](uint32_t kt, int i, v4i(&tf)[FT], v4i(&nf)[FN]) {
       const int8_t* bt = lds_t + (kt % SA) * ASL;
       const int8_t* bn = lds_n + (kt % SB) * BSL;
 #pragma unroll
-      for (int f = 0; f < FT; ++f) tf[f] = *(const v4i*)(bt + (wt0 + 32 * f) * 128 + off[i]);
+      for (int f = 0; f < FT; ++f) {
+        if constexpr (TS == 1) {
+          tf[f] = *(const v4i*)(bt + (wt0 + 32 * f) * 128 + off[i]);
+        } else {  // 16 values of the stage: half a section; a lane's 8 are two chunks
+          const int8_t* const r = bt + ((i >> 1) * BT + wt0 + 32 * f + fr) * 128;
+          const int c = 4 * (i & 1) + 2 * fh, key = (fr >> 1) & 7;
+          const v4f a = *(const v4f*)(r + (c ^ key) * 16), b = *(const v4f*)(r + ((c + 1) ^ key) * 16);
+          tf[f] = v4i{(int)bf16_pair(a.x, a.y), (int)bf16_pair(a.z, a.w), (int)bf16_pair(b.x, b.y),
+                      (int)bf16_pair(b.z, b.w)};
+        }
+      }
 #pragma unroll
       for (int j = 0; j < FN; ++j) nf[j] = *(const v4i*)(bn + (wn0 + 32 * j) * 128 + off[i]);
     };
@@ -135,8 +173,8 @@ struct TileStream {
       constexpr int N = decltype(n)::value, MF = FT * FN;
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        v16i& d = acc[i / FN][i % FN];
-        d = __builtin_amdgcn_mfma_i32_32x32x32_i8(nf[i % FN], tf[i / FN], decltype(first)::value ? v16i{} : d, 0, 0, 0);
+        Acc& d = acc[i / FN][i % FN];
+        d = mfma_op(nf[i % FN], tf[i / FN], decltype(first)::value ? Acc{} : d);
         const int lo = (i * N + MF - 1) / MF, hi = ((i + 1) * N + MF - 1) / MF;
         if (lo == hi) continue;
         __builtin_amdgcn_sched_barrier(0);
