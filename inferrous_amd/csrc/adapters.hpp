@@ -10,18 +10,8 @@ namespace w8a8 {
 
 static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// The distinct adapters of 32 rows, one after another: f(adapter, rows) with the
-// rows' bits.  Wave-uniform; lanes l and l + 32 hold row l's id.
-template <class F>
-__device__ __forceinline__ void each_adapter(uint32_t id, bool live, F f) {
-  uint32_t todo = (uint32_t)__ballot(live);
-  while (todo) {
-    const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)id, __builtin_ctz(todo));
-    const uint32_t rows = (uint32_t)__ballot(live && id == a);
-    todo &= ~rows;
-    f(a, rows);
-  }
-}
+// Values of a row of h's BF16 parts: the ranks, padded to whole 32s.
+__host__ __device__ constexpr uint32_t part_width(uint32_t rank) { return (rank + 31) / 32 * 32; }
 
 // How a call runs, a function of its sizes.
 struct AdapterPlan {

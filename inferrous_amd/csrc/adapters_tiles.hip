@@ -3,8 +3,8 @@
 //
 //   adapters_order          the sort, and the tiles: up to bt rows of one adapter;
 //   adapters_shrink_tiles   h's partial sums, tile x share of K, by bf16 MFMA;
-//   adapters_parts          h as two BF16 parts, high and low, whose products with
-//                           B are exact: 16 bits of h count, not 8;
+//   adapters_parts          scaling * h as two BF16 parts, high and low, whose
+//                           products with B are exact: 16 bits count, not 8;
 //   adapters_gemm           the projection over the sorted rows, its int8 sums
 //                           scaled in their registers and the second product
 //                           added to them by bf16 MFMA before the one store.
@@ -68,17 +68,21 @@ __global__ __launch_bounds__(64 * T::NW) void adapters_shrink_tiles(AdapterArgs 
   }
 }
 
-// high + low = the sum of the shares, to 16 bits; rows padded with zeros to a
-// multiple of 16 values.
-__global__ __launch_bounds__(256) void adapters_parts(const float* h, uint32_t m, uint32_t rank, uint32_t splits,
-                                                      uint16_t* high, uint16_t* low) {
-  const uint32_t quads = (rank + 15) / 16 * 4;
+// high + low = scaling * the sum of the shares, to 16 bits; rows padded with zeros
+// to a multiple of 32 values.
+__global__ __launch_bounds__(256) void adapters_parts(AdapterArgs a, const uint32_t* order, const float* h,
+                                                      uint32_t splits, uint16_t* high, uint16_t* low) {
+  const uint32_t quads = part_width(a.rank) / 4;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (size_t)m * quads) return;
-  const uint32_t j = (uint32_t)(i % quads) * 4;
+  if (i >= (size_t)a.m * quads) return;
+  const uint32_t p = (uint32_t)(i / quads), j = (uint32_t)(i % quads) * 4;
+  const uint32_t id = (uint32_t)a.ids[order[p]];
   v4f s{};
-  if (j < rank)
-    for (uint32_t t = 0; t < splits; ++t) s += *(const v4f*)(h + ((size_t)t * m + i / quads) * rank + j);
+  if (j < a.rank && id < a.adapters) {
+#pragma unroll 4
+    for (uint32_t t = 0; t < splits; ++t) s += *(const v4f*)(h + ((size_t)t * a.m + p) * a.rank + j);
+    s *= a.scaling[id];
+  }
   const uint32_t h0 = bf16_pair(s.x, s.y), h1 = bf16_pair(s.z, s.w);
   *(v2i*)(high + i * 4) = v2i{(int)h0, (int)h1};
   *(v2i*)(low + i * 4) = v2i{(int)bf16_pair(s.x - bf16_lo(h0), s.y - bf16_hi(h0)),
@@ -89,12 +93,22 @@ __global__ __launch_bounds__(256) void adapters_parts(const float* h, uint32_t m
 // operands (gemm.hip).
 constexpr uint32_t kStripTiles = 4;
 
+// After the K loop the rings' memory holds, 32 ranks at a time, the tile's B rows of
+// one adapter and its rows' two parts of h: one load from memory serves every
+// wave, and the next ranks (or adapter) are in flight while the waves multiply.
+// Rows of another adapter keep the value they had (a lane is one row).
 template <class T>
 __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, const uint32_t* order,
                                                               const uint16_t* high, const uint16_t* low,
                                                               uint32_t tiles_m, uint32_t tiles_n, bool wide) {
-  constexpr int STRIDE = T::WN + 4;  // f32 values of an LDS row, padded
-  static_assert(T::NW * 32 * STRIDE * 4 <= T::LDS, "the epilogue reuses the rings");
+  constexpr int PAIR = 40;          // BF16 values of an LDS row of 32, padded
+  constexpr int STRIDE = 64 + 4;    // f32 values of an LDS row of 64 columns, padded
+  constexpr int THREADS = 64 * T::NW;
+  constexpr int B_AT = 0, H_AT = T::BN * PAIR * 2, L_AT = H_AT + T::BT * PAIR * 2, W_AT = L_AT + T::BT * PAIR * 2;
+  constexpr int O_AT = W_AT + T::BN * 4;
+  static_assert(O_AT + T::NW * 32 * STRIDE * 4 <= T::LDS, "the epilogue reuses the rings");
+  static_assert(T::WN % 64 == 0 && T::BN * 4 % THREADS == 0 && T::BT * 4 % THREADS == 0, "whole loads");
+  constexpr int LB = T::BN * 4 / THREADS, LH = T::BT * 4 / THREADS;  // 16-byte loads of a thread
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
   const uint32_t G = tiles_m * tiles_n;
   uint32_t at = blockIdx.x;
@@ -110,87 +124,165 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
 
   const int lane = threadIdx.x & 63, half = lane >> 5, tl = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t wt0 = m0 + (wave / T::WAVES_N) * T::WT, cw = n0 + (wave % T::WAVES_N) * T::WN;
-  const uint32_t padded = (a.rank + 15) / 16 * 16;
-  float* const mine = (float*)lds + wave * 32 * STRIDE;
-  __syncthreads();  // every wave is done with the rings
+  const uint32_t wt = (wave / T::WAVES_N) * T::WT, wn = (wave % T::WAVES_N) * T::WN;
+  const uint32_t padded = part_width(a.rank), rows_in = min((uint32_t)T::BT, a.m - m0);
+  // the wave's rows
+  uint32_t row[T::FT], id[T::FT];
+  float asc[T::FT];
 #pragma unroll
   for (int f = 0; f < T::FT; ++f) {
-    const uint32_t p = wt0 + 32 * f + tl, pc = p < a.m ? p : m0;
-    const uint32_t row = order[pc];
-    const uint32_t id = p < a.m ? (uint32_t)a.ids[row] : ~0u;
-    const float asc = a.asc[row];
-    // a block of columns at a time: what the sums leave of the registers
+    const uint32_t r = wt + 32 * f + tl;
+    row[f] = order[m0 + (r < rows_in ? r : 0)];
+    id[f] = r < rows_in ? (uint32_t)a.ids[row[f]] : ~0u;
+    asc[f] = a.asc[row[f]];
+  }
+  // the tile's ids, every wave alike: lane l's are rows l, l + 64, ...
+  uint32_t tid[T::BT / 64];
 #pragma unroll
-    for (int j = 0; j < T::FN; ++j) {
-      float y[16];
+  for (int i = 0; i < T::BT / 64; ++i) {
+    const uint32_t r = lane + 64 * i;
+    tid[i] = r < rows_in ? (uint32_t)a.ids[order[m0 + r]] : ~0u;
+  }
+  __syncthreads();  // every wave is done with the rings
+  float* const tile_ws = (float*)(lds + W_AT);
+  for (int c = threadIdx.x; c < T::BN; c += THREADS) tile_ws[c] = a.ws[min(n0 + c, a.n - 1)];
+  __syncthreads();
+  v16f y[T::FT][T::FN];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const uint32_t c = cw + 32 * j + 8 * (v >> 2) + 4 * half + (v & 3);
-        y[v] = (float)s.acc[f][j][v] * asc * a.ws[c < a.n ? c : a.n - 1];
-      }
-      each_adapter(id, id < a.adapters, [&](uint32_t ad, uint32_t rows) {
-        const uint16_t* const b = a.b + ((size_t)ad * a.n + min(cw + 32 * j + tl, a.n - 1)) * a.rank + 8 * half;
-        const size_t ho = (size_t)pc * padded + 8 * half;
-        v16f d{};
-#pragma unroll 2
-        for (uint32_t k = 0; k < a.rank; k += 16) {
-          const v4i hi = *(const v4i*)(high + ho + k), lo = *(const v4i*)(low + ho + k);
-          const v4i bf = k + 8 * half < a.rank ? *(const v4i*)(b + k) : v4i{};
-          d = mfma_bf16(bf, hi, d);
-          d = mfma_bf16(bf, lo, d);
-        }
-        const float sc = a.scaling[ad];
-        if ((rows >> tl) & 1) {
+  for (int j = 0; j < T::FN; ++j)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) y[v] += sc * d[v];
-        }
-      });
-      // 32 rows through the wave's own LDS: whole runs of a row to memory
+    for (int q = 0; q < 4; ++q) {
+      const v4f w = *(const v4f*)(tile_ws + wn + 32 * j + 8 * q + 4 * half);
 #pragma unroll
-      for (int v = 0; v < 16; v += 4)
-        *(v4f*)(mine + tl * STRIDE + 32 * j + 2 * v + 4 * half) = v4f{y[v], y[v + 1], y[v + 2], y[v + 3]};
+      for (int f = 0; f < T::FT; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[f][j][4 * q + i] = (float)s.acc[f][j][4 * q + i] * asc[f] * w[i];
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (wide) {  // n % 8 == 0: 16-byte stores
-      constexpr int PER = T::WN / 8, ROWS = 64 / PER;
+  // Rows are sorted by adapter, those without one last: the tile's adapters follow
+  // each other, each from the row after the last one's.
+  auto at_row = [&](uint32_t r) {  // the id of tile row r, wave-uniform
+    uint32_t v = 0;
 #pragma unroll
-      for (int i = 0; i < 32; i += ROWS) {
-        const uint32_t r = i + lane / PER, c = (lane % PER) * 8;
-        const uint32_t to = (uint32_t)__shfl((int)row, (int)r, kWave);
-        if (wt0 + 32 * f + r >= a.m || cw + c >= a.n) continue;
-        const size_t o = (size_t)to * a.n + cw + c;
-        v4f lo = *(const v4f*)(mine + r * STRIDE + c), hi = *(const v4f*)(mine + r * STRIDE + c + 4);
-        if (a.residual) {
-          lo += *(const v4f*)(a.residual + o);
-          hi += *(const v4f*)(a.residual + o + 4);
+    for (int i = 0; i < T::BT / 64; ++i)
+      if ((r >> 6) == (uint32_t)i) v = (uint32_t)__builtin_amdgcn_readlane((int)tid[i], (int)(r & 63));
+    return v;
+  };
+  auto count = [&](uint32_t ad) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < T::BT / 64; ++i) c += (uint32_t)__popcll(__ballot(tid[i] == ad));
+    return c;
+  };
+  v4i rb[LB], rh[LH], rl[LH];
+  auto fetch = [&](uint32_t ad, uint32_t k) {
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      const uint32_t t = threadIdx.x + i * THREADS, kk = k + (t & 3) * 8;
+      rb[i] = kk < a.rank ? *(const v4i*)(a.b + ((size_t)ad * a.n + min(n0 + (t >> 2), a.n - 1)) * a.rank + kk) : v4i{};
+    }
+#pragma unroll
+    for (int i = 0; i < LH; ++i) {
+      const uint32_t t = threadIdx.x + i * THREADS, r = t >> 2;
+      const size_t o = (size_t)(m0 + (r < rows_in ? r : 0)) * padded + k + (t & 3) * 8;
+      rh[i] = *(const v4i*)(high + o);
+      rl[i] = *(const v4i*)(low + o);
+    }
+  };
+  uint32_t r0 = 0, ad = at_row(0);
+  if (ad < a.adapters) fetch(ad, 0);
+  while (ad < a.adapters) {
+    const uint32_t r1 = r0 + count(ad), next = r1 < rows_in ? at_row(r1) : ~0u;
+    for (uint32_t k = 0; k < a.rank; k += 32) {
+      __syncthreads();  // the last ranks are multiplied
+#pragma unroll
+      for (int i = 0; i < LB; ++i) {
+        const uint32_t t = threadIdx.x + i * THREADS;
+        *(v4i*)(lds + B_AT + (t >> 2) * PAIR * 2 + (t & 3) * 16) = rb[i];
+      }
+#pragma unroll
+      for (int i = 0; i < LH; ++i) {
+        const uint32_t t = threadIdx.x + i * THREADS;
+        *(v4i*)(lds + H_AT + (t >> 2) * PAIR * 2 + (t & 3) * 16) = rh[i];
+        *(v4i*)(lds + L_AT + (t >> 2) * PAIR * 2 + (t & 3) * 16) = rl[i];
+      }
+      __syncthreads();
+      if (k + 32 < a.rank) fetch(ad, k + 32);
+      else if (next < a.adapters) fetch(next, 0);
+#pragma unroll
+      for (int f = 0; f < T::FT; ++f) {
+        const bool on = id[f] == ad;
+        if (!__ballot(on)) continue;
+        v4i hi[2], lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int o = (wt + 32 * f + tl) * PAIR * 2 + 32 * i + 16 * half;
+          hi[i] = *(const v4i*)(lds + H_AT + o);
+          lo[i] = *(const v4i*)(lds + L_AT + o);
         }
-        if (a.out_dtype == W8A8_OUT_F32) {
-          float* const out = (float*)a.out + o;
-          *(v4f*)out = v4f{bf16_rne(lo.x), bf16_rne(lo.y), bf16_rne(lo.z), bf16_rne(lo.w)};
-          *(v4f*)(out + 4) = v4f{bf16_rne(hi.x), bf16_rne(hi.y), bf16_rne(hi.z), bf16_rne(hi.w)};
-        } else {
-          *(v4i*)((uint16_t*)a.out + o) = v4i{(int)bf16_pair(lo.x, lo.y), (int)bf16_pair(lo.z, lo.w),
-                                             (int)bf16_pair(hi.x, hi.y), (int)bf16_pair(hi.z, hi.w)};
+#pragma unroll
+        for (int j = 0; j < T::FN; ++j) {
+          v16f d = y[f][j];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const v4i b = *(const v4i*)(lds + B_AT + (wn + 32 * j + tl) * PAIR * 2 + 32 * i + 16 * half);
+            d = mfma_bf16(b, hi[i], d);
+            d = mfma_bf16(b, lo[i], d);
+          }
+#pragma unroll
+          for (int v = 0; v < 16; ++v) y[f][j][v] = on ? d[v] : y[f][j][v];
         }
       }
-    } else {
-      for (int r = 0; r < 32; ++r) {
-        const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)row, r);
-        if (wt0 + 32 * f + r >= a.m) break;
+    }
+    r0 = r1;
+    ad = next;
+  }
+  // 32 rows x 64 columns at a time through the wave's own LDS: whole runs of a row
+  // to memory
+  float* const mine = (float*)(lds + O_AT) + wave * 32 * STRIDE;
 #pragma unroll
-        for (int c = lane; c < T::WN; c += 64) {
-          if (cw + c >= a.n) continue;
+  for (int f = 0; f < T::FT; ++f)
+#pragma unroll
+    for (int j0 = 0; j0 < T::FN; j0 += 2) {
+      const uint32_t cw = n0 + wn + 32 * j0, rw = wt + 32 * f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4)
+          *(v4f*)(mine + tl * STRIDE + 32 * j + 2 * v + 4 * half) =
+              v4f{y[f][j0 + j][v], y[f][j0 + j][v + 1], y[f][j0 + j][v + 2], y[f][j0 + j][v + 3]};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (wide) {  // n % 8 == 0: 16-byte stores
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          const uint32_t r = i + (lane >> 3), c = (lane & 7) * 8;
+          const uint32_t to = (uint32_t)__shfl((int)row[f], (int)r, kWave);
+          if (rw + r >= rows_in || cw + c >= a.n) continue;
           const size_t o = (size_t)to * a.n + cw + c;
-          const float v = mine[r * STRIDE + c];
+          v4f lo = *(const v4f*)(mine + r * STRIDE + c), hi = *(const v4f*)(mine + r * STRIDE + c + 4);
+          if (a.residual) {
+            lo += *(const v4f*)(a.residual + o);
+            hi += *(const v4f*)(a.residual + o + 4);
+          }
+          if (a.out_dtype == W8A8_OUT_F32) {
+            float* const out = (float*)a.out + o;
+            *(v4f*)out = v4f{bf16_rne(lo.x), bf16_rne(lo.y), bf16_rne(lo.z), bf16_rne(lo.w)};
+            *(v4f*)(out + 4) = v4f{bf16_rne(hi.x), bf16_rne(hi.y), bf16_rne(hi.z), bf16_rne(hi.w)};
+          } else {
+            *(v4i*)((uint16_t*)a.out + o) = v4i{(int)bf16_pair(lo.x, lo.y), (int)bf16_pair(lo.z, lo.w),
+                                               (int)bf16_pair(hi.x, hi.y), (int)bf16_pair(hi.z, hi.w)};
+          }
+        }
+      } else if (cw + lane < a.n) {
+        for (uint32_t r = 0; r < 32 && rw + r < rows_in; ++r) {
+          const size_t o = (size_t)(uint32_t)__builtin_amdgcn_readlane((int)row[f], (int)r) * a.n + cw + lane;
+          const float v = mine[r * STRIDE + lane];
           store_routed(a.out, a.out_dtype, o, a.residual ? a.residual[o] + v : v);
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
 }
 
 // ------------------------------------------------------------------ launches
@@ -246,9 +338,9 @@ hipError_t launch_adapters_sorted(hipStream_t st, const AdapterArgs& a, const Ad
 }
 
 hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* ws) {
-  const size_t quads = (size_t)a.m * ((a.rank + 15) / 16 * 4);
-  hipLaunchKernelGGL(adapters_parts, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st,
-                     (const float*)(ws + p.h), a.m, a.rank, p.splits, (uint16_t*)(ws + p.high),
+  const size_t quads = (size_t)a.m * (part_width(a.rank) / 4);
+  hipLaunchKernelGGL(adapters_parts, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, a,
+                     (const uint32_t*)(ws + p.order), (const float*)(ws + p.h), p.splits, (uint16_t*)(ws + p.high),
                      (uint16_t*)(ws + p.low));
   const uint64_t big = (uint64_t)((a.m + 255) / 256) * ((a.n + 255) / 256);
   if (big >= 192) gemm_as<256, 256, 64, 128, 2, 3>(st, a, p, ws);

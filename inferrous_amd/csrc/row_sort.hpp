@@ -68,6 +68,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_counts(const int32_t* id
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < n; e += 64 * kSortWaves) {
     uint32_t sum = 0;
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) sum += hist[w * n + e];
     counts[(size_t)blockIdx.x * n + e] = sum;
   }
@@ -85,6 +86,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* part, uin
   if (lane == 63) part[wave] = s;
   __syncthreads();
   uint32_t before = 0, total = 0;
+#pragma unroll
   for (int w = 0; w < kSortWaves; ++w) {
     if (w < wave) before += part[w];
     total += part[w];
@@ -129,6 +131,7 @@ __device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, u
   uint32_t total = 0, before = 0;  // of class e: all its items, those of earlier workgroups
   if (e < n) {
     if (gridDim.x == 1) {
+#pragma unroll
       for (int w = 0; w < kSortWaves; ++w) total += hist[w * n + e];
     } else {
       for (uint32_t b = 0; b < gridDim.x; ++b) {
@@ -141,11 +144,13 @@ __device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, u
   uint32_t all;
   const uint32_t first = block_prefix(total, part, &all);
   if (e < n) {
-    uint32_t p = first + before;
+    uint32_t p = first + before, c[kSortWaves];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) c[w] = hist[w * n + e];
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = hist[w * n + e];
       hist[w * n + e] = p;
-      p += c;
+      p += c[w];
     }
   }
   firsts(first, total);
