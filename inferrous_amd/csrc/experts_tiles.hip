@@ -52,15 +52,11 @@ __device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t cols,
 // columns, in turn, so that a lane of a 32 x 32 block holds a column's gate sum
 // (v < 8) and its up sum (v + 8).
 template <class T>
-__global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_gate_up(ExpertsArgs a, ExpertsPlan plan,
-                                                                                  int8_t* codes, float* scales) {
+__device__ __forceinline__ void gate_up_tile(const ExpertsArgs& a, const ExpertsPlan& plan, const RowTile& t,
+                                             uint32_t group, int8_t* lds, int8_t* codes, float* scales) {
   constexpr int CSTRIDE = 144;  // bytes of a row of codes in LDS: 128 and a pad against bank conflicts
   constexpr int MAXES = T::WAVES_N * T::BT * 4;
   static_assert(T::BN == 256 && MAXES + T::BT * CSTRIDE <= T::LDS, "the epilogue reuses the rings");
-  __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
-  RowTile t;
-  uint32_t group;
-  if (!own_tile(plan, (a.inter + 127) / 128, t, group)) return;
   const uint32_t H = a.hidden, I = a.inter, c0 = group * 128, slots = a.m * a.k;
   const int8_t* const wg = a.w_gate + (size_t)t.of * I * H;
   const int8_t* const wu = a.w_up + (size_t)t.of * I * H;
@@ -147,31 +143,53 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_gate_u
   }
 }
 
+// A tile of few rows, an expert's last, takes the form of its height: the K loop's
+// time goes with the form's rows, not with those that are there.
+struct NoForm {};
+template <class T, class Half, class Quarter>
+__global__ __launch_bounds__(64 * T::NW, 2) void experts_gate_up(ExpertsArgs a, ExpertsPlan plan, int8_t* codes,
+                                                                 float* scales) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
+  RowTile t;
+  uint32_t group;
+  if (!own_tile(plan, (a.inter + 127) / 128, t, group)) return;
+  if constexpr (!std::is_same_v<Quarter, NoForm>) {
+    static_assert(Quarter::NW == T::NW && Quarter::LDS <= T::LDS, "forms of one launch");
+    if (t.rows <= (uint32_t)Quarter::BT) return gate_up_tile<Quarter>(a, plan, t, group, lds, codes, scales);
+  }
+  if constexpr (!std::is_same_v<Half, NoForm>) {
+    static_assert(Half::NW == T::NW && Half::LDS <= T::LDS, "forms of one launch");
+    if (t.rows <= (uint32_t)Half::BT) return gate_up_tile<Half>(a, plan, t, group, lds, codes, scales);
+  }
+  gate_up_tile<T>(a, plan, t, group, lds, codes, scales);
+}
+
 // ------------------------------------------------------------------ down
 // 16-bit fixed point of y against its block's largest finite magnitude: up to
 // 32766, with codes of their own for the infinities and NaN.
 constexpr float kYMost = 32766.0f;
 __device__ __forceinline__ int y_code(float y, float inv) {
-  if (__builtin_expect(!(__builtin_fabsf(y) < __builtin_inff()), 0)) return y != y ? -32768 : y > 0 ? 32767 : -32767;
+  if (!(__builtin_fabsf(y) < __builtin_inff())) return y != y ? -32768 : y > 0 ? 32767 : -32767;
   return (int)__builtin_rintf(y * inv);
 }
 __device__ __forceinline__ float y_value(int code, float s) {
-  if (__builtin_expect(code == -32768, 0)) return __builtin_nanf("");
-  if (__builtin_expect(code == 32767 || code == -32767, 0)) return code > 0 ? __builtin_inff() : -__builtin_inff();
+  if (code == -32768) return __builtin_nanf("");
+  if (code == 32767 || code == -32767) return code > 0 ? __builtin_inff() : -__builtin_inff();
   return (float)code * s;
+}
+// Two finite values' codes in one word: adding 1.5 * 2^23 rounds to the integer
+// that is the low half of the sum's bits.
+__device__ __forceinline__ uint32_t y_codes2(float a, float b, float inv) {
+  const uint32_t p = __float_as_uint(__builtin_fmaf(a, inv, 12582912.0f));
+  const uint32_t q = __float_as_uint(__builtin_fmaf(b, inv, 12582912.0f));
+  return __builtin_amdgcn_perm(q, p, 0x05040100u);
 }
 
 template <class T>
-__global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_down(ExpertsArgs a, ExpertsPlan plan,
-                                                                               const int8_t* codes,
-                                                                               const float* scales, int16_t* y,
-                                                                               float* yscale) {
+__device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t, uint32_t col, int8_t* lds,
+                                          const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
   constexpr int STRIDE = 144;  // bytes of a row of 64 codes in LDS, padded
   static_assert(T::WN == 64 && T::GROUPED && T::NW * T::WT * STRIDE <= T::LDS, "the epilogue reuses the rings");
-  __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
-  RowTile t;
-  uint32_t col;
-  if (!own_tile(plan, (a.hidden + T::BN - 1) / T::BN, t, col)) return;
   const uint32_t H = a.hidden, I = a.inter, c0 = col * T::BN, slots = a.m * a.k;
   const int8_t* const w = a.w_down + (size_t)t.of * H * I;
   T s;
@@ -188,9 +206,11 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_down(E
 #pragma unroll
   for (int j = 0; j < T::FN; ++j)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const uint32_t c = cw + 32 * j + 4 * half + 8 * (v >> 2) + (v & 3);
-      ws[j][v] = a.ws_down[(size_t)t.of * H + (c < H ? c : H - 1)];
+    for (int v = 0; v < 16; v += 4) {
+      const uint32_t c = cw + 32 * j + 4 * half + 2 * v;  // H % 16 == 0: four columns are in or out together
+      const float* const w4 = a.ws_down + (size_t)t.of * H + (c < H ? c : 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ws[j][v + i] = c < H ? w4[i] : 0.f;
     }
   __syncthreads();  // every wave is done with the rings
   int8_t* const mine = lds + wave * T::WT * STRIDE;
@@ -202,25 +222,37 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_down(E
     for (int j = 0; j < T::FN; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const float p = s.sum[f][j][v] * ws[j][v];
-        s.sum[f][j][v] = p;
-        const uint32_t c = cw + 32 * j + 4 * half + 8 * (v >> 2) + (v & 3), b = abs_bits(p);
-        if (c < H && b < kInfBits) most = max(most, b);
+        s.sum[f][j][v] *= ws[j][v];
+        most = max(most, abs_bits(s.sum[f][j][v]));
       }
     most = halves_max_u32(most);
-    const float big = __uint_as_float(most);
-    const float sc = __builtin_fmaxf(big * (1.0f / kYMost), 0x1p-120f), inv = 1.0f / sc;
+    const bool finite = most < kInfBits;
+    if (!finite) {  // the largest finite one; past H there may be NaN, which is never stored
+      most = 0;
+#pragma unroll
+      for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const uint32_t b = abs_bits(s.sum[f][j][v]);
+          if (b < kInfBits) most = max(most, b);
+        }
+      most = halves_max_u32(most);
+    }
+    const float sc = __builtin_fmaxf(__uint_as_float(most) * (1.0f / kYMost), 0x1p-120f);
+    const float inv = __builtin_amdgcn_rcpf(sc) * (1.0f - 0x1p-22f);  // no code past kYMost
     const uint32_t r = wt0 + 32 * f + tl;
 #pragma unroll
     for (int j = 0; j < T::FN; ++j)
 #pragma unroll
       for (int v = 0; v < 16; v += 4) {
-        int q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = y_code(s.sum[f][j][v + i], inv);
         v2i d;
-        d.x = (q[0] & 0xffff) | (q[1] << 16);
-        d.y = (q[2] & 0xffff) | (q[3] << 16);
+        if (finite) {
+          d.x = (int)y_codes2(s.sum[f][j][v], s.sum[f][j][v + 1], inv);
+          d.y = (int)y_codes2(s.sum[f][j][v + 2], s.sum[f][j][v + 3], inv);
+        } else {
+          d.x = (y_code(s.sum[f][j][v], inv) & 0xffff) | (y_code(s.sum[f][j][v + 1], inv) << 16);
+          d.y = (y_code(s.sum[f][j][v + 2], inv) & 0xffff) | (y_code(s.sum[f][j][v + 3], inv) << 16);
+        }
         *(v2i*)(mine + (32 * f + tl) * STRIDE + (32 * j + 4 * half + 2 * v) * 2) = d;
       }
     if (half == 0 && r < t.rows && cw < H) yscale[(size_t)(t.first + r) * nb + cw / 64] = sc;
@@ -236,27 +268,63 @@ __global__ __launch_bounds__(64 * T::NW, T::NW == 8 ? 2 : 1) void experts_down(E
   }
 }
 
+// A plan tile is `parts` of these; one of few rows takes the lower form.
+template <class T, class Half>
+__global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, ExpertsPlan plan, uint32_t parts,
+                                                              const int8_t* codes, const float* scales, int16_t* y,
+                                                              float* yscale) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
+  RowTile t;
+  uint32_t col;
+  if (!own_tile(plan, parts * ((a.hidden + T::BN - 1) / T::BN), t, col)) return;
+  const uint32_t skip = col % parts * T::BT;
+  if (skip >= t.rows) return;
+  t.first += skip;
+  t.rows = min(t.rows - skip, (uint32_t)T::BT);
+  col /= parts;
+  if constexpr (!std::is_same_v<Half, NoForm>) {
+    static_assert(Half::NW == T::NW && Half::BN == T::BN && Half::LDS <= T::LDS, "forms of one launch");
+    if (t.rows <= (uint32_t)Half::BT) return down_tile<Half>(a, t, col, lds, codes, scales, y, yscale);
+  }
+  down_tile<T>(a, t, col, lds, codes, scales, y, yscale);
+}
+
 // ------------------------------------------------------------------ sum
-// out[t, c .. c + 7] a thread, slots in order: the sum's order is fixed.
-__global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int32_t* pos, const int16_t* y,
-                                                       const float* yscale) {
-  const uint32_t H8 = a.hidden / 8, nb = (a.hidden + 63) / 64;
-  const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (size_t)a.m * H8) return;
-  const uint32_t row = (uint32_t)(at / H8), c = (uint32_t)(at % H8) * 8;
+// out[t, c .. c + 7] a thread, slots in order: the sum's order is fixed.  Eight
+// slots' rows are under way together; their positions and weights, one row's,
+// are wave-uniform.
+__global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int32_t* __restrict__ pos,
+                                                       const int16_t* __restrict__ y,
+                                                       const float* __restrict__ yscale) {
+  const uint32_t nb = (a.hidden + 63) / 64, row = blockIdx.x;
+  const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 8;
+  if (c >= a.hidden) return;
   float sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = 0.f;
-#pragma unroll 4
-  for (uint32_t j = 0; j < a.k; ++j) {
-    const int32_t p = pos[(size_t)row * a.k + j];
-    if (p < 0) continue;
-    const float w = a.weights[(size_t)row * a.k + j], s = yscale[(size_t)p * nb + c / 64];
-    const v4i v = *(const v4i*)(y + (size_t)p * a.hidden + c);
+  for (uint32_t j0 = 0; j0 < a.k; j0 += 8) {
+    v4i v[8];
+    float s[8], w[8];
+    bool on[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum[2 * i] = __builtin_fmaf(w, y_value((int)(int16_t)(v[i] & 0xffff), s), sum[2 * i]);
-      sum[2 * i + 1] = __builtin_fmaf(w, y_value(v[i] >> 16, s), sum[2 * i + 1]);
+    for (int j = 0; j < 8; ++j) {
+      const size_t slot = (size_t)row * a.k + j0 + j;
+      const int32_t p = j0 + j < a.k ? pos[slot] : -1;
+      on[j] = p >= 0;
+      if (on[j]) {
+        w[j] = a.weights[slot];
+        s[j] = yscale[(size_t)p * nb + c / 64];
+        v[j] = *(const v4i*)(y + (size_t)p * a.hidden + c);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (!on[j]) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum[2 * i] = __builtin_fmaf(w[j], y_value((int)(int16_t)(v[j][i] & 0xffff), s[j]), sum[2 * i]);
+        sum[2 * i + 1] = __builtin_fmaf(w[j], y_value(v[j][i] >> 16, s[j]), sum[2 * i + 1]);
+      }
     }
   }
   const size_t o = (size_t)row * a.hidden + c;
@@ -324,28 +392,46 @@ Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_
   return l;
 }
 
-template <int BT, int WT, int WN, int SA, int SB>
+template <int BT, int WT, int WN, int SA, int SB, bool TAIL>
+using GateUp = TileStream<BT, 256, WT, WN, SA, SB, false, TAIL>;
+template <int BT, int BN, int WT, int SA, int SB, bool TAIL>
+using Down = TileStream<BT, BN, WT, 64, SA, SB, true, TAIL>;
+
+template <class T, class Half, class Quarter>
 void gate_up_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t tiles, int8_t* codes,
                 float* scales) {
   const uint32_t grid = (tiles * ((a.inter + 127) / 128) + 7) / 8 * 8;
-  using Whole = TileStream<BT, 256, WT, WN, SA, SB, false, false>;
-  using Tail = TileStream<BT, 256, WT, WN, SA, SB, false, true>;
-  if (a.hidden % 128 == 0)
-    hipLaunchKernelGGL(experts_gate_up<Whole>, dim3(grid), dim3(64 * Whole::NW), 0, st, a, p, codes, scales);
-  else
-    hipLaunchKernelGGL(experts_gate_up<Tail>, dim3(grid), dim3(64 * Whole::NW), 0, st, a, p, codes, scales);
+  hipLaunchKernelGGL((experts_gate_up<T, Half, Quarter>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, codes, scales);
 }
 
-template <int BT, int BN, int WT, int SA, int SB>
-void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t tiles, const int8_t* codes,
-             const float* scales, int16_t* y, float* yscale) {
-  const uint32_t grid = (tiles * ((a.hidden + BN - 1) / BN) + 7) / 8 * 8;
-  using Whole = TileStream<BT, BN, WT, 64, SA, SB, true, false>;
-  using Tail = TileStream<BT, BN, WT, 64, SA, SB, true, true>;
-  if (a.inter % 128 == 0)
-    hipLaunchKernelGGL(experts_down<Whole>, dim3(grid), dim3(64 * Whole::NW), 0, st, a, p, codes, scales, y, yscale);
-  else
-    hipLaunchKernelGGL(experts_down<Tail>, dim3(grid), dim3(64 * Whole::NW), 0, st, a, p, codes, scales, y, yscale);
+template <bool TAIL>
+void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles, int8_t* codes,
+             float* scales) {
+  using T32 = GateUp<32, 32, 64, 2, 2, TAIL>;
+  using T64 = GateUp<64, 64, 32, 4, 4, TAIL>;
+  using T128 = GateUp<128, 64, 64, 3, 3, TAIL>;
+  using T256 = GateUp<256, 64, 128, 2, 3, TAIL>;
+  if (bt == 32) gate_up_as<T32, NoForm, NoForm>(st, a, p, tiles, codes, scales);
+  else if (bt == 64) gate_up_as<T64, NoForm, NoForm>(st, a, p, tiles, codes, scales);
+  else if (bt == 128) gate_up_as<T128, GateUp<64, 64, 32, 3, 3, TAIL>, NoForm>(st, a, p, tiles, codes, scales);
+  else gate_up_as<T256, T128, T64>(st, a, p, tiles, codes, scales);
+}
+
+template <class T, class Half>
+void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
+             const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
+  const uint32_t parts = bt / T::BT, grid = (tiles * parts * ((a.hidden + T::BN - 1) / T::BN) + 7) / 8 * 8;
+  hipLaunchKernelGGL((experts_down<T, Half>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, parts, codes, scales, y,
+                     yscale);
+}
+
+template <bool TAIL>
+void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
+          const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
+  if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y,
+                                                                             yscale);
 }
 }  // namespace
 
@@ -372,17 +458,11 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
                        counts);
   hipLaunchKernelGGL(experts_plan, dim3(blocks), dim3(64 * kSortWaves), lds, st, a.ids, slots, per, a.experts, counts,
                      bt, plan);
-  if (bt == 32) gate_up_as<32, 32, 64, 4, 4>(st, a, plan, tiles, codes, scales);
-  else if (bt == 64) gate_up_as<64, 64, 32, 4, 4>(st, a, plan, tiles, codes, scales);
-  else if (bt == 128) gate_up_as<128, 64, 64, 3, 3>(st, a, plan, tiles, codes, scales);
-  else gate_up_as<256, 64, 128, 2, 3>(st, a, plan, tiles, codes, scales);
-  if (bt == 32) down_as<32, 256, 32, 4, 4>(st, a, plan, tiles, codes, scales, y, yscale);
-  else if (bt == 64) down_as<64, 256, 32, 3, 3>(st, a, plan, tiles, codes, scales, y, yscale);
-  else if (bt == 128) down_as<128, 256, 64, 2, 3>(st, a, plan, tiles, codes, scales, y, yscale);
-  else down_as<256, 128, 64, 2, 3>(st, a, plan, tiles, codes, scales, y, yscale);
-  const size_t threads = (size_t)a.m * (a.hidden / 8);
-  hipLaunchKernelGGL(experts_combine, dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, st, a, plan.pos, y,
-                     yscale);
+  if (a.hidden % 128 == 0) gate_up<false>(st, a, plan, bt, tiles, codes, scales);
+  else gate_up<true>(st, a, plan, bt, tiles, codes, scales);
+  if (a.inter % 128 == 0) down<false>(st, a, plan, bt, tiles, codes, scales, y, yscale);
+  else down<true>(st, a, plan, bt, tiles, codes, scales, y, yscale);
+  hipLaunchKernelGGL(experts_combine, dim3(a.m, (a.hidden + 2047) / 2048), dim3(256), 0, st, a, plan.pos, y, yscale);
   return hipGetLastError();
 }
 
