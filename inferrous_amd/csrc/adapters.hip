@@ -116,6 +116,72 @@ __global__ __launch_bounds__(256) void adapters_expand(AdapterArgs a, const int3
   }
 }
 
+// One row: the projection by dot products and the second product with it.  A wave
+// holds two columns; each lane reads 16 bytes of a weight row at a time, and up to
+// 8 ranks of a column's adapter row.
+constexpr int kGemvCols = 2;
+__global__ __launch_bounds__(256) void adapters_gemv(AdapterArgs a, const float* __restrict__ h) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t c0 = (blockIdx.x * 4 + wave) * kGemvCols, id = (uint32_t)a.ids[0];
+  if (c0 >= a.n) return;
+  const int8_t* w[kGemvCols];
+  int sum[kGemvCols];
+#pragma unroll
+  for (int c = 0; c < kGemvCols; ++c) {
+    w[c] = a.w + (size_t)min(c0 + c, a.n - 1) * a.width;
+    sum[c] = 0;
+  }
+  auto add = [&](uint32_t o, auto runs) {
+    constexpr int R = decltype(runs)::value;
+    v4i x[R], v[R][kGemvCols];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+#pragma unroll
+      for (int c = 0; c < kGemvCols; ++c) v[u][c] = load_nt16(w[c] + o + 1024 * u);
+      x[u] = load16(a.q + o + 1024 * u);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // every load is under way before the first use
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+#pragma unroll
+      for (int c = 0; c < kGemvCols; ++c) sum[c] = dot16(v[u][c], x[u], sum[c]);
+  };
+  uint32_t o = 0;
+  for (; o + 4096 <= a.width; o += 4096) add(o + lane * 16, std::integral_constant<int, 4>{});
+  for (; o < a.width; o += 1024)
+    if (o + lane * 16 < a.width) add(o + lane * 16, std::integral_constant<int, 1>{});
+  float d[kGemvCols];
+#pragma unroll
+  for (int c = 0; c < kGemvCols; ++c) d[c] = 0.f;
+  if (id < a.adapters && lane * 8u < a.rank) {  // rank <= 256
+    const v4f h0 = *(const v4f*)(h + lane * 8), h1 = *(const v4f*)(h + lane * 8 + 4);
+#pragma unroll
+    for (int c = 0; c < kGemvCols; ++c) {
+      const v4i b = *(const v4i*)(a.b + ((size_t)id * a.n + min(c0 + c, a.n - 1)) * a.rank + lane * 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d[c] = __builtin_fmaf(bf16_lo((uint32_t)b[i]), i < 2 ? h0[2 * i] : h1[2 * i - 4], d[c]);
+        d[c] = __builtin_fmaf(bf16_hi((uint32_t)b[i]), i < 2 ? h0[2 * i + 1] : h1[2 * i - 3], d[c]);
+      }
+    }
+  }
+  int acc = 0;
+  float add_on = 0.f;
+#pragma unroll
+  for (int c = 0; c < kGemvCols; ++c) {
+    const int t = wave_sum_i32(sum[c]);
+    const float u = wave_sum_f32(d[c]);
+    if (lane == c) acc = t, add_on = u;
+  }
+  const uint32_t c = c0 + lane;
+  if (lane < kGemvCols && c < a.n) {
+    float y = (float)acc * a.asc[0] * a.ws[c];
+    if (id < a.adapters) y += a.scaling[id] * add_on;
+    store_routed(a.out, a.out_dtype, c, a.residual ? a.residual[c] + y : y);
+  }
+}
+
 // ------------------------------------------------------------------ plan
 // Up to this many rows, and this many values of adapter rows read for them, each
 // row reads its own adapter; sorted, an adapter is read once for its rows.
@@ -162,7 +228,13 @@ AdapterPlan adapter_plan(const AdapterArgs& a) {
 }
 
 size_t adapters_workspace_bytes(const AdapterArgs& a) { return adapter_plan(a).bytes; }
-bool adapters_fused(const AdapterArgs& a) { return adapter_plan(a).fused; }
+// One row whose direct form applies, and the fused tiles, need no projection of
+// their own.
+static bool one_row(const AdapterArgs& a, const AdapterPlan& p) { return a.m == 1 && !p.sorted; }
+bool adapters_fused(const AdapterArgs& a) {
+  const AdapterPlan p = adapter_plan(a);
+  return p.fused || one_row(a, p);
+}
 
 hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* workspace) {
   const AdapterPlan p = adapter_plan(a);
@@ -177,6 +249,8 @@ hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* wo
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, h); };
   if (a.x_bf16) go(J == 1 ? adapters_shrink<1, true> : J == 2 ? adapters_shrink<2, true> : adapters_shrink<8, true>);
   else go(J == 1 ? adapters_shrink<1, false> : J == 2 ? adapters_shrink<2, false> : adapters_shrink<8, false>);
+  if (one_row(a, p))
+    hipLaunchKernelGGL(adapters_gemv, dim3((a.n + 4 * kGemvCols - 1) / (4 * kGemvCols)), dim3(256), 0, st, a, h);
   return hipGetLastError();
 }
 

@@ -22,10 +22,9 @@ __global__ __launch_bounds__(256) void experts_act_slot(ExpertsArgs a, float* ac
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t c0 = (blockIdx.x * 4 + wave) * COLS;
   if (c0 >= a.inter) return;
-  for (uint32_t slot = blockIdx.y; slot < a.m * a.k; slot += gridDim.y) {
-    const uint32_t e = (uint32_t)a.ids[slot];
-    if (e >= a.experts) continue;
-    const uint32_t row = slot / a.k;
+  const uint32_t slot = blockIdx.y, row = slot / a.k, e = (uint32_t)a.ids[slot];
+  if (e >= a.experts) return;
+  {
     const int8_t* const q = a.q + (size_t)row * a.hidden;
     const int8_t *g[COLS], *u[COLS];
     int sg[COLS], su[COLS];
@@ -58,84 +57,95 @@ __global__ __launch_bounds__(256) void experts_act_slot(ExpertsArgs a, float* ac
   }
 }
 
-// codes[slot, I] and scales[slot, groups] of act: eight lanes of 16 values hold
-// a group, a wave eight groups.
-__global__ __launch_bounds__(64) void experts_codes(const float* act, uint32_t slots, uint32_t inter, int8_t* codes,
-                                                    float* scales) {
-  const int lane = threadIdx.x;
-  const uint32_t c = blockIdx.x * 1024 + lane * 16, groups = (inter + 127) / 128;
-  for (uint32_t slot = blockIdx.y; slot < slots; slot += gridDim.y) {
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = 0.f;
-    if (c < inter) {
-      const float* const p = act + (size_t)slot * inter + c;
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const v4f t = *(const v4f*)(p + i);
-        v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
-      }
-    }
-    bool nan;
-    uint32_t m = absmax_bits(v, kFloorBits, &nan);
-    m = max(m, dpp_u32<0xB1>(m));
-    m = max(m, dpp_u32<0x4E>(m));
-    m = max(m, dpp_u32<0x141>(m));  // row_half_mirror: the eight lanes of a group
-    const float s = __uint_as_float(m) / 127.0f, r = 1.0f / s;
-    if (c < inter) {
-      v4i out;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        out[i] = (int)codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
-      *(v4i*)(codes + (size_t)slot * inter + c) = out;
-      if ((lane & 7) == 0) scales[(size_t)slot * groups + c / 128] = s;
-    }
-  }
-}
-
-// out[t, c] over the row's slots: a wave holds COLS columns of one row.  Each
-// lane's 16 products lie in one group, so its part of a sum is scaled before
-// the lanes' parts are added.
+// out[t, c] over the row's slots.  The workgroup's eight waves first make the codes
+// of eight slots' next 1024 columns of act, a wave a slot (16 values a lane, so
+// that eight lanes hold a group of 128), and share them through LDS; meanwhile
+// each wave's weights for its COLS columns are on their way.  A lane's 16 products
+// lie in one group, so its part of a sum is scaled before the lanes' parts are
+// added.
 template <int COLS>
-__global__ __launch_bounds__(256) void experts_down_slot(ExpertsArgs a, const int8_t* codes, const float* scales) {
+__global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const float* act) {
+  __shared__ __attribute__((aligned(16))) v4i code[8][64];
+  __shared__ float scale[8][8];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t c0 = (blockIdx.x * 4 + wave) * COLS, groups = (a.inter + 127) / 128;
-  if (c0 >= a.hidden) return;
-  for (uint32_t row = blockIdx.y; row < a.m; row += gridDim.y) {
-    float total[COLS];
+  const uint32_t c0 = (blockIdx.x * 8 + wave) * COLS, row = blockIdx.y;
+  uint32_t col[COLS];
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) total[c] = 0.f;
-    for (uint32_t j = 0; j < a.k; ++j) {
-      const uint32_t slot = row * a.k + j, e = (uint32_t)a.ids[slot];
-      if (e >= a.experts) continue;
-      const float weight = a.weights[slot];
-      float sum[COLS];
+  for (int c = 0; c < COLS; ++c) col[c] = min(c0 + c, a.hidden - 1);
+  float total[COLS];
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
-      for (uint32_t o = lane * 16; o < a.inter; o += 1024) {
-        const v4i x = load16(codes + (size_t)slot * a.inter + o);
-        const float s = scales[(size_t)slot * groups + o / 128];
+  for (int c = 0; c < COLS; ++c) total[c] = 0.f;
+  for (uint32_t j0 = 0; j0 < a.k; j0 += 8) {
+    uint32_t e[8];  // past the last slot, or without an expert: ~0
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-          const size_t n = (size_t)e * a.hidden + min(c0 + c, a.hidden - 1);
-          sum[c] += (float)dot16(load_nt16(a.w_down + n * a.inter + o), x, 0) * s;
-        }
-      }
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t id = (uint32_t)a.ids[(size_t)row * a.k + min(j0 + j, a.k - 1)];
+      e[j] = j0 + j < a.k && id < a.experts ? id : ~0u;
+    }
+    float f[8][COLS];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int c = 0; c < COLS; ++c)
-        total[c] += sum[c] * (weight * a.ws_down[(size_t)e * a.hidden + min(c0 + c, a.hidden - 1)]);
-    }
-    float mine = 0.f;
+        f[j][c] = e[j] != ~0u ? a.weights[(size_t)row * a.k + j0 + j] * a.ws_down[(size_t)e[j] * a.hidden + col[c]] : 0.f;
+    for (uint32_t o0 = 0; o0 < a.inter; o0 += 1024) {
+      const uint32_t o = o0 + lane * 16;
+      const bool in = o < a.inter;
+      v4i w[8][COLS];
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-      const float t = wave_sum_f32(total[c]);
-      if (lane == c) mine = t;
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+          w[j][c] = v4i{0, 0, 0, 0};
+          if (e[j] != ~0u && in) w[j][c] = load_nt16(a.w_down + ((size_t)e[j] * a.hidden + col[c]) * a.inter + o);
+        }
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      const uint32_t slot = row * a.k + j0 + wave;
+      const bool mine = j0 + wave < a.k && (uint32_t)a.ids[min(slot, a.m * a.k - 1)] < a.experts;
+      if (mine && in) {
+        const float* const p = act + (size_t)slot * a.inter + o;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const v4f t = *(const v4f*)(p + i);
+          v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+        }
+      }
+      bool nan;
+      uint32_t m = absmax_bits(v, kFloorBits, &nan);
+      m = max(m, dpp_u32<0xB1>(m));
+      m = max(m, dpp_u32<0x4E>(m));
+      m = max(m, dpp_u32<0x141>(m));  // row_half_mirror: the eight lanes of a group
+      const float s = __uint_as_float(m) / 127.0f, r = 1.0f / s;
+      v4i q;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[i] = (int)codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
+      code[wave][lane] = q;
+      if ((lane & 7) == 0) scale[wave][lane >> 3] = s;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const v4i x = code[j][lane];
+        const float t = scale[j][lane >> 3];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+          if (e[j] != ~0u) total[c] += (float)dot16(w[j][c], x, 0) * t * f[j][c];
+      }
+      __syncthreads();
     }
-    if (lane < COLS && c0 + lane < a.hidden) {
-      const size_t o = (size_t)row * a.hidden + c0 + lane;
-      store_routed(a.out, a.out_dtype, o, a.residual ? a.residual[o] + mine : mine);
-    }
+  }
+  float mine = 0.f;
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    const float t = wave_sum_f32(total[c]);
+    if (lane == c) mine = t;
+  }
+  if (lane < COLS && c0 + lane < a.hidden) {
+    const size_t o = (size_t)row * a.hidden + c0 + lane;
+    store_routed(a.out, a.out_dtype, o, a.residual ? a.residual[o] + mine : mine);
   }
 }
 
@@ -147,24 +157,16 @@ static bool by_slot(uint32_t m) { return m <= 4; }
 
 size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
   if (!by_slot(m)) return experts_tiles_workspace_bytes(m, k, experts, hidden, inter);
-  const size_t slots = (size_t)m * k;
-  return up256(slots * inter * 4) + up256(slots * inter) + up256(slots * ((inter + 127) / 128) * 4);
+  return up256((size_t)m * k * inter * 4);  // act
 }
 
 hipError_t launch_experts(hipStream_t st, const ExpertsArgs& a, void* workspace) {
   if (!by_slot(a.m)) return launch_experts_tiles(st, a, workspace);
   const uint32_t slots = a.m * a.k;
-  char* p = (char*)workspace;
-  float* const act = (float*)p;
-  int8_t* const codes = (int8_t*)(p += up256((size_t)slots * a.inter * 4));
-  float* const scales = (float*)(p + up256((size_t)slots * a.inter));
+  float* const act = (float*)workspace;
   constexpr int CG = 2, CD = 2;
-  const uint32_t ys = slots < 65535u ? slots : 65535u, yr = a.m < 65535u ? a.m : 65535u;
-  hipLaunchKernelGGL(experts_act_slot<CG>, dim3((a.inter + 4 * CG - 1) / (4 * CG), ys), dim3(256), 0, st, a, act);
-  hipLaunchKernelGGL(experts_codes, dim3((a.inter + 1023) / 1024, ys), dim3(64), 0, st, act, slots, a.inter, codes,
-                     scales);
-  hipLaunchKernelGGL(experts_down_slot<CD>, dim3((a.hidden + 4 * CD - 1) / (4 * CD), yr), dim3(256), 0, st, a, codes,
-                     scales);
+  hipLaunchKernelGGL(experts_act_slot<CG>, dim3((a.inter + 4 * CG - 1) / (4 * CG), slots), dim3(256), 0, st, a, act);
+  hipLaunchKernelGGL(experts_down_slot<CD>, dim3((a.hidden + 8 * CD - 1) / (8 * CD), a.m), dim3(512), 0, st, a, act);
   return hipGetLastError();
 }
 

@@ -134,7 +134,160 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
   }
 }
 
+// Many rows: 16 lanes a row, four rows a wave, lane l of a row holding its experts
+// NV l .. NV l + NV - 1.  A round's reductions are four DPP steps for four rows at
+// once.  For 16 NV = experts, k <= 16 and groups of whole lanes (a power of two of
+// them).  The order of choice and every sum are route_rows' but for the softmax
+// sum's and the renormalising sum's order.
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+  return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(v)));
+}
+__device__ __forceinline__ float row_max_f32(float v) {
+  v = fmaxf(v, dpp_f32<0xB1>(v));
+  v = fmaxf(v, dpp_f32<0x4E>(v));
+  v = fmaxf(v, dpp_f32<0x141>(v));
+  return fmaxf(v, dpp_f32<0x140>(v));
+}
+__device__ __forceinline__ float row_sum_f32(float v) {
+  v += dpp_f32<0xB1>(v);
+  v += dpp_f32<0x4E>(v);
+  v += dpp_f32<0x141>(v);
+  return v + dpp_f32<0x140>(v);
+}
+__device__ __forceinline__ uint32_t row_min_u32(uint32_t v) {
+  v = min(v, dpp_u32<0xB1>(v));
+  v = min(v, dpp_u32<0x4E>(v));
+  v = min(v, dpp_u32<0x141>(v));
+  return min(v, dpp_u32<0x140>(v));
+}
+// The two largest of (a, b) and a lane at the other end of a DPP step.
+template <int CTRL>
+__device__ __forceinline__ void merge_two(float& a, float& b) {
+  const float c = dpp_f32<CTRL>(a), d = dpp_f32<CTRL>(b);
+  b = fmaxf(fminf(a, c), fmaxf(b, d));
+  a = fmaxf(a, c);
+}
+
+template <int NV>
+__global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
+  __shared__ __attribute__((aligned(16))) float sh[16][16 * NV];
+  const int lane = threadIdx.x & 63, li = lane & 15;
+  const uint32_t slot = threadIdx.x >> 4, row = blockIdx.x * 16 + slot;
+  const uint32_t r = min(row, a.m - 1);  // lanes of rows past the last one follow it, and store nothing
+  const float ninf = -__builtin_inff();
+  float* const score = sh[slot];
+  float x[NV], c[NV];
+  if (a.bf16) {
+    const uint16_t* const p = (const uint16_t*)a.logits + (size_t)r * a.experts + li * NV;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = __uint_as_float((uint32_t)p[i] << 16);
+  } else {
+    const float* const p = (const float*)a.logits + (size_t)r * a.experts + li * NV;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = p[i];
+  }
+  float top = ninf;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (x[i] != x[i]) x[i] = ninf;
+    top = fmaxf(top, x[i]);
+  }
+  if (a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) c[i] = 1.0f / (1.0f + expf(-x[i]));
+  } else {
+    top = row_max_f32(top);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      c[i] = x[i] == top ? (top == ninf ? 0.0f : 1.0f) : x[i] == ninf ? 0.f : expf(x[i] - top);
+      sum += c[i];
+    }
+    sum = row_sum_f32(sum);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) c[i] = sum > 0.f ? c[i] / sum : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) score[li * NV + i] = c[i];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (a.bias) c[i] += a.bias[li * NV + i];
+    if (x[i] == ninf || c[i] != c[i]) c[i] = ninf;
+    c[i] += 0.0f;  // -0 ties with +0
+  }
+  if (a.groups > 1) {
+    const uint32_t lanes = a.experts / a.groups / NV;  // of a group
+    float best = ninf, second = ninf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      second = fmaxf(second, fminf(best, c[i]));
+      best = fmaxf(best, c[i]);
+    }
+    if (lanes > 1) merge_two<0xB1>(best, second);
+    if (lanes > 2) merge_two<0x4E>(best, second);
+    if (lanes > 4) merge_two<0x141>(best, second);
+    const float mine = a.group_top == 2 && second > ninf ? best + second : best;
+    const uint32_t g = li / lanes;
+    uint32_t ahead = 0;
+    for (uint32_t o = 0; o < a.groups; ++o) {
+      const float other = __shfl(mine, (int)((lane & 48) + o * lanes), kWave);
+      ahead += other > mine || (other == mine && o < g);
+    }
+    if (ahead >= a.top_groups) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) c[i] = ninf;
+    }
+  }
+  int32_t id = -1;
+  for (uint32_t j = 0; j < a.k; ++j) {
+    float most = c[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) most = fmaxf(most, c[i]);
+    most = row_max_f32(most);
+    uint32_t at = 16 * NV;
+#pragma unroll
+    for (int i = NV - 1; i >= 0; --i)
+      if (c[i] == most) at = li * NV + i;
+    at = row_min_u32(at);
+    if ((uint32_t)li == j && most > ninf) id = (int32_t)at;
+    const uint32_t mine = at - li * NV;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (mine == (uint32_t)i) c[i] = ninf;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  float w = id >= 0 ? score[id] : 0.f;
+  if (a.renorm) {
+    const float sum = row_sum_f32(w);
+    w = sum > 0.f ? w / sum : 0.f;
+  }
+  if (row < a.m && (uint32_t)li < a.k) {
+    a.ids[(size_t)row * a.k + li] = id;
+    a.weights[(size_t)row * a.k + li] = w * a.scale;
+  }
+}
+
+// 16 lanes a row from this many rows on; below it a wave a row has the lower latency.
+constexpr uint32_t kQuadRows = 2048;
+
+static bool quads(const RouteArgs& a) {
+  if (a.m < kQuadRows || a.k > 16 || a.experts < 16 || a.experts > 256 || (a.experts & (a.experts - 1))) return false;
+  const uint32_t nv = a.experts / 16, per = a.experts / a.groups;
+  return a.groups == 1 || per % nv == 0;  // both powers of two: so are the group's lanes
+}
+
 hipError_t launch_route(hipStream_t st, const RouteArgs& a) {
+  if (quads(a)) {
+    auto k = a.experts == 16    ? route_quads<1>
+             : a.experts == 32  ? route_quads<2>
+             : a.experts == 64  ? route_quads<4>
+             : a.experts == 128 ? route_quads<8>
+                                : route_quads<16>;
+    hipLaunchKernelGGL(k, dim3((a.m + 15) / 16), dim3(256), 0, st, a);
+    return hipGetLastError();
+  }
   const uint32_t grid = (a.m + kRouteWaves - 1) / kRouteWaves;
   auto k = a.experts <= 64    ? route_rows<1>
            : a.experts <= 128 ? route_rows<2>

@@ -31,6 +31,7 @@ from .runtime import CudaContext, CudaStream, DeviceBuffer, is_capturing
 
 _OUT = {np.dtype(np.float32): _lib.OUT_F32, np.dtype(np.uint16): _lib.OUT_BF16,
         np.dtype(np.int32): _lib.OUT_I32}
+_F32, _U16, _I32, _I8 = (np.dtype(t) for t in (np.float32, np.uint16, np.int32, np.int8))
 _SCORES = {"softmax": _lib.ROUTE_SOFTMAX, "sigmoid": _lib.ROUTE_SIGMOID}
 
 
@@ -66,6 +67,13 @@ def _check_len(buf: DeviceBuffer, need: int, what: str):
         raise ValueError(f"{what} has {len(buf)} elements, needs at least {need}")
 
 
+def _needs(buf: DeviceBuffer, dtype: np.dtype, need: int, what: str):
+    if buf.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {buf.dtype}")
+    if len(buf) < need:
+        raise ValueError(f"{what} has {len(buf)} elements, needs at least {need}")
+
+
 class LoadedModule:
     """One instance per device context.  The split-K and selection
     workspaces are kept per stream (calls sharing one workspace must not
@@ -80,6 +88,7 @@ class LoadedModule:
         self.ctx = ctx
         self._select_ws: dict = {}
         self._gemm_ws: dict = {}
+        self._routed_bytes: dict = {}   # workspace bytes by entry point and shape
         self._retired: list = []   # outgrown workspaces a captured graph may still use
 
     # ------------------------------------------------------------ quantizers
@@ -661,9 +670,13 @@ class LoadedModule:
         check(lib().w8a8_linear_sequence_reset(), "linear_sequence_reset")
 
     # ------------------------------------------------------------ routed layers
-    def _routed_workspace(self, stream, nbytes: int):
+    def _routed_workspace(self, stream, size_of, *shape):
         """The stream's workspace (the split-K one: calls on a stream follow
-        each other), at least nbytes."""
+        each other), at least size_of(*shape) bytes, which a shape asks for
+        once."""
+        nbytes = self._routed_bytes.get((size_of, shape))
+        if nbytes is None:
+            nbytes = self._routed_bytes[(size_of, shape)] = getattr(lib(), size_of)(*shape)
         cur = self._gemm_ws.get(_key(stream))
         if cur is None or cur.nbytes < nbytes:
             self.reserve_workspace(nbytes, stream)
@@ -687,13 +700,12 @@ class LoadedModule:
             raise ValueError("route_experts: ids and weights must both hold M rows of K")
         if score not in _SCORES:
             raise ValueError(f"score {score!r}: one of {sorted(_SCORES)}")
-        if logits.dtype not in (np.float32, np.uint16):
+        if logits.dtype != _F32 and logits.dtype != _U16:
             raise TypeError(f"logits dtype {logits.dtype} not supported (float32/uint16)")
-        _expect(ids, np.int32, "ids")
-        _expect(weights, np.float32, "weights")
+        _needs(ids, _I32, 0, "ids")
+        _needs(weights, _F32, 0, "weights")
         if bias is not None:
-            _expect(bias, np.float32, "bias")
-            _check_len(bias, n_experts, "bias")
+            _needs(bias, _F32, n_experts, "bias")
         if m == 0:
             return
         check(lib().w8a8_route_experts(_h(stream), logits.ptr, _OUT[logits.dtype], m, n_experts, _SCORES[score],
@@ -718,23 +730,25 @@ class LoadedModule:
         inter = len(s0) // n_experts
         if len(out) != m * width or len(ids) != len(weights) or (m and len(ids) % m):
             raise ValueError("experts_mlp: out must hold M*width values, ids and weights M rows of K")
-        for b, dt, nm in ((q, np.int8, "q"), (asc, np.float32, "asc"), (ids, np.int32, "ids"),
-                          (weights, np.float32, "weights"), (w0, np.int8, "w_gate"), (s0, np.float32, "s_gate"),
-                          (w1, np.int8, "w_up"), (s1, np.float32, "s_up"), (wd, np.int8, "w_down"),
-                          (sd, np.float32, "s_down")):
-            _expect(b, dt, nm)
-        _check_len(q, m * width, "q")
-        for b, need, nm in ((w0, n_experts * inter * width, "w_gate"), (w1, n_experts * inter * width, "w_up"),
-                            (wd, n_experts * inter * width, "w_down"), (sd, n_experts * width, "s_down")):
-            _check_len(b, need, nm)
+        size = n_experts * inter * width
+        _needs(q, _I8, m * width, "q")
+        _needs(asc, _F32, m, "asc")
+        _needs(ids, _I32, 0, "ids")
+        _needs(weights, _F32, 0, "weights")
+        _needs(w0, _I8, size, "w_gate")
+        _needs(s0, _F32, 0, "s_gate")
+        _needs(w1, _I8, size, "w_up")
+        _needs(s1, _F32, 0, "s_up")
+        _needs(wd, _I8, size, "w_down")
+        _needs(sd, _F32, n_experts * width, "s_down")
         if residual is not None:
-            _expect(residual, np.float32, "residual")
+            _needs(residual, _F32, m * width, "residual")
             if len(residual) != m * width:
                 raise ValueError("residual must hold M*width values")
         if m == 0:
             return
         k = len(ids) // m
-        wp, wb = self._routed_workspace(stream, lib().w8a8_experts_mlp_workspace_bytes(m, k, n_experts, width, inter))
+        wp, wb = self._routed_workspace(stream, "w8a8_experts_mlp_workspace_bytes", m, k, n_experts, width, inter)
         check(lib().w8a8_experts_mlp(_h(stream), q.ptr, asc.ptr, m, width, ids.ptr, weights.ptr, k, n_experts, w0.ptr,
                                      s0.ptr, w1.ptr, s1.ptr, wd.ptr, sd.ptr, inter,
                                      None if residual is None else residual.ptr, out.ptr, _dtype_code(out), wp, wb),
@@ -756,24 +770,24 @@ class LoadedModule:
         if k <= 0 or count == 0 or len(a) % (count * k):
             raise ValueError("linear_adapters: a must hold len(scaling) adapters of rank rows of width")
         rank = len(a) // (count * k)
-        for buf, dt, nm in ((q, np.int8, "q"), (asc, np.float32, "asc"), (w, np.int8, "w"), (ws, np.float32, "ws"),
-                            (ids, np.int32, "ids"), (a, np.uint16, "a"), (b, np.uint16, "b"),
-                            (scaling, np.float32, "scaling")):
-            _expect(buf, dt, nm)
-        if x.dtype not in (np.float32, np.uint16):
+        _needs(q, _I8, m * k, "q")
+        _needs(asc, _F32, m, "asc")
+        _needs(w, _I8, n * k, "w")
+        _needs(ws, _F32, n, "ws")
+        _needs(ids, _I32, m, "ids")
+        _needs(a, _U16, 0, "a")
+        _needs(b, _U16, count * n * rank, "b")
+        _needs(scaling, _F32, 0, "scaling")
+        if x.dtype != _F32 and x.dtype != _U16:
             raise TypeError(f"x dtype {x.dtype} not supported (float32/uint16)")
-        _check_len(q, m * k, "q")
-        _check_len(w, n * k, "w")
         _check_len(x, m * k, "x")
-        _check_len(ids, m, "ids")
-        _check_len(b, count * n * rank, "b")
         if residual is not None:
-            _expect(residual, np.float32, "residual")
+            _needs(residual, _F32, m * n, "residual")
             if len(residual) != m * n:
                 raise ValueError("residual must hold M*N values")
         if m == 0 or n == 0:
             return
-        wp, wb = self._routed_workspace(stream, lib().w8a8_linear_adapters_workspace_bytes(m, n, k, rank, count))
+        wp, wb = self._routed_workspace(stream, "w8a8_linear_adapters_workspace_bytes", m, n, k, rank, count)
         check(lib().w8a8_linear_adapters(_h(stream), q.ptr, asc.ptr, m, w.ptr, ws.ptr, n, k, x.ptr, _OUT[x.dtype],
                                          ids.ptr, a.ptr, b.ptr, scaling.ptr, rank, count,
                                          None if residual is None else residual.ptr, out.ptr, _dtype_code(out), wp,

@@ -162,6 +162,27 @@ def test_route_groups_and_bias(env, e, groups, top_groups, k, group_top, score):
                 group_top=group_top)
 
 
+@pytest.mark.parametrize("e, groups, top_groups, group_top, k", [
+    (16, 1, 1, 1, 3), (16, 8, 3, 2, 5), (32, 4, 2, 1, 9), (64, 16, 7, 2, 16), (128, 1, 1, 1, 8), (256, 8, 4, 2, 8),
+    (256, 2, 1, 2, 16), (256, 32, 9, 2, 8), (240, 8, 4, 2, 8)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_many_rows(env, e, groups, top_groups, group_top, k, score):
+    """Enough rows for several to a wave; ties, masks and infinities among them."""
+    rng = np.random.default_rng(e + groups)
+    x = rng.standard_normal((2051, e)) * 2
+    x[5] = -INF
+    x[6] = NAN
+    x[7, 1:] = -INF
+    x[8] = 0.0
+    x[9] = np.repeat(np.arange(e // 4), 4) * -0.25
+    x[10, ::3] = INF
+    x[11, : e // 2] = -INF
+    x[12, ::2] = -INF
+    x[2050, e - 1] = 9.0
+    check_route(env, x, k, score=score, bias=rng.standard_normal(e) * 0.3 if score == "sigmoid" else None,
+                groups=groups, top_groups=top_groups, group_top=group_top, renorm=k != 9, scale=2.5, b16=e == 64)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_route_ties_masks_and_infinities(env, score, groups):
@@ -281,7 +302,7 @@ class Experts:
 
 
 @pytest.mark.parametrize("m, k, e, h, f", [
-    (1, 1, 1, 16, 16), (1, 8, 64, 256, 128), (1, 3, 5, 4096, 256), (2, 2, 4, 144, 400), (3, 8, 8, 128, 2064),
+    (1, 1, 1, 16, 16), (1, 8, 64, 256, 128), (1, 3, 5, 4096, 256), (1, 20, 24, 1040, 1168), (2, 2, 4, 144, 400), (3, 8, 8, 128, 2064),
     (4, 6, 16, 1040, 240), (7, 2, 3, 272, 144), (16, 8, 32, 512, 192), (33, 2, 4, 2000, 720), (64, 4, 128, 256, 384),
     (65, 1, 2, 512, 256), (130, 3, 5, 784, 272), (300, 2, 3, 384, 640), (600, 4, 6, 256, 128), (1100, 2, 2, 144, 272),
     (257, 1, 1, 640, 1024), (40, 7, 1000, 32, 48), (1000, 6, 1024, 48, 16)])
@@ -415,7 +436,7 @@ class Adapters:
 
 
 @pytest.mark.parametrize("m, n, k, rank, count", [
-    (1, 1, 16, 8, 1), (1, 33, 64, 8, 2), (1, 4096, 4096, 16, 3), (1, 515, 2000, 64, 4), (2, 300, 512, 24, 3),
+    (1, 1, 16, 8, 1), (1, 33, 64, 8, 2), (1, 4096, 4096, 16, 3), (1, 515, 2000, 64, 4), (1, 7, 5136, 256, 2), (64, 96, 4096, 128, 5), (2, 300, 512, 24, 3),
     (5, 1023, 784, 16, 7), (8, 256, 4096, 256, 2), (16, 640, 1024, 32, 40), (33, 129, 272, 128, 5),
     (64, 700, 1040, 40, 64), (65, 257, 128, 8, 3), (130, 500, 2000, 72, 9), (300, 320, 640, 16, 4),
     (513, 193, 400, 64, 1)])

@@ -127,7 +127,7 @@ def test_experts_method_refuses(kw):
              n_experts=8, out=Buf(192, B))
     a.update(kw)
     mod = LoadedModule(None)
-    mod._routed_workspace = lambda stream, nbytes: (A, nbytes)
+    mod._routed_workspace = lambda stream, size_of, *shape: (A, 1 << 40)
     with pytest.raises((ValueError, TypeError)):
         mod.experts_mlp(None, **a)
 
@@ -142,6 +142,6 @@ def test_adapters_method_refuses(kw):
              a=Buf(4 * 16 * 64, B), b=Buf(4 * 33 * 16, B), scaling=Buf(4, F), out=Buf(99, B))
     a.update(kw)
     mod = LoadedModule(None)
-    mod._routed_workspace = lambda stream, nbytes: (A, nbytes)
+    mod._routed_workspace = lambda stream, size_of, *shape: (A, 1 << 40)
     with pytest.raises((ValueError, TypeError)):
         mod.linear_adapters(None, **a)
