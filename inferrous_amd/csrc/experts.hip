@@ -83,28 +83,17 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
       const uint32_t id = (uint32_t)a.ids[(size_t)row * a.k + min(j0 + j, a.k - 1)];
       e[j] = j0 + j < a.k && id < a.experts ? id : ~0u;
     }
-    float f[8][COLS];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int c = 0; c < COLS; ++c)
-        f[j][c] = e[j] != ~0u ? a.weights[(size_t)row * a.k + j0 + j] * a.ws_down[(size_t)e[j] * a.hidden + col[c]] : 0.f;
+    // this wave's slot
+    const uint32_t slot = row * a.k + min(j0 + wave, a.k - 1);
+    const uint32_t id = (uint32_t)a.ids[slot];
+    const bool mine = j0 + wave < a.k && id < a.experts;
+    const float weight = a.weights[slot];
     for (uint32_t o0 = 0; o0 < a.inter; o0 += 1024) {
       const uint32_t o = o0 + lane * 16;
       const bool in = o < a.inter;
-      v4i w[8][COLS];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-          w[j][c] = v4i{0, 0, 0, 0};
-          if (e[j] != ~0u && in) w[j][c] = load_nt16(a.w_down + ((size_t)e[j] * a.hidden + col[c]) * a.inter + o);
-        }
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.f;
-      const uint32_t slot = row * a.k + j0 + wave;
-      const bool mine = j0 + wave < a.k && (uint32_t)a.ids[min(slot, a.m * a.k - 1)] < a.experts;
       if (mine && in) {
         const float* const p = act + (size_t)slot * a.inter + o;
 #pragma unroll
@@ -113,6 +102,18 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
           v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
         }
       }
+      v4i w[8][COLS];
+      float ws[8][COLS];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+          if (e[j] == ~0u) continue;
+          const size_t n = (size_t)e[j] * a.hidden + col[c];
+          w[j][c] = load_nt16(a.w_down + n * a.inter + (in ? o : 0));
+          ws[j][c] = a.ws_down[n];
+        }
+      __builtin_amdgcn_sched_barrier(0);  // the weights are under way while the codes are made
       bool nan;
       uint32_t m = absmax_bits(v, kFloorBits, &nan);
       m = max(m, dpp_u32<0xB1>(m));
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
       for (int i = 0; i < 4; ++i)
         q[i] = (int)codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
       code[wave][lane] = q;
-      if ((lane & 7) == 0) scale[wave][lane >> 3] = s;
+      if ((lane & 7) == 0) scale[wave][lane >> 3] = s * weight;
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -132,20 +133,20 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
         const float t = scale[j][lane >> 3];
 #pragma unroll
         for (int c = 0; c < COLS; ++c)
-          if (e[j] != ~0u) total[c] += (float)dot16(w[j][c], x, 0) * t * f[j][c];
+          if (e[j] != ~0u) total[c] += (float)dot16(w[j][c], x, 0) * t * ws[j][c];
       }
       __syncthreads();
     }
   }
-  float mine = 0.f;
+  float y = 0.f;
 #pragma unroll
   for (int c = 0; c < COLS; ++c) {
     const float t = wave_sum_f32(total[c]);
-    if (lane == c) mine = t;
+    if (lane == c) y = t;
   }
   if (lane < COLS && c0 + lane < a.hidden) {
     const size_t o = (size_t)row * a.hidden + c0 + lane;
-    store_routed(a.out, a.out_dtype, o, a.residual ? a.residual[o] + mine : mine);
+    store_routed(a.out, a.out_dtype, o, a.residual ? a.residual[o] + y : y);
   }
 }
 

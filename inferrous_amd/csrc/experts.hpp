@@ -16,15 +16,6 @@ struct ExpertsPlan {
   uint32_t* n_tiles;
 };
 
-// exp(x) as 2^(x log2 e) on v_exp_f32: the product's rounding error, which
-// grows with |x|, is put back to first order.
-__device__ __forceinline__ float exp_fast(float x) {
-  const float t = x * 1.44269502f;
-  const float lo = __builtin_fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;  // log2 e in two parts
-  const float e = __builtin_amdgcn_exp2f(t);
-  return e < __builtin_inff() && lo == lo ? __builtin_fmaf(e, lo * 0.693147182f, e) : e;  // infinite x: lo is NaN
-}
-
 // act of two projections, kept in f32 up to its codes.
 __device__ __forceinline__ float act_f32(int32_t g, int32_t u, float asc, float wg, float wu) {
   const float gate = (float)g * asc * wg, up = (float)u * asc * wu;

@@ -16,6 +16,15 @@
 
 namespace w8a8 {
 
+// 1 / (1 + exp(-x)) to about two units of the last place: v_exp_f32 on a split
+// product (exp_fast) and v_rcp_f32 with one Newton step, against 25 instructions
+// of expf and a division.
+__device__ __forceinline__ float sigmoid_f32(float x) {
+  const float d = 1.0f + exp_fast(-x);
+  const float r = __builtin_amdgcn_rcpf(d);
+  return d < __builtin_inff() ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : 0.0f;
+}
+
 // Order of choice: larger keys first.  0 is an expert that is out; -0 ties
 // with +0.
 __device__ __forceinline__ uint32_t choice_key(float c) {
@@ -26,7 +35,8 @@ __device__ __forceinline__ uint32_t choice_key(float c) {
 
 constexpr int kRouteWaves = 4;
 
-// One wave per row, lane l holding experts l, l + 64, ... (NE of them).
+// One wave per row, lane l holding experts l, l + 64, ... (NE of them): more
+// experts, groups or choices than route_quads takes.
 template <int NE>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
   __shared__ float sh[kRouteWaves][2 * 64 * NE];
@@ -51,7 +61,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
   float s[NE];
   if (a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < NE; ++i) s[i] = 1.0f / (1.0f + expf(-x[i]));
+    for (int i = 0; i < NE; ++i) s[i] = sigmoid_f32(x[i]);
   } else {
     float top = x[0];
 #pragma unroll
@@ -62,7 +72,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       // infinite logits share the row; a row that is all out has no score
-      s[i] = x[i] == top ? (top == ninf ? 0.0f : 1.0f) : expf(x[i] - top);
+      s[i] = x[i] == top ? (top == ninf ? 0.0f : 1.0f) : exp_fast(x[i] - top);
       if (x[i] == ninf) s[i] = 0.f;
       sum += s[i];
     }
@@ -134,11 +144,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
   }
 }
 
-// Many rows: 16 lanes a row, four rows a wave, lane l of a row holding its experts
-// NV l .. NV l + NV - 1.  A round's reductions are four DPP steps for four rows at
-// once.  For 16 NV = experts, k <= 16 and groups of whole lanes (a power of two of
-// them).  The order of choice and every sum are route_rows' but for the softmax
-// sum's and the renormalising sum's order.
+// 16 lanes a row, four rows a wave, lane l of a row holding its experts NV l ..
+// NV l + NV - 1: a round's reductions are four DPP steps for four rows at once.
+// For at most 16 NV = 256 experts, 16 groups and k <= 16.
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float v) {
   return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(v)));
@@ -171,22 +179,42 @@ __device__ __forceinline__ void merge_two(float& a, float& b) {
 
 template <int NV>
 __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
-  __shared__ __attribute__((aligned(16))) float sh[16][16 * NV];
+  __shared__ __attribute__((aligned(16))) float sh[32][16 * NV];  // scores, choice scores
   const int lane = threadIdx.x & 63, li = lane & 15;
   const uint32_t slot = threadIdx.x >> 4, row = blockIdx.x * 16 + slot;
   const uint32_t r = min(row, a.m - 1);  // lanes of rows past the last one follow it, and store nothing
   const float ninf = -__builtin_inff();
   float* const score = sh[slot];
   float x[NV], c[NV];
+  // an expert past the last one reads the last one's logit, and is out
+  const uint32_t last = a.experts - 1;
+  const size_t base = (size_t)r * a.experts;
+  float bias[NV];
+  auto loads = [&](auto load) {
+    if ((uint32_t)(li + 1) * NV <= a.experts) {  // every one of the lane's experts is there: whole vectors
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load(i, (uint32_t)(li * NV + i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load(i, min((uint32_t)(li * NV + i), last));
+    }
+  };
   if (a.bf16) {
-    const uint16_t* const p = (const uint16_t*)a.logits + (size_t)r * a.experts + li * NV;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = __uint_as_float((uint32_t)p[i] << 16);
+    const uint16_t* const p = (const uint16_t*)a.logits + base;
+    loads([&](int i, uint32_t e) { x[i] = __uint_as_float((uint32_t)p[e] << 16); });
   } else {
-    const float* const p = (const float*)a.logits + (size_t)r * a.experts + li * NV;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = p[i];
+    const float* const p = (const float*)a.logits + base;
+    loads([&](int i, uint32_t e) { x[i] = p[e]; });
   }
+  if (a.bias) {
+    loads([&](int i, uint32_t e) { bias[i] = a.bias[e]; });
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) bias[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((uint32_t)(li * NV + i) > last) x[i] = ninf;
   float top = ninf;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -195,13 +223,13 @@ __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
   }
   if (a.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) c[i] = 1.0f / (1.0f + expf(-x[i]));
+    for (int i = 0; i < NV; ++i) c[i] = sigmoid_f32(x[i]);
   } else {
     top = row_max_f32(top);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      c[i] = x[i] == top ? (top == ninf ? 0.0f : 1.0f) : x[i] == ninf ? 0.f : expf(x[i] - top);
+      c[i] = x[i] == top ? (top == ninf ? 0.0f : 1.0f) : x[i] == ninf ? 0.f : exp_fast(x[i] - top);
       sum += c[i];
     }
     sum = row_sum_f32(sum);
@@ -212,31 +240,56 @@ __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
   for (int i = 0; i < NV; ++i) score[li * NV + i] = c[i];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (a.bias) c[i] += a.bias[li * NV + i];
+    c[i] += bias[i];
     if (x[i] == ninf || c[i] != c[i]) c[i] = ninf;
     c[i] += 0.0f;  // -0 ties with +0
   }
   if (a.groups > 1) {
-    const uint32_t lanes = a.experts / a.groups / NV;  // of a group
-    float best = ninf, second = ninf;
+    const uint32_t per = a.experts / a.groups, lanes = per / NV;
+    if (per % NV == 0 && lanes <= 8 && (lanes & (lanes - 1)) == 0) {  // whole lanes, a power of two of them, a group
+      float best = ninf, second = ninf;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      second = fmaxf(second, fminf(best, c[i]));
-      best = fmaxf(best, c[i]);
-    }
-    if (lanes > 1) merge_two<0xB1>(best, second);
-    if (lanes > 2) merge_two<0x4E>(best, second);
-    if (lanes > 4) merge_two<0x141>(best, second);
-    const float mine = a.group_top == 2 && second > ninf ? best + second : best;
-    const uint32_t g = li / lanes;
-    uint32_t ahead = 0;
-    for (uint32_t o = 0; o < a.groups; ++o) {
-      const float other = __shfl(mine, (int)((lane & 48) + o * lanes), kWave);
-      ahead += other > mine || (other == mine && o < g);
-    }
-    if (ahead >= a.top_groups) {
+      for (int i = 0; i < NV; ++i) {
+        second = fmaxf(second, fminf(best, c[i]));
+        best = fmaxf(best, c[i]);
+      }
+      if (lanes > 1) merge_two<0xB1>(best, second);
+      if (lanes > 2) merge_two<0x4E>(best, second);
+      if (lanes > 4) merge_two<0x141>(best, second);
+      const float mine = a.group_top == 2 && second > ninf ? best + second : best;
+      const uint32_t g = li / lanes;
+      uint32_t ahead = 0;
+      for (uint32_t o = 0; o < a.groups; ++o) {
+        const float other = __shfl(mine, (int)((lane & 48) + o * lanes), kWave);
+        ahead += other > mine || (other == mine && o < g);
+      }
+      if (ahead >= a.top_groups) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) c[i] = ninf;
+        for (int i = 0; i < NV; ++i) c[i] = ninf;
+      }
+    } else {  // lane g scores group g, from LDS
+      float* const choice = sh[16 + slot];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) choice[li * NV + i] = c[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      float best = ninf, second = ninf;
+      if ((uint32_t)li < a.groups)
+        for (uint32_t j = 0; j < per; ++j) {
+          const float v = choice[li * per + j];
+          second = fmaxf(second, fminf(best, v));
+          best = fmaxf(best, v);
+        }
+      const float mine = a.group_top == 2 && second > ninf ? best + second : best;
+      uint32_t ahead = 0;
+      for (uint32_t o = 0; o < a.groups; ++o) {
+        const float other = __shfl(mine, (int)((lane & 48) + o), kWave);
+        ahead += other > mine || (other == mine && o < (uint32_t)li);
+      }
+      const uint32_t keep = (uint32_t)(__ballot((uint32_t)li < a.groups && ahead < a.top_groups) >> (lane & 48)) & 0xffff;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (!((keep >> ((uint32_t)(li * NV + i) / per & 15)) & 1)) c[i] = ninf;
     }
   }
   int32_t id = -1;
@@ -269,29 +322,18 @@ __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
   }
 }
 
-// 16 lanes a row from this many rows on; below it a wave a row has the lower latency.
-constexpr uint32_t kQuadRows = 2048;
-
-static bool quads(const RouteArgs& a) {
-  if (a.m < kQuadRows || a.k > 16 || a.experts < 16 || a.experts > 256 || (a.experts & (a.experts - 1))) return false;
-  const uint32_t nv = a.experts / 16, per = a.experts / a.groups;
-  return a.groups == 1 || per % nv == 0;  // both powers of two: so are the group's lanes
-}
-
 hipError_t launch_route(hipStream_t st, const RouteArgs& a) {
-  if (quads(a)) {
-    auto k = a.experts == 16    ? route_quads<1>
-             : a.experts == 32  ? route_quads<2>
-             : a.experts == 64  ? route_quads<4>
-             : a.experts == 128 ? route_quads<8>
+  if (a.experts <= 256 && a.k <= 16 && a.groups <= 16) {
+    auto k = a.experts <= 16    ? route_quads<1>
+             : a.experts <= 32  ? route_quads<2>
+             : a.experts <= 64  ? route_quads<4>
+             : a.experts <= 128 ? route_quads<8>
                                 : route_quads<16>;
     hipLaunchKernelGGL(k, dim3((a.m + 15) / 16), dim3(256), 0, st, a);
     return hipGetLastError();
   }
   const uint32_t grid = (a.m + kRouteWaves - 1) / kRouteWaves;
-  auto k = a.experts <= 64    ? route_rows<1>
-           : a.experts <= 128 ? route_rows<2>
-           : a.experts <= 256 ? route_rows<4>
+  auto k = a.experts <= 256   ? route_rows<4>
            : a.experts <= 512 ? route_rows<8>
                               : route_rows<16>;
   hipLaunchKernelGGL(k, dim3(grid), dim3(64 * kRouteWaves), 0, st, a);

@@ -27,6 +27,16 @@ __device__ __forceinline__ int wave_sum_i32(int v) {
          __builtin_amdgcn_readlane(v, 48);
 }
 
+// exp(x) as 2^(x log2 e) on v_exp_f32: the product's rounding error, which
+// grows with |x|, is put back to first order.
+__device__ __forceinline__ float exp_fast(float x) {
+  const float t = x * 1.44269502f;
+  const float lo = __builtin_fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;  // log2 e in two parts
+  const float e = __builtin_amdgcn_exp2f(t);
+  // past the range of 2^t, where e is 0 or infinite, lo is no correction
+  return e < __builtin_inff() && __builtin_fabsf(lo) < 1.0f ? __builtin_fmaf(e, lo * 0.693147182f, e) : e;
+}
+
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
