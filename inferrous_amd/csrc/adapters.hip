@@ -85,33 +85,45 @@ __global__ __launch_bounds__(256) void adapters_shrink(AdapterArgs a, float* h) 
 __global__ __launch_bounds__(256) void adapters_expand(AdapterArgs a, const int32_t* __restrict__ acc, uint32_t slabs,
                                                        const float* __restrict__ h, uint32_t splits) {
   const uint32_t c = blockIdx.x * 256 + threadIdx.x, cc = min(c, a.n - 1);
+  const size_t slab = (size_t)a.m * a.n;
   for (uint32_t row = blockIdx.y; row < a.m; row += gridDim.y) {
     const uint32_t id = (uint32_t)a.ids[row];
     const size_t o = (size_t)row * a.n + cc;
-    int32_t sum = acc[o];
-    for (uint32_t s = 1; s < slabs; ++s) sum += acc[o + (size_t)s * a.m * a.n];
+    int32_t part[4];  // four slabs' loads together
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s) part[s] = acc[o + min(s, slabs - 1) * slab];
     const float res = a.residual ? a.residual[o] : 0.f;
-    float y = (float)sum * a.asc[row] * a.ws[cc];
+    float d = 0.f;
     if (id < a.adapters) {
       const uint16_t* const b = a.b + ((size_t)id * a.n + cc) * a.rank;
-      float d = 0.f;
-#pragma unroll 2
-      for (uint32_t j = 0; j < a.rank; j += 8) {
-        const v4i bv = *(const v4i*)(b + j);
-        float hv[8];  // wave-uniform
+      for (uint32_t j0 = 0; j0 < a.rank; j0 += 32) {  // rank % 8 == 0
+        v4i bv[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hv[i] = h[(size_t)row * a.rank + j + i];
-        for (uint32_t s = 1; s < splits; ++s)
+        for (int q = 0; q < 4; ++q) bv[q] = *(const v4i*)(b + min(j0 + 8 * q, a.rank - 8));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) hv[i] += h[((size_t)s * a.m + row) * a.rank + j + i];
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t j = j0 + 8 * q;
+          if (j >= a.rank) break;
+          float hv[8];  // wave-uniform
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          d = __builtin_fmaf(bf16_lo((uint32_t)bv[i]), hv[2 * i], d);
-          d = __builtin_fmaf(bf16_hi((uint32_t)bv[i]), hv[2 * i + 1], d);
+          for (int i = 0; i < 8; ++i) hv[i] = h[(size_t)row * a.rank + j + i];
+          for (uint32_t s = 1; s < splits; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hv[i] += h[((size_t)s * a.m + row) * a.rank + j + i];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            d = __builtin_fmaf(bf16_lo((uint32_t)bv[q][i]), hv[2 * i], d);
+            d = __builtin_fmaf(bf16_hi((uint32_t)bv[q][i]), hv[2 * i + 1], d);
+          }
         }
       }
-      y += a.scaling[id] * d;
     }
+    int32_t sum = part[0];
+#pragma unroll
+    for (uint32_t s = 1; s < 4; ++s) sum += s < slabs ? part[s] : 0;
+    for (uint32_t s = 4; s < slabs; ++s) sum += acc[o + s * slab];
+    float y = (float)sum * a.asc[row] * a.ws[cc];
+    if (id < a.adapters) y += a.scaling[id] * d;
     if (c < a.n) store_routed(a.out, a.out_dtype, o, a.residual ? res + y : y);
   }
 }
@@ -183,17 +195,18 @@ __global__ __launch_bounds__(256) void adapters_gemv(AdapterArgs a, const float*
 }
 
 // ------------------------------------------------------------------ plan
-// Up to this many rows, and this many values of adapter rows read for them, each
-// row reads its own adapter; sorted, an adapter is read once for its rows.
+// Up to this many rows, or where few share an adapter, and up to this many values of
+// adapter rows read for them, each row reads its own adapter; sorted, an adapter is
+// read once for its rows.
 constexpr uint32_t kDirectRows = 64;
 constexpr uint64_t kDirectWork = 1u << 24;
 
 AdapterPlan adapter_plan(const AdapterArgs& a) {
   AdapterPlan p{};
   const uint32_t mean = a.m / std::min(a.m, a.adapters);
-  p.sorted = a.m > kDirectRows || (uint64_t)a.m * a.rank * a.width > kDirectWork;
   // The fused tiles multiply every adapter of 32 sorted rows with all of them.
-  p.fused = p.sorted && mean >= 16;
+  p.fused = a.m > kDirectRows && mean >= 16;
+  p.sorted = p.fused || (uint64_t)a.m * a.rank * a.width > kDirectWork;
   if (p.sorted) {
     const uint32_t all = (a.width * 2 + 127) / 128;  // stages of an adapter row
     p.bt = mean <= 48 ? 32 : 128;

@@ -154,20 +154,26 @@ __device__ __forceinline__ void gate_up_tile(const ExpertsArgs& a, const Experts
 
 // A tile of few rows, an expert's last, takes the form of its height: the K loop's
 // time goes with the form's rows, not with those that are there.
-struct NoForm {};
+struct NoForm {
+  static constexpr int LDS = 0;
+};
+template <class T>
+constexpr int lds_of() { return T::LDS; }
 template <class T, class Half, class Quarter>
 __global__ __launch_bounds__(64 * T::NW, 2) void experts_gate_up(ExpertsArgs a, ExpertsPlan plan, int8_t* codes,
                                                                  float* scales) {
-  __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
+  constexpr int kHalf = lds_of<Half>(), kQuarter = lds_of<Quarter>();
+  constexpr int kMost = kHalf > kQuarter ? kHalf : kQuarter;
+  __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS > kMost ? T::LDS : kMost];
   RowTile t;
   uint32_t group;
   if (!own_tile<T::BT>(plan, 1, (a.inter + 127) / 128, t, group)) return;
   if constexpr (!std::is_same_v<Quarter, NoForm>) {
-    static_assert(Quarter::NW == T::NW && Quarter::LDS <= T::LDS, "forms of one launch");
+    static_assert(Quarter::NW == T::NW, "forms of one launch");
     if (t.rows <= (uint32_t)Quarter::BT) return gate_up_tile<Quarter>(a, plan, t, group, lds, codes, scales);
   }
   if constexpr (!std::is_same_v<Half, NoForm>) {
-    static_assert(Half::NW == T::NW && Half::LDS <= T::LDS, "forms of one launch");
+    static_assert(Half::NW == T::NW, "forms of one launch");
     if (t.rows <= (uint32_t)Half::BT) return gate_up_tile<Half>(a, plan, t, group, lds, codes, scales);
   }
   gate_up_tile<T>(a, plan, t, group, lds, codes, scales);
@@ -424,7 +430,7 @@ void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
   using T256 = GateUp<256, 64, 128, 2, 3, TAIL>;
   if (bt == 32) gate_up_as<T32, NoForm, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 64) gate_up_as<T64, NoForm, NoForm>(st, a, p, tiles, codes, scales);
-  else if (bt == 128) gate_up_as<T128, GateUp<64, 64, 32, 3, 3, TAIL>, NoForm>(st, a, p, tiles, codes, scales);
+  else if (bt == 128) gate_up_as<T128, T64, NoForm>(st, a, p, tiles, codes, scales);
   else gate_up_as<T256, T128, T64>(st, a, p, tiles, codes, scales);
 }
 

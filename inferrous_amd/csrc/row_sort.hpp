@@ -18,11 +18,12 @@ namespace w8a8 {
 constexpr int kSortWaves = 16;
 constexpr uint32_t kSortClasses = 1024;
 constexpr uint32_t kSortBlock = 4096;
-constexpr uint32_t kSortBlocks = 256;  // workgroups at most
+constexpr int kSortRegs = kSortBlock / (64 * kSortWaves);  // items of a lane, held in registers
 
-// Items of a workgroup: all of them, or runs of at least 1024.
+// Items of a workgroup: all of them; or 1024, which more workgroups share; or the
+// most there can be, where the workgroups' counts would take longer to add.
 static inline uint32_t sort_per_block(uint32_t items) {
-  return items <= kSortBlock ? items : std::max<uint32_t>(1024, (items + kSortBlocks - 1) / kSortBlocks);
+  return items <= kSortBlock ? items : items <= 64 * kSortBlock ? 1024 : kSortBlock;
 }
 static inline uint32_t sort_blocks(uint32_t items) {
   const uint32_t per = sort_per_block(items);
@@ -42,17 +43,28 @@ __device__ __forceinline__ void sort_run(uint32_t items, uint32_t per_block, int
   end = min(begin + run, b1);
 }
 
+// The lane's items of its wave's run, as classes (~0: none), all loads together.
 template <bool REST>
-__device__ __forceinline__ void sort_count(const int32_t* ids, uint32_t classes, uint32_t begin, uint32_t end,
-                                           uint32_t* hist, int lane) {
-  const uint32_t n = classes + REST;
+__device__ __forceinline__ void sort_load(const int32_t* ids, uint32_t classes, uint32_t begin, uint32_t end, int lane,
+                                          uint32_t (&c)[kSortRegs]) {
+  int32_t id[kSortRegs];
+#pragma unroll
+  for (int i = 0; i < kSortRegs; ++i) {
+    const uint32_t at = begin + 64 * i + lane;
+    id[i] = begin < end ? ids[min(at, end - 1)] : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kSortRegs; ++i)
+    c[i] = begin + 64 * i + lane < end ? sort_class<REST>(id[i], classes) : ~0u;
+}
+
+__device__ __forceinline__ void sort_count(const uint32_t (&c)[kSortRegs], uint32_t n, uint32_t* hist, int lane) {
   for (uint32_t e = lane; e < n; e += 64) hist[e] = 0;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  for (uint32_t i = begin + lane; i < end; i += 64) {
-    const uint32_t e = sort_class<REST>(ids[i], classes);
-    if (e < n) atomicAdd(&hist[e], 1u);  // a count: any order gives it
-  }
+#pragma unroll
+  for (int i = 0; i < kSortRegs; ++i)
+    if (c[i] < n) atomicAdd(&hist[c[i]], 1u);  // a count: any order gives it
 }
 
 // counts[workgroup][class] of a sort over several workgroups.
@@ -64,7 +76,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_counts(const int32_t* id
   const uint32_t n = classes + REST;
   uint32_t begin, end;
   sort_run(items, per_block, wave, begin, end);
-  sort_count<REST>(ids, classes, begin, end, hist + wave * n, lane);
+  uint32_t c[kSortRegs];
+  sort_load<REST>(ids, classes, begin, end, lane, c);
+  sort_count(c, n, hist + wave * n, lane);
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < n; e += 64 * kSortWaves) {
     uint32_t sum = 0;
@@ -126,7 +140,9 @@ __device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, u
   const uint32_t e = threadIdx.x, n = classes + REST;
   uint32_t begin, end;
   sort_run(items, per_block, wave, begin, end);
-  sort_count<REST>(ids, classes, begin, end, hist + wave * n, lane);
+  uint32_t c[kSortRegs];
+  sort_load<REST>(ids, classes, begin, end, lane, c);
+  sort_count(c, n, hist + wave * n, lane);
   __syncthreads();
   uint32_t total = 0, before = 0;  // of class e: all its items, those of earlier workgroups
   if (e < n) {
@@ -134,23 +150,29 @@ __device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, u
 #pragma unroll
       for (int w = 0; w < kSortWaves; ++w) total += hist[w * n + e];
     } else {
-      for (uint32_t b = 0; b < gridDim.x; ++b) {
-        const uint32_t c = counts[(size_t)b * n + e];
-        if (b < blockIdx.x) before += c;
-        total += c;
+      for (uint32_t b0 = 0; b0 < gridDim.x; b0 += 16) {
+        uint32_t k[16];
+#pragma unroll
+        for (uint32_t b = 0; b < 16; ++b) k[b] = counts[(size_t)min(b0 + b, gridDim.x - 1) * n + e];
+#pragma unroll
+        for (uint32_t b = 0; b < 16; ++b) {
+          if (b0 + b >= gridDim.x) k[b] = 0;
+          if (b0 + b < blockIdx.x) before += k[b];
+          total += k[b];
+        }
       }
     }
   }
   uint32_t all;
   const uint32_t first = block_prefix(total, part, &all);
   if (e < n) {
-    uint32_t p = first + before, c[kSortWaves];
+    uint32_t p = first + before, k[kSortWaves];
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) c[w] = hist[w * n + e];
+    for (int w = 0; w < kSortWaves; ++w) k[w] = hist[w * n + e];
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       hist[w * n + e] = p;
-      p += c[w];
+      p += k[w];
     }
   }
   firsts(first, total);
@@ -158,21 +180,22 @@ __device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, u
   // Each wave walks its run in order.  Lanes of one class find each other by
   // ballots over the bits of its number; their order is their lanes'.
   uint32_t* const next = hist + wave * n;
-  for (uint32_t i0 = begin; i0 < end; i0 += 64) {
-    const uint32_t i = i0 + lane;
-    const uint32_t c = i < end ? sort_class<REST>(ids[i], classes) : ~0u;
-    const bool on = c < n;
+#pragma unroll
+  for (int g = 0; g < kSortRegs; ++g) {
+    if (begin + 64 * g >= end) break;
+    const uint32_t i = begin + 64 * g + lane;
+    const bool on = c[g] < n;
     uint64_t peers = __ballot(on);
 #pragma unroll
     for (int b = 0; b < 10; ++b) {
-      const uint64_t set = __ballot((c >> b) & 1);
-      peers &= ((c >> b) & 1) ? set : ~set;
+      const uint64_t set = __ballot((c[g] >> b) & 1);
+      peers &= ((c[g] >> b) & 1) ? set : ~set;
     }
     uint32_t p = 0;
-    if (on) p = next[c] + (uint32_t)__popcll(peers & ((1ull << lane) - 1));
+    if (on) p = next[c[g]] + (uint32_t)__popcll(peers & ((1ull << lane) - 1));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (on && (peers >> lane) == 1) next[c] = p + 1;  // the last of its peers
+    if (on && (peers >> lane) == 1) next[c[g]] = p + 1;  // the last of its peers
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (i < end) place(i, on ? (int32_t)p : -1);
