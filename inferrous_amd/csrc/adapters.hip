@@ -7,8 +7,8 @@
 // a row whose id is outside [0, n_adapters) taking the projection alone.  h and
 // both sums are held in f32.
 //
-// Here: row by row (a decode batch), out from the projection's exact sums; with
-// the rows sorted by adapter (prompts, and many rows): adapters_tiles.hip.
+// Here: row by row (decode batches, short prompts), out from the projection's exact
+// sums; with the rows sorted by adapter (longer prompts): adapters_tiles.hip.
 #include <algorithm>
 
 #include "adapters.hpp"
@@ -37,7 +37,8 @@ __global__ __launch_bounds__(256) void adapters_shrink(AdapterArgs a, float* h) 
   constexpr int U = J == 8 ? 2 : 8 / J;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t j0 = (blockIdx.x * 4 + wave) * J, row = blockIdx.y;
+  const uint32_t per_row = (a.rank + 4 * J - 1) / (4 * J), row = blockIdx.x / per_row;
+  const uint32_t j0 = (blockIdx.x % per_row * 4 + wave) * J;
   if (j0 >= a.rank) return;
   const uint32_t id = (uint32_t)a.ids[row];
   if (id >= a.adapters) return;
@@ -79,11 +80,10 @@ __global__ __launch_bounds__(256) void adapters_shrink(AdapterArgs a, float* h) 
   if (lane < J) h[(size_t)row * a.rank + j0 + lane] = mine;  // rank % 8 == 0
 }
 
-// out row by row from the projection's exact sums (`slabs` partial ones) and h
-// (`splits` partial ones): a thread holds a column, its adapter row one
-// contiguous run.
+// out row by row from the projection's exact sums (`slabs` partial ones) and h: a
+// thread holds a column, its adapter row one contiguous run.
 __global__ __launch_bounds__(256) void adapters_expand(AdapterArgs a, const int32_t* __restrict__ acc, uint32_t slabs,
-                                                       const float* __restrict__ h, uint32_t splits) {
+                                                       const float* __restrict__ h) {
   const uint32_t c = blockIdx.x * 256 + threadIdx.x, cc = min(c, a.n - 1);
   const size_t slab = (size_t)a.m * a.n;
   for (uint32_t row = blockIdx.y; row < a.m; row += gridDim.y) {
@@ -107,9 +107,6 @@ __global__ __launch_bounds__(256) void adapters_expand(AdapterArgs a, const int3
           float hv[8];  // wave-uniform
 #pragma unroll
           for (int i = 0; i < 8; ++i) hv[i] = h[(size_t)row * a.rank + j + i];
-          for (uint32_t s = 1; s < splits; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) hv[i] += h[((size_t)s * a.m + row) * a.rank + j + i];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             d = __builtin_fmaf(bf16_lo((uint32_t)bv[q][i]), hv[2 * i], d);
@@ -195,19 +192,27 @@ __global__ __launch_bounds__(256) void adapters_gemv(AdapterArgs a, const float*
 }
 
 // ------------------------------------------------------------------ plan
-// Up to this many rows, or where few share an adapter, and up to this many values of
-// adapter rows read for them, each row reads its own adapter; sorted, an adapter is
-// read once for its rows.
-constexpr uint32_t kDirectRows = 64;
-constexpr uint64_t kDirectWork = 1u << 24;
+// Row by row, every row reads its own adapter: m rank (n + width) values from L2,
+// at about 10 TB/s, beside the projection.  The fused tiles read an adapter once,
+// but run in the tiles' own time: 22 us more than the projection at width 4096, 43
+// at 12288 until the tiles fill the card, and 1.5 us for each 32 ranks of every
+// adapter after a tile's first.  Measured, rows / fused us at 4 adapters: 4096 x
+// 4096, rank 16, m = 512 (134 MB) 34.6 / 39.0, m = 1024 (268 MB) 56 / 42; rank 64, m
+// = 128 (134 MB) 29 / 40, m = 512 62 / 43; 4096 x 12288, rank 16, m = 512 (268 MB)
+// 59 / 70, m = 1024 104 / 77; 24576 x 4096, rank 32, m = 80 (147 MB) 41 / 41, m = 128
+// 50 / 42.
+static bool fused_leads(const AdapterArgs& a) {
+  if (a.m == 1) return false;
+  const double rows_us = (double)a.m * a.rank * ((double)a.n + a.width) * 2.0 / 10e6;
+  const uint32_t mean = a.m / std::min(a.m, a.adapters), met = std::min(a.m, 256u) / std::min(mean, 256u);
+  return rows_us > 8.0 + a.width / 400.0 + 1.5 * ((a.rank + 31) / 32) * (met > 1 ? met - 1 : 0);
+}
 
 AdapterPlan adapter_plan(const AdapterArgs& a) {
   AdapterPlan p{};
   const uint32_t mean = a.m / std::min(a.m, a.adapters);
-  // The fused tiles multiply every adapter of 32 sorted rows with all of them.
-  p.fused = a.m > kDirectRows && mean >= 16;
-  p.sorted = p.fused || (uint64_t)a.m * a.rank * a.width > kDirectWork;
-  if (p.sorted) {
+  p.fused = fused_leads(a);
+  if (p.fused) {
     const uint32_t all = (a.width * 2 + 127) / 128;  // stages of an adapter row
     p.bt = mean <= 48 ? 32 : 128;
     p.tiles = a.m / p.bt + std::min(a.m, a.adapters);
@@ -225,44 +230,33 @@ AdapterPlan adapter_plan(const AdapterArgs& a) {
     return o;
   };
   p.h = take((size_t)p.splits * a.m * a.rank * 4);
-  if (p.sorted) {
+  if (p.fused) {
     const uint32_t blocks = sort_blocks(a.m);
     p.order = take((size_t)a.m * 4);
     p.table = take((size_t)p.tiles * sizeof(RowTile));
     p.n_tiles = take(4);
     p.counts = take(blocks > 1 ? (size_t)blocks * (a.adapters + 1) * 4 : 0);
-    if (p.fused) {
-      p.high = take((size_t)a.m * part_width(a.rank) * 2);
-      p.low = take((size_t)a.m * part_width(a.rank) * 2);
-    }
+    p.high = take((size_t)a.m * part_width(a.rank) * 2);
+    p.low = take((size_t)a.m * part_width(a.rank) * 2);
   }
   p.bytes = at;
   return p;
 }
 
 size_t adapters_workspace_bytes(const AdapterArgs& a) { return adapter_plan(a).bytes; }
-// One row whose direct form applies, and the fused tiles, need no projection of
-// their own.
-static bool one_row(const AdapterArgs& a, const AdapterPlan& p) { return a.m == 1 && !p.sorted; }
-bool adapters_fused(const AdapterArgs& a) {
-  const AdapterPlan p = adapter_plan(a);
-  return p.fused || one_row(a, p);
-}
+bool adapters_fused(const AdapterArgs& a) { return a.m == 1 || adapter_plan(a).fused; }
 
 hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* workspace) {
   const AdapterPlan p = adapter_plan(a);
-  if (p.sorted) {
-    const hipError_t e = launch_adapters_sorted(st, a, p, (char*)workspace);
-    return e != hipSuccess || !p.fused ? e : launch_adapters_fused(st, a, p, (char*)workspace);
-  }
+  if (p.fused) return launch_adapters_fused(st, a, p, (char*)workspace);
   float* const h = (float*)((char*)workspace + p.h);
   // few values: one a wave; many: eight, which share their loads of x
   const int J = a.m * a.rank <= 1024 ? 1 : a.m * a.rank <= 4096 ? 2 : 8;
-  const dim3 grid((a.rank + 4 * J - 1) / (4 * J), a.m);
+  const dim3 grid((a.rank + 4 * J - 1) / (4 * J) * a.m);
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, h); };
   if (a.x_bf16) go(J == 1 ? adapters_shrink<1, true> : J == 2 ? adapters_shrink<2, true> : adapters_shrink<8, true>);
   else go(J == 1 ? adapters_shrink<1, false> : J == 2 ? adapters_shrink<2, false> : adapters_shrink<8, false>);
-  if (one_row(a, p))
+  if (a.m == 1)
     hipLaunchKernelGGL(adapters_gemv, dim3((a.n + 4 * kGemvCols - 1) / (4 * kGemvCols)), dim3(256), 0, st, a, h);
   return hipGetLastError();
 }
@@ -271,7 +265,7 @@ hipError_t launch_adapters_after(hipStream_t st, const AdapterArgs& a, const int
                                  const void* workspace) {
   const AdapterPlan p = adapter_plan(a);
   hipLaunchKernelGGL(adapters_expand, dim3((a.n + 255) / 256, std::min(a.m, 65535u)), dim3(256), 0, st, a, acc, slabs,
-                     (const float*)((const char*)workspace + p.h), p.splits);
+                     (const float*)((const char*)workspace + p.h));
   return hipGetLastError();
 }
 

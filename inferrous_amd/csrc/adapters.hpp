@@ -15,17 +15,15 @@ __host__ __device__ constexpr uint32_t part_width(uint32_t rank) { return (rank 
 
 // How a call runs, a function of its sizes.
 struct AdapterPlan {
-  bool sorted;   // the rows are sorted by adapter, and the first product runs in tiles of them
-  bool fused;    // the projection runs in tiles of the sorted rows, and adds the second product itself
-  uint32_t bt;   // sorted: rows of a tile of the first product
-  uint32_t tiles;   // sorted: tiles at most
+  bool fused;       // the rows are sorted by adapter, and the projection's tiles add the second product
+  uint32_t bt;      // (fused) rows of a tile of the first product
+  uint32_t tiles;   // tiles at most
   uint32_t splits;  // shares of K of the first product, each with partial sums of its own
-  uint32_t stages;  // sorted: 128-byte stages of an adapter row in a share
+  uint32_t stages;  // 128-byte stages of an adapter row in a share
   size_t h, order, table, n_tiles, counts, high, low, bytes;  // workspace offsets
 };
 AdapterPlan adapter_plan(const AdapterArgs& a);
 
-hipError_t launch_adapters_sorted(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* workspace);
 hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* workspace);
 
 }  // namespace w8a8

@@ -27,12 +27,12 @@ __global__ __launch_bounds__(64 * kSortWaves) void adapters_order(const int32_t*
       [&](uint32_t row, int32_t p) { order[p] = row; });
 }
 
-// h[share][p or row][j] of a tile: the token operand's rows are gathered, K is the
-// share's stages.  by_row: h is read row by row, not in the sorted order.
+// h[share][p][j] of a tile, in the sorted order: the token operand's rows are
+// gathered, K is the share's stages.
 template <class T>
 __global__ __launch_bounds__(64 * T::NW) void adapters_shrink_tiles(AdapterArgs a, const uint32_t* order,
                                                                     const RowTile* table, const uint32_t* n_tiles,
-                                                                    float* h, uint32_t stages, bool by_row) {
+                                                                    float* h, uint32_t stages) {
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
   if (blockIdx.x >= *n_tiles) return;
   const RowTile t = table[blockIdx.x];
@@ -56,8 +56,7 @@ __global__ __launch_bounds__(64 * T::NW) void adapters_shrink_tiles(AdapterArgs 
   for (int f = 0; f < T::FT; ++f) {
     const uint32_t r = wt0 + 32 * f + (lane & 31);
     if (r >= t.rows) continue;
-    const uint32_t p = by_row ? order[t.first + r] : t.first + r;
-    float* const to = h + ((size_t)blockIdx.y * a.m + p) * a.rank;
+    float* const to = h + ((size_t)blockIdx.y * a.m + t.first + r) * a.rank;
 #pragma unroll
     for (int j = 0; j < T::FN; ++j)
 #pragma unroll
@@ -293,7 +292,7 @@ void shrink_as(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char*
     using T = decltype(tile);
     hipLaunchKernelGGL(adapters_shrink_tiles<T>, dim3(p.tiles, p.splits), dim3(64 * T::NW), 0, st, a,
                        (const uint32_t*)(ws + p.order), (const RowTile*)(ws + p.table), (const uint32_t*)(ws + p.n_tiles),
-                       (float*)(ws + p.h), p.stages, !p.fused);
+                       (float*)(ws + p.h), p.stages);
   };
   if (a.x_bf16) go(TileStream<BT, BN, WT, WN, SA, SB, false, true, OP_BF16>{});
   else go(TileStream<BT, BN, WT, WN, SA, SB, false, true, OP_BF16_F32>{});
@@ -314,7 +313,7 @@ void gemm_as(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* w
 }
 }  // namespace
 
-hipError_t launch_adapters_sorted(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* ws) {
+hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* ws) {
   uint32_t* const counts = (uint32_t*)(ws + p.counts);
   const uint32_t blocks = sort_blocks(a.m), per = sort_per_block(a.m), lds = kSortWaves * (a.adapters + 1) * 4;
   if (blocks > 1)
@@ -334,10 +333,6 @@ hipError_t launch_adapters_sorted(hipStream_t st, const AdapterArgs& a, const Ad
     else if (rank == 128) shrink_as<128, 128, 64, 64, 3, 3>(st, a, p, ws);
     else shrink_as<128, 256, 64, 64, 2, 2>(st, a, p, ws);
   }
-  return hipGetLastError();
-}
-
-hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* ws) {
   const size_t quads = (size_t)a.m * (part_width(a.rank) / 4);
   hipLaunchKernelGGL(adapters_parts, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, a,
                      (const uint32_t*)(ws + p.order), (const float*)(ws + p.h), p.splits, (uint16_t*)(ws + p.high),

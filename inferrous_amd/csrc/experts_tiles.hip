@@ -414,6 +414,8 @@ using GateUp = TileStream<BT, 256, WT, WN, SA, SB, false, TAIL>;
 template <int BT, int BN, int WT, int SA, int SB, bool TAIL>
 using Down = TileStream<BT, BN, WT, 64, SA, SB, true, TAIL>;
 
+constexpr uint32_t kOnePerCu = 256;  // workgroups
+
 template <class T, class Half, class Quarter>
 void gate_up_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t tiles, int8_t* codes,
                 float* scales) {
@@ -428,7 +430,10 @@ void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
   using T64 = GateUp<64, 64, 32, 4, 4, TAIL>;
   using T128 = GateUp<128, 64, 64, 3, 3, TAIL>;
   using T256 = GateUp<256, 64, 128, 2, 3, TAIL>;
-  if (bt == 32) gate_up_as<T32, NoForm, NoForm>(st, a, p, tiles, codes, scales);
+  // 32 rows: two workgroups share a CU, or one has twice the stages under way
+  if (bt == 32 && tiles * ((a.inter + 127) / 128) <= kOnePerCu)
+    gate_up_as<GateUp<32, 32, 64, 4, 4, TAIL>, NoForm, NoForm>(st, a, p, tiles, codes, scales);
+  else if (bt == 32) gate_up_as<T32, NoForm, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 64) gate_up_as<T64, NoForm, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 128) gate_up_as<T128, T64, NoForm>(st, a, p, tiles, codes, scales);
   else gate_up_as<T256, T128, T64>(st, a, p, tiles, codes, scales);
@@ -445,7 +450,9 @@ void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
 template <bool TAIL>
 void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
           const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
-  if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  if (bt == 32 && tiles * ((a.hidden + 255) / 256) <= kOnePerCu)
+    down_as<Down<32, 256, 32, 4, 4, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
   else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
   else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y,
                                                                              yscale);

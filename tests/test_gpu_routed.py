@@ -445,6 +445,37 @@ def test_adapters(env, m, n, k, rank, count, x_bf16):
     Adapters(m, n, k, rank, count, seed=m + n).check(env, x_bf16=x_bf16)
 
 
+@pytest.mark.parametrize("m, n, k, rank, count", [
+    (600, 1024, 1040, 256, 2), (1500, 520, 528, 128, 3), (2100, 999, 400, 72, 1), (1100, 264, 2048, 200, 8),
+    (5000, 130, 144, 256, 3)])
+@pytest.mark.parametrize("x_bf16", [False, True])
+def test_adapters_where_the_tiles_lead(env, m, n, k, rank, count, x_bf16):
+    """Enough work for the sorted rows: runs of one adapter, many in one tile, rows
+    with none at the end, odd columns, both types of x and of out."""
+    rng = np.random.default_rng(m)
+    ids = np.where(np.arange(m) < 2 * m // 3, 0, np.arange(m) % (count + 1) - 1)
+    ids = rng.permutation(ids) if x_bf16 else ids
+    Adapters(m, n, k, rank, count, seed=m + n, ids=ids, residual=x_bf16).check(env, F32 if x_bf16 else np.uint16,
+                                                                                x_bf16=x_bf16)
+
+
+def test_adapters_in_tiles_keep_rows_apart(env):
+    """A NaN adapter reaches its own rows only, rows without one equal the projection,
+    and the same call gives the same bits."""
+    mod, s, _ = env
+    m, n, k = 900, 512, 512
+    ids = np.arange(m) % 4 - 1
+    c = Adapters(m, n, k, 256, 3, seed=4, ids=ids)
+    base = c.run(env)
+    assert np.array_equal(c.run(env), base)
+    out = dev(s, np.zeros(m * n, np.uint16))
+    mod.linear(s, None, *(dev(s, v) for v in (c.q, c.asc, c.w, c.ws)), k, out)
+    assert np.array_equal(base[ids < 0], values(out, s).reshape(m, n)[ids < 0])
+    c.b[2], c.a[2, 5] = NAN, INF
+    got = c.run(env)
+    assert np.array_equal(got[ids != 2], base[ids != 2]) and not np.isfinite(got[ids == 2]).any()
+
+
 @pytest.mark.parametrize("m", [1, 9, 140])
 def test_adapters_residual_in_f32(env, m):
     Adapters(m, 333, 400, 16, 3, seed=m, residual=True).check(env, F32)
