@@ -371,10 +371,18 @@ __global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int3
 // ------------------------------------------------------------------ launches
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Rows of a token tile: the smallest that holds an expert's mean share, so that
-// few tiles are half empty and few experts take two where one would do.
-static uint32_t tile_rows(uint32_t slots, uint32_t experts) {
+// Rows of a token tile, by an expert's mean share of the slots: the smallest that
+// holds it with room for the uneven shares of real routing.  An expert that takes
+// two tiles reads its weights twice, which large experts (above 8 MiB) cannot
+// afford; a tile too tall computes rows that are not there.  Measured, tile rows: us,
+// hidden 4096, inner 1024, 8 of 64: mean 16 32: 231, 64: 201; mean 25 64: 235, 128:
+// 209; mean 42 64: 238, 128: 216; mean 128 128: 269, 256: 300.  Hidden 2048, inner 768,
+// 8 of 128: mean 16 32: 138, 64: 138; mean 44 64: 157, 128: 173; mean 128 128: 223,
+// 256: 227.  Hidden 2000, inner 720, 3 of 20: mean 19 32: 37, 64: 45, 128: 38; mean 105
+// 128: 50, 256: 59.
+static uint32_t tile_rows(uint32_t slots, uint32_t experts, uint32_t hidden, uint32_t inter) {
   const uint32_t mean = slots / std::min(slots, experts);
+  if (3ull * hidden * inter > (8u << 20)) return mean <= 12 ? 32 : mean <= 20 ? 64 : mean <= 128 ? 128 : 256;
   return mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
 }
 
@@ -398,7 +406,7 @@ Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_
   };
   l.order = take(slots * 4);
   l.pos = take(slots * 4);
-  l.tiles = take((size_t)most_tiles((uint32_t)slots, experts, tile_rows((uint32_t)slots, experts)) * sizeof(RowTile));
+  l.tiles = take((size_t)most_tiles((uint32_t)slots, experts, tile_rows((uint32_t)slots, experts, hidden, inter)) * sizeof(RowTile));
   l.n_tiles = take(4);
   l.counts = take(blocks > 1 ? (size_t)blocks * experts * 4 : 0);
   l.codes = take(slots * inter);
@@ -434,7 +442,7 @@ void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
   if (bt == 32 && tiles * ((a.inter + 127) / 128) <= kOnePerCu)
     gate_up_as<GateUp<32, 32, 64, 4, 4, TAIL>, NoForm, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 32) gate_up_as<T32, NoForm, NoForm>(st, a, p, tiles, codes, scales);
-  else if (bt == 64) gate_up_as<T64, NoForm, NoForm>(st, a, p, tiles, codes, scales);
+  else if (bt == 64) gate_up_as<GateUp<64, 64, 64, 2, 2, TAIL>, T32, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 128) gate_up_as<T128, T64, NoForm>(st, a, p, tiles, codes, scales);
   else gate_up_as<T256, T128, T64>(st, a, p, tiles, codes, scales);
 }
@@ -474,7 +482,7 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
   int16_t* const y = (int16_t*)(p + l.y);
   float* const yscale = (float*)(p + l.yscale);
   uint32_t* const counts = (uint32_t*)(p + l.counts);
-  const uint32_t bt = tile_rows(slots, a.experts);
+  const uint32_t bt = tile_rows(slots, a.experts, a.hidden, a.inter);
   const uint32_t tiles = most_tiles(slots, a.experts, bt);
   const uint32_t blocks = sort_blocks(slots), per = sort_per_block(slots), lds = kSortWaves * a.experts * 4;
   if (blocks > 1)
