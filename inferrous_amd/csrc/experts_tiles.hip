@@ -205,7 +205,7 @@ template <class T>
 __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t, uint32_t col, int8_t* lds,
                                           const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
   constexpr int STRIDE = 144;  // bytes of a row of 64 codes in LDS, padded
-  static_assert(T::WN == 64 && T::GROUPED && T::NW * T::WT * STRIDE <= T::LDS, "the epilogue reuses the rings");
+  static_assert(T::WN % 64 == 0 && T::GROUPED && T::NW * T::WT * STRIDE <= T::LDS, "the epilogue reuses the rings");
   const uint32_t H = a.hidden, I = a.inter, c0 = col * T::BN, slots = a.m * a.k;
   const int8_t* const w = a.w_down + (size_t)t.of * H * I;
   T s;
@@ -217,75 +217,82 @@ __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wt0 = (wave / T::WAVES_N) * T::WT, half = lane >> 5, tl = lane & 31;
-  const uint32_t cw = c0 + (wave % T::WAVES_N) * 64;  // the wave's 64 columns
-  float ws[T::FN][16];
-#pragma unroll
-  for (int j = 0; j < T::FN; ++j)
-#pragma unroll
-    for (int v = 0; v < 16; v += 4) {
-      const uint32_t c = cw + 32 * j + 4 * half + 2 * v;  // H % 16 == 0: four columns are in or out together
-      const float* const w4 = a.ws_down + (size_t)t.of * H + (c < H ? c : 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ws[j][v + i] = c < H ? w4[i] : 0.f;
-    }
+  const uint32_t nb = (H + 63) / 64;
   __syncthreads();  // every wave is done with the rings
   int8_t* const mine = lds + wave * T::WT * STRIDE;
-  const uint32_t nb = (H + 63) / 64;
+  // blocks of 64 columns
 #pragma unroll
-  for (int f = 0; f < T::FT; ++f) {
-    uint32_t most = 0;
+  for (int j0 = 0; j0 < T::FN; j0 += 2) {
+    const uint32_t cw = c0 + (wave % T::WAVES_N) * T::WN + 32 * j0;
+    float ws[2][16];
 #pragma unroll
-    for (int j = 0; j < T::FN; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        s.sum[f][j][v] *= ws[j][v];
-        most = max(most, abs_bits(s.sum[f][j][v]));
-      }
-    most = halves_max_u32(most);
-    const bool finite = most < kInfBits;
-    if (!finite) {  // the largest finite one; past H there may be NaN, which is never stored
-      most = 0;
-#pragma unroll
-      for (int j = 0; j < T::FN; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const uint32_t b = abs_bits(s.sum[f][j][v]);
-          if (b < kInfBits) most = max(most, b);
-        }
-      most = halves_max_u32(most);
-    }
-    const float sc = __builtin_fmaxf(__uint_as_float(most) * (1.0f / kYMost), 0x1p-120f);
-    const float inv = __builtin_amdgcn_rcpf(sc) * (1.0f - 0x1p-22f);  // no code past kYMost
-    const uint32_t r = wt0 + 32 * f + tl;
-#pragma unroll
-    for (int j = 0; j < T::FN; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int v = 0; v < 16; v += 4) {
-        v2i d;
-        if (finite) {
-          d.x = (int)y_codes2(s.sum[f][j][v], s.sum[f][j][v + 1], inv);
-          d.y = (int)y_codes2(s.sum[f][j][v + 2], s.sum[f][j][v + 3], inv);
-        } else {
-          d.x = (y_code(s.sum[f][j][v], inv) & 0xffff) | (y_code(s.sum[f][j][v + 1], inv) << 16);
-          d.y = (y_code(s.sum[f][j][v + 2], inv) & 0xffff) | (y_code(s.sum[f][j][v + 3], inv) << 16);
-        }
-        *(v2i*)(mine + (32 * f + tl) * STRIDE + (32 * j + 4 * half + 2 * v) * 2) = d;
-      }
-    if (half == 0 && r < t.rows && cw < H) yscale[(size_t)(t.first + r) * nb + cw / 64] = finite ? sc : -sc;
-  }
-  // the wave's own rows back, whole lines to memory
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+        const uint32_t c = cw + 32 * j + 4 * half + 2 * v;  // H % 16 == 0: four columns are in or out together
+        const float* const w4 = a.ws_down + (size_t)t.of * H + (c < H ? c : 0);
 #pragma unroll
-  for (int i = 0; i < T::WT; i += 8) {
-    const uint32_t r = i + (lane >> 3), c = cw + (lane & 7) * 8;
-    if (wt0 + r < t.rows && c < H)
-      *(v4i*)(y + (size_t)(t.first + wt0 + r) * H + c) = *(const v4i*)(mine + r * STRIDE + (lane & 7) * 16);
+        for (int i = 0; i < 4; ++i) ws[j][v + i] = c < H ? w4[i] : 0.f;
+      }
+#pragma unroll
+    for (int f = 0; f < T::FT; ++f) {
+      uint32_t most = 0;
+      float y0[2][16];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          y0[j][v] = s.sum[f][j0 + j][v] * ws[j][v];
+          most = max(most, abs_bits(y0[j][v]));
+        }
+      most = halves_max_u32(most);
+      const bool finite = most < kInfBits;
+      if (!finite) {  // the largest finite one; past H there may be NaN, which is never stored
+        most = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const uint32_t b = abs_bits(y0[j][v]);
+            if (b < kInfBits) most = max(most, b);
+          }
+        most = halves_max_u32(most);
+      }
+      const float sc = __builtin_fmaxf(__uint_as_float(most) * (1.0f / kYMost), 0x1p-120f);
+      const float inv = __builtin_amdgcn_rcpf(sc) * (1.0f - 0x1p-22f);  // no code past kYMost
+      const uint32_t r = wt0 + 32 * f + tl;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+          v2i d;
+          if (finite) {
+            d.x = (int)y_codes2(y0[j][v], y0[j][v + 1], inv);
+            d.y = (int)y_codes2(y0[j][v + 2], y0[j][v + 3], inv);
+          } else {
+            d.x = (y_code(y0[j][v], inv) & 0xffff) | (y_code(y0[j][v + 1], inv) << 16);
+            d.y = (y_code(y0[j][v + 2], inv) & 0xffff) | (y_code(y0[j][v + 3], inv) << 16);
+          }
+          *(v2i*)(mine + (32 * f + tl) * STRIDE + (32 * j + 4 * half + 2 * v) * 2) = d;
+        }
+      if (half == 0 && r < t.rows && cw < H) yscale[(size_t)(t.first + r) * nb + cw / 64] = finite ? sc : -sc;
+    }
+    // the wave's own rows back, whole lines to memory
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < T::WT; i += 8) {
+      const uint32_t r = i + (lane >> 3), c = cw + (lane & 7) * 8;
+      if (wt0 + r < t.rows && c < H)
+        *(v4i*)(y + (size_t)(t.first + wt0 + r) * H + c) = *(const v4i*)(mine + r * STRIDE + (lane & 7) * 16);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // A plan tile is `parts` of these; one of few rows takes the lower form.
-template <class T, class Half>
+template <class T, class Half, class Quarter>
 __global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, ExpertsPlan plan, uint32_t parts,
                                                               const int8_t* codes, const float* scales, int16_t* y,
                                                               float* yscale) {
@@ -293,6 +300,10 @@ __global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, Exp
   RowTile t;
   uint32_t col;
   if (!own_tile<T::BT>(plan, parts, (a.hidden + T::BN - 1) / T::BN, t, col)) return;
+  if constexpr (!std::is_same_v<Quarter, NoForm>) {
+    static_assert(Quarter::NW == T::NW && Quarter::BN == T::BN && Quarter::LDS <= T::LDS, "forms of one launch");
+    if (t.rows <= (uint32_t)Quarter::BT) return down_tile<Quarter>(a, t, col, lds, codes, scales, y, yscale);
+  }
   if constexpr (!std::is_same_v<Half, NoForm>) {
     static_assert(Half::NW == T::NW && Half::BN == T::BN && Half::LDS <= T::LDS, "forms of one launch");
     if (t.rows <= (uint32_t)Half::BT) return down_tile<Half>(a, t, col, lds, codes, scales, y, yscale);
@@ -447,11 +458,11 @@ void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
   else gate_up_as<T256, T128, T64>(st, a, p, tiles, codes, scales);
 }
 
-template <class T, class Half>
+template <class T, class Half = NoForm, class Quarter = NoForm>
 void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
              const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
   const uint32_t parts = bt / T::BT, grid = (tiles * parts * ((a.hidden + T::BN - 1) / T::BN) + 7) / 8 * 8;
-  hipLaunchKernelGGL((experts_down<T, Half>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, parts, codes, scales, y,
+  hipLaunchKernelGGL((experts_down<T, Half, Quarter>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, parts, codes, scales, y,
                      yscale);
 }
 
@@ -459,9 +470,12 @@ template <bool TAIL>
 void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
           const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
   if (bt == 32 && tiles * ((a.hidden + 255) / 256) <= kOnePerCu)
-    down_as<Down<32, 256, 32, 4, 4, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
-  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
-  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>, NoForm>(st, a, p, bt, tiles, codes, scales, y, yscale);
+    down_as<Down<32, 256, 32, 4, 4, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
+  else if (bt == 256)
+    down_as<TileStream<256, 256, 64, 128, 2, 2, true, TAIL, OP_I8, true>, Down<128, 256, 64, 2, 2, TAIL>,
+            Down<64, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
   else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y,
                                                                              yscale);
 }

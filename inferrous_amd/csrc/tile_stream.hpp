@@ -23,6 +23,12 @@
 // i32 sums are scaled into f32 accumulators when the stage is done.  The scales
 // (f32, one per token row of the wave) ride as one more load of the token ring.
 //
+// BLOCKED (with GROUPED): a stage's sums are made block by block, each from the
+// stage's four fragments of its rows, and folded while the next block's are made:
+// the i32 sums take two blocks of registers, not FT * FN, and a wave can hold 64 x
+// 128 f32 sums.  A larger tile pulls fewer operand bytes per product, and a CU's
+// pull, about 28 bytes a clock, is what bounds these kernels.
+//
 // The op (OP) is the int8 one above or v_mfma_f32_32x32x16_bf16, whose fragments
 // are 16 bytes a lane too and whose result has the same layout.  K is then the
 // weight row's bytes, 2 a value.  OP_BF16_F32's token rows are f32, twice the
@@ -69,12 +75,13 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   return (__float_as_uint(bf16_rne(a)) >> 16) | (__float_as_uint(bf16_rne(b)) & 0xffff0000u);
 }
 
-template <int BT_, int BN_, int WT_, int WN_, int SA_, int SB_, bool GROUPED_, bool TAIL_, int OP_ = OP_I8>
+template <int BT_, int BN_, int WT_, int WN_, int SA_, int SB_, bool GROUPED_, bool TAIL_, int OP_ = OP_I8,
+          bool BLOCKED_ = false>
 struct TileStream {
   static constexpr int OP = OP_, TS = OP == OP_BF16_F32 ? 2 : 1;  // sections of a token row's stage
   using Acc = std::conditional_t<OP == OP_I8, v16i, v16f>;
   static constexpr int BT = BT_, BN = BN_, WT = WT_, WN = WN_, SA = SA_, SB = SB_;
-  static constexpr bool GROUPED = GROUPED_, TAIL = TAIL_;
+  static constexpr bool GROUPED = GROUPED_, TAIL = TAIL_, BLOCKED = BLOCKED_;
   static constexpr int WAVES_N = BN / WN, NW = (BT / WT) * WAVES_N;
   static constexpr int FT = WT / 32, FN = WN / 32;
   static constexpr int LT = TS * BT / 8 / NW, LN = BN / 8 / NW;  // row loads per wave per stage
@@ -86,8 +93,9 @@ struct TileStream {
   static_assert(LT >= 1 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads");
   static_assert(SA >= 2 && SB >= SA && SB <= 8 && (SA - 1) * LA + (SB - 1) * LN < 64, "ring depths");
   static_assert(LDS <= 160 * 1024, "LDS");
+  static_assert(!BLOCKED || (GROUPED && SA == 2 && SB == 2), "blocks of grouped sums, two stages");
 
-  Acc acc[FT][FN];
+  Acc acc[BLOCKED ? 1 : FT][BLOCKED ? 2 : FN];
   v16f sum[GROUPED ? FT : 1][GROUPED ? FN : 1];
 
   // token_row(r) / weight_row(r): the first byte of tile row r (any row of the
@@ -146,9 +154,55 @@ struct TileStream {
     for (int f = 0; f < FT; ++f)
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        acc[f][j] = Acc{};
+        if constexpr (!BLOCKED) acc[f][j] = Acc{};
         if constexpr (GROUPED) sum[f][j] = v16f{};
       }
+    if constexpr (BLOCKED) {
+      auto loads = [&](uint32_t kt) {
+#pragma unroll
+        for (int j = 0; j < LA; ++j) load_t(kt, j);
+#pragma unroll
+        for (int j = 0; j < LN; ++j) load_n(kt, j);
+      };
+      auto fold_block = [&](const Acc& a, float ts, v16f& to) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) to[v] = __builtin_fmaf((float)a[v], ts, to[v]);
+      };
+      loads(0);
+      for (uint32_t kt = 0; kt < KT; ++kt) {
+        await_loads<0>();                     // stage kt landed
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's reads of stage kt - 1 returned
+        __builtin_amdgcn_s_barrier();         // for every wave
+        if (kt + 1 < KT) loads(kt + 1);
+        const int8_t* const bt = lds_t + (kt % SA) * ASL + wt0 * 128;
+        const int8_t* const bn = lds_n + (kt % SB) * BSL + wn0 * 128;
+        v4i tf[FT][4], nf[4];
+        float ts[FT];
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+          ts[f] = *(const float*)(lds_s + (kt % SA) * SCL + (32 * f + fr) * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tf[f][i] = *(const v4i*)(bt + f * 4096 + off[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) nf[i] = *(const v4i*)(bn + j * 4096 + off[i]);
+#pragma unroll
+          for (int f = 0; f < FT; ++f) {
+            const int b = j * FT + f;
+            Acc& d = acc[0][b & 1];
+            d = mfma_op(nf[0], tf[f][0], Acc{});
+#pragma unroll
+            for (int i = 1; i < 4; ++i) d = mfma_op(nf[i], tf[f][i], d);
+            if (b > 0) fold_block(acc[0][(b - 1) & 1], ts[(b - 1) % FT], sum[(b - 1) % FT][(b - 1) / FT]);
+          }
+        }
+        constexpr int LAST = FT * FN - 1;
+        fold_block(acc[0][LAST & 1], ts[LAST % FT], sum[LAST % FT][LAST / FT]);
+      }
+      return;
+    } else {
     auto rd = [&](uint32_t kt, int i, v4i(&tf)[FT], v4i(&nf)[FN]) {
       const int8_t* bt = lds_t + (kt % SA) * ASL;
       const int8_t* bn = lds_n + (kt % SB) * BSL;
@@ -255,6 +309,7 @@ struct TileStream {
     mm(t0, n0, std::false_type{}, None{}, nothing);
     mm(t1, n1, std::false_type{}, None{}, nothing);
     fold();
+    }
   }
 };
 
