@@ -11,6 +11,8 @@
 //   live expert is left for get id -1 and weight 0;
 //   weight = s of the chosen (divided by the chosen ones' sum) * scale.
 // Every score, sum and weight is held in f32.
+#include <type_traits>
+
 #include "internal.hpp"
 #include "routed_common.hpp"
 
@@ -77,8 +79,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
       sum += s[i];
     }
     sum = wave_sum_f32(sum);
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) s[i] = sum > 0.f ? s[i] / sum : 0.f;
+    for (int i = 0; i < NE; ++i) s[i] *= inv;
   }
   uint32_t key[NE];
   float c[NE];
@@ -177,9 +180,23 @@ __device__ __forceinline__ void merge_two(float& a, float& b) {
   a = fmaxf(a, c);
 }
 
+// Lane (l + R) % 16's value, within the 16 lanes of a row.
+template <int R>
+__device__ __forceinline__ uint32_t row_rotate(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + R, 0xF, 0xF, false);  // row_ror
+}
+template <int R, class F>
+__device__ __forceinline__ void each_rotation(F f) {
+  if constexpr (R < 16) {
+    f(std::integral_constant<int, R>{});
+    each_rotation<R + 1>(f);
+  }
+}
+
 template <int NV>
 __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
   __shared__ __attribute__((aligned(16))) float sh[32][16 * NV];  // scores, choice scores
+  __shared__ uint2 lists[16][16];                                 // a row's candidates: choice score, expert
   const int lane = threadIdx.x & 63, li = lane & 15;
   const uint32_t slot = threadIdx.x >> 4, row = blockIdx.x * 16 + slot;
   const uint32_t r = min(row, a.m - 1);  // lanes of rows past the last one follow it, and store nothing
@@ -233,8 +250,9 @@ __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
       sum += c[i];
     }
     sum = row_sum_f32(sum);
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) c[i] = sum > 0.f ? c[i] / sum : 0.f;
+    for (int i = 0; i < NV; ++i) c[i] *= inv;
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) score[li * NV + i] = c[i];
@@ -292,22 +310,83 @@ __global__ __launch_bounds__(256) void route_quads(RouteArgs a) {
         if (!((keep >> ((uint32_t)(li * NV + i) / per & 15)) & 1)) c[i] = ninf;
     }
   }
+  // A bound on the k-th best: the k-th of every lane's two largest.  What is not
+  // below it, little more than k as a rule, goes to the row's lanes one each (LDS), and
+  // each counts the ones ahead of it.  More than 16, as after many ties: k rounds.
   int32_t id = -1;
-  for (uint32_t j = 0; j < a.k; ++j) {
-    float most = c[0];
+  float first = ninf, second = ninf;
 #pragma unroll
-    for (int i = 1; i < NV; ++i) most = fmaxf(most, c[i]);
-    most = row_max_f32(most);
-    uint32_t at = 16 * NV;
+  for (int i = 0; i < NV; ++i) {
+    second = fmaxf(second, fminf(first, c[i]));
+    first = fmaxf(first, c[i]);
+  }
+  uint32_t ahead1 = 0, ahead2 = 1;  // of the lane's first and second among the 32
+  each_rotation<1>([&](auto n) {
+    constexpr int R = decltype(n)::value;
+    const float f = __uint_as_float(row_rotate<R>(__float_as_uint(first)));
+    const float g = __uint_as_float(row_rotate<R>(__float_as_uint(second)));
+    ahead1 += (f > first) + (g > first);
+    ahead2 += (f > second) + (g > second);
+  });
+  // the smallest of those with fewer than k ahead: at least k values are not below it
+  float bound = ahead2 < a.k ? second : ahead1 < a.k ? first : __builtin_inff();
+  bound = -row_max_f32(-bound);
+  uint32_t mine = 0;
 #pragma unroll
-    for (int i = NV - 1; i >= 0; --i)
-      if (c[i] == most) at = li * NV + i;
-    at = row_min_u32(at);
-    if ((uint32_t)li == j && most > ninf) id = (int32_t)at;
-    const uint32_t mine = at - li * NV;
+  for (int i = 0; i < NV; ++i) mine += c[i] >= bound && c[i] > ninf;
+  uint32_t upto = mine;  // inclusive sums over the row's lanes
+  {
+    uint32_t t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto, 0x111, 0xF, 0xF, true);
+    upto += t;
+    t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto, 0x112, 0xF, 0xF, true);
+    upto += t;
+    t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto, 0x114, 0xF, 0xF, true);
+    upto += t;
+    t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto, 0x118, 0xF, 0xF, true);
+    upto += t;
+  }
+  const uint32_t count = ~row_min_u32(~upto);  // the row's largest
+  if (!__any(count > 16)) {
+    uint2* const list = lists[slot];
+    uint32_t at = upto - mine;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (mine == (uint32_t)i) c[i] = ninf;
+      if (c[i] >= bound && c[i] > ninf) list[at++] = make_uint2(__float_as_uint(c[i]), (uint32_t)(li * NV + i));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const bool on = (uint32_t)li < count;
+    const uint2 own = on ? list[li] : make_uint2(0xff800000u, 0xffffu);
+    const float v = __uint_as_float(own.x);
+    uint32_t ahead = 0;  // candidates lie in the order of their index: of equal ones the lower lane is ahead
+    each_rotation<1>([&](auto n) {
+      constexpr int R = decltype(n)::value;
+      const float o = __uint_as_float(row_rotate<R>(own.x));
+      const uint32_t oi = row_rotate<R>(own.y);
+      ahead += o > v || (o == v && oi < own.y);
+    });
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (on && ahead < 16) list[ahead].y = own.y;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if ((uint32_t)li < min(count, a.k)) id = (int32_t)list[li].y;
+  } else {
+    for (uint32_t j = 0; j < a.k; ++j) {
+      float most = c[0];
+#pragma unroll
+      for (int i = 1; i < NV; ++i) most = fmaxf(most, c[i]);
+      most = row_max_f32(most);
+      uint32_t at = 16 * NV;
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+        if (c[i] == most) at = li * NV + i;
+      at = row_min_u32(at);
+      if ((uint32_t)li == j && most > ninf) id = (int32_t)at;
+      const uint32_t gone = at - li * NV;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (gone == (uint32_t)i) c[i] = ninf;
+    }
   }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
