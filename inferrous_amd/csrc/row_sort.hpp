@@ -62,8 +62,7 @@ __device__ __forceinline__ void sort_load(const int32_t* ids, uint32_t classes, 
 // of its number (none for a lane of no class).
 __device__ __forceinline__ uint64_t sort_peers(uint32_t c, uint32_t n) {
   uint64_t peers = __ballot(c < n);
-#pragma unroll
-  for (int b = 0; b < 10; ++b) {
+  for (uint32_t b = 0; (1u << b) < n; ++b) {
     const uint64_t set = __ballot((c >> b) & 1);
     peers &= ((c >> b) & 1) ? set : ~set;
   }
