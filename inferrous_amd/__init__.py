@@ -5,7 +5,8 @@ A drop-in for the W8A8 linear-layer operators of bitemyapp/inferrous
 quantization, the M=1 v_dot4 decode GEMV, the INT8 MFMA GEMM for prefill and
 small batches, the fused per-token x per-channel dequant epilogue to BF16,
 and greedy selection over the lm_head logits (W8A8, or the reference's
-losslessly packed BF16 head).
+losslessly packed BF16 head).  Beside them, without a counterpart there: a
+router, the routed experts' W8A8 MLP, and low-rank adapters beside a projection.
 
 The compute lives in ``libinferrous_w8a8.so`` (hand-written HIP for gfx950,
 C ABI in ``include/inferrous_w8a8.h``).  This package is the host-side mirror

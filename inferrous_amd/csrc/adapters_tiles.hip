@@ -1,5 +1,8 @@
 // adapters_tiles.hip -- adapters beside a projection with the rows sorted by
-// adapter (adapters.hip has the definition).
+// adapter (adapters.hip has the definition).  4096 rows on 4096 x 12288, 6 adapters of
+// rank 64, with a residual: 224-240 us, the projection's tiles 195-220 of them (the
+// projection alone 175-183, 2.3 POPS); the large int8 library product's rate, 2.07
+// POPS, would take 203.
 //
 //   adapters_order          the sort, and the tiles: up to bt rows of one adapter;
 //   adapters_shrink_tiles   h's partial sums, tile x share of K, by bf16 MFMA;
@@ -28,7 +31,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void adapters_order(const int32_t*
 }
 
 // h[share][p][j] of a tile, in the sorted order: the token operand's rows are
-// gathered, K is the share's stages.
+// gathered, K is the share's stages.  4096 rows x 12288, rank 64: 26 us for 100 MB of x
+// and 50 MB of adapter rows, 5.8 TB/s; fragments straight from memory took 105 us, a
+// line for each 32 bytes.
 template <class T>
 __global__ __launch_bounds__(64 * T::NW) void adapters_shrink_tiles(AdapterArgs a, const uint32_t* order,
                                                                     const RowTile* table, const uint32_t* n_tiles,

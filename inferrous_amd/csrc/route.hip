@@ -147,6 +147,11 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_rows(RouteArgs a) {
   }
 }
 
+// What bounds it is instructions: about 1900 a wave for its four rows.  16384 rows of
+// 256 experts, k = 8, 4 of 8 groups: 12.4 us (17.8 MB; a copy of them takes 3.4); a wave
+// a row, whose reductions serve one row each, 27.  64 rows: 6.3 us, the same chain
+// once.
+//
 // 16 lanes a row, four rows a wave, lane l of a row holding its experts NV l ..
 // NV l + NV - 1: a round's reductions are four DPP steps for four rows at once.
 // For at most 16 NV = 256 experts, 16 groups and k <= 16.
