@@ -552,8 +552,8 @@ int w8a8_experts_mlp(void *stream, const int8_t *q, const float *asc, size_t m,
  * rank, k], b: BF16 [n_adapters, n, rank]; residual: f32 [m, n] or NULL.
  * Products and sums are held in f32, the projection's in exact i32.  rank: a
  * multiple of 8 up to 256 (pad a smaller one with zeros); n_adapters <= 1023; m
- * <= 2097120; x, a, b 16-byte aligned; q, w, k as for w8a8_linear.  Workspace as
- * for w8a8_experts_mlp.
+ * <= 2^21, n <= 2^22; x, a, b 16-byte aligned; q, w, k as for w8a8_linear.
+ * Workspace as for w8a8_experts_mlp.
  * out must not overlap an input. */
 size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k,
                                             uint32_t rank, uint32_t n_adapters);

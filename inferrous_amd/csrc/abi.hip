@@ -1438,7 +1438,7 @@ int w8a8_experts_mlp(void* stream, const int8_t* q, const float* asc, size_t m, 
 }
 
 static int check_adapters_shape(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters) {
-  if (m > kMaxAdapterRows || n > kU32Max || k == 0 || k % 16 != 0) return W8A8_ESHAPE;
+  if (m > kMaxAdapterRows || n > kMaxAdapterCols || k == 0 || k % 16 != 0) return W8A8_ESHAPE;
   if (rank == 0 || rank % 8 != 0 || rank > kMaxRank || n_adapters == 0 || n_adapters > kMaxAdapters)
     return W8A8_ESHAPE;
   return W8A8_OK;

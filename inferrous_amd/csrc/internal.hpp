@@ -235,7 +235,7 @@ struct RouteArgs {
 };
 constexpr uint32_t kMaxExperts = 1024, kMaxRouteGroups = 64, kMaxTopK = 64;
 constexpr uint32_t kMaxExpertWidth = 65536, kMaxExpertSlots = 1u << 24;  // of experts_mlp
-constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1023, kMaxAdapterRows = 65535 * 32;  // of linear_adapters
+constexpr uint32_t kMaxRank = 256, kMaxAdapters = 1023, kMaxAdapterRows = 1u << 21, kMaxAdapterCols = 1u << 22;  // of linear_adapters
 hipError_t launch_route(hipStream_t st, const RouteArgs& a);
 
 // The routed experts' SwiGLU products and their weighted sum (experts.hip).

@@ -357,6 +357,19 @@ def test_experts_non_finite_rows(env, m):
     assert np.array_equal(c.run(env)[0], np.zeros(144, F32))
 
 
+@pytest.mark.parametrize("m", [1, 40, 700])
+def test_experts_non_finite_scales_stay_in_their_columns(env, m):
+    """An infinite or NaN scale of one output column reaches that column only."""
+    c = Experts(m, 2, 3, 192, 144, seed=6, ids=np.tile([1, 2], (m, 1)))
+    want, err = c.want()
+    c.sd[2, 5], c.sd[1, 70], c.sd[2, 191] = INF, NAN, -INF
+    got = c.run(env)
+    bad = [5, 70, 191]
+    assert not np.isfinite(got[:, bad]).any() and np.isnan(got[:, 70]).all()
+    rest = np.setdiff1d(np.arange(192), bad)
+    close_bf16(got[:, rest], want[:, rest], err[:, rest])
+
+
 @pytest.mark.parametrize("m", [1, 70])
 def test_experts_same_bits_again_and_on_another_stream(env, m):
     c = Experts(m, 4, 8, 512, 256, seed=9)
@@ -457,6 +470,15 @@ def test_adapters_where_the_tiles_lead(env, m, n, k, rank, count, x_bf16):
     ids = rng.permutation(ids) if x_bf16 else ids
     Adapters(m, n, k, rank, count, seed=m + n, ids=ids, residual=x_bf16).check(env, F32 if x_bf16 else np.uint16,
                                                                                 x_bf16=x_bf16)
+
+
+def test_adapters_in_tiles_without_any(env):
+    """No row has an adapter: the projection, bit for bit."""
+    mod, s, _ = env
+    c = Adapters(900, 512, 512, 256, 3, seed=4, ids=np.full(900, -1))
+    out = dev(s, np.zeros(900 * 512, np.uint16))
+    mod.linear(s, None, *(dev(s, v) for v in (c.q, c.asc, c.w, c.ws)), 512, out)
+    assert np.array_equal(c.run(env), values(out, s).reshape(900, 512))
 
 
 def test_adapters_in_tiles_keep_rows_apart(env):

@@ -84,7 +84,8 @@ def adapters(**kw):
     (dict(), WELL), (dict(xt=_lib.OUT_BF16, res=A, dt=_lib.OUT_F32), WELL), (dict(m=0, q=None), _lib.OK),
     (dict(n=0, w=None), _lib.OK), (dict(dt=_lib.OUT_I32), _lib.EARG), (dict(xt=_lib.OUT_I32), _lib.EARG),
     (dict(k=72), _lib.ESHAPE), (dict(k=0), _lib.ESHAPE), (dict(r=0), _lib.ESHAPE), (dict(r=12), _lib.ESHAPE),
-    (dict(r=264), _lib.ESHAPE), (dict(c=0), _lib.ESHAPE), (dict(c=65537), _lib.ESHAPE),
+    (dict(r=264), _lib.ESHAPE), (dict(m=(1 << 21) + 1), _lib.ESHAPE), (dict(n=(1 << 22) + 1), _lib.ESHAPE),
+    (dict(c=1023), WELL), (dict(c=1024), _lib.ESHAPE), (dict(c=0), _lib.ESHAPE), (dict(c=65537), _lib.ESHAPE),
     *[({n: None}, _lib.ENULL) for n in ("q", "asc", "w", "ws", "x", "ids", "a", "b", "s", "out")],
     *[({n: A + 8}, _lib.EALIGN) for n in ("q", "w", "x", "a", "b", "wsp")],
     *[({n: A + 2}, _lib.EALIGN) for n in ("asc", "ws", "ids", "s", "res")],
