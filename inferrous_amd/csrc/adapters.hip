@@ -128,74 +128,101 @@ __global__ __launch_bounds__(256) void adapters_expand(AdapterArgs a, const int3
   }
 }
 
-// One row: the projection by dot products and the second product with it (4096 x
-// 4096, rank 16: 3.9 us, against 3.0 for the projection alone).  A wave
-// holds two columns; each lane reads 16 bytes of a weight row at a time, and up to
-// 8 ranks of a column's adapter row.
+// Few rows: the projection by dot products and the second product with
+// it, one launch less than the projection's own route and adapters_expand take.  A
+// wave holds two columns of every row; each lane reads 16 bytes of a weight row at a
+// time, and up to 8 ranks of a column's adapter row.
 constexpr int kGemvCols = 2;
+template <int M>
 __global__ __launch_bounds__(256) void adapters_gemv(AdapterArgs a, const float* __restrict__ h) {
+  constexpr int U = M == 1 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t c0 = (blockIdx.x * 4 + wave) * kGemvCols, id = (uint32_t)a.ids[0];
+  const uint32_t c0 = (blockIdx.x * 4 + wave) * kGemvCols;
   if (c0 >= a.n) return;
-  const int8_t* w[kGemvCols];
-  int sum[kGemvCols];
+  uint32_t id[M];
+  const int8_t *w[kGemvCols], *q[M];
+  int sum[M][kGemvCols];
 #pragma unroll
-  for (int c = 0; c < kGemvCols; ++c) {
-    w[c] = a.w + (size_t)min(c0 + c, a.n - 1) * a.width;
-    sum[c] = 0;
+  for (int r = 0; r < M; ++r) {
+    id[r] = (uint32_t)a.ids[r];
+    q[r] = a.q + (size_t)r * a.width;
+#pragma unroll
+    for (int c = 0; c < kGemvCols; ++c) sum[r][c] = 0;
   }
+#pragma unroll
+  for (int c = 0; c < kGemvCols; ++c) w[c] = a.w + (size_t)min(c0 + c, a.n - 1) * a.width;
   auto add = [&](uint32_t o, auto runs) {
     constexpr int R = decltype(runs)::value;
-    v4i x[R], v[R][kGemvCols];
+    v4i x[R][M], v[R][kGemvCols];
 #pragma unroll
     for (int u = 0; u < R; ++u) {
 #pragma unroll
       for (int c = 0; c < kGemvCols; ++c) v[u][c] = load_nt16(w[c] + o + 1024 * u);
-      x[u] = load16(a.q + o + 1024 * u);
+#pragma unroll
+      for (int r = 0; r < M; ++r) x[u][r] = load16(q[r] + o + 1024 * u);
     }
     __builtin_amdgcn_sched_barrier(0);  // every load is under way before the first use
 #pragma unroll
     for (int u = 0; u < R; ++u)
 #pragma unroll
-      for (int c = 0; c < kGemvCols; ++c) sum[c] = dot16(v[u][c], x[u], sum[c]);
+      for (int r = 0; r < M; ++r)
+#pragma unroll
+        for (int c = 0; c < kGemvCols; ++c) sum[r][c] = dot16(v[u][c], x[u][r], sum[r][c]);
   };
   uint32_t o = 0;
-  for (; o + 4096 <= a.width; o += 4096) add(o + lane * 16, std::integral_constant<int, 4>{});
+  for (; o + 1024 * U <= a.width; o += 1024 * U) add(o + lane * 16, std::integral_constant<int, U>{});
   for (; o < a.width; o += 1024)
     if (o + lane * 16 < a.width) add(o + lane * 16, std::integral_constant<int, 1>{});
-  float d[kGemvCols];
+  int acc = 0;
+  float delta = 0.f;
 #pragma unroll
-  for (int c = 0; c < kGemvCols; ++c) d[c] = 0.f;
-  if (id < a.adapters && lane * 8u < a.rank) {  // rank <= 256
-    const v4f h0 = *(const v4f*)(h + lane * 8), h1 = *(const v4f*)(h + lane * 8 + 4);
+  for (int r = 0; r < M; ++r) {
+    float d[kGemvCols];
 #pragma unroll
-    for (int c = 0; c < kGemvCols; ++c) {
-      const v4i b = *(const v4i*)(a.b + ((size_t)id * a.n + min(c0 + c, a.n - 1)) * a.rank + lane * 8);
+    for (int c = 0; c < kGemvCols; ++c) d[c] = 0.f;
+    if (id[r] < a.adapters && lane * 8u < a.rank) {  // rank <= 256
+      const float* const hr = h + (size_t)r * a.rank + lane * 8;
+      const v4f h0 = *(const v4f*)hr, h1 = *(const v4f*)(hr + 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        d[c] = __builtin_fmaf(bf16_lo((uint32_t)b[i]), i < 2 ? h0[2 * i] : h1[2 * i - 4], d[c]);
-        d[c] = __builtin_fmaf(bf16_hi((uint32_t)b[i]), i < 2 ? h0[2 * i + 1] : h1[2 * i - 3], d[c]);
+      for (int c = 0; c < kGemvCols; ++c) {
+        const v4i b = *(const v4i*)(a.b + ((size_t)id[r] * a.n + min(c0 + c, a.n - 1)) * a.rank + lane * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          d[c] = __builtin_fmaf(bf16_lo((uint32_t)b[i]), i < 2 ? h0[2 * i] : h1[2 * i - 4], d[c]);
+          d[c] = __builtin_fmaf(bf16_hi((uint32_t)b[i]), i < 2 ? h0[2 * i + 1] : h1[2 * i - 3], d[c]);
+        }
       }
     }
-  }
-  int acc = 0;
-  float add_on = 0.f;
 #pragma unroll
-  for (int c = 0; c < kGemvCols; ++c) {
-    const int t = wave_sum_i32(sum[c]);
-    const float u = wave_sum_f32(d[c]);
-    if (lane == c) acc = t, add_on = u;
+    for (int c = 0; c < kGemvCols; ++c) {
+      const int t = wave_sum_i32(sum[r][c]);
+      const float u = wave_sum_f32(d[c]);
+      if (lane == r * kGemvCols + c) acc = t, delta = u;
+    }
   }
-  const uint32_t c = c0 + lane;
-  if (lane < kGemvCols && c < a.n) {
-    float y = (float)acc * a.asc[0] * a.ws[c];
-    if (id < a.adapters) y += a.scaling[id] * add_on;
-    store_routed(a.out, a.out_dtype, c, a.residual ? a.residual[c] + y : y);
+  // lane kGemvCols r + c stores column c0 + c of row r
+  const uint32_t row = lane / kGemvCols, c = c0 + lane % kGemvCols;
+  if (row < (uint32_t)M && c < a.n) {
+    const size_t at = (size_t)row * a.n + c;
+    const uint32_t ad = (uint32_t)a.ids[row];
+    float y = (float)acc * a.asc[row] * a.ws[c];
+    if (ad < a.adapters) y += a.scaling[ad] * delta;
+    store_routed(a.out, a.out_dtype, at, a.residual ? a.residual[at] + y : y);
   }
 }
 
 // ------------------------------------------------------------------ plan
+// Few rows on a small projection: adapters_gemv, whose dot products per row cost
+// less than a launch while the rows past the first make at most 2^20 * 100 of them.
+// Measured, adapters_gemv / the projection's route and adapters_expand us: 4096 x 4096,
+// rank 16, m = 2 / 3 / 4 9.6 / 9.8 / 10.5 against 12.4 / 12.3 / 12.6; 4096 x 12288 14.0 /
+// 15.0 / 16.9 against 16.3; 24576 x 4096 22.3 / 24.7 / 28.6 against 22.3 / 22.0 / 22.0.
+constexpr uint32_t kGemvRows = 4;
+static bool gemv_leads(const AdapterArgs& a) {
+  return a.m == 1 || (a.m <= kGemvRows && (uint64_t)(a.m - 1) * a.n * a.width <= (100u << 20));
+}
+
 // Row by row, every row reads its own adapter: m rank (n + width) values from L2,
 // at about 10 TB/s, beside the projection.  The fused tiles read an adapter once,
 // but run in the tiles' own time: 22 us more than the projection at width 4096, 43
@@ -206,7 +233,7 @@ __global__ __launch_bounds__(256) void adapters_gemv(AdapterArgs a, const float*
 // 59 / 70, m = 1024 104 / 77; 24576 x 4096, rank 32, m = 80 (147 MB) 41 / 41, m = 128
 // 50 / 42.
 static bool fused_leads(const AdapterArgs& a) {
-  if (a.m == 1) return false;
+  if (gemv_leads(a)) return false;
   const double rows_us = (double)a.m * a.rank * ((double)a.n + a.width) * 2.0 / 10e6;
   const uint32_t mean = a.m / std::min(a.m, a.adapters), met = std::min(a.m, 256u) / std::min(mean, 256u);
   return rows_us > 8.0 + a.width / 400.0 + 1.5 * ((a.rank + 31) / 32) * (met > 1 ? met - 1 : 0);
@@ -248,7 +275,7 @@ AdapterPlan adapter_plan(const AdapterArgs& a) {
 }
 
 size_t adapters_workspace_bytes(const AdapterArgs& a) { return adapter_plan(a).bytes; }
-bool adapters_fused(const AdapterArgs& a) { return a.m == 1 || adapter_plan(a).fused; }
+bool adapters_fused(const AdapterArgs& a) { return gemv_leads(a) || adapter_plan(a).fused; }
 
 hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* workspace) {
   const AdapterPlan p = adapter_plan(a);
@@ -261,8 +288,10 @@ hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* wo
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, h); };
   if (a.x_bf16) go(J == 1 ? adapters_shrink<1, true> : J == 2 ? adapters_shrink<2, true> : adapters_shrink<8, true>);
   else go(J == 1 ? adapters_shrink<1, false> : J == 2 ? adapters_shrink<2, false> : adapters_shrink<8, false>);
-  if (a.m == 1)
-    hipLaunchKernelGGL(adapters_gemv, dim3((a.n + 4 * kGemvCols - 1) / (4 * kGemvCols)), dim3(256), 0, st, a, h);
+  if (gemv_leads(a)) {
+    auto k = a.m == 1 ? adapters_gemv<1> : a.m == 2 ? adapters_gemv<2> : a.m == 3 ? adapters_gemv<3> : adapters_gemv<4>;
+    hipLaunchKernelGGL(k, dim3((a.n + 4 * kGemvCols - 1) / (4 * kGemvCols)), dim3(256), 0, st, a, h);
+  }
   return hipGetLastError();
 }
 

@@ -677,10 +677,11 @@ class LoadedModule:
         nbytes = self._routed_bytes.get((size_of, shape))
         if nbytes is None:
             nbytes = self._routed_bytes[(size_of, shape)] = getattr(lib(), size_of)(*shape)
-        cur = self._gemm_ws.get(_key(stream))
+        key = stream.handle if stream is not None else None
+        cur = self._gemm_ws.get(key)
         if cur is None or cur.nbytes < nbytes:
             self.reserve_workspace(nbytes, stream)
-            cur = self._gemm_ws[_key(stream)]
+            cur = self._gemm_ws[key]
         return cur.ptr, cur.nbytes
 
     def route_experts(self, stream, logits: DeviceBuffer, n_experts: int, ids: DeviceBuffer,
@@ -694,23 +695,28 @@ class LoadedModule:
         (float32 [n_experts]) counts in the choice only, and ``groups`` /
         ``top_groups`` / ``group_top`` limit the choice to the best groups."""
         m = len(logits) // n_experts if n_experts > 0 else 0
-        if n_experts <= 0 or m * n_experts != len(logits):
-            raise ValueError("route_experts: logits must hold M rows of n_experts")
-        if len(ids) != len(weights) or (m and len(ids) % m) or (m and not len(ids)):
+        slots, dtype, code = len(ids), logits.dtype, _SCORES.get(score)
+        # one test of everything; what is wrong is found out after it
+        if not (n_experts > 0 and m * n_experts == len(logits) and slots == len(weights)
+                and (m == 0 or (slots > 0 and slots % m == 0)) and code is not None
+                and (dtype == _F32 or dtype == _U16) and ids.dtype == _I32 and weights.dtype == _F32
+                and (bias is None or (bias.dtype == _F32 and len(bias) >= n_experts))):
+            if n_experts <= 0 or m * n_experts != len(logits):
+                raise ValueError("route_experts: logits must hold M rows of n_experts")
+            if code is None:
+                raise ValueError(f"score {score!r}: one of {sorted(_SCORES)}")
+            if dtype != _F32 and dtype != _U16:
+                raise TypeError(f"logits dtype {dtype} not supported (float32/uint16)")
+            _needs(ids, _I32, 0, "ids")
+            _needs(weights, _F32, 0, "weights")
+            if bias is not None:
+                _needs(bias, _F32, n_experts, "bias")
             raise ValueError("route_experts: ids and weights must both hold M rows of K")
-        if score not in _SCORES:
-            raise ValueError(f"score {score!r}: one of {sorted(_SCORES)}")
-        if logits.dtype != _F32 and logits.dtype != _U16:
-            raise TypeError(f"logits dtype {logits.dtype} not supported (float32/uint16)")
-        _needs(ids, _I32, 0, "ids")
-        _needs(weights, _F32, 0, "weights")
-        if bias is not None:
-            _needs(bias, _F32, n_experts, "bias")
         if m == 0:
             return
-        check(lib().w8a8_route_experts(_h(stream), logits.ptr, _OUT[logits.dtype], m, n_experts, _SCORES[score],
+        check(lib().w8a8_route_experts(_h(stream), logits.ptr, _OUT[dtype], m, n_experts, code,
                                        None if bias is None else bias.ptr, groups, top_groups, group_top,
-                                       len(ids) // m, int(renorm), scale, ids.ptr, weights.ptr), "route_experts")
+                                       slots // m, renorm, scale, ids.ptr, weights.ptr), "route_experts")
 
     def experts_mlp(self, stream, q, asc, width: int, ids: DeviceBuffer, weights: DeviceBuffer, w0, s0, w1, s1, wd,
                     sd, n_experts: int, out, residual=None) -> None:
@@ -724,30 +730,30 @@ class LoadedModule:
         (float32 or uint16 BF16, [M, width]), with ``residual`` (float32)
         added.  The scratch space is the stream's workspace;
         ``reserve_workspace`` it before capturing a graph."""
-        m, width, n_experts = len(asc), int(width), int(n_experts)
-        if n_experts <= 0 or width <= 0 or len(s0) % n_experts or len(s1) != len(s0):
-            raise ValueError("experts_mlp: s_gate and s_up must hold n_experts rows of I")
-        inter = len(s0) // n_experts
-        if len(out) != m * width or len(ids) != len(weights) or (m and len(ids) % m):
-            raise ValueError("experts_mlp: out must hold M*width values, ids and weights M rows of K")
-        size = n_experts * inter * width
-        _needs(q, _I8, m * width, "q")
-        _needs(asc, _F32, m, "asc")
-        _needs(ids, _I32, 0, "ids")
-        _needs(weights, _F32, 0, "weights")
-        _needs(w0, _I8, size, "w_gate")
-        _needs(s0, _F32, 0, "s_gate")
-        _needs(w1, _I8, size, "w_up")
-        _needs(s1, _F32, 0, "s_up")
-        _needs(wd, _I8, size, "w_down")
-        _needs(sd, _F32, n_experts * width, "s_down")
-        if residual is not None:
-            _needs(residual, _F32, m * width, "residual")
-            if len(residual) != m * width:
-                raise ValueError("residual must hold M*width values")
+        m, width, n_experts, slots, columns = len(asc), int(width), int(n_experts), len(ids), len(s0)
+        inter = columns // n_experts if n_experts > 0 else 0
+        size, rows = columns * width, m * width
+        # one test of everything; what is wrong is found out after it
+        if not (n_experts > 0 and width > 0 and inter * n_experts == columns and len(s1) == columns
+                and len(out) == rows and slots == len(weights) and (m == 0 or slots % m == 0)
+                and len(q) >= rows and len(w0) >= size and len(w1) >= size and len(wd) >= size
+                and len(sd) >= n_experts * width
+                and q.dtype == w0.dtype == w1.dtype == wd.dtype == _I8 and ids.dtype == _I32
+                and asc.dtype == weights.dtype == s0.dtype == s1.dtype == sd.dtype == _F32
+                and (residual is None or (residual.dtype == _F32 and len(residual) == rows))):
+            if n_experts <= 0 or width <= 0 or inter * n_experts != columns or len(s1) != columns:
+                raise ValueError("experts_mlp: s_gate and s_up must hold n_experts rows of I")
+            for buf, dtype, need, what in ((q, _I8, rows, "q"), (asc, _F32, m, "asc"), (ids, _I32, 0, "ids"),
+                                           (weights, _F32, 0, "weights"), (w0, _I8, size, "w_gate"),
+                                           (s0, _F32, 0, "s_gate"), (w1, _I8, size, "w_up"), (s1, _F32, 0, "s_up"),
+                                           (wd, _I8, size, "w_down"), (sd, _F32, n_experts * width, "s_down")):
+                _needs(buf, dtype, need, what)
+            if residual is not None:
+                _needs(residual, _F32, rows, "residual")
+            raise ValueError("experts_mlp: out and residual must hold M*width values, ids and weights M rows of K")
         if m == 0:
             return
-        k = len(ids) // m
+        k = slots // m
         wp, wb = self._routed_workspace(stream, "w8a8_experts_mlp_workspace_bytes", m, k, n_experts, width, inter)
         check(lib().w8a8_experts_mlp(_h(stream), q.ptr, asc.ptr, m, width, ids.ptr, weights.ptr, k, n_experts, w0.ptr,
                                      s0.ptr, w1.ptr, s1.ptr, wd.ptr, sd.ptr, inter,
@@ -765,30 +771,31 @@ class LoadedModule:
         (float32) is added before the one rounding.  The scratch space is the
         stream's workspace; ``reserve_workspace`` it before capturing a
         graph."""
-        m, n, k = _shape(asc, ws, out, width)
-        count = len(scaling)
-        if k <= 0 or count == 0 or len(a) % (count * k):
-            raise ValueError("linear_adapters: a must hold len(scaling) adapters of rank rows of width")
-        rank = len(a) // (count * k)
-        _needs(q, _I8, m * k, "q")
-        _needs(asc, _F32, m, "asc")
-        _needs(w, _I8, n * k, "w")
-        _needs(ws, _F32, n, "ws")
-        _needs(ids, _I32, m, "ids")
-        _needs(a, _U16, 0, "a")
-        _needs(b, _U16, count * n * rank, "b")
-        _needs(scaling, _F32, 0, "scaling")
-        if x.dtype != _F32 and x.dtype != _U16:
-            raise TypeError(f"x dtype {x.dtype} not supported (float32/uint16)")
-        _check_len(x, m * k, "x")
-        if residual is not None:
+        m, n, k, count = len(asc), len(ws), int(width), len(scaling)
+        rank = len(a) // (count * k) if count and k > 0 else 0
+        dtype = x.dtype
+        # one test of everything; what is wrong is found out after it
+        if not (count and k > 0 and rank * count * k == len(a) and len(out) == m * n and len(q) >= m * k
+                and len(w) >= n * k and len(x) >= m * k and len(ids) >= m and len(b) >= count * n * rank
+                and q.dtype == w.dtype == _I8 and asc.dtype == ws.dtype == scaling.dtype == _F32
+                and ids.dtype == _I32 and a.dtype == b.dtype == _U16 and (dtype == _F32 or dtype == _U16)
+                and (residual is None or (residual.dtype == _F32 and len(residual) == m * n))):
+            _shape(asc, ws, out, width)
+            if k <= 0 or count == 0 or rank * count * k != len(a):
+                raise ValueError("linear_adapters: a must hold len(scaling) adapters of rank rows of width")
+            for buf, dt, need, what in ((q, _I8, m * k, "q"), (asc, _F32, m, "asc"), (w, _I8, n * k, "w"),
+                                        (ws, _F32, n, "ws"), (ids, _I32, m, "ids"), (a, _U16, 0, "a"),
+                                        (b, _U16, count * n * rank, "b"), (scaling, _F32, 0, "scaling")):
+                _needs(buf, dt, need, what)
+            if dtype != _F32 and dtype != _U16:
+                raise TypeError(f"x dtype {dtype} not supported (float32/uint16)")
+            _check_len(x, m * k, "x")
             _needs(residual, _F32, m * n, "residual")
-            if len(residual) != m * n:
-                raise ValueError("residual must hold M*N values")
+            raise ValueError("residual must hold M*N values")
         if m == 0 or n == 0:
             return
         wp, wb = self._routed_workspace(stream, "w8a8_linear_adapters_workspace_bytes", m, n, k, rank, count)
-        check(lib().w8a8_linear_adapters(_h(stream), q.ptr, asc.ptr, m, w.ptr, ws.ptr, n, k, x.ptr, _OUT[x.dtype],
+        check(lib().w8a8_linear_adapters(_h(stream), q.ptr, asc.ptr, m, w.ptr, ws.ptr, n, k, x.ptr, _OUT[dtype],
                                          ids.ptr, a.ptr, b.ptr, scaling.ptr, rank, count,
                                          None if residual is None else residual.ptr, out.ptr, _dtype_code(out), wp,
                                          wb), "linear_adapters")

@@ -449,7 +449,7 @@ class Adapters:
 
 
 @pytest.mark.parametrize("m, n, k, rank, count", [
-    (1, 1, 16, 8, 1), (1, 33, 64, 8, 2), (1, 4096, 4096, 16, 3), (1, 515, 2000, 64, 4), (1, 7, 5136, 256, 2), (64, 96, 4096, 128, 5), (2, 300, 512, 24, 3),
+    (1, 1, 16, 8, 1), (1, 33, 64, 8, 2), (1, 4096, 4096, 16, 3), (1, 515, 2000, 64, 4), (1, 7, 5136, 256, 2), (64, 96, 4096, 128, 5), (2, 300, 512, 24, 3), (2, 33, 4112, 256, 2), (3, 1030, 2064, 40, 5), (4, 515, 1008, 16, 3), (4, 8200, 4096, 8, 2),
     (5, 1023, 784, 16, 7), (8, 256, 4096, 256, 2), (16, 640, 1024, 32, 40), (33, 129, 272, 128, 5),
     (64, 700, 1040, 40, 64), (65, 257, 128, 8, 3), (130, 500, 2000, 72, 9), (300, 320, 640, 16, 4),
     (513, 193, 400, 64, 1)])
