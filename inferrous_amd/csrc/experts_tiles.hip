@@ -65,8 +65,9 @@ __device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t parts
 // (v < 8) and its up sum (v + 8).
 // Few rows an expert: the weight stream bounds it, two workgroups a CU (81 experts of
 // hidden 2048, inner 768 met by 128 slots, 255 MB: 41 us, 6.2 TB/s; one workgroup with
-// four stages 45).  Many: the matrix cores, busy 55% of the time at the clock that
-// the board's power leaves (256-row tiles, 550 G operations in 345-365 us).
+// four stages 45).  Many: the matrix cores, busy 55-60% of the time at the clock
+// that the board's power leaves (256-row tiles, 550 G operations in 330-340 us, 285 of
+// them without the epilogue, which issues about 30 instructions a value of act).
 template <class T>
 __device__ __forceinline__ void gate_up_tile(const ExpertsArgs& a, const ExpertsPlan& plan, const RowTile& t,
                                              uint32_t group, int8_t* lds, int8_t* codes, float* scales) {

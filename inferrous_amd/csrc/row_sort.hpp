@@ -69,6 +69,17 @@ __device__ __forceinline__ uint64_t sort_peers(uint32_t c, uint32_t n) {
   return c < n ? peers : 0;
 }
 
+// Of every group of 64 that the wave's run has: up to 1024 items among 16 waves leave
+// a wave one group or none.
+__device__ __forceinline__ void sort_all_peers(const uint32_t (&c)[kSortRegs], uint32_t begin, uint32_t end, uint32_t n,
+                                               uint64_t (&peers)[kSortRegs]) {
+#pragma unroll
+  for (int i = 0; i < kSortRegs; ++i) {
+    peers[i] = 0;
+    if (begin + 64 * i < end) peers[i] = sort_peers(c[i], n);
+  }
+}
+
 // hist[class] of a wave's items.  One lane of each class adds its peers: atomics
 // of 64 equal classes, which sorted requests bring, took 10 of the sort's 13 us at
 // 4096 items of 7 classes.
@@ -95,8 +106,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_counts(const int32_t* id
   uint32_t c[kSortRegs];
   uint64_t peers[kSortRegs];
   sort_load<REST>(ids, classes, begin, end, lane, c);
-#pragma unroll
-  for (int i = 0; i < kSortRegs; ++i) peers[i] = sort_peers(c[i], n);
+  sort_all_peers(c, begin, end, n, peers);
   sort_count(c, peers, n, hist + wave * n, lane);
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < n; e += 64 * kSortWaves) {
@@ -162,8 +172,7 @@ __device__ __forceinline__ void sort_items(const int32_t* ids, uint32_t items, u
   uint32_t c[kSortRegs];
   uint64_t peers[kSortRegs];
   sort_load<REST>(ids, classes, begin, end, lane, c);
-#pragma unroll
-  for (int i = 0; i < kSortRegs; ++i) peers[i] = sort_peers(c[i], n);
+  sort_all_peers(c, begin, end, n, peers);
   sort_count(c, peers, n, hist + wave * n, lane);
   __syncthreads();
   uint32_t total = 0, before = 0;  // of class e: all its items, those of earlier workgroups
