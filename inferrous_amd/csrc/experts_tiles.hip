@@ -13,9 +13,8 @@
 //                      128-column groups, each scaled into f32 sums;
 //   experts_combine    out = residual + sum over a row's slots of weight * y.
 //
-// y goes through memory as 16-bit fixed point against the largest magnitude of
-// 64 columns of its row: half the bytes of f32, which would be the pass's largest
-// stream, at an error below 2^-16 of that magnitude, 2^-8 of what BF16 would add.
+// y goes through memory in f32, the pass's largest stream: a sum over slots is of
+// f32 values, and a column much larger than its neighbours costs them nothing.
 #include "experts.hpp"
 #include "tile_stream.hpp"
 
@@ -188,27 +187,6 @@ __global__ __launch_bounds__(64 * T::NW, 2) void experts_gate_up(ExpertsArgs a, 
 }
 
 // ------------------------------------------------------------------ down
-// 16-bit fixed point of y against its block's largest finite magnitude: up to
-// 32766, with codes of their own for the infinities and NaN; a block that has
-// any of them has its scale's sign set.
-constexpr float kYMost = 32766.0f;
-__device__ __forceinline__ int y_code(float y, float inv) {
-  if (!(__builtin_fabsf(y) < __builtin_inff())) return y != y ? -32768 : y > 0 ? 32767 : -32767;
-  return (int)__builtin_rintf(y * inv);
-}
-__device__ __forceinline__ float y_value(int code) {  // in units of the scale
-  if (code == -32768) return __builtin_nanf("");
-  if (code == 32767 || code == -32767) return code > 0 ? __builtin_inff() : -__builtin_inff();
-  return (float)code;
-}
-// Two finite values' codes in one word: adding 1.5 * 2^23 rounds to the integer
-// that is the low half of the sum's bits.
-__device__ __forceinline__ uint32_t y_codes2(float a, float b, float inv) {
-  const uint32_t p = __float_as_uint(__builtin_fmaf(a, inv, 12582912.0f));
-  const uint32_t q = __float_as_uint(__builtin_fmaf(b, inv, 12582912.0f));
-  return __builtin_amdgcn_perm(q, p, 0x05040100u);
-}
-
 // What bounds it at many rows is the CU's operand pull, 28 bytes a clock, not the f32
 // folding: 128 x 128 tiles (two workgroups a CU) took 313 us for 4096 rows x 8 of 64
 // experts, hidden 4096, inner 1024 (275 G operations); without the folding the same,
@@ -216,9 +194,9 @@ __device__ __forceinline__ uint32_t y_codes2(float a, float b, float inv) {
 // 256 x 128 tiles with three stages 310-333, 128 x 128 with four 393-410.
 template <class T>
 __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t, uint32_t col, int8_t* lds,
-                                          const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
-  constexpr int STRIDE = 144;  // bytes of a row of 64 codes in LDS, padded
-  static_assert(T::WN % 64 == 0 && T::GROUPED && T::NW * T::WT * STRIDE <= T::LDS, "the epilogue reuses the rings");
+                                          const int8_t* codes, const float* scales, float* y) {
+  constexpr int STRIDE = 64 + 4;  // f32 values of an LDS row of 64 columns, padded
+  static_assert(T::WN % 64 == 0 && T::GROUPED && T::NW * 32 * STRIDE * 4 <= T::LDS, "the epilogue reuses the rings");
   const uint32_t H = a.hidden, I = a.inter, c0 = col * T::BN, slots = a.m * a.k;
   const int8_t* const w = a.w_down + (size_t)t.of * H * I;
   T s;
@@ -230,10 +208,9 @@ __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wt0 = (wave / T::WAVES_N) * T::WT, half = lane >> 5, tl = lane & 31;
-  const uint32_t nb = (H + 63) / 64;
   __syncthreads();  // every wave is done with the rings
-  int8_t* const mine = lds + wave * T::WT * STRIDE;
-  // blocks of 64 columns
+  float* const mine = (float*)lds + wave * 32 * STRIDE;
+  // 32 rows x 64 columns at a time through the wave's own LDS, whole lines to memory
 #pragma unroll
   for (int j0 = 0; j0 < T::FN; j0 += 2) {
     const uint32_t cw = c0 + (wave % T::WAVES_N) * T::WN + 32 * j0;
@@ -245,151 +222,89 @@ __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t
         const uint32_t c = cw + 32 * j + 4 * half + 2 * v;  // H % 16 == 0: four columns are in or out together
         const float* const w4 = a.ws_down + (size_t)t.of * H + (c < H ? c : 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ws[j][v + i] = c < H ? w4[i] : 0.f;
+        for (int i = 0; i < 4; ++i) ws[j][v + i] = w4[i];
       }
 #pragma unroll
     for (int f = 0; f < T::FT; ++f) {
-      uint32_t most = 0;
-      float y0[2][16];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          y0[j][v] = s.sum[f][j0 + j][v] * ws[j][v];
-          most = max(most, abs_bits(y0[j][v]));
-        }
-      most = halves_max_u32(most);
-      const bool finite = most < kInfBits;
-      if (!finite) {  // the largest finite one; past H there may be NaN, which is never stored
-        most = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const uint32_t b = abs_bits(y0[j][v]);
-            if (b < kInfBits) most = max(most, b);
-          }
-        most = halves_max_u32(most);
-      }
-      const float sc = __builtin_fmaxf(__uint_as_float(most) * (1.0f / kYMost), 0x1p-120f);
-      const float inv = __builtin_amdgcn_rcpf(sc) * (1.0f - 0x1p-22f);  // no code past kYMost
-      const uint32_t r = wt0 + 32 * f + tl;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 4) {
-          v2i d;
-          if (finite) {
-            d.x = (int)y_codes2(y0[j][v], y0[j][v + 1], inv);
-            d.y = (int)y_codes2(y0[j][v + 2], y0[j][v + 3], inv);
-          } else {
-            d.x = (y_code(y0[j][v], inv) & 0xffff) | (y_code(y0[j][v + 1], inv) << 16);
-            d.y = (y_code(y0[j][v + 2], inv) & 0xffff) | (y_code(y0[j][v + 3], inv) << 16);
-          }
-          *(v2i*)(mine + (32 * f + tl) * STRIDE + (32 * j + 4 * half + 2 * v) * 2) = d;
+          const auto& sum = s.sum[f][j0 + j];
+          *(v4f*)(mine + tl * STRIDE + 32 * j + 2 * v + 4 * half) =
+              v4f{sum[v] * ws[j][v], sum[v + 1] * ws[j][v + 1], sum[v + 2] * ws[j][v + 2], sum[v + 3] * ws[j][v + 3]};
         }
-      if (half == 0 && r < t.rows && cw < H) yscale[(size_t)(t.first + r) * nb + cw / 64] = finite ? sc : -sc;
-    }
-    // the wave's own rows back, whole lines to memory
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < T::WT; i += 8) {
-      const uint32_t r = i + (lane >> 3), c = cw + (lane & 7) * 8;
-      if (wt0 + r < t.rows && c < H)
-        *(v4i*)(y + (size_t)(t.first + wt0 + r) * H + c) = *(const v4i*)(mine + r * STRIDE + (lane & 7) * 16);
+      for (int i = 0; i < 32; i += 4) {
+        const uint32_t r = i + (lane >> 4), c = cw + (lane & 15) * 4, row = wt0 + 32 * f + r;
+        if (row < t.rows && c < H)
+          *(v4f*)(y + (size_t)(t.first + row) * H + c) = *(const v4f*)(mine + r * STRIDE + (lane & 15) * 4);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // A plan tile is `parts` of these; one of few rows takes the lower form.
 template <class T, class Half, class Quarter>
 __global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, ExpertsPlan plan, uint32_t parts,
-                                                              const int8_t* codes, const float* scales, int16_t* y,
-                                                              float* yscale) {
+                                                              const int8_t* codes, const float* scales, float* y) {
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
   RowTile t;
   uint32_t col;
   if (!own_tile<T::BT>(plan, parts, (a.hidden + T::BN - 1) / T::BN, t, col)) return;
   if constexpr (!std::is_same_v<Quarter, NoForm>) {
     static_assert(Quarter::NW == T::NW && Quarter::BN == T::BN && Quarter::LDS <= T::LDS, "forms of one launch");
-    if (t.rows <= (uint32_t)Quarter::BT) return down_tile<Quarter>(a, t, col, lds, codes, scales, y, yscale);
+    if (t.rows <= (uint32_t)Quarter::BT) return down_tile<Quarter>(a, t, col, lds, codes, scales, y);
   }
   if constexpr (!std::is_same_v<Half, NoForm>) {
     static_assert(Half::NW == T::NW && Half::BN == T::BN && Half::LDS <= T::LDS, "forms of one launch");
-    if (t.rows <= (uint32_t)Half::BT) return down_tile<Half>(a, t, col, lds, codes, scales, y, yscale);
+    if (t.rows <= (uint32_t)Half::BT) return down_tile<Half>(a, t, col, lds, codes, scales, y);
   }
-  down_tile<T>(a, t, col, lds, codes, scales, y, yscale);
+  down_tile<T>(a, t, col, lds, codes, scales, y);
 }
 
 // ------------------------------------------------------------------ sum
-// out[t, c .. c + 7] a thread, slots in order: the sum's order is fixed.  Eight
+// out[t, c .. c + 3] a thread, slots in order: the sum's order is fixed.  Eight
 // slots' rows are under way together; their positions and weights, one row's,
-// are wave-uniform.  4096 rows of 8 slots, hidden 4096: 301 MB in 56 us, 5.4 TB/s, the
-// rate of a large copy.
+// are wave-uniform.
 __global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int32_t* __restrict__ pos,
-                                                       const int16_t* __restrict__ y,
-                                                       const float* __restrict__ yscale) {
-  const uint32_t nb = (a.hidden + 63) / 64, row = blockIdx.x;
-  const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 8;
+                                                       const float* __restrict__ y) {
+  const uint32_t row = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= a.hidden) return;
-  float sum[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+  v4f sum{};
   for (uint32_t j0 = 0; j0 < a.k; j0 += 8) {
-    v4i v[8];
-    float s[8];
+    v4f v[8];
     int32_t p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = pos[(size_t)row * a.k + min(j0 + j, a.k - 1)];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const size_t at = (size_t)max(p[j], 0);  // a slot without an expert reads a row that it does not use
-      s[j] = yscale[at * nb + c / 64];
-      v[j] = *(const v4i*)(y + at * a.hidden + c);
-    }
+    for (int j = 0; j < 8; ++j)  // a slot without an expert reads a row that it does not use
+      v[j] = *(const v4f*)(y + (size_t)max(p[j], 0) * a.hidden + c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (j0 + j >= a.k || p[j] < 0) continue;
-      const float w = a.weights[(size_t)row * a.k + j0 + j] * __builtin_fabsf(s[j]);
-      if (s[j] > 0.f) {
+      const float w = a.weights[(size_t)row * a.k + j0 + j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum[2 * i] = __builtin_fmaf(w, (float)(int16_t)(v[j][i] & 0xffff), sum[2 * i]);
-          sum[2 * i + 1] = __builtin_fmaf(w, (float)(v[j][i] >> 16), sum[2 * i + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum[2 * i] = __builtin_fmaf(w, y_value((int)(int16_t)(v[j][i] & 0xffff)), sum[2 * i]);
-          sum[2 * i + 1] = __builtin_fmaf(w, y_value(v[j][i] >> 16), sum[2 * i + 1]);
-        }
-      }
+      for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(w, v[j][i], sum[i]);
     }
   }
   const size_t o = (size_t)row * a.hidden + c;
   if (a.residual) {
+    const v4f r = *(const v4f*)(a.residual + o);
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      const v4f r = *(const v4f*)(a.residual + o + i);
-#pragma unroll
-      for (int l = 0; l < 4; ++l) sum[i + l] = r[l] + sum[i + l];
-    }
+    for (int i = 0; i < 4; ++i) sum[i] = r[i] + sum[i];
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum[i] = bf16_rne(sum[i]);
+  for (int i = 0; i < 4; ++i) sum[i] = bf16_rne(sum[i]);
   if (a.out_dtype == W8A8_OUT_F32) {
-    float* const out = (float*)a.out + o;
-    *(v4f*)out = v4f{sum[0], sum[1], sum[2], sum[3]};
-    *(v4f*)(out + 4) = v4f{sum[4], sum[5], sum[6], sum[7]};
+    *(v4f*)((float*)a.out + o) = sum;
   } else {
-    v4i out;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      out[i] = (int)((__float_as_uint(sum[2 * i]) >> 16) | (__float_as_uint(sum[2 * i + 1]) & 0xffff0000u));
-    *(v4i*)((uint16_t*)a.out + o) = out;
+    *(v2i*)((uint16_t*)a.out + o) = v2i{(int)((__float_as_uint(sum[0]) >> 16) | (__float_as_uint(sum[1]) & 0xffff0000u)),
+                                        (int)((__float_as_uint(sum[2]) >> 16) | (__float_as_uint(sum[3]) & 0xffff0000u))};
   }
 }
 
@@ -417,7 +332,7 @@ static uint32_t most_tiles(uint32_t slots, uint32_t experts, uint32_t bt) {
 
 namespace {
 struct Layout {
-  size_t order, pos, tiles, n_tiles, counts, codes, scales, y, yscale, bytes;
+  size_t order, pos, tiles, n_tiles, counts, codes, scales, y, bytes;
 };
 Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
   const size_t slots = (size_t)m * k;
@@ -436,8 +351,7 @@ Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_
   l.counts = take(blocks > 1 ? (size_t)blocks * experts * 4 : 0);
   l.codes = take(slots * inter);
   l.scales = take(slots * ((inter + 127) / 128) * 4);
-  l.y = take(slots * hidden * 2);
-  l.yscale = take(slots * ((hidden + 63) / 64) * 4);
+  l.y = take(slots * hidden * 4);
   l.bytes = at;
   return l;
 }
@@ -474,24 +388,22 @@ void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
 
 template <class T, class Half = NoForm, class Quarter = NoForm>
 void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
-             const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
+             const int8_t* codes, const float* scales, float* y) {
   const uint32_t parts = bt / T::BT, grid = (tiles * parts * ((a.hidden + T::BN - 1) / T::BN) + 7) / 8 * 8;
-  hipLaunchKernelGGL((experts_down<T, Half, Quarter>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, parts, codes, scales, y,
-                     yscale);
+  hipLaunchKernelGGL((experts_down<T, Half, Quarter>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, parts, codes, scales, y);
 }
 
 template <bool TAIL>
 void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
-          const int8_t* codes, const float* scales, int16_t* y, float* yscale) {
+          const int8_t* codes, const float* scales, float* y) {
   if (bt == 32 && tiles * ((a.hidden + 255) / 256) <= kOnePerCu)
-    down_as<Down<32, 256, 32, 4, 4, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
-  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
-  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
+    down_as<Down<32, 256, 32, 4, 4, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
+  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
+  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
   else if (bt == 256)
     down_as<TileStream<256, 256, 64, 128, 2, 2, true, TAIL, OP_I8, true>, Down<128, 256, 64, 2, 2, TAIL>,
-            Down<64, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y, yscale);
-  else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y,
-                                                                             yscale);
+            Down<64, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
+  else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
 }
 }  // namespace
 
@@ -507,8 +419,7 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
                          (uint32_t*)(p + l.n_tiles)};
   int8_t* const codes = (int8_t*)(p + l.codes);
   float* const scales = (float*)(p + l.scales);
-  int16_t* const y = (int16_t*)(p + l.y);
-  float* const yscale = (float*)(p + l.yscale);
+  float* const y = (float*)(p + l.y);
   uint32_t* const counts = (uint32_t*)(p + l.counts);
   const uint32_t bt = tile_rows(slots, a.experts, a.hidden, a.inter);
   const uint32_t tiles = most_tiles(slots, a.experts, bt);
@@ -520,9 +431,9 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
                      bt, plan);
   if (a.hidden % 128 == 0) gate_up<false>(st, a, plan, bt, tiles, codes, scales);
   else gate_up<true>(st, a, plan, bt, tiles, codes, scales);
-  if (a.inter % 128 == 0) down<false>(st, a, plan, bt, tiles, codes, scales, y, yscale);
-  else down<true>(st, a, plan, bt, tiles, codes, scales, y, yscale);
-  hipLaunchKernelGGL(experts_combine, dim3(a.m, (a.hidden + 2047) / 2048), dim3(256), 0, st, a, plan.pos, y, yscale);
+  if (a.inter % 128 == 0) down<false>(st, a, plan, bt, tiles, codes, scales, y);
+  else down<true>(st, a, plan, bt, tiles, codes, scales, y);
+  hipLaunchKernelGGL(experts_combine, dim3(a.m, (a.hidden + 1023) / 1024), dim3(256), 0, st, a, plan.pos, y);
   return hipGetLastError();
 }
 
