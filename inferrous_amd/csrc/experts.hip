@@ -130,7 +130,7 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
       v4i q;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        q[i] = (int)act_codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
+        q[i] = (int)codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
       code[wave][lane] = q;
       if ((lane & 7) == 0) scale[wave][lane >> 3] = s * weight;
       __syncthreads();

@@ -16,23 +16,16 @@ struct ExpertsPlan {
   uint32_t* n_tiles;
 };
 
-// act of two projections, kept in f32 up to its codes.  exp(-gate) goes straight to
-// v_exp_f32: its error, 2^-23.7 |gate|, is far below a code's step, 1 / 127 of the
-// group's maximum, wherever act is not negligible.
+// act of two projections, kept in f32 up to its codes: SiLU from t = exp(-|gate|), in
+// (0, 1], as gate * (gate < 0 ? t : 1) / (1 + t), the reciprocal by v_rcp_f32 and one
+// Newton step: the divisor is never large, where v_rcp_f32 has no normal result.
+// Below -128 t is 0.  About 3 units of the last place.
 __device__ __forceinline__ float act_f32(int32_t g, int32_t u, float asc, float wg, float wu) {
   const float gate = (float)g * asc * wg, up = (float)u * asc * wu;
-  return gate * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gate * -1.44269502f)) * up;
-}
-
-// Four codes of act at scale s, r = RN(1 / s): v r is within 2^-23 of v / s, 1.6e-5 of a
-// code at most, so that only a value that close to a half takes the other neighbour;
-// adding 1.5 * 2^23 rounds to the integer that is the low byte.  An infinite s
-// gives zeros.  `slow` as in codes4.  Two instructions a value, where the correctly
-// rounded quotients take eight.
-__device__ __forceinline__ uint32_t act_codes4(float a, float b, float c, float d, float s, float r, bool slow) {
-  if (slow) return pack4(a, b, c, d, s);
-  auto bits = [&](float v) { return __float_as_uint(__builtin_fmaf(v, r, 12582912.0f)); };
-  return __builtin_amdgcn_perm(bits(b), bits(a), 0x0c0c0400u) | __builtin_amdgcn_perm(bits(d), bits(c), 0x04000c0cu);
+  const float t = exp_above_m128(__builtin_fmaxf(-__builtin_fabsf(gate), -128.0f)), d = 1.0f + t;
+  float r = __builtin_amdgcn_rcpf(d);
+  r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+  return gate * (gate < 0.f ? t : 1.0f) * r * up;
 }
 
 size_t experts_tiles_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);

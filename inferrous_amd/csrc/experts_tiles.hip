@@ -148,7 +148,7 @@ __device__ __forceinline__ void gate_up_tile(const ExpertsArgs& a, const Experts
 #pragma unroll
       for (int v = 0; v < 8; v += 4)
         *(uint32_t*)(rows + r * CSTRIDE + (wn * T::FN + j) * 16 + 4 * half + 2 * v) =
-            act_codes4(act[f][j][v], act[f][j][v + 1], act[f][j][v + 2], act[f][j][v + 3], sc, inv, slow);
+            codes4(act[f][j][v], act[f][j][v + 1], act[f][j][v + 2], act[f][j][v + 3], sc, inv, slow);
     if (wn == 0 && half == 0 && r < t.rows) scales[(size_t)group * slots + t.first + r] = sc;
   }
   __syncthreads();

@@ -37,6 +37,15 @@ __device__ __forceinline__ float exp_fast(float x) {
   return e < __builtin_inff() && __builtin_fabsf(lo) < 1.0f ? __builtin_fmaf(e, lo * 0.693147182f, e) : e;
 }
 
+// exp(x) for x in [-128, 0], where the correction is small and neither part can
+// overflow: exp_fast without its tests.
+__device__ __forceinline__ float exp_above_m128(float x) {
+  const float t = x * 1.44269502f;
+  const float lo = __builtin_fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, lo * 0.693147182f, e);
+}
+
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, load
-from test_gpu_routed import Experts, close_bf16
+from test_gpu_routed import Experts, bf16, close_bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,48 @@ def test_experts_large_columns_cost_their_neighbours_nothing(env, m):
     c.sd[:, 70] *= 1e5
     rest = np.setdiff1d(np.arange(192), [5, 70])
     close_bf16(c.run(env)[:, rest], want[:, rest], err[:, rest])
+
+
+@pytest.mark.parametrize("m", ROWS)
+def test_experts_codes_round_ties_to_even(env, m):
+    """act exactly at the half-way points of its codes, for a scale that is no power
+    of two: gate is 32, whose sigmoid is 1 in f32, and up k + 1/2 times the scale.
+    The codes' products are exact, so the outputs are the definition's in BF16."""
+    h, f = 128, 128
+    c = Experts(m, 1, 1, h, f, ids=np.zeros((m, 1), np.int32))
+    c.q[:] = 0
+    c.q[:, :2] = 1                                # column 0 of gate's rows, column 1 of up's
+    c.asc[:], c.weights[:] = 1.0, 1.0
+    c.wg[:], c.wu[:], c.wd[:] = 0, 0, 0
+    c.wg[0, :, 0] = 32
+    c.sg[:], c.sd[:] = 1.0, 1.0
+    steps = np.arange(f) % 63 + 0.5               # act in units of the scale
+    steps[1::2] *= -1
+    steps[0] = 127.0                              # act's largest: the scale is 3 exactly
+    c.wu[0, :, 1] = 2 * steps
+    c.wu[0, 0, 1] = 127
+    c.su[:] = 3.0 / 64.0                          # 32 * 2 steps * 3 / 64 = 3 steps
+    c.su[0, 0] = 3.0 / 32.0
+    c.wd[0, np.arange(h), np.arange(f)] = 1       # output column i is code i's value
+    assert np.array_equal(c.run(env), np.tile(bf16(3.0 * np.rint(steps)), (m, 1)))
+
+
+@pytest.mark.parametrize("m", ROWS)
+def test_experts_act_is_held_in_f32(env, m):
+    """One act value to each group of 128 columns, gates from -60 to 20, less its 64-bit
+    value as the residual: what is left is act's error.  exp 1 unit and a rounding, a
+    reciprocal 1 unit, and eight products, quotients and sums of half a unit: 12 *
+    2^-24 of the value, below 2^-20."""
+    gates = np.array([-60, -55, -47, -38, -33, -27, -21, -16, -11, -7, -3, -1, 1, 4, 9, 20], np.float64)
+    h, f = 16, 16 * 128
+    c = Experts(m, 1, 1, h, f, residual=True, ids=np.zeros((m, 1), np.int32))
+    c.q[:], c.wg[:], c.wu[:], c.wd[:] = 0, 0, 0, 0
+    c.q[:, 0] = 1
+    c.asc[:], c.weights[:], c.sg[:], c.sd[:] = 1.0, 1.0, 1.0, 1.0
+    c.wg[0, ::128, 0], c.wu[0, ::128, 0] = gates, 1
+    silu = gates / (1.0 + np.exp(-gates))
+    c.su[0, ::128] = 2.0 ** -np.floor(np.log2(np.abs(silu)))   # act between 1 and 2
+    c.wd[0, np.arange(h), np.arange(h) * 128] = 1
+    act = silu * c.su[0, ::128].astype(np.float64)
+    c.residual[:] = -act
+    assert np.all(np.abs(c.run(env)) <= 2.0 ** -20 * np.abs(act))
