@@ -62,12 +62,65 @@ __global__ __launch_bounds__(256) void experts_act_slot(ExpertsArgs a, float* ac
   }
 }
 
+// Sixteen values of act (0 past inter), and their codes and the scale of their group
+// of 128, which eight lanes hold.
+__device__ __forceinline__ void load_act(const float* p, bool in, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  if (in) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const v4f t = *(const v4f*)(p + i);
+      v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+    }
+  }
+}
+__device__ __forceinline__ v4i code_act(const float (&v)[16], float& s) {
+  bool nan;
+  uint32_t m = absmax_bits(v, kFloorBits, &nan);
+  m = max(m, dpp_u32<0xB1>(m));
+  m = max(m, dpp_u32<0x4E>(m));
+  m = max(m, dpp_u32<0x141>(m));  // row_half_mirror: the eight lanes of a group
+  s = __uint_as_float(m) / 127.0f;
+  const float r = 1.0f / s;
+  v4i q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q[i] = (int)codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
+  return q;
+}
+
+// One column's weighted sum in the definition's order, a slot's whole sum before its
+// wsd and its weight: what experts_down_slot makes of parts that were not finite.
+__device__ __forceinline__ float down_in_order(const ExpertsArgs& a, const float* act, uint32_t row, uint32_t col,
+                                               int lane) {
+  float out = 0.f;
+  for (uint32_t j = 0; j < a.k; ++j) {
+    const uint32_t slot = row * a.k + j, e = (uint32_t)a.ids[slot];
+    if (e >= a.experts) continue;
+    const size_t n = (size_t)e * a.hidden + col;
+    float sum = 0.f;
+    for (uint32_t o0 = 0; o0 < a.inter; o0 += 1024) {
+      const uint32_t o = o0 + lane * 16;
+      const bool in = o < a.inter;
+      float v[16], s;
+      load_act(act + (size_t)slot * a.inter + o, in, v);
+      const v4i q = code_act(v, s);
+      sum += (float)dot16(load16(a.w_down + n * a.inter + (in ? o : 0)), q, 0) * s;
+    }
+    const float y = wave_sum_f32(sum) * a.ws_down[n];
+    out += a.weights[slot] * y;
+  }
+  return out;
+}
+
 // out[t, c] over the row's slots.  The workgroup's eight waves first make the codes
 // of eight slots' next 1024 columns of act, a wave a slot (16 values a lane, so
 // that eight lanes hold a group of 128), and share them through LDS; meanwhile
 // each wave's weights for its COLS columns are on their way.  A lane's 16 products
-// lie in one group, so its part of a sum is scaled before the lanes' parts are
-// added.  8 slots of hidden 4096, inner 1024 (33.5 MB): 9.4 us, 3.6 TB/s: ids, then
+// lie in one group, so its part of a sum is scaled, by s, weight and wsd, before the
+// lanes' parts are added.  Parts of both signs or of 0 make NaN of an infinite wsd or
+// weight: a column that is not finite is summed again, in order.  8 slots of hidden 4096, inner 1024 (33.5 MB): 9.4 us, 3.6 TB/s: ids, then
 // act and weights, codes, sums follow each other.  With the codes made by a launch
 // of their own 10.8 + 2.5 us; one column a wave 8.9-9.3.
 template <int COLS>
@@ -99,16 +152,7 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
       const uint32_t o = o0 + lane * 16;
       const bool in = o < a.inter;
       float v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
-      if (mine && in) {
-        const float* const p = act + (size_t)slot * a.inter + o;
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const v4f t = *(const v4f*)(p + i);
-          v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
-        }
-      }
+      load_act(act + (size_t)slot * a.inter + o, mine && in, v);
       v4i w[8][COLS];
       float ws[8][COLS];
 #pragma unroll
@@ -121,17 +165,8 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
           ws[j][c] = a.ws_down[n];
         }
       __builtin_amdgcn_sched_barrier(0);  // the weights are under way while the codes are made
-      bool nan;
-      uint32_t m = absmax_bits(v, kFloorBits, &nan);
-      m = max(m, dpp_u32<0xB1>(m));
-      m = max(m, dpp_u32<0x4E>(m));
-      m = max(m, dpp_u32<0x141>(m));  // row_half_mirror: the eight lanes of a group
-      const float s = __uint_as_float(m) / 127.0f, r = 1.0f / s;
-      v4i q;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        q[i] = (int)codes4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s, r, nan || s < kFastScaleMin);
-      code[wave][lane] = q;
+      float s;
+      code[wave][lane] = code_act(v, s);
       if ((lane & 7) == 0) scale[wave][lane >> 3] = s * weight;
       __syncthreads();
 #pragma unroll
@@ -148,7 +183,8 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
   float y = 0.f;
 #pragma unroll
   for (int c = 0; c < COLS; ++c) {
-    const float t = wave_sum_f32(total[c]);
+    float t = wave_sum_f32(total[c]);
+    if (!(__builtin_fabsf(t) < __builtin_inff())) t = down_in_order(a, act, row, col[c], lane);
     if (lane == c) y = t;
   }
   if (lane < COLS && c0 + lane < a.hidden) {

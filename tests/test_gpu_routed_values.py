@@ -82,3 +82,36 @@ def test_experts_act_is_held_in_f32(env, m):
     act = silu * c.su[0, ::128].astype(np.float64)
     c.residual[:] = -act
     assert np.all(np.abs(c.run(env)) <= 2.0 ** -20 * np.abs(act))
+
+
+@pytest.mark.parametrize("m", ROWS)
+def test_experts_infinite_column_scale(env, m):
+    """y = ws_down * a finite sum: an infinite scale of one column gives an infinity of
+    the sum's sign, in every form, and leaves the other columns alone."""
+    c = Experts(m, 2, 3, 192, 144, seed=m + 1, ids=np.tile([1, 2], (m, 1)))
+    want, err = c.want()
+    c.sd[1, 5] = 0.0                              # column 5 of expert 2 alone
+    w5, e5 = c.want()
+    c.sd[1, 5], c.sd[2, 5] = 1.0, INF
+    got = c.run(env)
+    sure = np.abs(w5[:, 5]) > e5[:, 5]
+    assert sure.mean() > 0.9
+    assert np.array_equal(got[sure, 5], np.where(w5[sure, 5] > 0, INF, -INF))
+    rest = np.arange(192) != 5
+    close_bf16(got[:, rest], want[:, rest], err[:, rest])
+
+
+@pytest.mark.parametrize("m", ROWS)
+def test_experts_infinite_weight(env, m):
+    """An infinite weight of one slot gives infinities of its product's signs."""
+    c = Experts(m, 2, 3, 192, 144, seed=m + 2, ids=np.tile([1, 2], (m, 1)))
+    want, err = c.want()
+    w = c.weights[0].copy()
+    c.weights[0] = 1.0, 0.0
+    one, bound = (v[0] for v in c.want())
+    c.weights[0] = INF, w[1]
+    got = c.run(env)
+    sure = np.abs(one) > bound
+    assert sure.mean() > 0.9
+    assert np.array_equal(got[0, sure], np.where(one[sure] > 0, INF, -INF))
+    close_bf16(got[1:], want[1:], err[1:])
