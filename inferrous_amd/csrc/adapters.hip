@@ -267,8 +267,7 @@ AdapterPlan adapter_plan(const AdapterArgs& a) {
     p.table = take((size_t)p.tiles * sizeof(RowTile));
     p.n_tiles = take(4);
     p.counts = take(blocks > 1 ? (size_t)blocks * (a.adapters + 1) * 4 : 0);
-    p.high = take((size_t)a.m * part_width(a.rank) * 2);
-    p.low = take((size_t)a.m * part_width(a.rank) * 2);
+    p.scaled = take((size_t)a.m * part_width(a.rank) * 4);
   }
   p.bytes = at;
   return p;

@@ -10,7 +10,7 @@ namespace w8a8 {
 
 static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Values of a row of h's BF16 parts: the ranks, padded to whole 32s.
+// Values of a row of scaling * h: the ranks, padded to whole 32s.
 __host__ __device__ constexpr uint32_t part_width(uint32_t rank) { return (rank + 31) / 32 * 32; }
 
 // How a call runs, a function of its sizes.
@@ -20,7 +20,7 @@ struct AdapterPlan {
   uint32_t tiles;   // tiles at most
   uint32_t splits;  // shares of K of the first product, each with partial sums of its own
   uint32_t stages;  // 128-byte stages of an adapter row in a share
-  size_t h, order, table, n_tiles, counts, high, low, bytes;  // workspace offsets
+  size_t h, order, table, n_tiles, counts, scaled, bytes;  // workspace offsets
 };
 AdapterPlan adapter_plan(const AdapterArgs& a);
 

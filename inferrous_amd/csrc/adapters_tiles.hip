@@ -6,11 +6,12 @@
 //
 //   adapters_order          the sort, and the tiles: up to bt rows of one adapter;
 //   adapters_shrink_tiles   h's partial sums, tile x share of K, by bf16 MFMA;
-//   adapters_parts          scaling * h as two BF16 parts, high and low, whose
-//                           products with B are exact: 16 bits count, not 8;
+//   adapters_scale          scaling * h, the shares of K added;
 //   adapters_gemm           the projection over the sorted rows, its int8 sums
 //                           scaled in their registers and the second product
-//                           added to them by bf16 MFMA before the one store.
+//                           added to them by bf16 MFMA before the one store: of
+//                           scaling * h as three BF16 parts, whose sum is the f32
+//                           value and whose products with B are exact.
 #include "adapters.hpp"
 
 namespace w8a8 {
@@ -72,10 +73,9 @@ __global__ __launch_bounds__(64 * T::NW) void adapters_shrink_tiles(AdapterArgs 
   }
 }
 
-// high + low = scaling * the sum of the shares, to 16 bits; rows padded with zeros
-// to a multiple of 32 values.
-__global__ __launch_bounds__(256) void adapters_parts(AdapterArgs a, const uint32_t* order, const float* h,
-                                                      uint32_t splits, uint16_t* high, uint16_t* low) {
+// scaling * the sum of the shares; rows padded with zeros to a multiple of 32 values.
+__global__ __launch_bounds__(256) void adapters_scale(AdapterArgs a, const uint32_t* order, const float* h,
+                                                      uint32_t splits, float* scaled) {
   const uint32_t quads = part_width(a.rank) / 4;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (size_t)a.m * quads) return;
@@ -87,10 +87,16 @@ __global__ __launch_bounds__(256) void adapters_parts(AdapterArgs a, const uint3
     for (uint32_t t = 0; t < splits; ++t) s += *(const v4f*)(h + ((size_t)t * a.m + p) * a.rank + j);
     s *= a.scaling[id];
   }
-  const uint32_t h0 = bf16_pair(s.x, s.y), h1 = bf16_pair(s.z, s.w);
-  *(v2i*)(high + i * 4) = v2i{(int)h0, (int)h1};
-  *(v2i*)(low + i * 4) = v2i{(int)bf16_pair(s.x - bf16_lo(h0), s.y - bf16_hi(h0)),
-                             (int)bf16_pair(s.z - bf16_lo(h1), s.w - bf16_hi(h1))};
+  *(v4f*)(scaled + i * 4) = s;
+}
+
+// Three parts of v, BF16 values in their high halves: each holds the next 8 of v's 24
+// bits, cut off, so that their sum is v.
+__device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
+  part[0] = __float_as_uint(v) & 0xffff0000u;
+  const float rest = v - __uint_as_float(part[0]);
+  part[1] = __float_as_uint(rest) & 0xffff0000u;
+  part[2] = __float_as_uint(rest - __uint_as_float(part[1]));
 }
 
 // M tiles of a strip: the tiles that an XCD runs at once share panels of both
@@ -98,21 +104,20 @@ __global__ __launch_bounds__(256) void adapters_parts(AdapterArgs a, const uint3
 constexpr uint32_t kStripTiles = 4;
 
 // After the K loop the rings' memory holds, 32 ranks at a time, the tile's B rows of
-// one adapter and its rows' two parts of h: one load from memory serves every
+// one adapter and its rows' three parts of h: one load from memory serves every
 // wave, and the next ranks (or adapter) are in flight while the waves multiply.
 // Rows of another adapter keep the value they had (a lane is one row).
 template <class T>
 __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, const uint32_t* order,
-                                                              const uint16_t* high, const uint16_t* low,
-                                                              uint32_t tiles_m, uint32_t tiles_n, bool wide) {
+                                                              const float* scaled, uint32_t tiles_m, uint32_t tiles_n, bool wide) {
   constexpr int PAIR = 40;          // BF16 values of an LDS row of 32, padded
   constexpr int STRIDE = 64 + 4;    // f32 values of an LDS row of 64 columns, padded
   constexpr int THREADS = 64 * T::NW;
-  constexpr int B_AT = 0, H_AT = T::BN * PAIR * 2, L_AT = H_AT + T::BT * PAIR * 2, W_AT = L_AT + T::BT * PAIR * 2;
+  constexpr int B_AT = 0, H_AT = T::BN * PAIR * 2, H_SIZE = T::BT * PAIR * 2, W_AT = H_AT + 3 * H_SIZE;
   constexpr int O_AT = W_AT + T::BN * 4;
   static_assert(O_AT + T::NW * 32 * STRIDE * 4 <= T::LDS, "the epilogue reuses the rings");
   static_assert(T::WN % 64 == 0 && T::BN * 4 % THREADS == 0 && T::BT * 4 % THREADS == 0, "whole loads");
-  constexpr int LB = T::BN * 4 / THREADS, LH = T::BT * 4 / THREADS;  // 16-byte loads of a thread
+  constexpr int LB = T::BN * 4 / THREADS, LH = T::BT * 8 / THREADS;  // 16-byte loads of a thread
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
   const uint32_t G = tiles_m * tiles_n;
   uint32_t at = blockIdx.x;
@@ -177,7 +182,8 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
     for (int i = 0; i < T::BT / 64; ++i) c += (uint32_t)__popcll(__ballot(tid[i] == ad));
     return c;
   };
-  v4i rb[LB], rh[LH], rl[LH];
+  v4i rb[LB];
+  v4f rh[LH];
   auto fetch = [&](uint32_t ad, uint32_t k) {
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
@@ -186,10 +192,8 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
     }
 #pragma unroll
     for (int i = 0; i < LH; ++i) {
-      const uint32_t t = threadIdx.x + i * THREADS, r = t >> 2;
-      const size_t o = (size_t)(m0 + (r < rows_in ? r : 0)) * padded + k + (t & 3) * 8;
-      rh[i] = *(const v4i*)(high + o);
-      rl[i] = *(const v4i*)(low + o);
+      const uint32_t t = threadIdx.x + i * THREADS, r = t >> 3;
+      rh[i] = *(const v4f*)(scaled + (size_t)(m0 + (r < rows_in ? r : 0)) * padded + k + (t & 7) * 4);
     }
   };
   uint32_t r0 = 0, ad = at_row(0);
@@ -206,8 +210,14 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
 #pragma unroll
       for (int i = 0; i < LH; ++i) {
         const uint32_t t = threadIdx.x + i * THREADS;
-        *(v4i*)(lds + H_AT + (t >> 2) * PAIR * 2 + (t & 3) * 16) = rh[i];
-        *(v4i*)(lds + L_AT + (t >> 2) * PAIR * 2 + (t & 3) * 16) = rl[i];
+        uint32_t q[4][3];
+#pragma unroll
+        for (int l = 0; l < 4; ++l) split3(rh[i][l], q[l]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          *(v2i*)(lds + H_AT + p * H_SIZE + (t >> 3) * PAIR * 2 + (t & 7) * 8) =
+              v2i{(int)__builtin_amdgcn_perm(q[1][p], q[0][p], 0x07060302u),
+                  (int)__builtin_amdgcn_perm(q[3][p], q[2][p], 0x07060302u)};
       }
       __syncthreads();
       if (k + 32 < a.rank) fetch(ad, k + 32);
@@ -216,21 +226,20 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
       for (int f = 0; f < T::FT; ++f) {
         const bool on = id[f] == ad;
         if (!__ballot(on)) continue;
-        v4i hi[2], lo[2];
+        v4i hp[3][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int o = (wt + 32 * f + tl) * PAIR * 2 + 32 * i + 16 * half;
-          hi[i] = *(const v4i*)(lds + H_AT + o);
-          lo[i] = *(const v4i*)(lds + L_AT + o);
-        }
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            hp[p][i] = *(const v4i*)(lds + H_AT + p * H_SIZE + (wt + 32 * f + tl) * PAIR * 2 + 32 * i + 16 * half);
 #pragma unroll
         for (int j = 0; j < T::FN; ++j) {
           v16f d = y[f][j];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const v4i b = *(const v4i*)(lds + B_AT + (wn + 32 * j + tl) * PAIR * 2 + 32 * i + 16 * half);
-            d = mfma_bf16(b, hi[i], d);
-            d = mfma_bf16(b, lo[i], d);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) d = mfma_bf16(b, hp[p][i], d);
           }
 #pragma unroll
           for (int v = 0; v < 16; ++v) y[f][j][v] = on ? d[v] : y[f][j][v];
@@ -311,7 +320,7 @@ void gemm_as(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* w
   auto go = [&](auto tile) {
     using T = decltype(tile);
     hipLaunchKernelGGL(adapters_gemm<T>, dim3(tm * tn), dim3(64 * T::NW), 0, st, a, (const uint32_t*)(ws + p.order),
-                       (const uint16_t*)(ws + p.high), (const uint16_t*)(ws + p.low), tm, tn, wide);
+                       (const float*)(ws + p.scaled), tm, tn, wide);
   };
   if (a.width % 128 == 0) go(TileStream<BT, BN, WT, WN, SA, SB, false, false>{});
   else go(TileStream<BT, BN, WT, WN, SA, SB, false, true>{});
@@ -339,9 +348,8 @@ hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const Ada
     else shrink_as<128, 256, 64, 64, 2, 2>(st, a, p, ws);
   }
   const size_t quads = (size_t)a.m * (part_width(a.rank) / 4);
-  hipLaunchKernelGGL(adapters_parts, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, a,
-                     (const uint32_t*)(ws + p.order), (const float*)(ws + p.h), p.splits, (uint16_t*)(ws + p.high),
-                     (uint16_t*)(ws + p.low));
+  hipLaunchKernelGGL(adapters_scale, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, a,
+                     (const uint32_t*)(ws + p.order), (const float*)(ws + p.h), p.splits, (float*)(ws + p.scaled));
   const uint64_t big = (uint64_t)((a.m + 255) / 256) * ((a.n + 255) / 256);
   if (big >= 192) gemm_as<256, 256, 64, 128, 2, 3>(st, a, p, ws);
   else gemm_as<128, 128, 64, 64, 2, 3>(st, a, p, ws);

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, load
-from test_gpu_routed import Experts, bf16, close_bf16
+from test_gpu_routed import Adapters, Experts, bf16, close_bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,31 @@ def test_experts_infinite_weight(env, m):
     assert sure.mean() > 0.9
     assert np.array_equal(got[0, sure], np.where(one[sure] > 0, INF, -INF))
     close_bf16(got[1:], want[1:], err[1:])
+
+
+# ------------------------------------------------------------------ adapters
+# rows, columns, width, rank, adapters: row by row (one kernel, and two), with the rows sorted
+# by adapter and tiles of 128 and of 256.
+ADAPTED = [(1, 40, 64, 8, 2), (4, 40, 64, 8, 2), (30, 130, 272, 16, 3), (900, 512, 512, 256, 3),
+           (4096, 3088, 144, 16, 4)]
+
+
+def bare(m, n, k, rank, count):
+    """Rows of adapter r % count whose projection is 0 and whose h is x[0] alone."""
+    c = Adapters(m, n, k, rank, count, ids=np.arange(m) % count)
+    c.x[:], c.w[:], c.a[:], c.b[:], c.scaling[:] = 0, 0, 0, 0, 1.0
+    c.q[:] = 0
+    c.x[:, 0], c.a[:, :, 0] = 1.0, 1.0
+    return c
+
+
+@pytest.mark.parametrize("m, n, k, rank, count", ADAPTED)
+def test_adapters_keep_every_bit_of_h(env, m, n, k, rank, count):
+    """h[i] = 1 + 2^-9 + 2^-e less h[7] = 1 + 2^-9: what is left is h's last bits."""
+    e = np.array([12, 15, 18, 20, 23])
+    c = bare(m, n, k, rank, count)
+    c.x[:, 1:3] = 1.0
+    c.a[:, :, 1], c.a[:, :5, 2] = 2.0 ** -9, 2.0 ** -e.astype(F32)
+    i = np.arange(n) % 5
+    c.b[:, np.arange(n), i], c.b[:, :, 7] = 1.0, -1.0
+    assert np.array_equal(c.run(env), np.tile(2.0 ** -e[i].astype(F32), (m, 1)))
