@@ -73,7 +73,9 @@ __global__ __launch_bounds__(64 * T::NW) void adapters_shrink_tiles(AdapterArgs 
   }
 }
 
-// scaling * the sum of the shares; rows padded with zeros to a multiple of 32 values.
+// scaling * the sum of the shares, without an infinite scaling (adapters_gemm); rows
+// padded with zeros to a multiple of 32 values.
+__device__ __forceinline__ bool infinite(float v) { return __builtin_fabsf(v) == __builtin_inff(); }
 __global__ __launch_bounds__(256) void adapters_scale(AdapterArgs a, const uint32_t* order, const float* h,
                                                       uint32_t splits, float* scaled) {
   const uint32_t quads = part_width(a.rank) / 4;
@@ -85,18 +87,25 @@ __global__ __launch_bounds__(256) void adapters_scale(AdapterArgs a, const uint3
   if (j < a.rank && id < a.adapters) {
 #pragma unroll 4
     for (uint32_t t = 0; t < splits; ++t) s += *(const v4f*)(h + ((size_t)t * a.m + p) * a.rank + j);
-    s *= a.scaling[id];
+    const float scaling = a.scaling[id];
+    if (!infinite(scaling)) s *= scaling;
   }
   *(v4f*)(scaled + i * 4) = s;
 }
 
 // Three parts of v, BF16 values in their high halves: each holds the next 8 of v's 24
-// bits, cut off, so that their sum is v.
+// bits, cut off, so that their sum is v.  An infinite B times a part of 0 would be NaN:
+// such a part is 2^-48 v, far below f32's last bit of the products' sum.  Every part of
+// an infinity or NaN is v.
 __device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
+  const float least = v * 0x1p-48f;
   part[0] = __float_as_uint(v) & 0xffff0000u;
-  const float rest = v - __uint_as_float(part[0]);
+  float rest = v - __uint_as_float(part[0]);
+  rest = rest != 0.f ? rest : least;
   part[1] = __float_as_uint(rest) & 0xffff0000u;
-  part[2] = __float_as_uint(rest - __uint_as_float(part[1]));
+  rest -= __uint_as_float(part[1]);
+  part[2] = __float_as_uint(rest != 0.f ? rest : least);
+  if (!(__builtin_fabsf(v) < __builtin_inff())) part[0] = part[1] = part[2] = v != v ? 0x7fc00000u : __float_as_uint(v);
 }
 
 // M tiles of a strip: the tiles that an XCD runs at once share panels of both
@@ -137,13 +146,14 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
   const uint32_t padded = part_width(a.rank), rows_in = min((uint32_t)T::BT, a.m - m0);
   // the wave's rows
   uint32_t row[T::FT], id[T::FT];
-  float asc[T::FT];
+  float asc[T::FT], scaling[T::FT];
 #pragma unroll
   for (int f = 0; f < T::FT; ++f) {
     const uint32_t r = wt + 32 * f + tl;
     row[f] = order[m0 + (r < rows_in ? r : 0)];
     id[f] = r < rows_in ? (uint32_t)a.ids[row[f]] : ~0u;
     asc[f] = a.asc[row[f]];
+    scaling[f] = id[f] < a.adapters ? a.scaling[id[f]] : 0.f;
   }
   // the tile's ids, every wave alike: lane l's are rows l, l + 64, ...
   uint32_t tid[T::BT / 64];
@@ -167,6 +177,24 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[f][j][4 * q + i] = (float)s.acc[f][j][4 * q + i] * asc[f] * w[i];
     }
+  // An infinite scaling multiplies the row's whole second product, as in the definition:
+  // its row starts from 0 here (NaN where the projection is not finite).
+  bool odd[T::FT], any_odd = false;
+#pragma unroll
+  for (int f = 0; f < T::FT; ++f) {
+    odd[f] = infinite(scaling[f]);
+    any_odd |= odd[f];
+  }
+  any_odd = __any(any_odd);
+  auto times = [&](auto factor) {
+#pragma unroll
+    for (int f = 0; f < T::FT; ++f)
+#pragma unroll
+      for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) y[f][j][v] = odd[f] ? y[f][j][v] * factor(f) : y[f][j][v];
+  };
+  if (any_odd) times([](int) { return 0.f; });
   // Rows are sorted by adapter, those without one last: the tile's adapters follow
   // each other, each from the row after the last one's.
   auto at_row = [&](uint32_t r) {  // the id of tile row r, wave-uniform
@@ -249,6 +277,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, co
     r0 = r1;
     ad = next;
   }
+  if (any_odd) times([&](int f) { return scaling[f]; });
   // 32 rows x 64 columns at a time through the wave's own LDS: whole runs of a row
   // to memory
   float* const mine = (float*)(lds + O_AT) + wave * 32 * STRIDE;

@@ -143,3 +143,39 @@ def test_adapters_keep_every_bit_of_h(env, m, n, k, rank, count):
     i = np.arange(n) % 5
     c.b[:, np.arange(n), i], c.b[:, :, 7] = 1.0, -1.0
     assert np.array_equal(c.run(env), np.tile(2.0 ** -e[i].astype(F32), (m, 1)))
+
+
+@pytest.mark.parametrize("m, n, k, rank, count", ADAPTED)
+@pytest.mark.parametrize("what", ["x", "a", "b", "scaling", "largest"])
+def test_adapters_infinities(env, m, n, k, rank, count, what):
+    """An infinity of x, A, B or the scaling gives infinities of the products' signs in
+    its rows, and h may be the largest f32; the other rows keep their values."""
+    c = bare(m, n, k, rank, count)
+    sign = np.where(np.arange(n) % 3 == 1, -1.0, 1.0).astype(F32)
+    c.b[:] = sign[None, :, None]
+    mine = np.arange(m) == 0 if what in ("x", "largest") else c.ids == 0
+    want = np.where(mine[:, None], INF, float(rank)) * sign
+    if what == "x":
+        c.x[0, 0] = INF
+    elif what == "a":
+        c.a[0, 3, 0] = INF
+    elif what == "b":
+        c.b[0, 7, 5] = INF
+        want = np.tile(rank * sign, (m, 1))
+        want[mine, 7] = INF
+    elif what == "scaling":
+        c.scaling[0] = -INF
+        want[mine] = -want[mine]
+    else:  # less than 2^128, but no BF16 value between
+        c.x[0, :3] = 255 * 2.0 ** 120, 2.0 ** 119, 255 * 2.0 ** 110
+        c.x[1:, 1:3] = 0.0
+        c.a[:, :, :3] = 0.0
+        c.a[:, 2, :3] = 1.0
+        c.b[:, :, :] = (sign * 2.0 ** -100)[None, :, None]
+        want = np.zeros((m, n))
+        want[0] = (255 * 2.0 ** 20 + 2.0 ** 19 + 255 * 2.0 ** 10) * sign
+        want[1:] = 2.0 ** -100 * sign
+        want = bf16(want)
+    with np.errstate(invalid="ignore"):
+        got = c.run(env)
+    assert np.array_equal(got, want.astype(F32))
