@@ -324,7 +324,10 @@ int w8a8_malloc(void** ptr, size_t bytes) {
   if (bytes == 0) bytes = 16;
   void* p = nullptr;
   hipError_t e = hipMalloc(&p, bytes);
-  if (e != hipSuccess) return hip_status(e);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();  // returned here: no later launch's
+    return hip_status(e);
+  }
   e = hipMemset(p, 0, bytes);
   if (e == hipSuccess) e = hipDeviceSynchronize();
   if (e != hipSuccess) {

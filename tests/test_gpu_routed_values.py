@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from inferrous_amd import CudaContext, load
+from inferrous_amd import CudaContext, DeviceBuffer, W8A8Error, load
 from test_gpu_routed import Adapters, Experts, bf16, close_bf16
 
 pytestmark = pytest.mark.gpu
@@ -179,3 +179,12 @@ def test_adapters_infinities(env, m, n, k, rank, count, what):
     with np.errstate(invalid="ignore"):
         got = c.run(env)
     assert np.array_equal(got, want.astype(F32))
+
+
+# ------------------------------------------------------------------ workspaces
+def test_a_refused_allocation_is_no_later_calls_error(env):
+    """An allocation that cannot be had raises, and the launch after it does not report
+    its error once more."""
+    with pytest.raises(W8A8Error):
+        DeviceBuffer(1 << 50, np.uint8)
+    Experts(3, 2, 4, 64, 48).check(env)
