@@ -79,7 +79,7 @@ class LoadedModule:
     workspaces are kept per stream (calls sharing one workspace must not
     overlap, and ops on different streams may), and an outgrown workspace is
     kept alive, not freed, because a graph captured earlier holds its
-    address.  While a stream is being captured no workspace is allocated."""
+    address (its successor is twice as large, so they stay few).  While a stream is being captured no workspace is allocated."""
 
     # lm_head of the Qwen3 family: selection workspace sized for it up front
     _SELECT_ROWS = 151936
@@ -180,16 +180,27 @@ class LoadedModule:
 
     # ------------------------------------------------------------ projections
     def reserve_workspace(self, nbytes: int, stream: CudaStream | None = None) -> None:
-        """Make ``stream``'s split-K workspace at least nbytes (call before
-        capturing a graph of large prefill projections)."""
+        """Make ``stream``'s workspace (split-K slabs, the routed layers' scratch
+        space) at least nbytes; call it before capturing a graph of ops that
+        use one.  The first workspace is nbytes; one that is outgrown is
+        followed by twice its size or nbytes, whichever is more, so that what
+        is kept for graphs captured earlier stays below the workspace in use."""
         cur = self._gemm_ws.get(_key(stream))
-        if cur is None or cur.nbytes < nbytes:
-            if is_capturing(stream):
-                raise W8A8Error(_lib.EWORKSPACE, "split-K workspace cannot grow while the stream is captured; "
-                                "call reserve_workspace before capturing")
-            if cur is not None:
-                self._retired.append(cur)
-            self._gemm_ws[_key(stream)] = DeviceBuffer((nbytes + 15) // 16 * 16, np.uint8)
+        if cur is not None and cur.nbytes >= nbytes:
+            return
+        if is_capturing(stream):
+            raise W8A8Error(_lib.EWORKSPACE, "the workspace cannot grow while the stream is captured; "
+                            "call reserve_workspace before capturing")
+        need = (nbytes + 15) // 16 * 16
+        if cur is None:
+            self._gemm_ws[_key(stream)] = DeviceBuffer(need, np.uint8)
+            return
+        try:
+            grown = DeviceBuffer(max(need, 2 * cur.nbytes), np.uint8)
+        except W8A8Error:   # no memory for twice the size: the need alone
+            grown = DeviceBuffer(need, np.uint8)
+        self._retired.append(cur)
+        self._gemm_ws[_key(stream)] = grown
 
     def _workspace_for(self, stream, m: int, n: int, k: int, path: int, split: bool = False):
         if path == _lib.PATH_MFMA and m > 4 and not split:
