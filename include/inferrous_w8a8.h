@@ -530,10 +530,17 @@ int w8a8_route_experts(void *stream, const void *logits, int logits_dtype,
  * q, the weights, residual and out 16-byte aligned; m * top_k <= 2^24.  The workspace
  * (256-byte aligned, at least w8a8_experts_mlp_workspace_bytes) is written
  * before it is read; calls sharing one must not overlap.  out must not
- * overlap an input. */
+ * overlap an input.
+ * The need is not monotone in m (the form depends on it): a buffer shared by
+ * every batch size up to max_m, or held by graphs of several, is sized with
+ * w8a8_experts_mlp_workspace_bytes_upto, the largest need over m = 1 ..
+ * max_m. */
 size_t w8a8_experts_mlp_workspace_bytes(size_t m, uint32_t top_k,
                                         uint32_t n_experts, uint32_t hidden,
                                         uint32_t inter);
+size_t w8a8_experts_mlp_workspace_bytes_upto(size_t max_m, uint32_t top_k,
+                                             uint32_t n_experts,
+                                             uint32_t hidden, uint32_t inter);
 int w8a8_experts_mlp(void *stream, const int8_t *q, const float *asc, size_t m,
                      uint32_t hidden, const int32_t *ids, const float *weights,
                      uint32_t top_k, uint32_t n_experts, const int8_t *w_gate,
@@ -553,10 +560,14 @@ int w8a8_experts_mlp(void *stream, const int8_t *q, const float *asc, size_t m,
  * Products and sums are held in f32, the projection's in exact i32.  rank: a
  * multiple of 8 up to 256 (pad a smaller one with zeros); n_adapters <= 1023; m
  * <= 2^21, n <= 2^22; x, a, b 16-byte aligned; q, w, k as for w8a8_linear.
- * Workspace as for w8a8_experts_mlp.
+ * Workspace as for w8a8_experts_mlp, its need not monotone in m either: 4096 x
+ * 4096, rank 16, 4 adapters needs 10 MB at 128 rows and less than 1 MB at 1024.
  * out must not overlap an input. */
 size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k,
                                             uint32_t rank, uint32_t n_adapters);
+size_t w8a8_linear_adapters_workspace_bytes_upto(size_t max_m, size_t n,
+                                                 uint32_t k, uint32_t rank,
+                                                 uint32_t n_adapters);
 int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
                          size_t m, const int8_t *w, const float *ws, size_t n,
                          uint32_t k, const void *x, int x_dtype,

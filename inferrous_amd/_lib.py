@@ -98,8 +98,10 @@ SIGNATURES: dict[str, tuple] = {
     "w8a8_linear_sequence_reset": (I, []),
     "w8a8_route_experts": (I, [P, P, I, S, U32, I, P, U32, U32, U32, U32, I, F, P, P]),
     "w8a8_experts_mlp_workspace_bytes": (S, [S, U32, U32, U32, U32]),
+    "w8a8_experts_mlp_workspace_bytes_upto": (S, [S, U32, U32, U32, U32]),
     "w8a8_experts_mlp": (I, [P, P, P, S, U32, P, P, U32, U32, P, P, P, P, P, P, U32, P, P, I, P, S]),
     "w8a8_linear_adapters_workspace_bytes": (S, [S, S, U32, U32, U32]),
+    "w8a8_linear_adapters_workspace_bytes_upto": (S, [S, S, U32, U32, U32]),
     "w8a8_linear_adapters": (I, [P, P, P, S, P, P, S, U32, P, I, P, P, P, P, U32, U32, P, P, I, P, S]),
     "w8a8_synth_i8": (I, [P, P, S, U64, U64]),
     "w8a8_synth_f32": (I, [P, P, S, U64, U64, F, F]),

@@ -1401,6 +1401,16 @@ size_t w8a8_experts_mlp_workspace_bytes(size_t m, uint32_t top_k, uint32_t n_exp
   return experts_workspace_bytes((uint32_t)m, top_k, n_experts, hidden, inter);
 }
 
+// Every m: tile heights, the sort's workgroups and the tables they size change with it.
+size_t w8a8_experts_mlp_workspace_bytes_upto(size_t max_m, uint32_t top_k, uint32_t n_experts, uint32_t hidden,
+                                             uint32_t inter) {
+  size_t most = 0;
+  max_m = std::min<size_t>(max_m, kMaxExpertSlots);
+  for (size_t m = 1; m <= max_m; ++m)
+    most = std::max(most, w8a8_experts_mlp_workspace_bytes(m, top_k, n_experts, hidden, inter));
+  return most;
+}
+
 int w8a8_experts_mlp(void* stream, const int8_t* q, const float* asc, size_t m, uint32_t hidden, const int32_t* ids,
                      const float* weights, uint32_t top_k, uint32_t n_experts, const int8_t* w_gate,
                      const float* ws_gate, const int8_t* w_up, const float* ws_up, const int8_t* w_down,
@@ -1462,6 +1472,15 @@ size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k, uint
   const size_t part = up256(adapters_workspace_bytes(a));
   return adapters_fused(a) ? part
                            : part + up256(m * n * 4) + w8a8_linear_workspace_bytes_path(m, n, k, W8A8_PATH_AUTO);
+}
+
+size_t w8a8_linear_adapters_workspace_bytes_upto(size_t max_m, size_t n, uint32_t k, uint32_t rank,
+                                                 uint32_t n_adapters) {
+  size_t most = 0;
+  max_m = std::min<size_t>(max_m, kMaxAdapterRows);
+  for (size_t m = 1; m <= max_m; ++m)
+    most = std::max(most, w8a8_linear_adapters_workspace_bytes(m, n, k, rank, n_adapters));
+  return most;
 }
 
 int w8a8_linear_adapters(void* stream, const int8_t* q, const float* asc, size_t m, const int8_t* w, const float* ws,

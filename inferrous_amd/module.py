@@ -695,6 +695,16 @@ class LoadedModule:
             cur = self._gemm_ws[key]
         return cur.ptr, cur.nbytes
 
+    @staticmethod
+    def experts_mlp_workspace_bytes(max_rows: int, top_k: int, n_experts: int, width: int, inter: int) -> int:
+        """What ``reserve_workspace`` needs for ``experts_mlp`` of up to max_rows rows."""
+        return lib().w8a8_experts_mlp_workspace_bytes_upto(max_rows, top_k, n_experts, width, inter)
+
+    @staticmethod
+    def linear_adapters_workspace_bytes(max_rows: int, n: int, width: int, rank: int, adapters: int) -> int:
+        """What ``reserve_workspace`` needs for ``linear_adapters`` of up to max_rows rows."""
+        return lib().w8a8_linear_adapters_workspace_bytes_upto(max_rows, n, width, rank, adapters)
+
     def route_experts(self, stream, logits: DeviceBuffer, n_experts: int, ids: DeviceBuffer,
                       weights: DeviceBuffer, score: str = "softmax", bias: DeviceBuffer | None = None,
                       groups: int = 1, top_groups: int = 1, group_top: int = 1, renorm: bool = True,
@@ -740,7 +750,8 @@ class LoadedModule:
         [n_experts, width, I], float32 [n_experts, width]), into ``out``
         (float32 or uint16 BF16, [M, width]), with ``residual`` (float32)
         added.  The scratch space is the stream's workspace;
-        ``reserve_workspace`` it before capturing a graph."""
+        ``reserve_workspace(experts_mlp_workspace_bytes(...))`` before
+        capturing a graph."""
         m, width, n_experts, slots, columns = len(asc), int(width), int(n_experts), len(ids), len(s0)
         inter = columns // n_experts if n_experts > 0 else 0
         size, rows = columns * width, m * width
@@ -780,8 +791,9 @@ class LoadedModule:
         (uint16 BF16 [adapters, rank, width]), ``b`` (uint16 BF16 [adapters,
         N, rank]) and ``scaling`` (float32 [adapters]); ``residual``
         (float32) is added before the one rounding.  The scratch space is the
-        stream's workspace; ``reserve_workspace`` it before capturing a
-        graph."""
+        stream's workspace;
+        ``reserve_workspace(linear_adapters_workspace_bytes(...))`` before
+        capturing a graph."""
         m, n, k, count = len(asc), len(ws), int(width), len(scaling)
         rank = len(a) // (count * k) if count and k > 0 else 0
         dtype = x.dtype

@@ -50,3 +50,30 @@ def test_growth_without_the_memory_for_it_takes_the_need(mod, monkeypatch):
     monkeypatch.setattr(module, "DeviceBuffer", Full)
     mod.reserve_workspace(1700)
     assert mod._gemm_ws[None].nbytes == 1712
+
+
+SHAPES = [("experts_mlp", (8, 64, 4096, 1024)), ("experts_mlp", (2, 8, 512, 4096)), ("experts_mlp", (1, 1024, 16, 16)),
+          ("linear_adapters", (4096, 4096, 16, 4)), ("linear_adapters", (6144, 4096, 32, 40)),
+          ("linear_adapters", (4096, 12288, 64, 6))]
+
+
+@pytest.mark.parametrize("op, shape", SHAPES)
+def test_one_workspace_serves_every_batch_up_to_its_rows(mod, op, shape):
+    """Sized for the largest batch, no smaller one asks for more: the need is not
+    monotone in the rows."""
+    rows = 2000 if shape[0] < 16 else 1100
+    size = getattr(_lib.lib(), f"w8a8_{op}_workspace_bytes")
+    needs = [size(m, *shape) for m in range(1, rows + 1)]
+    most = getattr(LoadedModule, f"{op}_workspace_bytes")(rows, *shape)
+    assert most == max(needs) > 0
+    mod.reserve_workspace(most)
+    for m in range(1, rows + 1):
+        mod._routed_workspace(None, f"w8a8_{op}_workspace_bytes", m, *shape)
+    assert not mod._retired
+
+
+def test_sizes_for_no_rows_and_refused_shapes():
+    assert LoadedModule.experts_mlp_workspace_bytes(0, 8, 64, 4096, 1024) == 0
+    assert LoadedModule.experts_mlp_workspace_bytes(4, 8, 64, 4096, 1000) == 0
+    assert LoadedModule.linear_adapters_workspace_bytes(0, 4096, 4096, 16, 4) == 0
+    assert LoadedModule.linear_adapters_workspace_bytes(8, 4096, 4096, 12, 4) == 0
