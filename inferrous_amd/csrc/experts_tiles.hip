@@ -268,43 +268,47 @@ __global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, Exp
 }
 
 // ------------------------------------------------------------------ sum
+constexpr uint32_t kCombineRows = 1u << 22;  // workgroups: their threads stay below 2^32
+
 // out[t, c .. c + 3] a thread, slots in order: the sum's order is fixed.  Eight
 // slots' rows are under way together; their positions and weights, one row's,
 // are wave-uniform.
 __global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int32_t* __restrict__ pos,
                                                        const float* __restrict__ y) {
-  const uint32_t row = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= a.hidden) return;
-  v4f sum{};
-  for (uint32_t j0 = 0; j0 < a.k; j0 += 8) {
-    v4f v[8];
-    int32_t p[8];
+  for (uint32_t row = blockIdx.x; row < a.m; row += gridDim.x) {
+    v4f sum{};
+    for (uint32_t j0 = 0; j0 < a.k; j0 += 8) {
+      v4f v[8];
+      int32_t p[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = pos[(size_t)row * a.k + min(j0 + j, a.k - 1)];
+      for (int j = 0; j < 8; ++j) p[j] = pos[(size_t)row * a.k + min(j0 + j, a.k - 1)];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)  // a slot without an expert reads a row that it does not use
-      v[j] = *(const v4f*)(y + (size_t)max(p[j], 0) * a.hidden + c);
+      for (int j = 0; j < 8; ++j)  // a slot without an expert reads a row that it does not use
+        v[j] = *(const v4f*)(y + (size_t)max(p[j], 0) * a.hidden + c);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j0 + j >= a.k || p[j] < 0) continue;
-      const float w = a.weights[(size_t)row * a.k + j0 + j];
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j >= a.k || p[j] < 0) continue;
+        const float w = a.weights[(size_t)row * a.k + j0 + j];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(w, v[j][i], sum[i]);
+        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(w, v[j][i], sum[i]);
+      }
     }
-  }
-  const size_t o = (size_t)row * a.hidden + c;
-  if (a.residual) {
-    const v4f r = *(const v4f*)(a.residual + o);
+    const size_t o = (size_t)row * a.hidden + c;
+    if (a.residual) {
+      const v4f r = *(const v4f*)(a.residual + o);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = r[i] + sum[i];
-  }
+      for (int i = 0; i < 4; ++i) sum[i] = r[i] + sum[i];
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum[i] = bf16_rne(sum[i]);
-  if (a.out_dtype == W8A8_OUT_F32) {
-    *(v4f*)((float*)a.out + o) = sum;
-  } else {
-    *(v2i*)((uint16_t*)a.out + o) = v2i{(int)((__float_as_uint(sum[0]) >> 16) | (__float_as_uint(sum[1]) & 0xffff0000u)),
-                                        (int)((__float_as_uint(sum[2]) >> 16) | (__float_as_uint(sum[3]) & 0xffff0000u))};
+    for (int i = 0; i < 4; ++i) sum[i] = bf16_rne(sum[i]);
+    if (a.out_dtype == W8A8_OUT_F32) {
+      *(v4f*)((float*)a.out + o) = sum;
+    } else {
+      *(v2i*)((uint16_t*)a.out + o) = v2i{(int)((__float_as_uint(sum[0]) >> 16) | (__float_as_uint(sum[1]) & 0xffff0000u)),
+                                          (int)((__float_as_uint(sum[2]) >> 16) | (__float_as_uint(sum[3]) & 0xffff0000u))};
+    }
   }
 }
 
@@ -433,7 +437,8 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
   else gate_up<true>(st, a, plan, bt, tiles, codes, scales);
   if (a.inter % 128 == 0) down<false>(st, a, plan, bt, tiles, codes, scales, y);
   else down<true>(st, a, plan, bt, tiles, codes, scales, y);
-  hipLaunchKernelGGL(experts_combine, dim3(a.m, (a.hidden + 1023) / 1024), dim3(256), 0, st, a, plan.pos, y);
+  hipLaunchKernelGGL(experts_combine, dim3(std::min(a.m, kCombineRows), (a.hidden + 1023) / 1024), dim3(256), 0, st, a,
+                     plan.pos, y);
   return hipGetLastError();
 }
 

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, DeviceBuffer, W8A8Error, load
-from test_gpu_routed import Adapters, Experts, bf16, close_bf16
+from test_gpu_routed import Adapters, Experts, bf16, close_bf16, from_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +188,22 @@ def test_a_refused_allocation_is_no_later_calls_error(env):
     with pytest.raises(W8A8Error):
         DeviceBuffer(1 << 50, np.uint8)
     Experts(3, 2, 4, 64, 48).check(env)
+
+
+# ------------------------------------------------------------------ limits
+def test_experts_at_the_most_slots(env):
+    """2^24 rows of one slot, the documented limit: a period of rows again and again,
+    each with the outputs of its first."""
+    mod, s, _ = env
+    m, period, h, f, e = 1 << 24, 1 << 12, 16, 16, 5
+    c = Experts(period, 1, e, h, f, seed=7)
+    c.ids = np.random.default_rng(8).integers(-1, e, (period, 1)).astype(np.int32)
+    want, err = c.want()
+    rows = [np.tile(a, (m // period,) + (1,) * (a.ndim - 1)) for a in (c.q, c.asc, c.ids, c.weights)]
+    q, asc, ids, weights = (DeviceBuffer.from_host(s, a) for a in rows)
+    mats = [DeviceBuffer.from_host(s, a) for a in (c.wg, c.sg, c.wu, c.su, c.wd, c.sd)]
+    out = DeviceBuffer(m * h, np.uint16)
+    mod.experts_mlp(s, q, asc, h, ids, weights, *mats, e, out)
+    got = out.to_host_vec(s).reshape(-1, period * h)
+    close_bf16(from_bits(got[0]).reshape(period, h), want, err)
+    assert (got == got[0]).all()
