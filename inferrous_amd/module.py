@@ -687,6 +687,8 @@ class LoadedModule:
         once."""
         nbytes = self._routed_bytes.get((size_of, shape))
         if nbytes is None:
+            if len(self._routed_bytes) >= 4096:   # batches of any number of rows
+                self._routed_bytes.clear()
             nbytes = self._routed_bytes[(size_of, shape)] = getattr(lib(), size_of)(*shape)
         key = stream.handle if stream is not None else None
         cur = self._gemm_ws.get(key)

@@ -77,3 +77,11 @@ def test_sizes_for_no_rows_and_refused_shapes():
     assert LoadedModule.experts_mlp_workspace_bytes(4, 8, 64, 4096, 1000) == 0
     assert LoadedModule.linear_adapters_workspace_bytes(0, 4096, 4096, 16, 4) == 0
     assert LoadedModule.linear_adapters_workspace_bytes(8, 4096, 4096, 12, 4) == 0
+
+
+def test_sizes_kept_by_shape_stay_bounded(mod):
+    """A server's batches have any number of rows: the sizes kept do not grow with them."""
+    for m in range(1, 6000):
+        ptr, nbytes = mod._routed_workspace(None, "w8a8_linear_adapters_workspace_bytes", m, 64, 64, 8, 2)
+        assert nbytes >= _lib.lib().w8a8_linear_adapters_workspace_bytes(m, 64, 64, 8, 2)
+    assert len(mod._routed_bytes) <= 4096
