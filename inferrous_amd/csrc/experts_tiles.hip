@@ -37,24 +37,16 @@ __global__ __launch_bounds__(64 * kSortWaves) void experts_plan(const int32_t* i
       });
 }
 
-// The rows and the column tile of a workgroup, or false where it has none.  A plan
-// tile is `parts` units of BT rows.  Each XCD takes a contiguous run of the work, a
-// unit's columns next to each other.  Strips of 2, 4 or 8 units walking the columns
-// together were slower: 4096 rows x 8 of 64 experts, gate and up 323 against 349-352
-// us, down 293 against 304-317.
-template <uint32_t BT>
-__device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t parts, uint32_t cols, RowTile& t,
-                                         uint32_t& col) {
-  const uint32_t work = *plan.n_tiles * parts * cols, per = (work + 7) / 8;
+// The rows and the column tile of a workgroup, or false where it has none.  Each XCD
+// takes a contiguous run of the work, a tile's columns next to each other.  Strips of
+// 2, 4 or 8 tiles walking the columns together were slower: 4096 rows x 8 of 64
+// experts, gate and up 323 against 349-352 us, down 293 against 304-317.
+__device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t cols, RowTile& t, uint32_t& col) {
+  const uint32_t work = *plan.n_tiles * cols, per = (work + 7) / 8;
   const uint32_t at = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per || at >= work) return false;
-  const uint32_t unit = at / cols;
   col = at % cols;
-  t = plan.tiles[unit / parts];
-  const uint32_t skip = unit % parts * BT;
-  if (skip >= t.rows) return false;
-  t.first += skip;
-  t.rows = min(t.rows - skip, BT);
+  t = plan.tiles[at / cols];
   return true;
 }
 
@@ -174,7 +166,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void experts_gate_up(ExpertsArgs a, 
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS > kMost ? T::LDS : kMost];
   RowTile t;
   uint32_t group;
-  if (!own_tile<T::BT>(plan, 1, (a.inter + 127) / 128, t, group)) return;
+  if (!own_tile(plan, (a.inter + 127) / 128, t, group)) return;
   if constexpr (!std::is_same_v<Quarter, NoForm>) {
     static_assert(Quarter::NW == T::NW, "forms of one launch");
     if (t.rows <= (uint32_t)Quarter::BT) return gate_up_tile<Quarter>(a, plan, t, group, lds, codes, scales);
@@ -248,14 +240,14 @@ __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t
   }
 }
 
-// A plan tile is `parts` of these; one of few rows takes the lower form.
+// A tile of few rows takes the lower form.
 template <class T, class Half, class Quarter>
-__global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, ExpertsPlan plan, uint32_t parts,
-                                                              const int8_t* codes, const float* scales, float* y) {
+__global__ __launch_bounds__(64 * T::NW, 2) void experts_down(ExpertsArgs a, ExpertsPlan plan, const int8_t* codes,
+                                                              const float* scales, float* y) {
   __shared__ __attribute__((aligned(1024))) int8_t lds[T::LDS];
   RowTile t;
   uint32_t col;
-  if (!own_tile<T::BT>(plan, parts, (a.hidden + T::BN - 1) / T::BN, t, col)) return;
+  if (!own_tile(plan, (a.hidden + T::BN - 1) / T::BN, t, col)) return;
   if constexpr (!std::is_same_v<Quarter, NoForm>) {
     static_assert(Quarter::NW == T::NW && Quarter::BN == T::BN && Quarter::LDS <= T::LDS, "forms of one launch");
     if (t.rows <= (uint32_t)Quarter::BT) return down_tile<Quarter>(a, t, col, lds, codes, scales, y);
@@ -391,23 +383,23 @@ void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
 }
 
 template <class T, class Half = NoForm, class Quarter = NoForm>
-void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
+void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t tiles,
              const int8_t* codes, const float* scales, float* y) {
-  const uint32_t parts = bt / T::BT, grid = (tiles * parts * ((a.hidden + T::BN - 1) / T::BN) + 7) / 8 * 8;
-  hipLaunchKernelGGL((experts_down<T, Half, Quarter>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, parts, codes, scales, y);
+  const uint32_t grid = (tiles * ((a.hidden + T::BN - 1) / T::BN) + 7) / 8 * 8;
+  hipLaunchKernelGGL((experts_down<T, Half, Quarter>), dim3(grid), dim3(64 * T::NW), 0, st, a, p, codes, scales, y);
 }
 
 template <bool TAIL>
 void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
           const int8_t* codes, const float* scales, float* y) {
   if (bt == 32 && tiles * ((a.hidden + 255) / 256) <= kOnePerCu)
-    down_as<Down<32, 256, 32, 4, 4, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
-  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
-  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
+    down_as<Down<32, 256, 32, 4, 4, TAIL>>(st, a, p, tiles, codes, scales, y);
+  else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>>(st, a, p, tiles, codes, scales, y);
+  else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>>(st, a, p, tiles, codes, scales, y);
   else if (bt == 256)
     down_as<TileStream<256, 256, 64, 128, 2, 2, true, TAIL, OP_I8, true>, Down<128, 256, 64, 2, 2, TAIL>,
-            Down<64, 256, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
-  else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, bt, tiles, codes, scales, y);
+            Down<64, 256, 32, 2, 2, TAIL>>(st, a, p, tiles, codes, scales, y);
+  else down_as<Down<128, 128, 64, 2, 2, TAIL>, Down<64, 128, 32, 2, 2, TAIL>>(st, a, p, tiles, codes, scales, y);
 }
 }  // namespace
 
