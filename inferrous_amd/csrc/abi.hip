@@ -1459,8 +1459,6 @@ static int check_adapters_shape(size_t m, size_t n, uint32_t k, uint32_t rank, u
 
 // The workspace: the adapters' part, then, unless they run with the projection in
 // one kernel, the projection's sums [m, n] and its own workspace.
-static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
-
 size_t w8a8_linear_adapters_workspace_bytes(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters) {
   if (m == 0 || n == 0 || check_adapters_shape(m, n, k, rank, n_adapters) != W8A8_OK) return 0;
   AdapterArgs a{};

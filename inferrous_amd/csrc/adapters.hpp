@@ -8,8 +8,6 @@
 
 namespace w8a8 {
 
-static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
-
 // Values of a row of scaling * h: the ranks, padded to whole 32s.
 __host__ __device__ constexpr uint32_t part_width(uint32_t rank) { return (rank + 31) / 32 * 32; }
 

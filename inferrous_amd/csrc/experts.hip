@@ -193,8 +193,6 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
   }
 }
 
-static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
-
 // Slot by slot every slot reads its expert's weights; expert by expert the experts
 // that are met are read once, in four launches instead of two.  The slots' form
 // runs while what it reads more costs less than those launches: about 140 MB.

@@ -305,8 +305,6 @@ __global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int3
 }
 
 // ------------------------------------------------------------------ launches
-static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
-
 // Rows of a token tile, by an expert's mean share of the slots: the smallest that
 // holds it with room for the uneven shares of real routing.  An expert that takes
 // two tiles reads its weights twice, which large experts (above 8 MiB) cannot

@@ -223,6 +223,9 @@ uint32_t seq_max_rows(uint32_t grid);
 hipError_t launch_sequence(hipStream_t st, const SeqEntry* tab, uint32_t count, uint32_t base, uint32_t* ctl,
                            uint64_t* keys, uint32_t* token, uint64_t spin, uint32_t grid);
 
+// Bytes of a workspace's part: whole 256s.
+static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
+
 // The router of a layer of experts (route.hip).
 struct RouteArgs {
   const void* logits;  // [m, experts], f32 or BF16
