@@ -99,6 +99,28 @@ int w8a8_diag_argmax_route(size_t n, uint32_t k, int32_t *route,
 int w8a8_diag_grouped_route(size_t m, uint32_t k, int count, const size_t *n,
                             int32_t *route, size_t route_len);
 
+/* The forms that w8a8_experts_mlp and w8a8_linear_adapters take, decided on the
+ * host from the sizes alone and returned as W8A8_DIAG_FORM_LEN int32 values
+ * (unused ones 0), so that tests can say which kernels a shape runs.
+ * Experts: [0] 1 slot by slot, 2 expert by expert; then for 2 [1] rows of a token
+ * tile, [2] tiles at most, [3] workgroups of the sort, [4] gate and up with
+ * four stages at 32 rows, [5] down with four stages at 32 rows, [6] a short last
+ * stage of gate's and up's K, [7] of down's.
+ * Adapters: [0] 1 one kernel after the first product, 2 row by row, 3 rows sorted
+ * by adapter; for 1 and 2 [1] values of the first product a wave; for 3 [1] rows
+ * and [2] ranks of a tile of the first product, [3] its shares of K, [4]
+ * workgroups of the sort, [5] rows and columns of the projection's tiles, [6] a
+ * short last stage of its K.
+ * W8A8_ESHAPE for sizes that the operator refuses (all 0 for no rows),
+ * W8A8_EWORKSPACE when form_len is short. */
+#define W8A8_DIAG_FORM_LEN 8
+int w8a8_diag_experts_form(size_t m, uint32_t top_k, uint32_t n_experts,
+                           uint32_t hidden, uint32_t inter, int32_t *form,
+                           size_t form_len);
+int w8a8_diag_adapters_form(size_t m, size_t n, uint32_t k, uint32_t rank,
+                            uint32_t n_adapters, int32_t *form,
+                            size_t form_len);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,8 @@
 
 #include "../../include/inferrous_w8a8.h"
 #include "../../include/inferrous_w8a8_diag.h"
+#include "adapters.hpp"
+#include "experts.hpp"
 #include "internal.hpp"
 
 using namespace w8a8;
@@ -1545,6 +1547,49 @@ int w8a8_linear_adapters(void* stream, const int8_t* q, const float* asc, size_t
   }
   if (s != W8A8_OK) return s;
   return hip_status(launch_adapters_after(st, t, acc, slabs, workspace));
+}
+
+int w8a8_diag_experts_form(size_t m, uint32_t top_k, uint32_t n_experts, uint32_t hidden, uint32_t inter,
+                           int32_t* form, size_t form_len) {
+  if (!form) return W8A8_ENULL;
+  if (form_len < W8A8_DIAG_FORM_LEN) return W8A8_EWORKSPACE;
+  std::fill(form, form + W8A8_DIAG_FORM_LEN, 0);
+  const int s = check_experts_shape(m, top_k, n_experts, hidden, inter);
+  if (s != W8A8_OK || m == 0) return s;
+  if (experts_by_slot((uint32_t)m, top_k, n_experts, hidden, inter)) {
+    form[0] = 1;
+    return W8A8_OK;
+  }
+  const ExpertsTilesForm f = experts_tiles_form((uint32_t)m, top_k, n_experts, hidden, inter);
+  const int32_t all[] = {2, (int32_t)f.bt, (int32_t)f.tiles, (int32_t)f.sort_blocks, f.gate_deep, f.down_deep,
+                         f.gate_tail, f.down_tail};
+  std::copy(std::begin(all), std::end(all), form);
+  return W8A8_OK;
+}
+
+int w8a8_diag_adapters_form(size_t m, size_t n, uint32_t k, uint32_t rank, uint32_t n_adapters, int32_t* form,
+                            size_t form_len) {
+  if (!form) return W8A8_ENULL;
+  if (form_len < W8A8_DIAG_FORM_LEN) return W8A8_EWORKSPACE;
+  std::fill(form, form + W8A8_DIAG_FORM_LEN, 0);
+  const int s = check_adapters_shape(m, n, k, rank, n_adapters);
+  if (s != W8A8_OK || m == 0 || n == 0) return s;
+  AdapterArgs a{};
+  a.m = (uint32_t)m;
+  a.n = (uint32_t)n;
+  a.width = k;
+  a.rank = rank;
+  a.adapters = n_adapters;
+  const AdapterPlan p = adapter_plan(a);
+  form[0] = p.fused ? 3 : p.gemv ? 1 : 2;
+  form[1] = (int32_t)(p.fused ? p.bt : p.values);
+  if (!p.fused) return W8A8_OK;
+  form[2] = (int32_t)p.ranks;
+  form[3] = (int32_t)p.splits;
+  form[4] = (int32_t)sort_blocks(a.m);
+  form[5] = (int32_t)p.tile;
+  form[6] = p.tail;
+  return W8A8_OK;
 }
 
 }  // extern "C"

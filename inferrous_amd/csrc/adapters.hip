@@ -242,8 +242,12 @@ static bool fused_leads(const AdapterArgs& a) {
 AdapterPlan adapter_plan(const AdapterArgs& a) {
   AdapterPlan p{};
   const uint32_t mean = a.m / std::min(a.m, a.adapters);
+  p.gemv = gemv_leads(a);
   p.fused = fused_leads(a);
   if (p.fused) {
+    p.ranks = a.rank <= 32 ? 32 : a.rank <= 64 ? 64 : a.rank <= 128 ? 128 : 256;
+    p.tile = (uint64_t)((a.m + 255) / 256) * ((a.n + 255) / 256) >= 192 ? 256 : 128;
+    p.tail = a.width % 128 != 0;
     const uint32_t all = (a.width * 2 + 127) / 128;  // stages of an adapter row
     p.bt = mean <= 48 ? 32 : 128;
     p.tiles = a.m / p.bt + std::min(a.m, a.adapters);
@@ -252,6 +256,9 @@ AdapterPlan adapter_plan(const AdapterArgs& a) {
     p.stages = std::max((all + want - 1) / want, std::min(all, 8u));
     p.splits = (all + p.stages - 1) / p.stages;
   } else {
+    // few values: one a wave; many: eight, which share their loads of x (64 rows of
+    // rank 32 at width 4096, one / two / eight: 3.9 / 4.3 / 6.9 us)
+    p.values = a.m * a.rank <= 4096 ? 1 : a.m * a.rank <= 16384 ? 2 : 8;
     p.splits = 1;
   }
   size_t at = 0;
@@ -274,20 +281,21 @@ AdapterPlan adapter_plan(const AdapterArgs& a) {
 }
 
 size_t adapters_workspace_bytes(const AdapterArgs& a) { return adapter_plan(a).bytes; }
-bool adapters_fused(const AdapterArgs& a) { return gemv_leads(a) || adapter_plan(a).fused; }
+bool adapters_fused(const AdapterArgs& a) {
+  const AdapterPlan p = adapter_plan(a);
+  return p.gemv || p.fused;
+}
 
 hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* workspace) {
   const AdapterPlan p = adapter_plan(a);
   if (p.fused) return launch_adapters_fused(st, a, p, (char*)workspace);
   float* const h = (float*)((char*)workspace + p.h);
-  // few values: one a wave; many: eight, which share their loads of x (64 rows of
-  // rank 32 at width 4096, one / two / eight: 3.9 / 4.3 / 6.9 us)
-  const int J = a.m * a.rank <= 4096 ? 1 : a.m * a.rank <= 16384 ? 2 : 8;
+  const uint32_t J = p.values;
   const dim3 grid((a.rank + 4 * J - 1) / (4 * J) * a.m);
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a, h); };
   if (a.x_bf16) go(J == 1 ? adapters_shrink<1, true> : J == 2 ? adapters_shrink<2, true> : adapters_shrink<8, true>);
   else go(J == 1 ? adapters_shrink<1, false> : J == 2 ? adapters_shrink<2, false> : adapters_shrink<8, false>);
-  if (gemv_leads(a)) {
+  if (p.gemv) {
     auto k = a.m == 1 ? adapters_gemv<1> : a.m == 2 ? adapters_gemv<2> : a.m == 3 ? adapters_gemv<3> : adapters_gemv<4>;
     hipLaunchKernelGGL(k, dim3((a.n + 4 * kGemvCols - 1) / (4 * kGemvCols)), dim3(256), 0, st, a, h);
   }

@@ -13,7 +13,12 @@ __host__ __device__ constexpr uint32_t part_width(uint32_t rank) { return (rank 
 
 // How a call runs, a function of its sizes.
 struct AdapterPlan {
+  bool gemv;        // few rows: the projection and the second product in one kernel
   bool fused;       // the rows are sorted by adapter, and the projection's tiles add the second product
+  uint32_t values;  // (not fused) values of h that a wave sums: 1, 2 or 8
+  uint32_t ranks;   // (fused) ranks of a tile of the first product: 32, 64, 128 or 256
+  uint32_t tile;    // (fused) rows and columns of the projection's tiles: 128 or 256
+  bool tail;        // (fused) the last stage of the projection's K is short
   uint32_t bt;      // (fused) rows of a tile of the first product
   uint32_t tiles;   // tiles at most
   uint32_t splits;  // shares of K of the first product, each with partial sums of its own

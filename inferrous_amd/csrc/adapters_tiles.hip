@@ -351,8 +351,8 @@ void gemm_as(hipStream_t st, const AdapterArgs& a, const AdapterPlan& p, char* w
     hipLaunchKernelGGL(adapters_gemm<T>, dim3(tm * tn), dim3(64 * T::NW), 0, st, a, (const uint32_t*)(ws + p.order),
                        (const float*)(ws + p.scaled), tm, tn, wide);
   };
-  if (a.width % 128 == 0) go(TileStream<BT, BN, WT, WN, SA, SB, false, false>{});
-  else go(TileStream<BT, BN, WT, WN, SA, SB, false, true>{});
+  if (p.tail) go(TileStream<BT, BN, WT, WN, SA, SB, false, true>{});
+  else go(TileStream<BT, BN, WT, WN, SA, SB, false, false>{});
 }
 }  // namespace
 
@@ -364,7 +364,7 @@ hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const Ada
                        counts);
   hipLaunchKernelGGL(adapters_order, dim3(blocks), dim3(64 * kSortWaves), lds, st, a.ids, a.m, per, a.adapters, counts,
                      p.bt, (uint32_t*)(ws + p.order), (RowTile*)(ws + p.table), (uint32_t*)(ws + p.n_tiles));
-  const int rank = a.rank <= 32 ? 32 : a.rank <= 64 ? 64 : a.rank <= 128 ? 128 : 256;
+  const uint32_t rank = p.ranks;
   if (p.bt == 32) {
     if (rank == 32) shrink_as<32, 32, 32, 32, 4, 4>(st, a, p, ws);
     else if (rank == 64) shrink_as<32, 64, 32, 32, 4, 4>(st, a, p, ws);
@@ -379,8 +379,7 @@ hipError_t launch_adapters_fused(hipStream_t st, const AdapterArgs& a, const Ada
   const size_t quads = (size_t)a.m * (part_width(a.rank) / 4);
   hipLaunchKernelGGL(adapters_scale, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, a,
                      (const uint32_t*)(ws + p.order), (const float*)(ws + p.h), p.splits, (float*)(ws + p.scaled));
-  const uint64_t big = (uint64_t)((a.m + 255) / 256) * ((a.n + 255) / 256);
-  if (big >= 192) gemm_as<256, 256, 64, 128, 2, 3>(st, a, p, ws);
+  if (p.tile == 256) gemm_as<256, 256, 64, 128, 2, 3>(st, a, p, ws);
   else gemm_as<128, 128, 64, 64, 2, 3>(st, a, p, ws);
   return hipGetLastError();
 }

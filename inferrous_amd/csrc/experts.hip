@@ -200,19 +200,19 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
 // 49.8 / 55.1, 12 rows (136 MB) 71.6 / 61.7; hidden 4096, inner 2048, 2 of 16, 8 rows
 // (139 MB) 68.6 / 74.1, 12 rows (251 MB) 98.1 / 76.5; hidden 2048, inner 1024, 2 of 8, 16
 // rows (151 MB) 33.2 / 35.8.
-static bool by_slot(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
+bool experts_by_slot(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
   if (m > 64) return false;
   const double slots = (double)m * k, met = experts * (1.0 - std::pow(1.0 - std::min(1.0, (double)k / experts), (double)m));
   return (slots - met) * 3.0 * hidden * inter <= 140e6;
 }
 
 size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
-  if (!by_slot(m, k, experts, hidden, inter)) return experts_tiles_workspace_bytes(m, k, experts, hidden, inter);
+  if (!experts_by_slot(m, k, experts, hidden, inter)) return experts_tiles_workspace_bytes(m, k, experts, hidden, inter);
   return up256((size_t)m * k * inter * 4);  // act
 }
 
 hipError_t launch_experts(hipStream_t st, const ExpertsArgs& a, void* workspace) {
-  if (!by_slot(a.m, a.k, a.experts, a.hidden, a.inter)) return launch_experts_tiles(st, a, workspace);
+  if (!experts_by_slot(a.m, a.k, a.experts, a.hidden, a.inter)) return launch_experts_tiles(st, a, workspace);
   const uint32_t slots = a.m * a.k;
   float* const act = (float*)workspace;
   constexpr int CG = 2, CD = 2;

@@ -28,6 +28,16 @@ __device__ __forceinline__ float act_f32(int32_t g, int32_t u, float asc, float 
   return gate * (gate < 0.f ? t : 1.0f) * r * up;
 }
 
+bool experts_by_slot(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);
+
+// How a call runs expert by expert, a function of its sizes.
+struct ExpertsTilesForm {
+  uint32_t bt, tiles;            // rows of a token tile, and how many tiles there can be
+  uint32_t sort_blocks;          // workgroups of the sort
+  bool gate_deep, down_deep;     // 32 rows: one workgroup a CU with twice the stages under way
+  bool gate_tail, down_tail;     // the last stage of K is short
+};
+ExpertsTilesForm experts_tiles_form(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);
 size_t experts_tiles_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter);
 hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* workspace);
 

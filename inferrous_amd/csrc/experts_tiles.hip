@@ -320,8 +320,19 @@ static uint32_t tile_rows(uint32_t slots, uint32_t experts, uint32_t hidden, uin
   return mean <= 24 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
 }
 
-static uint32_t most_tiles(uint32_t slots, uint32_t experts, uint32_t bt) {
-  return slots / bt + std::min(slots, experts);
+constexpr uint32_t kOnePerCu = 256;  // workgroups
+
+ExpertsTilesForm experts_tiles_form(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
+  const uint32_t slots = m * k;
+  ExpertsTilesForm f{};
+  f.bt = tile_rows(slots, experts, hidden, inter);
+  f.tiles = slots / f.bt + std::min(slots, experts);
+  f.sort_blocks = sort_blocks(slots);
+  f.gate_deep = f.bt == 32 && f.tiles * ((inter + 127) / 128) <= kOnePerCu;
+  f.down_deep = f.bt == 32 && f.tiles * ((hidden + 255) / 256) <= kOnePerCu;
+  f.gate_tail = hidden % 128 != 0;
+  f.down_tail = inter % 128 != 0;
+  return f;
 }
 
 namespace {
@@ -330,7 +341,7 @@ struct Layout {
 };
 Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
   const size_t slots = (size_t)m * k;
-  const uint32_t blocks = sort_blocks((uint32_t)slots);
+  const ExpertsTilesForm f = experts_tiles_form(m, k, experts, hidden, inter);
   Layout l{};
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -340,9 +351,9 @@ Layout layout(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_
   };
   l.order = take(slots * 4);
   l.pos = take(slots * 4);
-  l.tiles = take((size_t)most_tiles((uint32_t)slots, experts, tile_rows((uint32_t)slots, experts, hidden, inter)) * sizeof(RowTile));
+  l.tiles = take((size_t)f.tiles * sizeof(RowTile));
   l.n_tiles = take(4);
-  l.counts = take(blocks > 1 ? (size_t)blocks * experts * 4 : 0);
+  l.counts = take(f.sort_blocks > 1 ? (size_t)f.sort_blocks * experts * 4 : 0);
   l.codes = take(slots * inter);
   l.scales = take(slots * ((inter + 127) / 128) * 4);
   l.y = take(slots * hidden * 4);
@@ -355,8 +366,6 @@ using GateUp = TileStream<BT, 256, WT, WN, SA, SB, false, TAIL>;
 template <int BT, int BN, int WT, int SA, int SB, bool TAIL>
 using Down = TileStream<BT, BN, WT, 64, SA, SB, true, TAIL>;
 
-constexpr uint32_t kOnePerCu = 256;  // workgroups
-
 template <class T, class Half, class Quarter>
 void gate_up_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t tiles, int8_t* codes,
                 float* scales) {
@@ -365,14 +374,15 @@ void gate_up_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint
 }
 
 template <bool TAIL>
-void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles, int8_t* codes,
+void gate_up(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, const ExpertsTilesForm& form, int8_t* codes,
              float* scales) {
+  const uint32_t bt = form.bt, tiles = form.tiles;
   using T32 = GateUp<32, 32, 64, 2, 2, TAIL>;
   using T64 = GateUp<64, 64, 32, 4, 4, TAIL>;
   using T128 = GateUp<128, 64, 64, 3, 3, TAIL>;
   using T256 = GateUp<256, 64, 128, 2, 3, TAIL>;
   // 32 rows: two workgroups share a CU, or one has twice the stages under way
-  if (bt == 32 && tiles * ((a.inter + 127) / 128) <= kOnePerCu)
+  if (form.gate_deep)
     gate_up_as<GateUp<32, 32, 64, 4, 4, TAIL>, NoForm, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 32) gate_up_as<T32, NoForm, NoForm>(st, a, p, tiles, codes, scales);
   else if (bt == 64) gate_up_as<GateUp<64, 64, 64, 2, 2, TAIL>, T32, NoForm>(st, a, p, tiles, codes, scales);
@@ -388,9 +398,10 @@ void down_as(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_
 }
 
 template <bool TAIL>
-void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, uint32_t bt, uint32_t tiles,
+void down(hipStream_t st, const ExpertsArgs& a, const ExpertsPlan& p, const ExpertsTilesForm& form,
           const int8_t* codes, const float* scales, float* y) {
-  if (bt == 32 && tiles * ((a.hidden + 255) / 256) <= kOnePerCu)
+  const uint32_t bt = form.bt, tiles = form.tiles;
+  if (form.down_deep)
     down_as<Down<32, 256, 32, 4, 4, TAIL>>(st, a, p, tiles, codes, scales, y);
   else if (bt == 32) down_as<Down<32, 256, 32, 2, 2, TAIL>>(st, a, p, tiles, codes, scales, y);
   else if (bt == 64) down_as<Down<64, 128, 32, 3, 3, TAIL>>(st, a, p, tiles, codes, scales, y);
@@ -415,18 +426,17 @@ hipError_t launch_experts_tiles(hipStream_t st, const ExpertsArgs& a, void* work
   float* const scales = (float*)(p + l.scales);
   float* const y = (float*)(p + l.y);
   uint32_t* const counts = (uint32_t*)(p + l.counts);
-  const uint32_t bt = tile_rows(slots, a.experts, a.hidden, a.inter);
-  const uint32_t tiles = most_tiles(slots, a.experts, bt);
-  const uint32_t blocks = sort_blocks(slots), per = sort_per_block(slots), lds = kSortWaves * a.experts * 4;
+  const ExpertsTilesForm form = experts_tiles_form(a.m, a.k, a.experts, a.hidden, a.inter);
+  const uint32_t blocks = form.sort_blocks, per = sort_per_block(slots), lds = kSortWaves * a.experts * 4;
   if (blocks > 1)
     hipLaunchKernelGGL(sort_counts<false>, dim3(blocks), dim3(64 * kSortWaves), lds, st, a.ids, slots, per, a.experts,
                        counts);
   hipLaunchKernelGGL(experts_plan, dim3(blocks), dim3(64 * kSortWaves), lds, st, a.ids, slots, per, a.experts, counts,
-                     bt, plan);
-  if (a.hidden % 128 == 0) gate_up<false>(st, a, plan, bt, tiles, codes, scales);
-  else gate_up<true>(st, a, plan, bt, tiles, codes, scales);
-  if (a.inter % 128 == 0) down<false>(st, a, plan, bt, tiles, codes, scales, y);
-  else down<true>(st, a, plan, bt, tiles, codes, scales, y);
+                     form.bt, plan);
+  if (form.gate_tail) gate_up<true>(st, a, plan, form, codes, scales);
+  else gate_up<false>(st, a, plan, form, codes, scales);
+  if (form.down_tail) down<true>(st, a, plan, form, codes, scales, y);
+  else down<false>(st, a, plan, form, codes, scales, y);
   hipLaunchKernelGGL(experts_combine, dim3(std::min(a.m, kCombineRows), (a.hidden + 1023) / 1024), dim3(256), 0, st, a,
                      plan.pos, y);
   return hipGetLastError();
