@@ -227,11 +227,12 @@ static bool gemv_leads(const AdapterArgs& a) {
 // at about 10 TB/s, beside the projection.  The fused tiles read an adapter once,
 // but run in the tiles' own time: 22 us more than the projection at width 4096, 43
 // at 12288 until the tiles fill the card, and 1.5 us for each 32 ranks of every
-// adapter after a tile's first.  Measured, rows / fused us at 4 adapters: 4096 x
-// 4096, rank 16, m = 512 (134 MB) 34.6 / 39.0, m = 1024 (268 MB) 56 / 42; rank 64, m
-// = 128 (134 MB) 29 / 40, m = 512 62 / 43; 4096 x 12288, rank 16, m = 512 (268 MB)
-// 59 / 70, m = 1024 104 / 77; 24576 x 4096, rank 32, m = 80 (147 MB) 41 / 41, m = 128
-// 50 / 42.
+// adapter after a tile's first.  Measured, rows / fused us at 4 adapters, on the same
+// weights again: 4096 x 4096, rank 16, m = 512 (134 MB) 32.8 / 39.8, m = 1024 (268 MB) 53 /
+// 41; rank 64, m = 128 (134 MB) 30 / 43, m = 512 63 / 46; 4096 x 12288, rank 16, m = 512
+// (268 MB) 55 / 69, m = 1024 99 / 77; 24576 x 4096, rank 32, m = 80 (147 MB) 40 / 42, m = 128
+// 49 / 43.  On weights of each pass's own: 35 / 44, 58 / 51; 30 / 48, 66 / 51; 65 / 96, 113
+// / 100; 42 / 53, 50 / 55.
 static bool fused_leads(const AdapterArgs& a) {
   if (gemv_leads(a)) return false;
   const double rows_us = (double)a.m * a.rank * ((double)a.n + a.width) * 2.0 / 10e6;

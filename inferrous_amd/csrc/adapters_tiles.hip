@@ -1,8 +1,8 @@
 // adapters_tiles.hip -- adapters beside a projection with the rows sorted by
 // adapter (adapters.hip has the definition).  4096 rows on 4096 x 12288, 6 adapters of
-// rank 64, with a residual: 224-240 us, the projection's tiles 195-220 of them (the
-// projection alone 175-183, 2.3 POPS); the large int8 library product's rate, 2.07
-// POPS, would take 203.
+// rank 64, with a residual: 229-231 us a pass among others, the projection's tiles 193 at
+// the least and 208-220 in a run of passes (the projection alone 175-183); the large int8
+// library product's rate, 2.07 POPS, would take 203.
 //
 //   adapters_order          the sort, and the tiles: up to bt rows of one adapter;
 //   adapters_shrink_tiles   h's partial sums, tile x share of K, by bf16 MFMA;
@@ -118,7 +118,8 @@ constexpr uint32_t kStripTiles = 4;
 // Rows of another adapter keep the value they had (a lane is one row).
 template <class T>
 __global__ __launch_bounds__(64 * T::NW, 2) void adapters_gemm(AdapterArgs a, const uint32_t* order,
-                                                              const float* scaled, uint32_t tiles_m, uint32_t tiles_n, bool wide) {
+                                                              const float* scaled, uint32_t tiles_m,
+                                                              uint32_t tiles_n, bool wide) {
   constexpr int PAIR = 40;          // BF16 values of an LDS row of 32, padded
   constexpr int STRIDE = 64 + 4;    // f32 values of an LDS row of 64 columns, padded
   constexpr int THREADS = 64 * T::NW;

@@ -120,9 +120,10 @@ __device__ __forceinline__ float down_in_order(const ExpertsArgs& a, const float
 // each wave's weights for its COLS columns are on their way.  A lane's 16 products
 // lie in one group, so its part of a sum is scaled, by s, weight and wsd, before the
 // lanes' parts are added.  Parts of both signs or of 0 make NaN of an infinite wsd or
-// weight: a column that is not finite is summed again, in order.  8 slots of hidden 4096, inner 1024 (33.5 MB): 9.4 us, 3.6 TB/s: ids, then
-// act and weights, codes, sums follow each other.  With the codes made by a launch
-// of their own 10.8 + 2.5 us; one column a wave 8.9-9.3.
+// weight: a column that is not finite is summed again, in order.  8 slots of hidden
+// 4096, inner 1024 (33.5 MB): 9.4 us, 3.6 TB/s: ids, then act and weights, codes, sums
+// follow each other.  With the codes made by a launch of their own 10.8 + 2.5 us; one
+// column a wave level.
 template <int COLS>
 __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const float* act) {
   __shared__ __attribute__((aligned(16))) v4i code[8][64];
@@ -196,18 +197,23 @@ __global__ __launch_bounds__(512) void experts_down_slot(ExpertsArgs a, const fl
 // Slot by slot every slot reads its expert's weights; expert by expert the experts
 // that are met are read once, in four launches instead of two.  The slots' form
 // runs while what it reads more costs less than those launches: about 140 MB.
-// Measured, slots / experts us: hidden 2048, inner 768, 8 of 128, 8 rows (63 MB more)
-// 49.8 / 55.1, 12 rows (136 MB) 71.6 / 61.7; hidden 4096, inner 2048, 2 of 16, 8 rows
-// (139 MB) 68.6 / 74.1, 12 rows (251 MB) 98.1 / 76.5; hidden 2048, inner 1024, 2 of 8, 16
-// rows (151 MB) 33.2 / 35.8.
+// Measured on weights of each pass's own, slots / experts us: hidden 4096, inner 1024, 8
+// of 64, 4 rows (69 MB more) 65.0 / 78.3, 6 rows (160 MB) 92.6 / 112; hidden 2048, inner
+// 768, 8 of 128, 8 rows (58 MB) 51.5 / 59.3, 12 rows (127 MB) 73.4 / 70.6; hidden 4096,
+// inner 2048, 2 of 16, 6 rows (80 MB) 55.6 / 61.9, 8 rows (138 MB) 70.9 / 66.4, 12 rows
+// (282 MB) 101 / 71; hidden 2048, inner 1024, 2 of 8, 12 rows (102 MB) 28.9 / 32.9, 16 rows
+// (151 MB) 36.0 / 33.0.  Of small experts the slots' form takes more than its bytes:
+// hidden 512, inner 256, 4 of 32, 32 rows (38 MB) 18.3 / 18.9, 64 rows (88 MB) 31.8 / 19.0.
 bool experts_by_slot(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
   if (m > 64) return false;
-  const double slots = (double)m * k, met = experts * (1.0 - std::pow(1.0 - std::min(1.0, (double)k / experts), (double)m));
+  const double slots = (double)m * k;
+  const double met = experts * (1.0 - std::pow(1.0 - std::min(1.0, (double)k / experts), (double)m));
   return (slots - met) * 3.0 * hidden * inter <= 140e6;
 }
 
 size_t experts_workspace_bytes(uint32_t m, uint32_t k, uint32_t experts, uint32_t hidden, uint32_t inter) {
-  if (!experts_by_slot(m, k, experts, hidden, inter)) return experts_tiles_workspace_bytes(m, k, experts, hidden, inter);
+  if (!experts_by_slot(m, k, experts, hidden, inter))
+    return experts_tiles_workspace_bytes(m, k, experts, hidden, inter);
   return up256((size_t)m * k * inter * 4);  // act
 }
 

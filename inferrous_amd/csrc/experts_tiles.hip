@@ -3,7 +3,7 @@
 // slots' products summed row by row.  The definition is in experts.hip.
 //
 // For 4096 rows x 8 of 64 experts, hidden 4096, inner 1024 (825 G operations; the
-// large int8 library product's rate, 2.07 POPS, would take 398 us): 643-690 us.
+// large int8 library product's rate, 2.07 POPS, would take 398 us): 700-718 us.
 //
 //   experts_plan       sorts the slots (a counting sort that keeps their order)
 //                      and lists the token tiles: up to BT rows of one expert;
@@ -55,10 +55,11 @@ __device__ __forceinline__ bool own_tile(const ExpertsPlan& plan, uint32_t cols,
 // columns, in turn, so that a lane of a 32 x 32 block holds a column's gate sum
 // (v < 8) and its up sum (v + 8).
 // Few rows an expert: the weight stream bounds it, two workgroups a CU (81 experts of
-// hidden 2048, inner 768 met by 128 slots, 255 MB: 41 us, 6.2 TB/s; one workgroup with
-// four stages 45).  Many: the matrix cores, busy 55-60% of the time at the clock
-// that the board's power leaves (256-row tiles, 550 G operations in 330-340 us, 285 of
-// them without the epilogue, which issues about 30 instructions a value of act).
+// hidden 2048, inner 768 met by 128 slots, 255 MB: 40 us, 6.4 TB/s; one workgroup with
+// four stages 45).  Many (256-row tiles, 550 G operations): 325 us at the least and 365
+// in a run of passes, whose power lowers the clock.  The matrix cores are busy 55% of
+// a CU's own time and the VALU, most of it the epilogue, 27%, one after the other;
+// CUs are idle for 17% at the end.
 template <class T>
 __device__ __forceinline__ void gate_up_tile(const ExpertsArgs& a, const ExpertsPlan& plan, const RowTile& t,
                                              uint32_t group, int8_t* lds, int8_t* codes, float* scales) {
@@ -179,11 +180,13 @@ __global__ __launch_bounds__(64 * T::NW, 2) void experts_gate_up(ExpertsArgs a, 
 }
 
 // ------------------------------------------------------------------ down
-// What bounds it at many rows is the CU's operand pull, 28 bytes a clock, not the f32
-// folding: 128 x 128 tiles (two workgroups a CU) took 313 us for 4096 rows x 8 of 64
-// experts, hidden 4096, inner 1024 (275 G operations); without the folding the same,
-// without the epilogue 225-266; 256 x 256 tiles, half the pull, 287.  128 x 256 and
-// 256 x 128 tiles with three stages 310-333, 128 x 128 with four 393-410.
+// At many rows no unit bounds it alone: in 256 x 256 tiles of 4096 rows x 8 of 64 experts,
+// hidden 4096, inner 1024 (275 G operations, 287 us at the least, 309 in a run of passes)
+// the matrix cores are busy 27% of a CU's own time, the VALU 38%, the loads' addressing
+// 43%, and the vector cache waits for L2 58%: with one workgroup a CU and 8 stages a
+// tile they follow each other.  128 x 128 tiles (two workgroups a CU): 309 and 337.
+// When y was 16 bits wide: 128 x 256 and 256 x 128 tiles with three stages 310-333, 128 x
+// 128 with four 393-410, against 313 and 287.
 template <class T>
 __device__ __forceinline__ void down_tile(const ExpertsArgs& a, const RowTile& t, uint32_t col, int8_t* lds,
                                           const int8_t* codes, const float* scales, float* y) {
@@ -302,8 +305,9 @@ __global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int3
     if (a.out_dtype == W8A8_OUT_F32) {
       *(v4f*)((float*)a.out + o) = sum;
     } else {
-      *(v2i*)((uint16_t*)a.out + o) = v2i{(int)((__float_as_uint(sum[0]) >> 16) | (__float_as_uint(sum[1]) & 0xffff0000u)),
-                                          (int)((__float_as_uint(sum[2]) >> 16) | (__float_as_uint(sum[3]) & 0xffff0000u))};
+      const uint32_t lo = (__float_as_uint(sum[0]) >> 16) | (__float_as_uint(sum[1]) & 0xffff0000u);
+      const uint32_t hi = (__float_as_uint(sum[2]) >> 16) | (__float_as_uint(sum[3]) & 0xffff0000u);
+      *(v2i*)((uint16_t*)a.out + o) = v2i{(int)lo, (int)hi};
     }
   }
 }
@@ -312,12 +316,13 @@ __global__ __launch_bounds__(256) void experts_combine(ExpertsArgs a, const int3
 // Rows of a token tile, by an expert's mean share of the slots: the smallest that
 // holds it with room for the uneven shares of real routing.  An expert that takes
 // two tiles reads its weights twice, which large experts (above 8 MiB) cannot
-// afford; a tile too tall computes rows that are not there.  Measured, tile rows: us,
-// hidden 4096, inner 1024, 8 of 64: mean 16 32: 231, 64: 201; mean 25 64: 235, 128:
-// 209; mean 42 64: 238, 128: 216; mean 128 128: 269, 256: 300.  Hidden 2048, inner 768,
-// 8 of 128: mean 16 32: 138, 64: 138; mean 44 64: 157, 128: 173; mean 128 128: 223,
-// 256: 227.  Hidden 2000, inner 720, 3 of 20: mean 19 32: 37, 64: 45, 128: 38; mean 105
-// 128: 50, 256: 59.
+// afford; a tile too tall computes rows that are not there.  Measured on weights of
+// each pass's own, tile rows: us, hidden 4096, inner 1024, 8 of 64: mean 16 32: 213, 64:
+// 182; mean 25 64: 217, 128: 193; mean 42 64: 229, 128: 215; mean 128 128: 277, 256: 312;
+// mean 150 128: 315, 256: 314.  Hidden 2048, inner 768, 8 of 128: mean 16 32: 140, 64:
+// 139; mean 44 64: 161, 128: 176; mean 128 128: 239, 256: 244; mean 144 128: 251, 256: 260.
+// Hidden 2000, inner 720, 3 of 20: mean 19 32: 46, 64: 55, 128: 48; mean 50 64: 58, 128:
+// 57; mean 105 128: 63, 256: 75.
 static uint32_t tile_rows(uint32_t slots, uint32_t experts, uint32_t hidden, uint32_t inter) {
   const uint32_t mean = slots / std::min(slots, experts);
   if (3ull * hidden * inter > (8u << 20)) return mean <= 12 ? 32 : mean <= 20 ? 64 : mean <= 128 ? 128 : 256;

@@ -26,8 +26,7 @@
 // BLOCKED (with GROUPED): a stage's sums are made block by block, each from the
 // stage's four fragments of its rows, and folded while the next block's are made:
 // the i32 sums take two blocks of registers, not FT * FN, and a wave can hold 64 x
-// 128 f32 sums.  A larger tile pulls fewer operand bytes per product, and a CU's
-// pull, about 28 bytes a clock, is what bounds these kernels.
+// 128 f32 sums.  A larger tile pulls fewer operand bytes per product.
 //
 // The op (OP) is the int8 one above or v_mfma_f32_32x32x16_bf16, whose fragments
 // are 16 bytes a lane too and whose result has the same layout.  K is then the
