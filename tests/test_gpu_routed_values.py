@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, DeviceBuffer, W8A8Error, load
-from test_gpu_routed import Adapters, Experts, bf16, close_bf16, from_bits
+from test_gpu_routed import Adapters, Experts, bf16, bf16_bits, close_bf16, from_bits, values
 
 pytestmark = pytest.mark.gpu
 
@@ -206,4 +206,48 @@ def test_experts_at_the_most_slots(env):
     mod.experts_mlp(s, q, asc, h, ids, weights, *mats, e, out)
     got = out.to_host_vec(s).reshape(-1, period * h)
     close_bf16(from_bits(got[0]).reshape(period, h), want, err)
+    assert (got == got[0]).all()
+
+
+def at_the_end(s, count, part):
+    """A buffer of `count` parts, zeros but for the last one."""
+    buf = DeviceBuffer(count * part.size, part.dtype)
+    DeviceBuffer.view_of(buf, (count - 1) * part.size, part.size).copy_from_host(s, part.reshape(-1))
+    return buf
+
+
+@pytest.mark.parametrize("m", [2, 200])
+def test_experts_weights_past_four_gib(env, m):
+    """The last of 270 experts of 4096 x 4096: its weights lie above 2^32 bytes."""
+    mod, s, _ = env
+    h = f = 4096
+    e = 270
+    c = Experts(m, 1, 1, h, f, seed=m, ids=np.zeros((m, 1), np.int32))
+    mats = [at_the_end(s, e, a) for a in (c.wg, c.sg, c.wu, c.su, c.wd, c.sd)]
+    assert len(mats[0]) > 1 << 32
+    q, asc, ids, weights = (DeviceBuffer.from_host(s, a) for a in (c.q, c.asc, np.full(m, e - 1, np.int32), c.weights))
+    out = DeviceBuffer(m * h, np.uint16)
+    mod.experts_mlp(s, q, asc, h, ids, weights, *mats, e, out)
+    close_bf16(values(out, s).reshape(m, h), *c.want())
+
+
+@pytest.mark.parametrize("m", [4, 40, 4000])
+def test_adapters_past_four_gib(env, m):
+    """The last of 1023 adapters of rank 256, rows again and again: row by row and with the
+    rows sorted, every row has the outputs of its first."""
+    mod, s, _ = env
+    n = k = 8320
+    count, rank, period = 1023, 256, 4
+    c = Adapters(period, n, k, rank, 1, seed=m, ids=[0, -1, 0, 0])
+    a, b = at_the_end(s, count, bf16_bits(c.a)), at_the_end(s, count, bf16_bits(c.b))
+    assert a.nbytes > 1 << 32 and b.nbytes > 1 << 32
+    scaling = at_the_end(s, count, c.scaling)
+    reps = m // period
+    q, asc, x, ids = (DeviceBuffer.from_host(s, np.concatenate([v] * reps)) for v in (
+        c.q, c.asc, bf16_bits(c.x), np.where(c.ids == 0, count - 1, -1).astype(np.int32)))
+    out = DeviceBuffer(m * n, np.uint16)
+    mod.linear_adapters(s, q, asc, DeviceBuffer.from_host(s, c.w), DeviceBuffer.from_host(s, c.ws), k, x, ids, a, b,
+                        scaling, out)
+    got = values(out, s).reshape(reps, period, n)
+    close_bf16(got[0], *c.want())
     assert (got == got[0]).all()
