@@ -577,6 +577,103 @@ int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
                          const float *residual, void *out, int out_dtype,
                          void *workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------ attention
+ * What runs between the qkv and the o projection.  The reference's kernels for
+ * it (`prepare_qk`, `attention_prefill`, `attention`, src/kernels.rs:1290-2161,
+ * call sites src/gpu.rs:624-696) keep one request's keys and values in BF16;
+ * these take batches, and hold them in 8 bits in pages.
+ *
+ * Heads: `heads` query heads share `kv_heads` key/value heads, heads / kv_heads
+ * neighbours each; head_dim is 64 or 128.
+ *
+ * Batches: rows of n_seq sequences one after another; sequence i has rows
+ * starts[i] .. starts[i + 1] - 1 (int32 [n_seq + 1], not decreasing; cut to [0,
+ * m]).  Rows of no sequence are left as they were in every output.
+ *
+ * The cache of one layer: pages of W8A8_PAGE_TOKENS tokens.  codes[pages][kv_heads]
+ * holds of each the keys [tokens][head_dim], then the values [head_dim][tokens],
+ * e4m3 codes (OCP: largest 448, 0x7f and 0xff NaN); scales[pages][kv_heads][2]
+ * their scales, powers of two: a value is code * scale.  table[n_seq][table_width]
+ * names each sequence's pages in order: token t is slot t % 64 of page table[t /
+ * 64].  A page number outside [0, pages) stands for no page: nothing is written
+ * there, and its tokens are not seen.
+ *
+ * w8a8_prepare_qk: of each row, every query and key head normalised and rotated,
+ *   n = x / sqrt(mean(x^2) + eps) * gain     (gain NULL: n = x)
+ *   (a cos - b sin, b cos + a sin)           (a, b: n's halves; cos and sin:
+ *                                             the halves of rope[position])
+ * in f32, rounded once, to q_out[m, heads, head_dim] and, where not NULL,
+ * k_out[m, kv_heads, head_dim]; v_out (or NULL) is v as BF16.  q, k and v (F32 or
+ * BF16, dtype) are rows of heads * head_dim values with q_stride, k_stride and
+ * v_stride values from row to row: a qkv projection's output, or three.
+ * Position: past[i] (NULL: 0) plus the row's place in sequence i.  starts NULL:
+ * one row a sequence, n_seq == m.  A position not below rope_rows gives NaN.
+ * With codes (then scales and table too) the f32 keys and the values are also
+ * appended to the cache at their positions, beyond the table's width not.  A
+ * page's scale is the smallest 2^e, e >= -100, with 448 * 2^e at least the largest
+ * finite magnitude of its tokens, or the scale it had if past[i] lies inside the
+ * page and that is larger; if it grows, the codes before past[i] are rounded to it.
+ * NaN and infinities become NaN codes.  Slots behind the last token are left as
+ * they were.  A page may be in the table of one sequence that writes to it.
+ * starts, past, table and scales 4-byte, everything else 16-byte aligned; strides
+ * multiples of 8. */
+#define W8A8_PAGE_TOKENS 64
+int w8a8_prepare_qk(void *stream, const void *q, size_t q_stride, const void *k,
+                    size_t k_stride, const void *v, size_t v_stride, int dtype,
+                    size_t m, uint32_t heads, uint32_t kv_heads,
+                    uint32_t head_dim, const float *q_gain,
+                    const float *k_gain, float eps, const float *rope,
+                    uint32_t rope_rows, const int32_t *starts,
+                    const int32_t *past, uint32_t n_seq, uint16_t *q_out,
+                    uint16_t *k_out, uint16_t *v_out, uint8_t *codes,
+                    float *scales, uint32_t pages, const int32_t *table,
+                    uint32_t table_width);
+
+/* Causal attention of whole prompts: row r of a sequence sees its rows up to r,
+ *   out[r] = sum_j softmax_j(scale * q[r] . k[j]) v[j]
+ * q, k, v: BF16 rows as above (k and v as w8a8_prepare_qk leaves them, v also
+ * straight from a projection); starts NULL: one sequence of m rows.  Products and
+ * sums are held in f32, probabilities in BF16.  out: [m, heads, head_dim], F32
+ * (holding BF16 values) or BF16.  scale: positive.  What a row does not see never
+ * reaches it, whatever it holds. */
+int w8a8_attention_prefill(void *stream, const uint16_t *q, size_t q_stride,
+                           const uint16_t *k, size_t k_stride,
+                           const uint16_t *v, size_t v_stride, size_t m,
+                           uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, const int32_t *starts,
+                           uint32_t n_seq, float scale, void *out,
+                           int out_dtype);
+
+/* One query row of each of m sequences over the cache: q[m, heads, head_dim]
+ * (BF16), row i over the first lengths[i] tokens of its sequence (cut to what
+ * table[i] can name; 0 or less: out is 0).  Rows of one sequence (draft tokens)
+ * may repeat its pages with lengths of their own.  out, scale: as above.  The
+ * workspace (256-byte aligned) is written before it is read; calls sharing one must
+ * not overlap.  w8a8_attention_decode_workspace_bytes does not fall with m: a
+ * buffer for the largest batch serves every smaller one (with the same
+ * table_width). */
+size_t w8a8_attention_decode_workspace_bytes(size_t m, uint32_t heads,
+                                             uint32_t kv_heads,
+                                             uint32_t head_dim,
+                                             uint32_t table_width);
+int w8a8_attention_decode(void *stream, const uint16_t *q, size_t m,
+                          uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                          const uint8_t *codes, const float *scales,
+                          uint32_t pages, const int32_t *lengths,
+                          const int32_t *table, uint32_t table_width,
+                          float scale, void *out, int out_dtype,
+                          void *workspace, size_t workspace_bytes);
+
+/* Pages src[i] to dst[i], i < n, of each of `layers` caches that lie one after
+ * another (codes [layers][pages]..., scales likewise), codes and scales: what
+ * forking a sequence (its last, partly filled page) and compacting need.  Pairs
+ * with a page outside [0, pages) are skipped.  No page may be a destination twice,
+ * nor a source and a destination. */
+int w8a8_copy_pages(void *stream, uint8_t *codes, float *scales,
+                    uint32_t layers, uint32_t pages, uint32_t kv_heads,
+                    uint32_t head_dim, const int32_t *src, const int32_t *dst,
+                    uint32_t n);
+
 /* ------------------------------------------------------------------ synthetic
  * Seeded generators for benches and tests (no reference counterpart; the
  * reference loads exported bundles, src/model.rs:46-165).  Pure functions of

@@ -17,6 +17,7 @@ PATH_AUTO, PATH_DOT4, PATH_MFMA = 0, 1, 2
 NOALLOC_MAX_ROWS = 262144  # W8A8_NOALLOC_MAX_ROWS
 SEQ_SELECT = 1  # W8A8_SEQ_SELECT
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+PAGE_TOKENS = 64  # W8A8_PAGE_TOKENS
 
 
 class SeqEntry(ctypes.Structure):
@@ -103,6 +104,12 @@ SIGNATURES: dict[str, tuple] = {
     "w8a8_linear_adapters_workspace_bytes": (S, [S, S, U32, U32, U32]),
     "w8a8_linear_adapters_workspace_bytes_upto": (S, [S, S, U32, U32, U32]),
     "w8a8_linear_adapters": (I, [P, P, P, S, P, P, S, U32, P, I, P, P, P, P, U32, U32, P, P, I, P, S]),
+    "w8a8_prepare_qk": (I, [P, P, S, P, S, P, S, I, S, U32, U32, U32, P, P, F, P, U32, P, P, U32, P, P, P, P, P, U32, P,
+                            U32]),
+    "w8a8_attention_prefill": (I, [P, P, S, P, S, P, S, S, U32, U32, U32, P, U32, F, P, I]),
+    "w8a8_attention_decode_workspace_bytes": (S, [S, U32, U32, U32, U32]),
+    "w8a8_attention_decode": (I, [P, P, S, U32, U32, U32, P, P, U32, P, P, U32, F, P, I, P, S]),
+    "w8a8_copy_pages": (I, [P, P, P, U32, U32, U32, U32, P, P, U32]),
     "w8a8_synth_i8": (I, [P, P, S, U64, U64]),
     "w8a8_synth_f32": (I, [P, P, S, U64, U64, F, F]),
 }

@@ -22,7 +22,8 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libinferrous_w8a8.so"
 SOURCES = ["abi.hip", "quantize.hip", "gemv.hip", "gemm.hip", "head.hip", "synth.hip", "sequence.hip",
-           "route.hip", "experts.hip", "experts_tiles.hip", "adapters.hip", "adapters_tiles.hip"]
+           "route.hip", "experts.hip", "experts_tiles.hip", "adapters.hip", "adapters_tiles.hip",
+           "kv_cache.hip", "attention_prefill.hip", "attention_decode.hip"]
 ARCH = "gfx950"
 
 

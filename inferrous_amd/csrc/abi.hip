@@ -1158,6 +1158,180 @@ int w8a8_diag_grouped_route(size_t m, uint32_t k, int count, const size_t* n, in
   return W8A8_OK;
 }
 
+// ---- attention
+
+// Threads of a launch stay below 2^32.
+static constexpr uint64_t kMaxBlocks256 = (1u << 24) - 1;
+
+static int check_heads(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return W8A8_ESHAPE;
+  if (heads == 0 || kv_heads == 0 || heads > kMaxHeads || heads % kv_heads != 0) return W8A8_ESHAPE;
+  return m > kMaxAttentionRows ? W8A8_ESHAPE : W8A8_OK;
+}
+
+// Rows of `values` values, `stride` from row to row.
+static bool good_stride(size_t stride, size_t values) { return stride >= values && stride % 8 == 0 && stride <= kU32Max; }
+
+int w8a8_prepare_qk(void* stream, const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v,
+                    size_t v_stride, int dtype, size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                    const float* q_gain, const float* k_gain, float eps, const float* rope, uint32_t rope_rows,
+                    const int32_t* starts, const int32_t* past, uint32_t n_seq, uint16_t* q_out, uint16_t* k_out,
+                    uint16_t* v_out, uint8_t* codes, float* scales, uint32_t pages, const int32_t* table,
+                    uint32_t table_width) {
+  if (dtype != W8A8_OUT_F32 && dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  if (!(eps >= 0.f)) return W8A8_EARG;
+  const int s = check_heads(m, heads, kv_heads, head_dim);
+  if (s != W8A8_OK) return s;
+  if (!good_stride(q_stride, (size_t)heads * head_dim) || !good_stride(k_stride, (size_t)kv_heads * head_dim) ||
+      !good_stride(v_stride, (size_t)kv_heads * head_dim))
+    return W8A8_ESHAPE;
+  if (rope_rows == 0 || (!starts && n_seq != m) || (starts && n_seq == 0) || n_seq > kMaxAttentionRows) return W8A8_ESHAPE;
+  if (codes && (pages == 0 || pages > 0x7fffffffu || table_width == 0 || table_width > kMaxTableWidth)) return W8A8_ESHAPE;
+  if (m == 0) return W8A8_OK;
+  if (!q || !k || !v || !rope || !q_out || (codes && (!scales || !table))) return W8A8_ENULL;
+  if (!al(q, 16) || !al(k, 16) || !al(v, 16) || !al(q_gain, 16) || !al(k_gain, 16) || !al(rope, 16) || !al(q_out, 16) ||
+      !al(k_out, 16) || !al(v_out, 16) || !al(codes, 16) || !al(scales, 4) || !al(starts, 4) || !al(past, 4) ||
+      !al(table, 4))
+    return W8A8_EALIGN;
+  PrepareArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.bf16 = dtype == W8A8_OUT_BF16;
+  a.m = (uint32_t)m;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.q_gain = q_gain;
+  a.k_gain = k_gain;
+  a.eps = eps;
+  a.rope = rope;
+  a.rope_rows = rope_rows;
+  a.starts = starts;
+  a.past = past;
+  a.seqs = n_seq;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.codes = codes;
+  a.scales = codes ? scales : nullptr;
+  a.pages = codes ? pages : 0;
+  a.table = codes ? table : nullptr;
+  a.width = codes ? table_width : 0;
+  if (prepare_qk_blocks(a) > kMaxBlocks256) return W8A8_ESHAPE;
+  if (!ready()) return W8A8_EINIT;
+  return hip_status(launch_prepare_qk((hipStream_t)stream, a));
+}
+
+int w8a8_attention_prefill(void* stream, const uint16_t* q, size_t q_stride, const uint16_t* k, size_t k_stride,
+                           const uint16_t* v, size_t v_stride, size_t m, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, const int32_t* starts, uint32_t n_seq, float scale, void* out,
+                           int out_dtype) {
+  if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  if (!(scale > 0.f) || scale > 3e38f) return W8A8_EARG;
+  const int s = check_heads(m, heads, kv_heads, head_dim);
+  if (s != W8A8_OK) return s;
+  if (!good_stride(q_stride, (size_t)heads * head_dim) || !good_stride(k_stride, (size_t)kv_heads * head_dim) ||
+      !good_stride(v_stride, (size_t)kv_heads * head_dim))
+    return W8A8_ESHAPE;
+  if (n_seq == 0 || (!starts && n_seq != 1) || n_seq > kMaxAttentionRows) return W8A8_ESHAPE;
+  if (m == 0) return W8A8_OK;
+  if (!q || !k || !v || !out) return W8A8_ENULL;
+  if (!al(q, 16) || !al(k, 16) || !al(v, 16) || !al(out, 16) || !al(starts, 4)) return W8A8_EALIGN;
+  PrefillArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.m = (uint32_t)m;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.starts = starts;
+  a.seqs = n_seq;
+  a.scale = scale;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  if (attention_prefill_blocks(a) > kMaxBlocks256 / 2) return W8A8_ESHAPE;  // of 512 threads
+  if (!ready()) return W8A8_EINIT;
+  return hip_status(launch_attention_prefill((hipStream_t)stream, a));
+}
+
+// m * splits(m) rises and falls with m while there are splits (fewer than 512
+// workgroups without them): the largest of the smaller batches.
+size_t w8a8_attention_decode_workspace_bytes(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                             uint32_t table_width) {
+  if (check_heads(m, heads, kv_heads, head_dim) != W8A8_OK || table_width > kMaxTableWidth) return 0;
+  size_t most = 0;
+  for (uint32_t n = 1; n <= std::min<size_t>(m, 512); ++n)
+    most = std::max(most, attention_decode_partial_bytes(n, heads, kv_heads, head_dim, table_width));
+  return most;
+}
+
+int w8a8_attention_decode(void* stream, const uint16_t* q, size_t m, uint32_t heads, uint32_t kv_heads,
+                          uint32_t head_dim, const uint8_t* codes, const float* scales, uint32_t pages,
+                          const int32_t* lengths, const int32_t* table, uint32_t table_width, float scale, void* out,
+                          int out_dtype, void* workspace, size_t workspace_bytes) {
+  if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
+  if (!(scale > 0.f) || scale > 3e38f) return W8A8_EARG;
+  const int s = check_heads(m, heads, kv_heads, head_dim);
+  if (s != W8A8_OK) return s;
+  if (pages == 0 || pages > 0x7fffffffu || table_width == 0 || table_width > kMaxTableWidth) return W8A8_ESHAPE;
+  if (attention_decode_blocks((uint32_t)m, heads, kv_heads, table_width) > kMaxBlocks256) return W8A8_ESHAPE;
+  if (m == 0) return W8A8_OK;
+  if (!q || !codes || !scales || !lengths || !table || !out) return W8A8_ENULL;
+  if (!al(q, 16) || !al(codes, 16) || !al(out, 16) || !al(scales, 4) || !al(lengths, 4) || !al(table, 4))
+    return W8A8_EALIGN;
+  const size_t need = attention_decode_partial_bytes((uint32_t)m, heads, kv_heads, head_dim, table_width);
+  if (need && (!workspace || workspace_bytes < need)) return W8A8_EWORKSPACE;
+  if (need && !al(workspace, 256)) return W8A8_EALIGN;
+  if (!ready()) return W8A8_EINIT;
+  DecodeArgs a{};
+  a.q = q;
+  a.m = (uint32_t)m;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.codes = codes;
+  a.scales = scales;
+  a.pages = pages;
+  a.lengths = lengths;
+  a.table = table;
+  a.width = table_width;
+  a.scale = scale;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  return hip_status(launch_attention_decode((hipStream_t)stream, a, workspace));
+}
+
+int w8a8_copy_pages(void* stream, uint8_t* codes, float* scales, uint32_t layers, uint32_t pages, uint32_t kv_heads,
+                    uint32_t head_dim, const int32_t* src, const int32_t* dst, uint32_t n) {
+  const int s = check_heads(0, kv_heads, kv_heads, head_dim);
+  if (s != W8A8_OK) return s;
+  if (layers == 0 || pages == 0 || pages > 0x7fffffffu) return W8A8_ESHAPE;
+  CopyPagesArgs a{};
+  a.codes = codes;
+  a.scales = scales;
+  a.layers = layers;
+  a.pages = pages;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.src = src;
+  a.dst = dst;
+  a.n = n;
+  if (layers > kMaxBlocks256 || n > kMaxBlocks256 || copy_pages_blocks(a) > kMaxBlocks256) return W8A8_ESHAPE;
+  if (n == 0) return W8A8_OK;
+  if (!codes || !scales || !src || !dst) return W8A8_ENULL;
+  if (!al(codes, 16) || !al(scales, 4) || !al(src, 4) || !al(dst, 4)) return W8A8_EALIGN;
+  if (!ready()) return W8A8_EINIT;
+  return hip_status(launch_copy_pages((hipStream_t)stream, a));
+}
+
 int w8a8_synth_i8(void* stream, int8_t* out, size_t n, uint64_t seed, uint64_t stream_id) {
   if (n == 0) return W8A8_OK;
   if (!out) return W8A8_ENULL;

@@ -286,6 +286,80 @@ hipError_t launch_adapters_before(hipStream_t st, const AdapterArgs& a, void* wo
 hipError_t launch_adapters_after(hipStream_t st, const AdapterArgs& a, const int32_t* acc, uint32_t slabs,
                                  const void* workspace);
 
+// ---- attention: between the qkv and the o projection
+// A page of the cache: kPageTokens tokens; of each key/value head the keys' codes
+// [kPageTokens][head_dim], then the values' [head_dim][kPageTokens], e4m3, and a
+// power-of-two scale of each.
+constexpr uint32_t kPageTokens = 64;
+__host__ __device__ constexpr size_t page_head_bytes(uint32_t head_dim) { return (size_t)2 * kPageTokens * head_dim; }
+constexpr uint32_t kMaxHeads = 1024, kMaxAttentionRows = 1u << 24, kMaxTableWidth = 1u << 24;
+
+// prepare_qk (kv_cache.hip): rows' heads normalised, rotated and appended.
+struct PrepareArgs {
+  const void *q, *k, *v;  // [m] rows of heads * dim values, f32 or BF16
+  size_t q_stride, k_stride, v_stride;  // values between rows
+  int bf16;
+  uint32_t m, heads, kv_heads, dim;
+  const float *q_gain, *k_gain;  // [dim], optional
+  float eps;
+  const float* rope;             // [rope_rows][dim]: cosines, then sines
+  uint32_t rope_rows;
+  const int32_t* starts;         // [seqs + 1], or null: one row a sequence
+  const int32_t* past;           // [seqs], or null
+  uint32_t seqs;
+  uint16_t *q_out, *k_out, *v_out;  // dense BF16; k_out and v_out optional
+  uint8_t* codes;                // one layer's cache, optional with scales
+  float* scales;
+  uint32_t pages;
+  const int32_t* table;          // [seqs][width]
+  uint32_t width;
+};
+uint64_t prepare_qk_blocks(const PrepareArgs& a);  // workgroups of the launch
+hipError_t launch_prepare_qk(hipStream_t st, const PrepareArgs& a);
+
+struct CopyPagesArgs {
+  uint8_t* codes;  // [layers][pages][kv_heads][2 * kPageTokens * dim]
+  float* scales;   // [layers][pages][kv_heads][2]
+  uint32_t layers, pages, kv_heads, dim;
+  const int32_t *src, *dst;
+  uint32_t n;
+};
+uint64_t copy_pages_blocks(const CopyPagesArgs& a);
+hipError_t launch_copy_pages(hipStream_t st, const CopyPagesArgs& a);
+
+// attention_prefill.hip
+struct PrefillArgs {
+  const uint16_t *q, *k, *v;  // BF16 rows
+  size_t q_stride, k_stride, v_stride;
+  uint32_t m, heads, kv_heads, dim;
+  const int32_t* starts;  // [seqs + 1], or null: one sequence
+  uint32_t seqs;
+  float scale;
+  void* out;  // [m][heads][dim]
+  int out_dtype;  // F32 or BF16
+};
+uint64_t attention_prefill_blocks(const PrefillArgs& a);
+hipError_t launch_attention_prefill(hipStream_t st, const PrefillArgs& a);
+
+// attention_decode.hip
+struct DecodeArgs {
+  const uint16_t* q;  // [m][heads][dim] BF16
+  uint32_t m, heads, kv_heads, dim;
+  const uint8_t* codes;
+  const float* scales;
+  uint32_t pages;
+  const int32_t* lengths;  // [m]
+  const int32_t* table;    // [m][width]
+  uint32_t width;
+  float scale;
+  void* out;
+  int out_dtype;
+};
+// Bytes of the parts that a batch of exactly m rows leaves for a second launch to join (0: none).
+size_t attention_decode_partial_bytes(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width);
+uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width);
+hipError_t launch_attention_decode(hipStream_t st, const DecodeArgs& a, void* workspace);
+
 hipError_t launch_synth_i8(hipStream_t st, int8_t* out, size_t n, uint64_t seed, uint64_t stream_id);
 hipError_t launch_synth_f32(hipStream_t st, float* out, size_t n, uint64_t seed, uint64_t stream_id,
                             float lo, float hi);

@@ -1,0 +1,293 @@
+// kv_cache.hip -- the cache of keys and values: what prepare_qk appends to it
+// beside normalising and rotating the heads, and copies of its pages.
+//
+//   n = x / sqrt(mean(x^2) + eps) * gain         (a head's x[D]; optional)
+//   (a', b') = (a cos - b sin, b cos + a sin)    (a, b: n's halves)
+//   s = the smallest 2^e, e >= -100, with 448 * 2^e >= the page's largest |x|
+//   code = e4m3(x / s), nearest even; NaN and infinities are NaN codes
+// Norms, rotations and maxima are held in f32 and rounded once: to BF16 in the
+// outputs, to e4m3 in the cache.
+//
+// A scale is a power of two, so that x / s is exact, a larger one later only
+// shifts the codes that are there (exact but for e4m3's subnormals), and the
+// readers' conversion to BF16 (v_cvt_scalef32_pk_bf16_fp8) applies it for free.
+#include <algorithm>
+
+#include "attention.hpp"
+
+namespace w8a8 {
+
+// The scale of a largest magnitude given as f32 bits: 448 = 1.75 * 2^8.
+__device__ __forceinline__ float page_scale(uint32_t top) {
+  const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
+}
+__device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float(0x7f000000u - __float_as_uint(s)); }
+
+// Four codes; |v| <= 448, or v is not finite.
+__device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  return (uint32_t)w;
+}
+__device__ __forceinline__ uint32_t codes_times(uint32_t w, float f) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return codes_of(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+}
+
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = abs_bits(x);
+  return b < kInfBits ? b : 0u;
+}
+
+// A lane's share of a head: four values of each half, so that a rotation's
+// pairs are in one lane.
+struct Share {
+  float lo[4], hi[4];
+};
+
+template <int D, bool BF16IN>
+__device__ __forceinline__ Share load_share(const void* rows, size_t at, int i) {
+  Share x;
+  if constexpr (BF16IN) {
+    const uint16_t* p = (const uint16_t*)rows + at + 4 * i;
+    const v2u a = *(const v2u*)p, b = *(const v2u*)(p + D / 2);
+    x.lo[0] = bf16_lo(a.x), x.lo[1] = bf16_hi(a.x), x.lo[2] = bf16_lo(a.y), x.lo[3] = bf16_hi(a.y);
+    x.hi[0] = bf16_lo(b.x), x.hi[1] = bf16_hi(b.x), x.hi[2] = bf16_lo(b.y), x.hi[3] = bf16_hi(b.y);
+  } else {
+    const float* p = (const float*)rows + at + 4 * i;
+    const v4f a = *(const v4f*)p, b = *(const v4f*)(p + D / 2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.lo[j] = a[j], x.hi[j] = b[j];
+  }
+  return x;
+}
+
+template <int D>
+__device__ __forceinline__ void store_share(uint16_t* out, size_t at, int i, const Share& x) {
+  uint16_t* p = out + at + 4 * i;
+  *(v2u*)p = v2u{pack_bf16(x.lo[0], x.lo[1]), pack_bf16(x.lo[2], x.lo[3])};
+  *(v2u*)(p + D / 2) = v2u{pack_bf16(x.hi[0], x.hi[1]), pack_bf16(x.hi[2], x.hi[3])};
+}
+
+// The sum over the D / 8 lanes of a head (8 or 16, within a DPP row).
+template <int D>
+__device__ __forceinline__ float head_sum(float v) {
+  auto add = [&](auto other) { v = v + other; };
+  add(__uint_as_float(dpp_u32<0xB1>(__float_as_uint(v))));
+  add(__uint_as_float(dpp_u32<0x4E>(__float_as_uint(v))));
+  add(__uint_as_float(dpp_u32<0x141>(__float_as_uint(v))));
+  if constexpr (D == 128) add(__uint_as_float(dpp_u32<0x140>(__float_as_uint(v))));
+  return v;
+}
+
+template <int D>
+__device__ __forceinline__ void norm_rotate(Share& x, const float* gain, float eps, const float* rope, uint32_t rope_rows,
+                                            uint32_t pos, int i) {
+  if (gain) {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x.lo[j], x.lo[j], __builtin_fmaf(x.hi[j], x.hi[j], ss));
+    // v_rsq_f32: one unit of the last place
+    const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<D>(ss), 1.0f / D, eps));
+    const v4f a = *(const v4f*)(gain + 4 * i), b = *(const v4f*)(gain + D / 2 + 4 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.lo[j] = x.lo[j] * inv * a[j], x.hi[j] = x.hi[j] * inv * b[j];
+  }
+  const bool known = pos < rope_rows;
+  const float* r = rope + (size_t)(known ? pos : 0u) * D + 4 * i;
+  const v4f c = *(const v4f*)r, s = *(const v4f*)(r + D / 2);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = x.lo[j], b = x.hi[j];
+    x.lo[j] = known ? __builtin_fmaf(a, c[j], -(b * s[j])) : __builtin_nanf("");
+    x.hi[j] = known ? __builtin_fmaf(b, c[j], a * s[j]) : __builtin_nanf("");
+  }
+}
+
+constexpr uint32_t kPrepareHeads = 4;  // query heads of one workgroup
+
+// A unit is the rows that one sequence brings to one page.  Of a unit, one
+// workgroup takes a key/value head (its 64 x D keys and values: whole blocks of
+// the cache, so that their scale is one workgroup's) and one takes kPrepareHeads
+// query heads.  D / 8 lanes hold a head.
+template <int D, bool BF16IN>
+__global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t blocks) {
+  constexpr int LPH = D / 8, GROUPS = 256 / LPH, SLOTS = 64 / GROUPS;  // lanes of a head, heads in flight, tokens of a group
+  __shared__ uint32_t red[2][4];
+  const uint32_t unit = blockIdx.x / blocks, part = blockIdx.x % blocks;
+  const int tid = threadIdx.x, i = tid % LPH, group = tid / LPH;
+  uint32_t seq = unit, index = 0, lo = unit, n = 1;
+  if (a.starts) {
+    const auto count = [&](uint32_t s) {
+      const RowRange r = rows_of(a.starts, s, a.m);
+      const uint32_t p = a.past ? (uint32_t)max(a.past[s], 0) : 0u, rows = r.hi - r.lo;
+      return rows ? (p + rows - 1) / kPageTokens - p / kPageTokens + 1 : 0u;
+    };
+    if (!find_unit(unit, a.seqs, count, &seq, &index)) return;
+    const RowRange r = rows_of(a.starts, seq, a.m);
+    lo = r.lo;
+    n = r.hi - r.lo;
+  }
+  const uint32_t past = a.past ? (uint32_t)max(a.past[seq], 0) : 0u;
+  const uint32_t page = past / kPageTokens + index;  // of the sequence
+  const uint32_t first = max(past, page * kPageTokens), last = min(past + n, (page + 1) * kPageTokens);
+  const uint32_t n0 = first - page * kPageTokens, n1 = last - page * kPageTokens;  // the unit's slots of the page
+  const uint32_t row0 = lo + (first - past);
+
+  if (part >= a.kv_heads) {
+    const uint32_t h0 = (part - a.kv_heads) * kPrepareHeads, heads = min(kPrepareHeads, a.heads - h0);
+    for (uint32_t u = group; u < (n1 - n0) * heads; u += GROUPS) {
+      const uint32_t t = u / heads, h = h0 + u % heads;
+      Share x = load_share<D, BF16IN>(a.q, (size_t)(row0 + t) * a.q_stride + (size_t)h * D, i);
+      norm_rotate<D>(x, a.q_gain, a.eps, a.rope, a.rope_rows, first + t, i);
+      store_share<D>(a.q_out, ((size_t)(row0 + t) * a.heads + h) * D, i, x);
+    }
+    return;
+  }
+
+  const uint32_t h = part;
+  Share k[SLOTS], v[SLOTS];
+  uint32_t k_top = 0, v_top = 0;
+#pragma unroll
+  for (int j = 0; j < SLOTS; ++j) {
+    const uint32_t slot = SLOTS * group + j;
+    k[j] = v[j] = Share{};
+    if (slot >= n0 && slot < n1) {  // the same for a head's lanes
+      const size_t row = row0 + (slot - n0);
+      k[j] = load_share<D, BF16IN>(a.k, row * a.k_stride + (size_t)h * D, i);
+      v[j] = load_share<D, BF16IN>(a.v, row * a.v_stride + (size_t)h * D, i);
+      norm_rotate<D>(k[j], a.k_gain, a.eps, a.rope, a.rope_rows, first + (slot - n0), i);
+      if (a.k_out) store_share<D>(a.k_out, (row * a.kv_heads + h) * D, i, k[j]);
+      if (a.v_out) store_share<D>(a.v_out, (row * a.kv_heads + h) * D, i, v[j]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      k_top = max(k_top, max(finite_bits(k[j].lo[e]), finite_bits(k[j].hi[e])));
+      v_top = max(v_top, max(finite_bits(v[j].lo[e]), finite_bits(v[j].hi[e])));
+    }
+  }
+  if (!a.codes || page >= a.width) return;
+  const int32_t id = a.table[(size_t)seq * a.width + page];
+  if (id < 0 || (uint32_t)id >= a.pages) return;
+  uint8_t* const codes = a.codes + ((size_t)id * a.kv_heads + h) * page_head_bytes(D);
+  uint8_t* const vcodes = codes + kPageTokens * D;
+  float* const scales = a.scales + ((size_t)id * a.kv_heads + h) * 2;
+  const float k_was = n0 ? scales[0] : 0.f, v_was = n0 ? scales[1] : 0.f;
+
+  k_top = wave_max_u32(k_top);
+  v_top = wave_max_u32(v_top);
+  if ((tid & 63) == 0) red[0][tid >> 6] = k_top, red[1][tid >> 6] = v_top;
+  __syncthreads();
+  k_top = max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3]));
+  v_top = max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]));
+  const float k_s = fmaxf(page_scale(k_top), k_was), v_s = fmaxf(page_scale(v_top), v_was);
+  if (tid == 0) scales[0] = k_s, scales[1] = v_s;
+
+  // a larger scale: the codes that are there move down
+  if (n0 && k_s > k_was) {
+    const float f = k_was * pow2_inverse(k_s);
+    for (uint32_t w = tid; w < n0 * (D / 4); w += 256) ((uint32_t*)codes)[w] = codes_times(((uint32_t*)codes)[w], f);
+  }
+  if (n0 && v_s > v_was) {
+    const float f = v_was * pow2_inverse(v_s);
+    for (uint32_t w = tid; w < D * (kPageTokens / 4); w += 256) {
+      const uint32_t slot = w % (kPageTokens / 4) * 4;
+      if (slot >= n0) continue;
+      const uint32_t keep = n0 - slot < 4 ? 0xffffffffu << 8 * (n0 - slot) : 0u;  // later slots' bytes
+      uint32_t* const p = (uint32_t*)vcodes + w;
+      *p = (codes_times(*p, f) & ~keep) | (*p & keep);
+    }
+  }
+  __syncthreads();  // a word of the values' codes may hold old tokens and new ones
+
+  const float k_r = pow2_inverse(k_s), v_r = pow2_inverse(v_s);
+  uint32_t held[8] = {};  // of each of the lane's columns, its slots' value codes
+#pragma unroll
+  for (int j = 0; j < SLOTS; ++j) {
+    const uint32_t slot = SLOTS * group + j;
+    const Share &x = k[j], &y = v[j];
+    if (slot >= n0 && slot < n1) {
+      uint32_t* const p = (uint32_t*)(codes + slot * D) + i;
+      p[0] = codes_of(x.lo[0] * k_r, x.lo[1] * k_r, x.lo[2] * k_r, x.lo[3] * k_r);
+      p[D / 8] = codes_of(x.hi[0] * k_r, x.hi[1] * k_r, x.hi[2] * k_r, x.hi[3] * k_r);
+    }
+    const uint32_t a0 = codes_of(y.lo[0] * v_r, y.lo[1] * v_r, y.lo[2] * v_r, y.lo[3] * v_r);
+    const uint32_t a1 = codes_of(y.hi[0] * v_r, y.hi[1] * v_r, y.hi[2] * v_r, y.hi[3] * v_r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      held[e] |= (a0 >> 8 * e & 0xffu) << 8 * j;
+      held[4 + e] |= (a1 >> 8 * e & 0xffu) << 8 * j;
+    }
+  }
+  const uint32_t s0 = SLOTS * group;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    uint8_t* const p = vcodes + (size_t)(4 * i + e % 4 + e / 4 * (D / 2)) * kPageTokens + s0;
+    if (s0 >= n0 && s0 + SLOTS <= n1) {
+      if constexpr (SLOTS == 4)
+        *(uint32_t*)p = held[e];
+      else
+        *(uint16_t*)p = (uint16_t)held[e];
+    } else {
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j)
+        if (s0 + j >= n0 && s0 + j < n1) p[j] = (uint8_t)(held[e] >> 8 * j);
+    }
+  }
+}
+
+static uint32_t prepare_parts(const PrepareArgs& a) { return a.kv_heads + (a.heads + kPrepareHeads - 1) / kPrepareHeads; }
+
+// Every unit has a row, and a sequence's pages hold 64 of its rows but for two.
+uint64_t prepare_qk_blocks(const PrepareArgs& a) {
+  const uint64_t units = a.starts ? std::min<uint64_t>(a.m, a.m / kPageTokens + (uint64_t)2 * a.seqs) : a.m;
+  return units * prepare_parts(a);
+}
+
+hipError_t launch_prepare_qk(hipStream_t st, const PrepareArgs& a) {
+  const uint32_t blocks = prepare_parts(a);
+  const dim3 grid((uint32_t)prepare_qk_blocks(a));
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, blocks); };
+  if (a.dim == 128)
+    a.bf16 ? go(prepare_qk_kernel<128, true>) : go(prepare_qk_kernel<128, false>);
+  else
+    a.bf16 ? go(prepare_qk_kernel<64, true>) : go(prepare_qk_kernel<64, false>);
+  return hipGetLastError();
+}
+
+constexpr uint32_t kCopyBytes = 16384;  // of one workgroup
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(CopyPagesArgs a, uint32_t chunks) {
+  const uint32_t chunk = blockIdx.x % chunks, pair = blockIdx.x / chunks % a.n, layer = blockIdx.x / chunks / a.n;
+  const int32_t from = a.src[pair], to = a.dst[pair];
+  if (from < 0 || to < 0 || (uint32_t)from >= a.pages || (uint32_t)to >= a.pages || from == to) return;
+  const size_t bytes = a.kv_heads * page_head_bytes(a.dim);
+  const size_t f = (size_t)layer * a.pages + from, t = (size_t)layer * a.pages + to;
+  const uint8_t* const p = a.codes + f * bytes;
+  uint8_t* const q = a.codes + t * bytes;
+  const size_t at = (size_t)chunk * kCopyBytes + threadIdx.x * 16;
+  v4u w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (at + j * 4096 < bytes) w[j] = __builtin_nontemporal_load((const v4u*)(p + at + j * 4096));
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (at + j * 4096 < bytes) __builtin_nontemporal_store(w[j], (v4u*)(q + at + j * 4096));
+  if (chunk == 0)
+    for (uint32_t s = threadIdx.x; s < 2 * a.kv_heads; s += 256)
+      a.scales[t * 2 * a.kv_heads + s] = a.scales[f * 2 * a.kv_heads + s];
+}
+
+static uint32_t copy_chunks(const CopyPagesArgs& a) {
+  return (uint32_t)((a.kv_heads * page_head_bytes(a.dim) + kCopyBytes - 1) / kCopyBytes);
+}
+uint64_t copy_pages_blocks(const CopyPagesArgs& a) { return (uint64_t)a.layers * a.n * copy_chunks(a); }
+
+hipError_t launch_copy_pages(hipStream_t st, const CopyPagesArgs& a) {
+  hipLaunchKernelGGL(copy_pages_kernel, dim3((uint32_t)copy_pages_blocks(a)), dim3(256), 0, st, a, copy_chunks(a));
+  return hipGetLastError();
+}
+
+}  // namespace w8a8

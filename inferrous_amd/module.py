@@ -27,6 +27,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import W8A8Error, check, lib
+from .kv_cache import KvCache
 from .runtime import CudaContext, CudaStream, DeviceBuffer, is_capturing
 
 _OUT = {np.dtype(np.float32): _lib.OUT_F32, np.dtype(np.uint16): _lib.OUT_BF16,
@@ -72,6 +73,16 @@ def _needs(buf: DeviceBuffer, dtype: np.dtype, need: int, what: str):
         raise TypeError(f"{what} must be {dtype}, got {buf.dtype}")
     if len(buf) < need:
         raise ValueError(f"{what} has {len(buf)} elements, needs at least {need}")
+
+
+def _table_width(table: DeviceBuffer | None, seqs: int) -> int:
+    """Pages of a row of a page table of seqs rows."""
+    if table is None:
+        raise ValueError("a page table is required")
+    _needs(table, _I32, seqs, "table")
+    if seqs and len(table) % seqs:
+        raise ValueError("the table must hold one row of pages a sequence")
+    return len(table) // seqs if seqs else 0
 
 
 class LoadedModule:
@@ -681,15 +692,17 @@ class LoadedModule:
         check(lib().w8a8_linear_sequence_reset(), "linear_sequence_reset")
 
     # ------------------------------------------------------------ routed layers
-    def _routed_workspace(self, stream, size_of, *shape):
+    def _routed_workspace(self, stream, size_of, *shape, none_if_zero=False):
         """The stream's workspace (the split-K one: calls on a stream follow
         each other), at least size_of(*shape) bytes, which a shape asks for
-        once."""
+        once; none_if_zero: (None, 0) for a shape that needs none."""
         nbytes = self._routed_bytes.get((size_of, shape))
         if nbytes is None:
             if len(self._routed_bytes) >= 4096:   # batches of any number of rows
                 self._routed_bytes.clear()
             nbytes = self._routed_bytes[(size_of, shape)] = getattr(lib(), size_of)(*shape)
+        if none_if_zero and not nbytes:
+            return None, 0
         key = stream.handle if stream is not None else None
         cur = self._gemm_ws.get(key)
         if cur is None or cur.nbytes < nbytes:
@@ -824,6 +837,158 @@ class LoadedModule:
                                          ids.ptr, a.ptr, b.ptr, scaling.ptr, rank, count,
                                          None if residual is None else residual.ptr, out.ptr, _dtype_code(out), wp,
                                          wb), "linear_adapters")
+
+    # ------------------------------------------------------------ attention
+    def prepare_qk(self, stream, q: DeviceBuffer, heads: int, kv_heads: int, head_dim: int, rope: DeviceBuffer,
+                   q_out: DeviceBuffer, k: DeviceBuffer | None = None, v: DeviceBuffer | None = None,
+                   q_gain: DeviceBuffer | None = None, k_gain: DeviceBuffer | None = None,
+                   starts: DeviceBuffer | None = None, past: DeviceBuffer | None = None,
+                   k_out: DeviceBuffer | None = None, v_out: DeviceBuffer | None = None,
+                   cache: KvCache | None = None, table: DeviceBuffer | None = None, layer: int = 0,
+                   eps: float = 1e-6) -> None:
+        """Query and key heads normalised and rotated, keys and values into the
+        cache (w8a8_prepare_qk; `prepare_qk` with the caches of
+        src/kernels.rs:1290-1488).  ``q`` is a qkv projection's rows [M, (heads
+        + 2 kv_heads) * head_dim], or the query rows alone beside ``k`` and
+        ``v`` (all float32 or uint16 BF16); M comes from ``q_out`` (uint16 [M,
+        heads, head_dim]).  ``rope`` is float32 [positions, head_dim], cosines
+        then sines; ``q_gain`` / ``k_gain`` float32 [head_dim], None for no
+        norm.  ``starts`` (int32 [S + 1]): the sequences' rows, None for one
+        row each; ``past`` (int32 [S]): their tokens so far, None for none.
+        ``k_out`` / ``v_out`` (uint16 [M, kv_heads, head_dim]) and ``cache``
+        with ``table`` (int32 [S, width]) are optional."""
+        heads, kv_heads, dim = int(heads), int(kv_heads), int(head_dim)
+        width, kv_width = heads * dim, kv_heads * dim
+        if width <= 0 or kv_width <= 0 or len(q_out) % width:
+            raise ValueError("prepare_qk: q_out must hold M rows of heads * head_dim")
+        m = len(q_out) // width
+        seqs = m if starts is None else len(starts) - 1
+        dtype = q.dtype
+        code = _OUT.get(dtype)
+        if dtype != _F32 and dtype != _U16:
+            raise TypeError(f"q dtype {dtype} not supported (float32/uint16)")
+        _needs(q_out, _U16, 0, "q_out")
+        if seqs < 0 or (starts is not None and starts.dtype != _I32):
+            raise TypeError("starts must be int32 [S + 1]")
+        if (k is None) != (v is None):
+            raise ValueError("k and v go together")
+        size = q.dtype.itemsize
+        if k is None:
+            stride = width + 2 * kv_width
+            _check_len(q, m * stride, "q")
+            strides = (stride, stride, stride)
+            kp, vp = q.ptr + width * size, q.ptr + (width + kv_width) * size
+        else:
+            strides = (width, kv_width, kv_width)
+            _check_len(q, m * width, "q")
+            _needs(k, dtype, m * kv_width, "k")
+            _needs(v, dtype, m * kv_width, "v")
+            kp, vp = k.ptr, v.ptr
+        _needs(rope, _F32, dim, "rope")
+        for buf, dt, need, what in ((q_gain, _F32, dim, "q_gain"), (k_gain, _F32, dim, "k_gain"),
+                                    (past, _I32, seqs, "past"), (k_out, _U16, m * kv_width, "k_out"),
+                                    (v_out, _U16, m * kv_width, "v_out")):
+            if buf is not None:
+                _needs(buf, dt, need, what)
+        codes = scales = table_ptr = None
+        pages = columns = 0
+        if cache is not None:
+            if cache.kv_heads != kv_heads or cache.head_dim != dim:
+                raise ValueError("the cache has other heads")
+            columns = _table_width(table, seqs)
+            (codes, scales), pages, table_ptr = cache.layer(layer), cache.pages, table.ptr
+        elif table is not None:
+            raise ValueError("a table names the pages of a cache")
+        if m == 0 or seqs == 0:
+            return
+        ptr = lambda b: None if b is None else b.ptr  # noqa: E731
+        check(lib().w8a8_prepare_qk(_h(stream), q.ptr, strides[0], kp, strides[1], vp, strides[2], code, m, heads,
+                                    kv_heads, dim, ptr(q_gain), ptr(k_gain), eps, rope.ptr, len(rope) // dim,
+                                    ptr(starts), ptr(past), seqs, q_out.ptr, ptr(k_out), ptr(v_out), codes, scales,
+                                    pages, table_ptr, columns), "prepare_qk")
+
+    def attention_prefill(self, stream, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer, heads: int, kv_heads: int,
+                          head_dim: int, out: DeviceBuffer, starts: DeviceBuffer | None = None,
+                          scale: float | None = None, v_stride: int | None = None) -> None:
+        """Causal attention of whole prompts packed one after another
+        (w8a8_attention_prefill; `attention_prefill` of src/kernels.rs:1489-2161):
+        ``q`` (uint16 BF16 [M, heads, head_dim]) and ``k``, ``v`` (uint16 [M,
+        kv_heads, head_dim]) as ``prepare_qk`` leaves them, into ``out``
+        (float32 or uint16, as q).  ``v_stride``: values between the rows of
+        ``v``, for one that is columns of a projection's output.  ``starts``
+        (int32 [S + 1]): the sequences' rows, None for one sequence.  ``scale``:
+        head_dim ** -0.5 by default."""
+        heads, kv_heads, dim = int(heads), int(kv_heads), int(head_dim)
+        width, kv_width = heads * dim, kv_heads * dim
+        if width <= 0 or kv_width <= 0 or len(out) % width:
+            raise ValueError("attention_prefill: out must hold M rows of heads * head_dim")
+        m, dtype = len(out) // width, out.dtype
+        if dtype != _F32 and dtype != _U16:
+            raise TypeError(f"out dtype {dtype} not supported (float32/uint16)")
+        stride = kv_width if v_stride is None else int(v_stride)
+        _needs(q, _U16, m * width, "q")
+        _needs(k, _U16, m * kv_width, "k")
+        _needs(v, _U16, (m - 1) * stride + kv_width if m else 0, "v")
+        seqs = 1
+        if starts is not None:
+            _needs(starts, _I32, 1, "starts")
+            seqs = len(starts) - 1
+        if m == 0 or seqs == 0:
+            return
+        check(lib().w8a8_attention_prefill(_h(stream), q.ptr, width, k.ptr, kv_width, v.ptr, stride, m, heads,
+                                           kv_heads, dim, None if starts is None else starts.ptr, seqs,
+                                           dim ** -0.5 if scale is None else scale, out.ptr, _OUT[dtype]),
+              "attention_prefill")
+
+    @staticmethod
+    def attention_decode_workspace_bytes(max_rows: int, heads: int, kv_heads: int, head_dim: int,
+                                         table_width: int) -> int:
+        """What ``reserve_workspace`` needs for ``attention_decode`` of up to max_rows rows."""
+        return lib().w8a8_attention_decode_workspace_bytes(max_rows, heads, kv_heads, head_dim, table_width)
+
+    def attention_decode(self, stream, q: DeviceBuffer, cache: KvCache, lengths: DeviceBuffer, table: DeviceBuffer,
+                         heads: int, out: DeviceBuffer, layer: int = 0, scale: float | None = None) -> None:
+        """One query row of each sequence over the cache (w8a8_attention_decode;
+        `attention` of src/kernels.rs:1489-2161): ``q`` (uint16 BF16 [M,
+        heads, head_dim]) over the first ``lengths`` (int32 [M]) tokens of the
+        pages that ``table`` (int32 [M, width]) names, into ``out`` (float32 or
+        uint16, as q).  ``scale``: head_dim ** -0.5 by default.  The scratch
+        space is the stream's workspace;
+        ``reserve_workspace(attention_decode_workspace_bytes(...))`` before
+        capturing a graph."""
+        heads, dim, kv_heads = int(heads), cache.head_dim, cache.kv_heads
+        width, dtype = heads * dim, out.dtype
+        if width <= 0 or len(out) % width:
+            raise ValueError("attention_decode: out must hold M rows of heads * head_dim")
+        m = len(out) // width
+        if dtype != _F32 and dtype != _U16:
+            raise TypeError(f"out dtype {dtype} not supported (float32/uint16)")
+        _needs(q, _U16, m * width, "q")
+        _needs(lengths, _I32, m, "lengths")
+        columns = _table_width(table, m)
+        codes, scales = cache.layer(layer)
+        if m == 0:
+            return
+        if heads % kv_heads:
+            raise ValueError("the query heads must be a multiple of the cache's heads")
+        wp, wb = self._routed_workspace(stream, "w8a8_attention_decode_workspace_bytes", m, heads, kv_heads, dim,
+                                        columns, none_if_zero=True)
+        check(lib().w8a8_attention_decode(_h(stream), q.ptr, m, heads, kv_heads, dim, codes, scales, cache.pages,
+                                          lengths.ptr, table.ptr, columns, dim ** -0.5 if scale is None else scale,
+                                          out.ptr, _OUT[dtype], wp, wb), "attention_decode")
+
+    def copy_pages(self, stream, cache: KvCache, src: DeviceBuffer, dst: DeviceBuffer) -> None:
+        """Pages ``src`` to ``dst`` (int32, one length) of every layer of a
+        cache (w8a8_copy_pages; no counterpart in the reference): the pairs
+        that ``PagePool.extend`` and ``PagePool.compact`` return."""
+        _needs(src, _I32, 0, "src")
+        _needs(dst, _I32, 0, "dst")
+        n = len(src)
+        if len(dst) != n:
+            raise ValueError("copy_pages: src and dst must have one length")
+        if n:
+            check(lib().w8a8_copy_pages(_h(stream), cache.codes.ptr, cache.scales.ptr, cache.layers, cache.pages,
+                                        cache.kv_heads, cache.head_dim, src.ptr, dst.ptr, n), "copy_pages")
 
     # ------------------------------------------------------------ synthetic
     def synth_i8(self, stream, out: DeviceBuffer, seed: int, stream_id: int) -> None:
