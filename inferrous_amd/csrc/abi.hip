@@ -1262,12 +1262,17 @@ int w8a8_attention_prefill(void* stream, const uint16_t* q, size_t q_stride, con
   return hip_status(launch_attention_prefill((hipStream_t)stream, a));
 }
 
-// m * splits(m) rises and falls with m while there are splits (fewer than 512
-// workgroups without them): the largest of the smaller batches.
+static int check_decode_shape(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t table_width) {
+  const int s = check_heads(m, heads, kv_heads, head_dim);
+  if (s != W8A8_OK) return s;
+  if (table_width == 0 || table_width > kMaxTableWidth || m * table_width > 0x7fffffffu) return W8A8_ESHAPE;
+  return attention_decode_blocks((uint32_t)m, heads, kv_heads, table_width) > kMaxBlocks256 ? W8A8_ESHAPE : W8A8_OK;
+}
+
 size_t w8a8_attention_decode_workspace_bytes(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                                              uint32_t table_width) {
-  if (check_heads(m, heads, kv_heads, head_dim) != W8A8_OK || table_width > kMaxTableWidth) return 0;
-  size_t most = 0;
+  if (m == 0 || check_decode_shape(m, heads, kv_heads, head_dim, table_width) != W8A8_OK) return 0;
+  size_t most = 0;  // the need rises and falls with m while there are splits, fewer than 512 rows
   for (uint32_t n = 1; n <= std::min<size_t>(m, 512); ++n)
     most = std::max(most, attention_decode_partial_bytes(n, heads, kv_heads, head_dim, table_width));
   return most;
@@ -1279,10 +1284,9 @@ int w8a8_attention_decode(void* stream, const uint16_t* q, size_t m, uint32_t he
                           int out_dtype, void* workspace, size_t workspace_bytes) {
   if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
   if (!(scale > 0.f) || scale > 3e38f) return W8A8_EARG;
-  const int s = check_heads(m, heads, kv_heads, head_dim);
+  const int s = check_decode_shape(m, heads, kv_heads, head_dim, table_width);
   if (s != W8A8_OK) return s;
-  if (pages == 0 || pages > 0x7fffffffu || table_width == 0 || table_width > kMaxTableWidth) return W8A8_ESHAPE;
-  if (attention_decode_blocks((uint32_t)m, heads, kv_heads, table_width) > kMaxBlocks256) return W8A8_ESHAPE;
+  if (pages == 0 || pages > 0x7fffffffu) return W8A8_ESHAPE;
   if (m == 0) return W8A8_OK;
   if (!q || !codes || !scales || !lengths || !table || !out) return W8A8_ENULL;
   if (!al(q, 16) || !al(codes, 16) || !al(out, 16) || !al(scales, 4) || !al(lengths, 4) || !al(table, 4))

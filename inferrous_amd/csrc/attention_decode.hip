@@ -3,8 +3,8 @@
 //   s_j = scale * q . (k_scale k_j),  o = sum_j exp(s_j - m) (v_scale v_j) / sum_j exp(s_j - m)
 //
 // The cache's bytes bound it: 2 * D a token and key/value head, read once.  A
-// workgroup takes a sequence's key/value head and a run of its pages, a wave
-// every fourth page of the run; up to 16 of the query heads that share the
+// workgroup takes a sequence's key/value head, alone or with other workgroups that
+// share its pages, and a wave one page at a time; up to 16 of the query heads that share the
 // key/value head are the 16 columns of v_mfma_f32_16x16x32_bf16, which so
 // costs the same for one head or 16.
 //
@@ -32,17 +32,24 @@ constexpr uint32_t kDecodeHeads = 16;  // query heads of a workgroup
 
 struct DecodeSplit {
   uint32_t tiles;   // workgroups a key/value head's query heads take
-  uint32_t splits;  // runs of a sequence's pages
+  uint32_t chunk;   // pages of a workgroup
+  uint32_t splits;  // workgroups of the widest sequence
 };
 
-// Runs of pages: enough workgroups for twice the CUs where a run keeps eight
-// pages of the widest sequence or more.
+constexpr uint32_t kMaxSplits = 64;
+// Splits that a join of so many waves a head takes.
+constexpr uint32_t join_splits(int waves) { return waves == 1 ? 16 : kMaxSplits; }
+
+// Splits: two workgroups a CU where a wave keeps a page.  More, where the longest
+// sequences bound a large batch, gains less there than the join costs: 64 sequences
+// of up to 4096 tokens, 59 us alone, 60-65 us in 2 to 8 splits.
 static DecodeSplit decode_split(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width) {
   DecodeSplit d;
   d.tiles = (heads / kv_heads + kDecodeHeads - 1) / kDecodeHeads;
-  const uint64_t units = (uint64_t)m * kv_heads * d.tiles, want = 2 * 256;
-  const uint32_t most = std::max(1u, std::min(64u, width / 8));
-  d.splits = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, (want + units - 1) / units));
+  const uint64_t units = (uint64_t)m * kv_heads * d.tiles;
+  const uint32_t splits = (uint32_t)std::min<uint64_t>(kMaxSplits, std::max<uint64_t>(1, 512 / units));
+  d.chunk = ((width + splits - 1) / splits + kDecodeWaves - 1) / kDecodeWaves * kDecodeWaves;
+  d.splits = (width + d.chunk - 1) / d.chunk;
   return d;
 }
 
@@ -56,20 +63,42 @@ __device__ __forceinline__ v4u widen(uint32_t a, uint32_t b, float s) {
              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false)),
              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true))};
 }
-// Across the four lane groups of a head's column.
-__device__ __forceinline__ float groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, kWave));
-  return fmaxf(v, __shfl_xor(v, 32, kWave));
-}
-__device__ __forceinline__ float groups_sum(float v) {
-  v += __shfl_xor(v, 16, kWave);
-  return v + __shfl_xor(v, 32, kWave);
+// Four neighbouring outputs.
+__device__ __forceinline__ void store4(const DecodeArgs& a, size_t at, v4f x) {
+  const uint32_t lo = pack_bf16(x[0], x[1]), hi = pack_bf16(x[2], x[3]);
+  if (a.out_dtype == W8A8_OUT_BF16)
+    *(v2u*)((uint16_t*)a.out + at) = v2u{lo, hi};
+  else
+    *(v4u*)((float*)a.out + at) = v4u{lo << 16, lo & 0xffff0000u, hi << 16, hi & 0xffff0000u};
 }
 
-// partial: [m][kv_heads][tiles][splits] of {float m, l}[16] and O[16][D], or null
-// with one split.
+// Across the four lane groups of a head's column (rows of 16 lanes): a row beside
+// its neighbour, then a half beside the other.
+template <class Op>
+__device__ __forceinline__ float across_groups(float v, Op op) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+__device__ __forceinline__ float groups_max(float v) {
+  return across_groups(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  return across_groups(v, [](float a, float b) { return a + b; });
+}
+
+// A page's codes as the two products take them.
 template <int D>
-__global__ __launch_bounds__(256) void attention_decode_kernel(DecodeArgs a, DecodeSplit d, float* partial) {
+struct PageCodes {
+  v4u k[4][D / 64], v[D / 16];
+  float scale;  // of the keys in even lanes, of the values in odd ones
+};
+
+// partial: of sequences with more pages than a chunk, of each row, head and split its
+// unscaled sum o[D], then of each {m, l}.
+template <int D>
+__global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, DecodeSplit d, float* partial) {
   constexpr int HALVES = D / 64, TILES = D / 16;
   __shared__ float sh_m[4][16], sh_l[4][16];
   __shared__ float sh_o[4][16][D + 4];
@@ -85,9 +114,30 @@ __global__ __launch_bounds__(256) void attention_decode_kernel(DecodeArgs a, Dec
   const uint32_t head0 = h * group + tile * kDecodeHeads, live = min(kDecodeHeads, group - tile * kDecodeHeads);
 
   const int32_t* const table = a.table + (size_t)row * a.width;
+  uint32_t p = split * d.chunk + wave;  // the wave's first page: it does not wait for the length
+  // The numbers of the wave's next 64 pages, one a lane.  (Vector loads, as the
+  // scales' are: a scalar load's result is waited for with all that are in flight,
+  // and these miss the caches.)
+  const auto ids_from = [&](uint32_t page) { return table[min(page + lane * kDecodeWaves, a.width - 1)]; };
+  int32_t ids = ids_from(p);
   const uint32_t len = min((uint32_t)max(a.lengths[row], 0), a.width * kPageTokens);
-  const uint32_t pages = (len + kPageTokens - 1) / kPageTokens, run = (pages + d.splits - 1) / d.splits;
-  const uint32_t p0 = min(split * run, pages), p1 = min(p0 + run, pages);
+  const uint32_t pages = (len + kPageTokens - 1) / kPageTokens, end = min(pages, (split + 1) * d.chunk);
+  if (split != 0 && split * d.chunk >= pages) return;  // the sequence ends before
+  const auto known = [&](int32_t i) { return i >= 0 && (uint32_t)i < a.pages; };
+
+  const auto load = [&](PageCodes<D>& x, int32_t i) {
+    const size_t at = (size_t)(known(i) ? i : 0) * a.kv_heads + h;
+    const uint8_t* const codes = a.codes + at * page_head_bytes(D);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int f = 0; f < HALVES; ++f)
+        x.k[t][f] = *(const v4u*)(codes + (16 * (c >> 2) + 4 * t + (c & 3)) * D + 64 * f + 16 * g);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      x.v[t] = *(const v4u*)(codes + kPageTokens * D + (16 * t + c) * kPageTokens + 16 * g);
+    x.scale = a.scales[2 * at + (lane & 1)];
+  };
 
   v4u q[2 * HALVES];
 #pragma unroll
@@ -97,36 +147,25 @@ __global__ __launch_bounds__(256) void attention_decode_kernel(DecodeArgs a, Dec
       q[s] = *(const v4u*)(a.q + ((size_t)row * a.heads + head0 + c) * D + 64 * (s / 2) + 16 * g + 8 * (s % 2));
   }
   const float to_log2 = a.scale * kLog2e;
-  const size_t head_bytes = page_head_bytes(D);
   float m = -__builtin_inff(), l = 0.f;
   v4f o[TILES] = {};
-  for (uint32_t p = p0 + wave; p < p1; p += kDecodeWaves) {
-    const int32_t id = table[p];
-    if (id < 0 || (uint32_t)id >= a.pages) continue;
-    const uint8_t* const codes = a.codes + ((size_t)id * a.kv_heads + h) * head_bytes;
-    const float* const scales = a.scales + ((size_t)id * a.kv_heads + h) * 2;
-    const float ks = scales[0], vs = scales[1];
-    v4u k[4][HALVES], v[TILES];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int f = 0; f < HALVES; ++f)
-        k[t][f] = *(const v4u*)(codes + (16 * (c >> 2) + 4 * t + (c & 3)) * D + 64 * f + 16 * g);
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) v[t] = *(const v4u*)(codes + kPageTokens * D + (16 * t + c) * kPageTokens + 16 * g);
+
+  const auto attend = [&](PageCodes<D>& x, uint32_t page) {
+    const float ks = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x.scale), 0));
+    const float vs = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x.scale), 1));
     float s[16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       v4f acc = {};
 #pragma unroll
       for (int f = 0; f < HALVES; ++f) {
-        acc = mfma16(widen(k[t][f].x, k[t][f].y, ks), q[2 * f], acc);
-        acc = mfma16(widen(k[t][f].z, k[t][f].w, ks), q[2 * f + 1], acc);
+        acc = mfma16(widen(x.k[t][f].x, x.k[t][f].y, ks), q[2 * f], acc);
+        acc = mfma16(widen(x.k[t][f].z, x.k[t][f].w, ks), q[2 * f + 1], acc);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i] * to_log2;
     }
-    const uint32_t left = len - p * kPageTokens;  // tokens of the page, 64 but in the last one
+    const uint32_t left = len - page * kPageTokens;  // tokens of the page, 64 but in the last one
     if (left < kPageTokens) {
       // what lies behind the last token may be any bytes, NaN among them
       const int mine = (int)left - 16 * g;
@@ -137,7 +176,7 @@ __global__ __launch_bounds__(256) void attention_decode_kernel(DecodeArgs a, Dec
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int keep = mine - 4 * w;
-          v[t][w] &= keep >= 4 ? ~0u : keep <= 0 ? 0u : ~0u >> 8 * (4 - keep);
+          x.v[t][w] &= keep >= 4 ? ~0u : keep <= 0 ? 0u : ~0u >> 8 * (4 - keep);
         }
     }
     float top = s[0];
@@ -162,9 +201,17 @@ __global__ __launch_bounds__(256) void attention_decode_kernel(DecodeArgs a, Dec
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      o[t] = mfma16(widen(v[t].x, v[t].y, vs), w[0], o[t]);
-      o[t] = mfma16(widen(v[t].z, v[t].w, vs), w[1], o[t]);
+      o[t] = mfma16(widen(x.v[t].x, x.v[t].y, vs), w[0], o[t]);
+      o[t] = mfma16(widen(x.v[t].z, x.v[t].w, vs), w[1], o[t]);
     }
+  };
+  for (uint32_t n = 0; p < end; p += kDecodeWaves, ++n) {
+    if (n == 64) ids = ids_from(p), n = 0;
+    const int32_t id = __builtin_amdgcn_readlane(ids, (int)n);
+    if (!known(id)) continue;
+    PageCodes<D> x;
+    load(x, id);
+    attend(x, p);
   }
   l = groups_sum(l);
   if (g == 0) sh_m[wave][c] = m, sh_l[wave][c] = l;
@@ -177,91 +224,110 @@ __global__ __launch_bounds__(256) void attention_decode_kernel(DecodeArgs a, Dec
   float mm = sh_m[0][hd];
 #pragma unroll
   for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sh_m[w][hd]);
-  float ll = 0.f, oo[D / 16] = {};
+  float ll = 0.f;
+  v4f oo[D / 64] = {};
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     const float mw = sh_m[w][hd], f = mw == mm ? 1.f : exp2_fast(mw - mm);
     ll += sh_l[w][hd] * f;
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) oo[j] += sh_o[w][hd][part * (D / 16) + j] * f;
+    for (int j = 0; j < D / 64; ++j) oo[j] += *(const v4f*)&sh_o[w][hd][64 * j + 4 * part] * f;
   }
-  if (partial) {
-    float* const at = partial + (((size_t)row * a.kv_heads + h) * d.tiles + tile) * d.splits * (16 * (D + 2)) +
-                      (size_t)split * (16 * (D + 2));
-    if (part == 0) at[2 * hd] = mm, at[2 * hd + 1] = ll;
+  const size_t at = (size_t)row * a.heads + head0 + hd;
+  if (pages > d.chunk) {
+    float* const ml = partial + (size_t)a.m * a.heads * d.splits * D;
+    if (part == 0) *(float2*)(ml + 2 * (at * d.splits + split)) = float2{mm, ll};
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) at[32 + hd * D + part * (D / 16) + j] = oo[j];
+    for (int j = 0; j < D / 64; ++j) *(v4f*)(partial + (at * d.splits + split) * D + 64 * j + 4 * part) = oo[j];
     return;
   }
   const float r = ll == 0.f ? 0.f : 1.f / ll;
-  const size_t at = ((size_t)row * a.heads + head0 + hd) * D + part * (D / 16);
 #pragma unroll
-  for (int j = 0; j < D / 16; j += 2) {
-    const uint32_t pair = pack_bf16(oo[j] * r, oo[j + 1] * r);
-    if (a.out_dtype == W8A8_OUT_BF16)
-      *(uint32_t*)((uint16_t*)a.out + at + j) = pair;
-    else
-      *(v2u*)((float*)a.out + at + j) = v2u{pair << 16, pair & 0xffff0000u};
-  }
+  for (int j = 0; j < D / 64; ++j) store4(a, at * D + 64 * j + 4 * part, oo[j] * r);
 }
 
-// One wave for a row's head: the splits' parts joined.
-template <int D>
-__global__ __launch_bounds__(64) void attention_join_kernel(DecodeArgs a, DecodeSplit d, const float* partial) {
-  const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, group = a.heads / a.kv_heads;
-  const uint32_t h = head / group, tile = head % group / kDecodeHeads, hd = head % group % kDecodeHeads;
-  const float* const at = partial + (((size_t)row * a.kv_heads + h) * d.tiles + tile) * d.splits * (16 * (D + 2));
-  const int lane = threadIdx.x;
-  constexpr size_t step = 16 * (D + 2);
-  const float m = (uint32_t)lane < d.splits ? at[lane * step + 2 * hd] : -__builtin_inff();
-  const float l = (uint32_t)lane < d.splits ? at[lane * step + 2 * hd + 1] : 0.f;
-  float mm = m;
+// A row's head, of WAVES waves: the splits' parts joined, each by the D / 4 threads
+// of a group, and the groups' results by the first.
+template <int D, int WAVES>
+__global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a, DecodeSplit d, const float* partial) {
+  constexpr uint32_t LANES = D / 4, GROUPS = 64 * WAVES / LANES, EACH = join_splits(WAVES) / GROUPS, HEADS = 4 / WAVES;
+  __shared__ float sh_m[HEADS][GROUPS], sh_l[HEADS][GROUPS];
+  __shared__ v4f sh_o[HEADS][GROUPS][LANES];
+  const uint32_t mine = threadIdx.x / (64 * WAVES), i = threadIdx.x % LANES, group = threadIdx.x % (64 * WAVES) / LANES;
+  const uint64_t at = (uint64_t)blockIdx.x * HEADS + mine;
+  const bool real = at < (uint64_t)a.m * a.heads;
+  const float* const ml = partial + (size_t)a.m * a.heads * d.splits * D;
+  const uint32_t len = real ? min((uint32_t)max(a.lengths[at / a.heads], 0), a.width * kPageTokens) : 0u;
+  uint32_t splits = ((len + kPageTokens - 1) / kPageTokens + d.chunk - 1) / d.chunk;
+  if (splits == 1) splits = 0;  // the output is there
+  float2 part[EACH];
+  v4f x[EACH];
+  // (requested before the length is known; what a short sequence did not write is not used)
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o, kWave));
-  const float f = m == mm ? 1.f : exp2_fast(m - mm);
-  float ll = l * f;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) ll += __shfl_xor(ll, o, kWave);
-  float oo[D / 64] = {};
-  for (uint32_t s = 0; s < d.splits; ++s) {
-    const float fs = __shfl(f, (int)s, kWave);
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) oo[j] += at[s * step + 32 + hd * D + lane * (D / 64) + j] * fs;
+  for (uint32_t e = 0; e < EACH; ++e) {
+    const uint32_t s = group + e * GROUPS;
+    const size_t from = real && s < d.splits ? at * d.splits + s : 0;
+    part[e] = *(const float2*)(ml + 2 * from);
+    x[e] = *(const v4f*)(partial + from * D + 4 * i);
   }
-  const float r = ll == 0.f ? 0.f : 1.f / ll;
-  const size_t to = ((size_t)row * a.heads + head) * D + lane * (D / 64);
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j) {
-    const uint32_t w = pack_bf16(oo[j] * r, 0.f);
-    if (a.out_dtype == W8A8_OUT_BF16)
-      ((uint16_t*)a.out)[to + j] = (uint16_t)w;
-    else
-      ((float*)a.out)[to + j] = bf16_lo(w);
+  for (uint32_t e = 0; e < EACH; ++e)
+    if (group + e * GROUPS >= splits) part[e] = float2{-__builtin_inff(), 0.f}, x[e] = v4f{};
+  float m = part[0].x;
+#pragma unroll
+  for (uint32_t e = 1; e < EACH; ++e) m = fmaxf(m, part[e].x);
+  float l = 0.f;
+  v4f o = {};
+#pragma unroll
+  for (uint32_t e = 0; e < EACH; ++e) {
+    const float f = part[e].x == m ? 1.f : exp2_fast(part[e].x - m);
+    l += part[e].y * f;
+    o += x[e] * f;
   }
+  if (i == 0) sh_m[mine][group] = m, sh_l[mine][group] = l;
+  sh_o[mine][group][i] = o;
+  __syncthreads();
+  if (group != 0 || splits == 0) return;
+#pragma unroll
+  for (uint32_t e = 1; e < GROUPS; ++e) m = fmaxf(m, sh_m[mine][e]);
+  l = 0.f;
+  o = v4f{};
+#pragma unroll
+  for (uint32_t e = 0; e < GROUPS; ++e) {
+    const float f = sh_m[mine][e] == m ? 1.f : exp2_fast(sh_m[mine][e] - m);
+    l += sh_l[mine][e] * f;
+    o += sh_o[mine][e][i] * f;
+  }
+  store4(a, at * D + 4 * i, o * (l == 0.f ? 0.f : 1.f / l));
 }
 
 size_t attention_decode_partial_bytes(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width) {
   const DecodeSplit d = decode_split(m, heads, kv_heads, width);
-  return d.splits > 1 ? (size_t)m * kv_heads * d.tiles * d.splits * 16 * (dim + 2) * sizeof(float) : 0;
+  return d.splits > 1 ? (size_t)m * heads * d.splits * (dim + 2) * sizeof(float) : 0;
 }
 
 uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width) {
   const DecodeSplit d = decode_split(std::max(1u, m), heads, kv_heads, width);
-  return std::max((uint64_t)m * kv_heads * d.tiles * d.splits, (uint64_t)m * heads / 4);  // of 256 threads
+  return std::max((uint64_t)m * kv_heads * d.tiles * d.splits, (uint64_t)m * heads);
+}
+
+template <int D>
+static void launch_decode(hipStream_t st, const DecodeArgs& a, float* partial) {
+  const DecodeSplit d = decode_split(a.m, a.heads, a.kv_heads, a.width);
+  const dim3 grid(a.m * a.kv_heads * d.tiles * d.splits), block(256);
+  hipLaunchKernelGGL(attention_decode_kernel<D>, grid, block, 0, st, a, d, partial);
+  if (d.splits == 1) return;
+  if (d.splits <= join_splits(1))
+    hipLaunchKernelGGL((attention_join_kernel<D, 1>), dim3((a.m * a.heads + 3) / 4), block, 0, st, a, d, (const float*)partial);
+  else
+    hipLaunchKernelGGL((attention_join_kernel<D, 4>), dim3(a.m * a.heads), block, 0, st, a, d, (const float*)partial);
 }
 
 hipError_t launch_attention_decode(hipStream_t st, const DecodeArgs& a, void* workspace) {
-  const DecodeSplit d = decode_split(a.m, a.heads, a.kv_heads, a.width);
-  float* const partial = d.splits > 1 ? (float*)workspace : nullptr;
-  const dim3 grid(a.m * a.kv_heads * d.tiles * d.splits);
-  auto go = [&](auto kernel, auto join) {
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, d, partial);
-    if (partial) hipLaunchKernelGGL(join, dim3(a.m * a.heads), dim3(64), 0, st, a, d, (const float*)partial);
-  };
   if (a.dim == 128)
-    go(attention_decode_kernel<128>, attention_join_kernel<128>);
+    launch_decode<128>(st, a, (float*)workspace);
   else
-    go(attention_decode_kernel<64>, attention_join_kernel<64>);
+    launch_decode<64>(st, a, (float*)workspace);
   return hipGetLastError();
 }
 
