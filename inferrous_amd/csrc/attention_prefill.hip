@@ -31,11 +31,17 @@ constexpr int kTileKeys = 64, kPrefillWaves = 8;
 
 // 16 keys of 32 columns of the values in LDS, as the first operand: lane l's
 // column is l % 32 and its keys 4 (l / 32) + {0..3, 8..11}.
-__device__ __forceinline__ v4u read_columns(const uint8_t* at0, const uint8_t* at1) {
+__device__ __forceinline__ v4u read_columns(uint32_t at0, uint32_t at1) {
   typedef __attribute__((address_space(3))) v4s* lds_v4s;
-  const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)at0));
-  const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)at1));
+  const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)at0));
+  const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)at1));
   return v4u{a.x, a.y, b.x, b.y};
+}
+__device__ __forceinline__ v4u read_row(uint32_t at) {
+  return *(const __attribute__((address_space(3))) v4u*)(uintptr_t)at;
+}
+__device__ __forceinline__ void write_lds(uint32_t at, v2u x) {
+  *(__attribute__((address_space(3))) v2u*)(uintptr_t)at = x;
 }
 __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -89,12 +95,11 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
 
   // the lane's row: a query and a head
   const uint64_t rows = (uint64_t)len * group, first = (uint64_t)tile * ROWS;
-  const uint64_t flat = first + 32 * wave + col;
-  const bool mine = flat < rows;
-  const uint32_t query = (uint32_t)((mine ? flat : rows - 1) / group), member = (uint32_t)((mine ? flat : rows - 1) % group);
-  const uint32_t last_query = (uint32_t)((std::min<uint64_t>(first + ROWS, rows) - 1) / group);
-  const uint32_t wave_first = (uint32_t)(std::min<uint64_t>(first + 32 * wave, rows - 1) / group);
-  const uint32_t wave_last = (uint32_t)(std::min<uint64_t>(first + 32 * wave + 31, rows - 1) / group);
+  const uint32_t first_query = (uint32_t)(first / group), first_member = (uint32_t)(first % group);
+  const auto query_of = [&](uint32_t row) { return min(first_query + (first_member + row) / group, len - 1); };
+  const bool mine = first + 32 * wave + col < rows;
+  const uint32_t query = query_of(32 * wave + col), member = (first_member + 32 * wave + col) % group;
+  const uint32_t last_query = query_of(ROWS - 1), wave_first = query_of(32 * wave), wave_last = query_of(32 * wave + 31);
   const uint32_t tiles = last_query / kTileKeys + 1;    // of the workgroup
   const uint32_t own = wave_last / kTileKeys + 1;       // with a key that a row of the wave sees
   const uint32_t whole = (wave_first + 1) / kTileKeys;  // of those, without one that a row does not see
@@ -111,18 +116,35 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
   const uint16_t* const kbase = a.k + (size_t)r.lo * a.k_stride + (size_t)head * D;
   const uint16_t* const vbase = a.v + (size_t)r.lo * a.v_stride + (size_t)head * D;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  const auto load_tile = [&](uint32_t t, const uint16_t* base, size_t stride, uint32_t to, auto swizzle) {
-    const uint32_t last = len - 1 - min(t * kTileKeys, len - 1);  // rows behind it are that one again
-    const void* const from = base + (size_t)min(t * kTileKeys, len - 1) * stride;
+  // Requests of the wave's part of a tile: row row0 of its first load, and 1024 / (2 D)
+  // rows on for each more.  Rows behind the sequence, which no row sees, are a part of its last one.
+  constexpr int APART = 1024 / (2 * D);
+  const uint32_t row0 = wave * (LOADS * APART) + lane / CH;
+  uint32_t key_from[LOADS], value_from[LOADS];
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int at = (wave * LOADS + j) * 64 + lane, row = at / CH, ch = at % CH;  // where it lands
-      load_to_lds(from, min((uint32_t)row, last) * ((uint32_t)stride * 2) + (ch ^ swizzle(row)) * 16,
-                  to + (wave * LOADS + j) * 1024);
-    }
+  for (int j = 0; j < LOADS; ++j) {
+    const int row = row0 + j * APART, ch = lane % CH;
+    key_from[j] = row * ((uint32_t)a.k_stride * 2) + (ch ^ key_swizzle(row)) * 16;
+    value_from[j] = row * ((uint32_t)a.v_stride * 2) + (ch ^ value_swizzle(row)) * 16;
+  }
+  const auto load_one = [&](uint32_t t, const uint16_t* base, uint32_t stride, uint32_t from, uint32_t to) {
+    const uint32_t top = min(t * kTileKeys, len - 1), last = min(len - 1 - top, (uint32_t)kTileKeys - 1);
+    load_to_lds(base + (size_t)top * stride, min(from, last * stride * 2 + (2 * D - 16)), to);
   };
-  const auto load_keys = [&](uint32_t t) { load_tile(t, kbase, a.k_stride, lds0 + t % 3 * TILE, key_swizzle); };
-  const auto load_values = [&](uint32_t t) { load_tile(t, vbase, a.v_stride, lds0 + (3 + t % 3) * TILE, value_swizzle); };
+  const auto load_key = [&](uint32_t t, int j) {
+    load_one(t, kbase, (uint32_t)a.k_stride, key_from[j], lds0 + t % 3 * TILE + (wave * LOADS + j) * 1024);
+  };
+  const auto load_value = [&](uint32_t t, int j) {
+    load_one(t, vbase, (uint32_t)a.v_stride, value_from[j], lds0 + (3 + t % 3) * TILE + (wave * LOADS + j) * 1024);
+  };
+  const auto load_keys = [&](uint32_t t) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load_key(t, j);
+  };
+  const auto load_values = [&](uint32_t t) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) load_value(t, j);
+  };
 
   // Where the lane's fragments lie in a tile: of the keys, step i's are at key_at ^
   // 32 i (its two chunks differ from the first step's in bits that the swizzle only
@@ -131,93 +153,92 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
   const int vrow = 4 * half + ((lane & 15) >> 2);
   const uint32_t value_at = vrow * (2 * D) + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle(vrow)) * 16 + (lane & 1) * 8;
 
-  const float to_log2 = a.scale * kLog2e;
+  // in a scalar register: a product with a sum of three vector registers is slower
+  const float to_log2 = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(a.scale * kLog2e)));
   float m = -__builtin_inff(), l = 0.f;
   v16f o[COLS] = {}, s[2];
   v4u p[4];
-  const auto scores = [&](uint32_t t) {
-    const uint8_t* const kb = lds + t % 3 * TILE;
-    s[0] = s[1] = v16f{};
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = mfma32(*(const v4u*)(kb + (key_at ^ (32 * i)) + 32 * b * (2 * D)), q[i], s[b]);
+  // v_med3 with infinity: a maximum without fmaxf's care for signalling NaN
+  const auto larger = [](float x, float y) { return __builtin_amdgcn_fmed3f(x, y, __builtin_inff()); };
+  const v2bf one = {(__bf16)1.f, (__bf16)1.f};
+  const auto key = [&](uint32_t t, int b, int i) {
+    return read_row(lds0 + t % 3 * TILE + (key_at ^ (32 * i)) + 32 * b * (2 * D));
   };
-  const auto softmax = [&](uint32_t t, auto masked) {
-    if (masked && t >= whole) {
+  // the largest of 32 keys' scores, for both of the row's lanes
+  const auto top_of = [&](const v16f& x) {
+    float tops[2] = {x[0], x[1]};
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t * kTileKeys + 32 * b + 8 * (i / 4) + 4 * half + i % 4 > query) s[b][i] = -__builtin_inff();
-    }
-    float top = s[0][0];  // v_med3 with infinity: a maximum without fmaxf's care for signalling NaN
-#pragma unroll
-    for (int i = 1; i < 32; ++i) top = __builtin_amdgcn_fmed3f(top, s[i / 16][i % 16], __builtin_inff());
+    for (int i = 2; i < 16; ++i) tops[i % 2] = larger(tops[i % 2], x[i]);
+    return larger(tops[0], tops[1]);
+  };
+  // of both of the row's lanes, as a power of two
+  const auto both = [&](float top) {
     const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-    top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * to_log2;
-    if (__ballot(top > m + 8.f || m == -__builtin_inff())) {
-      const float to = fmaxf(m, top);
-      const float f = to == m ? 1.f : exp2_fast(m - to);
-      m = to;
-      l *= f;
+    return fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * to_log2;
+  };
+  // m, or a new one if the scores are far above it, and what sums so far are scaled by for that
+  const auto raised = [&](float top) { return top > m + 8.f || m == -__builtin_inff() ? fmaxf(m, top) : m; };
+  const auto factor = [&](float to) { return to == m ? 1.f : exp2_fast(m - to); };
+  const auto rescale = [&](float f) {
+    if (__ballot(f != 1.f)) {
 #pragma unroll
       for (int c = 0; c < COLS; ++c) o[c] *= f;
     }
-    const v2bf one = {(__bf16)1.f, (__bf16)1.f};
+  };
+  // probabilities of 32 keys, and their sum
+  const auto soften = [&](const v16f& x, v4u* to) {
+    float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t pair = pack_bf16(exp2_fast(__builtin_fmaf(s[b][2 * i], to_log2, -m)),
-                                        exp2_fast(__builtin_fmaf(s[b][2 * i + 1], to_log2, -m)));
-        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pair), one, l, false);
-        p[2 * b + i / 4][i % 4] = pair;
-      }
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t pair = pack_bf16(exp2_fast(__builtin_fmaf(x[2 * i], to_log2, -m)),
+                                      exp2_fast(__builtin_fmaf(x[2 * i + 1], to_log2, -m)));
+      sums[i % 2] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pair), one, sums[i % 2], false);
+      to[i / 4][i % 4] = pair;
+    }
+    return sums[0] + sums[1];
   };
   const auto values = [&](uint32_t t, int i, int c) {
-    const uint8_t* const at = lds + (3 + t % 3) * TILE + (value_at ^ (64 * c)) + 16 * i * (2 * D);
+    const uint32_t at = lds0 + (3 + t % 3) * TILE + (value_at ^ (64 * c)) + 16 * i * (2 * D);
     return read_columns(at, at + 8 * (2 * D));
   };
-  const auto add_values = [&](uint32_t t) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) o[c] = mfma32(values(t, i, c), p[i], o[c]);
-  };
-  // The same for a tile that some of the rows see in part.
+  // adds a tile that some of the rows see in part
   const auto add_seen_values = [&](uint32_t t) {
-    uint32_t odd = 0;  // values on the diagonal's tile that a zero probability would make NaN
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i)
+    v4u v[2][COLS];
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) {
-        const v4u bad = not_finite(values(t, i, c));
-        odd |= bad.x | bad.y | bad.z | bad.w;
-      }
-    if (!__ballot(odd != 0)) {
-      add_values(t);
-      return;
-    }
-    // what is finite first, then the rest key by key, and only into the rows that see the key
+    for (int c = 0; c < COLS; ++c) v[0][c] = values(t, 0, c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (i < 3) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) v[(i + 1) % 2][c] = values(t, i + 1, c);
+      }
+      uint32_t odd = 0;  // bits 15 and 31 if there is a value that a probability of zero would make NaN
 #pragma unroll
       for (int c = 0; c < COLS; ++c) {
-        const v4u v = values(t, i, c);
-        o[c] = mfma32(v & ~not_finite(v), p[i], o[c]);
+        const v4u x = (v[i % 2][c] & 0x7f807f80u) + 0x00800080u;
+        odd |= x.x | x.y | x.z | x.w;
       }
-#pragma unroll 1
-      for (int key = 0; key < 16; ++key) {
-        const int slot = (key >> 3) * 4 + (key & 3);  // of the lanes of half (key >> 2) & 1
-        const uint32_t part = half == ((key >> 2) & 1) ? 0xffffu << 16 * (slot & 1) : 0u;
-        const v4u only = {slot / 2 == 0 ? part : 0u, slot / 2 == 1 ? part : 0u, slot / 2 == 2 ? part : 0u,
-                          slot / 2 == 3 ? part : 0u};
-        const bool seen = t * kTileKeys + 16 * i + key <= query;
+      // what is finite first, then the rest key by key, and only into the rows that see the key
+      const bool rest = __ballot(odd & 0x80008000u);
+      if (rest) {
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-          const v4u v = values(t, i, c);
-          const v16f with = mfma32(v & not_finite(v) & only, p[i], o[c]);
+        for (int c = 0; c < COLS; ++c) v[i % 2][c] &= ~not_finite(v[i % 2][c]);
+      }
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) o[c] = mfma32(v[i % 2][c], p[i], o[c]);
+      if (!rest) continue;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) {
+        v4u w = values(t, i, c);
+        w &= not_finite(w);
+#pragma unroll 1
+        for (int key = 0; key < 16; ++key) {
+          const int slot = (key >> 3) * 4 + (key & 3);  // of the lanes of half (key >> 2) & 1
+          const uint32_t part = half == ((key >> 2) & 1) ? 0xffffu << 16 * (slot & 1) : 0u;
+          const v4u only = {slot / 2 == 0 ? part : 0u, slot / 2 == 1 ? part : 0u, slot / 2 == 2 ? part : 0u,
+                            slot / 2 == 3 ? part : 0u};
+          const bool seen = t * kTileKeys + 16 * i + key <= query;
+          const v16f with = mfma32(w & only, p[i], o[c]);
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[c][e] = seen ? with[e] : o[c][e];
         }
@@ -225,79 +246,180 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
     }
   };
 
-  // Two waves share a SIMD.  Half of the waves run half a turn behind, so that one of
-  // the two feeds the matrix cores (a tile's scores and the sums of the tile before)
-  // while the other works on its softmax.  In turn t a wave requests keys t + 2 and
-  // values t + 1, into the buffers that all waves left before the barrier; at the turn's
-  // second barrier what it requested a turn ago has arrived, for all to read after
-  // the next one.
-  const bool behind = wave >= NW / 2;
   load_keys(0);
-  load_keys(1);
   load_values(0);
-  arrived<2 * LOADS>();
-  if (behind) meet();
+  if (tiles > 1) load_keys(1);
   uint32_t t = 0;
   // tiles that every row of the workgroup sees as a whole
-  const uint32_t plain = (uint32_t)(first / group + 1) / kTileKeys;
+  const uint32_t plain = (first_query + 1) / kTileKeys;
+  arrived<0>();
+  meet();
   if (plain) {
-    meet();
-    load_keys(2);
-    load_values(1);
-    scores(0);
-    arrived<2 * LOADS>();
-    meet();
-    softmax(0, std::false_type{});
+    v16f s0, s1;
+    v4u p0[2], p1[2], kf[STEPS], vf[STEPS];
+    static_assert(STEPS == 2 * COLS, "a read for each product");
+    uint32_t key_lies[STEPS], value_lies[COLS];  // in the tiles that are read next
+    float next_m, next_f;  // for the keys whose scores come next
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) key_lies[i] = lds0 + (key_at ^ (32 * i));
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) value_lies[c] = lds0 + (3 * TILE) + (value_at ^ (64 * c));
+    const auto read_key = [&](int b, int i) { kf[i] = read_row(key_lies[i] + 32 * b * (2 * D)); };
+    const auto read_value = [&](int b, int j) {
+      const uint32_t at = value_lies[j % COLS] + (2 * b + j / COLS) * 16 * (2 * D);
+      vf[j] = read_columns(at, at + 8 * (2 * D));
+    };
+    // Scores of the next 32 keys, sums of the last 32 and the softmax of those between,
+    // in one stream: a product, the reads for one that is STEPS products away and a part
+    // of the softmax in every step.
+    const auto unit = [&](const v16f& now, v16f& next, const v4u* before, v4u* to, int bv, int bk, auto sum, auto load) {
+      constexpr int EACH = 16 / (2 * STEPS);
+      float sums[2] = {0.f, 0.f}, x[16], tops[2], top;
+      m = next_m;
+      const float f = next_f;
+      next = v16f{};
+      const auto pack = [&](int i) {
+        const uint32_t pair = pack_bf16(x[2 * i], x[2 * i + 1]);
+        sums[i % 2] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pair), one, sums[i % 2], false);
+        to[i / 4][i % 4] = pair;
+      };
+#pragma unroll
+      for (int k = 0; k < 2 * STEPS; ++k) {
+        if (k < STEPS) {
+          next = mfma32(kf[k], q[k], next);
+          if (sum) read_value(bv, k);
+        } else {
+          const int j = k - STEPS;
+          if (sum) o[j % COLS] = mfma32(vf[j], before[j / COLS], o[j % COLS]);
+          read_key(bk, j);
+        }
+#pragma unroll
+        for (int e = k * EACH; e < (k + 1) * EACH; ++e) {
+          if (e % 2 == 0 && e) pack(e / 2 - 1);
+          x[e] = exp2_fast(__builtin_fmaf(now[e], to_log2, -m));
+        }
+        constexpr int FROM = STEPS + STEPS / 4, MANY = 32 / STEPS;
+        if (k >= FROM && k < FROM + STEPS / 2) {
+#pragma unroll
+          for (int e = (k - FROM) * MANY; e < (k - FROM + 1) * MANY; ++e)
+            tops[e % 2] = e < 2 ? next[e] : larger(tops[e % 2], next[e]);
+        }
+        if (k == 2 * STEPS - 2) top = both(larger(tops[0], tops[1]));
+        if (k == 2 * STEPS - 1) {
+          next_m = raised(top);
+          next_f = factor(next_m);
+        }
+        if (k % (STEPS / LOADS) == 1) load(k / (STEPS / LOADS));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      pack(7);
+      l = __builtin_fmaf(l, f, sums[0] + sums[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(to[i]));
+      asm volatile("" : "+v"(l), "+v"(next_m), "+v"(next_f));
+      rescale(f);
+    };
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) read_key(0, i);
+    s0 = v16f{};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) s0 = mfma32(kf[i], q[i], s0);
+    next_m = raised(both(top_of(s0)));
+    next_f = 1.f;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) read_key(1, i);
+    uint32_t key_buffer = 0, value_buffer = 0;
+    const auto keys_on = [&] {
+      const uint32_t by = key_buffer == 2 ? (uint32_t)(-2 * TILE) : (uint32_t)TILE;
+      key_buffer = key_buffer == 2 ? 0 : key_buffer + 1;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) key_lies[i] += by;
+    };
+    const auto values_on = [&] {
+      const uint32_t by = value_buffer == 2 ? (uint32_t)(-2 * TILE) : (uint32_t)TILE;
+      value_buffer = value_buffer == 2 ? 0 : value_buffer + 1;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) value_lies[c] += by;
+    };
+    keys_on();
+    unit(s0, s1, p1, p0, 1, 0, std::false_type{}, [&](int j) { j < LOADS ? load_key(2, j) : load_value(1, j - LOADS); });
+    unit(s1, s0, p0, p1, 0, 1, std::true_type{}, [](int) {});
 #pragma unroll 1
     for (t = 1; t < plain; ++t) {
+      arrived<0>();
       meet();
-      load_keys(t + 2);
-      load_values(t + 1);
-      __builtin_amdgcn_s_setprio(1);
-      add_values(t - 1);
-      scores(t);
-      // reads of LDS run eight ahead of the products
-      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-      for (int i = 0; i < 4 * COLS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * STEPS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      arrived<2 * LOADS>();
-      meet();
-      softmax(t, std::false_type{});
+      keys_on();
+      unit(s0, s1, p1, p0, 1, 0, std::true_type{}, [&](int j) { j < LOADS ? load_key(t + 2, j) : load_value(t + 1, j - LOADS); });
+      values_on();
+      unit(s1, s0, p0, p1, 0, 1, std::true_type{}, [](int) {});
     }
+    // what is left of the last keys; the scores that were taken ahead are not used
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      read_value(1, j);
+      o[j % COLS] = mfma32(vf[j], p1[j / COLS], o[j % COLS]);
+    }
+    arrived<0>();
+    meet();
   }
 #pragma unroll 1
-  for (; t <= tiles; ++t) {
-    meet();
-    if (t < tiles) {
+  for (; t < tiles; ++t) {
+    if (t + 1 < tiles) {
       load_keys(t + 2);
       load_values(t + 1);
     }
-    __builtin_amdgcn_s_setprio(1);
-    if (t > 0 && t <= whole)
-      add_values(t - 1);
-    else if (t > 0 && t <= own)
-      add_seen_values(t - 1);
-    if (t < own) scores(t);
-    __builtin_amdgcn_s_setprio(0);
-    arrived<2 * LOADS>();
-    meet();
-    if (t < own) softmax(t, std::true_type{});
+    if (t < own) {
+      s[0] = s[1] = v16f{};
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = mfma32(key(t, b, i), q[i], s[b]);
+      if (t >= whole) {
+        const int seen = (int)(query - t * kTileKeys) - 4 * half;  // the last key, from the lane's first
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * b + 8 * (i / 4) + i % 4 > seen) s[b][i] = -__builtin_inff();
+      }
+      const float to = raised(both(larger(top_of(s[0]), top_of(s[1])))), f = factor(to);
+      m = to;
+      l = __builtin_fmaf(l, f, soften(s[0], p) + soften(s[1], p + 2));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(p[i]));  // here: the scores would not fit beside the values
+      rescale(f);
+      add_seen_values(t);
+    }
+    if (t + 1 < tiles) {
+      arrived<0>();
+      meet();
+    }
   }
-  if (!behind) meet();
-  arrived<0>();
 
   l += __shfl_xor(l, 32, kWave);
-  if (!mine) return;
   const float inv = 1.f / l;
+  if (a.out_dtype == W8A8_OUT_BF16) {
+    // through LDS, so that a store's lanes write whole rows
+    meet();
+    const uint32_t part = lds0 + wave * (32 * 2 * D);
+#pragma unroll
+    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        write_lds(part + col * (2 * D) + ((4 * c + i) ^ key_swizzle(col)) * 16 + 8 * half,
+                  v2u{pack_bf16(o[c][4 * i] * inv, o[c][4 * i + 1] * inv), pack_bf16(o[c][4 * i + 2] * inv, o[c][4 * i + 3] * inv)});
+#pragma unroll
+    for (int j = 0; j < 32 / (64 / CH); ++j) {
+      const uint32_t row = j * (64 / CH) + lane / CH;
+      const uint32_t to = first_member + 32 * wave + row;
+      const v4u x = read_row(part + row * (2 * D) + ((lane % CH) ^ key_swizzle(row)) * 16);
+      if (first + 32 * wave + row < rows)
+        *(v4u*)((uint16_t*)a.out + ((size_t)(r.lo + first_query + to / group) * a.heads + head * group + to % group) * D +
+                lane % CH * 8) = x;
+    }
+    return;
+  }
+  if (!mine) return;
   const size_t at = ((size_t)(r.lo + query) * a.heads + head * group + member) * D;
 #pragma unroll
   for (int c = 0; c < COLS; ++c)
@@ -305,11 +427,7 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
     for (int i = 0; i < 4; ++i) {
       const uint32_t x = pack_bf16(o[c][4 * i] * inv, o[c][4 * i + 1] * inv);
       const uint32_t y = pack_bf16(o[c][4 * i + 2] * inv, o[c][4 * i + 3] * inv);
-      const size_t to = at + 32 * c + 8 * i + 4 * half;
-      if (a.out_dtype == W8A8_OUT_BF16)
-        *(v2u*)((uint16_t*)a.out + to) = v2u{x, y};
-      else
-        *(v4u*)((float*)a.out + to) = v4u{x << 16, x & 0xffff0000u, y << 16, y & 0xffff0000u};
+      *(v4u*)((float*)a.out + at + 32 * c + 8 * i + 4 * half) = v4u{x << 16, x & 0xffff0000u, y << 16, y & 0xffff0000u};
     }
 }
 
