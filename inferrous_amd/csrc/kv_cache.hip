@@ -12,6 +12,7 @@
 // shifts the codes that are there (exact but for e4m3's subnormals), and the
 // readers' conversion to BF16 (v_cvt_scalef32_pk_bf16_fp8) applies it for free.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.hpp"
 
@@ -47,22 +48,40 @@ struct Share {
   float lo[4], hi[4];
 };
 
+// What a lane reads for a share: loads of many shares are under way before the
+// first is used.
 template <int D, bool BF16IN>
-__device__ __forceinline__ Share load_share(const void* rows, size_t at, int i) {
-  Share x;
-  if constexpr (BF16IN) {
-    const uint16_t* p = (const uint16_t*)rows + at + 4 * i;
-    const v2u a = *(const v2u*)p, b = *(const v2u*)(p + D / 2);
-    x.lo[0] = bf16_lo(a.x), x.lo[1] = bf16_hi(a.x), x.lo[2] = bf16_lo(a.y), x.lo[3] = bf16_hi(a.y);
-    x.hi[0] = bf16_lo(b.x), x.hi[1] = bf16_hi(b.x), x.hi[2] = bf16_lo(b.y), x.hi[3] = bf16_hi(b.y);
-  } else {
-    const float* p = (const float*)rows + at + 4 * i;
-    const v4f a = *(const v4f*)p, b = *(const v4f*)(p + D / 2);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x.lo[j] = a[j], x.hi[j] = b[j];
+struct Read {
+  typename std::conditional<BF16IN, v2u, v4f>::type lo, hi;
+  __device__ __forceinline__ void start(const void* rows, size_t at, int i) {
+    const uint8_t* p = (const uint8_t*)rows + (at + 4 * i) * (BF16IN ? 2 : 4);
+    lo = *(const decltype(lo)*)p;
+    hi = *(const decltype(hi)*)(p + D / 2 * (BF16IN ? 2 : 4));
   }
-  return x;
-}
+  __device__ __forceinline__ Share share() const {
+    Share x;
+    if constexpr (BF16IN) {
+      x.lo[0] = bf16_lo(lo.x), x.lo[1] = bf16_hi(lo.x), x.lo[2] = bf16_lo(lo.y), x.lo[3] = bf16_hi(lo.y);
+      x.hi[0] = bf16_lo(hi.x), x.hi[1] = bf16_hi(hi.x), x.hi[2] = bf16_lo(hi.y), x.hi[3] = bf16_hi(hi.y);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.lo[j] = lo[j], x.hi[j] = hi[j];
+    }
+    return x;
+  }
+};
+
+// The lane's cosines and sines of a position; NaN if the table has no such row.
+template <int D>
+struct Angles {
+  v4f c, s;
+  bool known;
+  __device__ __forceinline__ void start(const float* rope, uint32_t rope_rows, uint32_t pos, int i) {
+    known = pos < rope_rows;
+    const float* r = rope + (size_t)(known ? pos : 0u) * D + 4 * i;
+    c = *(const v4f*)r, s = *(const v4f*)(r + D / 2);
+  }
+};
 
 template <int D>
 __device__ __forceinline__ void store_share(uint16_t* out, size_t at, int i, const Share& x) {
@@ -82,44 +101,50 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
+// The lane's gains, if there is a norm.
 template <int D>
-__device__ __forceinline__ void norm_rotate(Share& x, const float* gain, float eps, const float* rope, uint32_t rope_rows,
-                                            uint32_t pos, int i) {
-  if (gain) {
+struct Gains {
+  v4f a, b;
+  __device__ __forceinline__ void start(const float* gain, int i) {
+    if (gain) a = *(const v4f*)(gain + 4 * i), b = *(const v4f*)(gain + D / 2 + 4 * i);
+  }
+};
+
+template <int D>
+__device__ __forceinline__ void norm_rotate(Share& x, bool norm, const Gains<D>& g, float eps, const Angles<D>& r) {
+  if (norm) {
     float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x.lo[j], x.lo[j], __builtin_fmaf(x.hi[j], x.hi[j], ss));
     // v_rsq_f32: one unit of the last place
     const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<D>(ss), 1.0f / D, eps));
-    const v4f a = *(const v4f*)(gain + 4 * i), b = *(const v4f*)(gain + D / 2 + 4 * i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x.lo[j] = x.lo[j] * inv * a[j], x.hi[j] = x.hi[j] * inv * b[j];
+    for (int j = 0; j < 4; ++j) x.lo[j] = x.lo[j] * inv * g.a[j], x.hi[j] = x.hi[j] * inv * g.b[j];
   }
-  const bool known = pos < rope_rows;
-  const float* r = rope + (size_t)(known ? pos : 0u) * D + 4 * i;
-  const v4f c = *(const v4f*)r, s = *(const v4f*)(r + D / 2);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float a = x.lo[j], b = x.hi[j];
-    x.lo[j] = known ? __builtin_fmaf(a, c[j], -(b * s[j])) : __builtin_nanf("");
-    x.hi[j] = known ? __builtin_fmaf(b, c[j], a * s[j]) : __builtin_nanf("");
+    x.lo[j] = r.known ? __builtin_fmaf(a, r.c[j], -(b * r.s[j])) : __builtin_nanf("");
+    x.hi[j] = r.known ? __builtin_fmaf(b, r.c[j], a * r.s[j]) : __builtin_nanf("");
   }
 }
 
-constexpr uint32_t kPrepareHeads = 4;  // query heads of one workgroup
+constexpr uint32_t kPrepareHeads = 4;  // query heads that a group of lanes takes of one token
 
 // A unit is the rows that one sequence brings to one page.  Of a unit, one
 // workgroup takes a key/value head (its 64 x D keys and values: whole blocks of
-// the cache, so that their scale is one workgroup's) and one takes kPrepareHeads
-// query heads.  D / 8 lanes hold a head.
-template <int D, bool BF16IN>
+// the cache, so that their scale is one workgroup's).  The queries of GROUPS of its
+// tokens and of kPrepareHeads heads are one workgroup's, too; if every sequence
+// brings one row (ONE), GROUPS heads of it are.  D / 8 lanes hold a head.
+template <int D, bool BF16IN, bool ONE>
 __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t blocks) {
   constexpr int LPH = D / 8, GROUPS = 256 / LPH, SLOTS = 64 / GROUPS;  // lanes of a head, heads in flight, tokens of a group
   __shared__ uint32_t red[2][4];
+  __shared__ __align__(16) uint32_t turned[ONE ? 1 : D * kPageTokens / 4];  // the page's value codes
   const uint32_t unit = blockIdx.x / blocks, part = blockIdx.x % blocks;
   const int tid = threadIdx.x, i = tid % LPH, group = tid / LPH;
   uint32_t seq = unit, index = 0, lo = unit, n = 1;
-  if (a.starts) {
+  if constexpr (!ONE) {
     const auto count = [&](uint32_t s) {
       const RowRange r = rows_of(a.starts, s, a.m);
       const uint32_t p = a.past ? (uint32_t)max(a.past[s], 0) : 0u, rows = r.hi - r.lo;
@@ -137,35 +162,58 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
   const uint32_t row0 = lo + (first - past);
 
   if (part >= a.kv_heads) {
-    const uint32_t h0 = (part - a.kv_heads) * kPrepareHeads, heads = min(kPrepareHeads, a.heads - h0);
-    for (uint32_t u = group; u < (n1 - n0) * heads; u += GROUPS) {
-      const uint32_t t = u / heads, h = h0 + u % heads;
-      Share x = load_share<D, BF16IN>(a.q, (size_t)(row0 + t) * a.q_stride + (size_t)h * D, i);
-      norm_rotate<D>(x, a.q_gain, a.eps, a.rope, a.rope_rows, first + t, i);
-      store_share<D>(a.q_out, ((size_t)(row0 + t) * a.heads + h) * D, i, x);
+    constexpr uint32_t TIMES = ONE ? 1 : kPrepareHeads, HEADS = ONE ? GROUPS : kPrepareHeads;
+    const uint32_t sets = (a.heads + HEADS - 1) / HEADS, set = (part - a.kv_heads) % sets;
+    const uint32_t t = ONE ? 0u : (part - a.kv_heads) / sets * GROUPS + group, h0 = set * HEADS + (ONE ? group : 0u);
+    if (t >= n1 - n0 || h0 >= a.heads) return;
+    const size_t row = row0 + t;
+    Read<D, BF16IN> in[TIMES];
+    Angles<D> angles;
+    Gains<D> gains;
+#pragma unroll
+    for (uint32_t j = 0; j < TIMES; ++j) in[j].start(a.q, row * a.q_stride + (size_t)min(h0 + j, a.heads - 1) * D, i);
+    angles.start(a.rope, a.rope_rows, first + t, i);
+    gains.start(a.q_gain, i);
+#pragma unroll
+    for (uint32_t j = 0; j < TIMES; ++j) {
+      Share x = in[j].share();
+      norm_rotate<D>(x, a.q_gain, gains, a.eps, angles);
+      if (h0 + j < a.heads) store_share<D>(a.q_out, (row * a.heads + h0 + j) * D, i, x);
     }
     return;
   }
 
   const uint32_t h = part;
-  Share k[SLOTS], v[SLOTS];
+  Share k[SLOTS] = {}, v[SLOTS] = {};
   uint32_t k_top = 0, v_top = 0;
+  const uint32_t s0 = SLOTS * group;
+  if (s0 < n1 && s0 + SLOTS > n0) {  // the same for a head's lanes
+    Read<D, BF16IN> k_in[SLOTS], v_in[SLOTS];
+    Angles<D> angles[SLOTS];
+    Gains<D> gains;
 #pragma unroll
-  for (int j = 0; j < SLOTS; ++j) {
-    const uint32_t slot = SLOTS * group + j;
-    k[j] = v[j] = Share{};
-    if (slot >= n0 && slot < n1) {  // the same for a head's lanes
-      const size_t row = row0 + (slot - n0);
-      k[j] = load_share<D, BF16IN>(a.k, row * a.k_stride + (size_t)h * D, i);
-      v[j] = load_share<D, BF16IN>(a.v, row * a.v_stride + (size_t)h * D, i);
-      norm_rotate<D>(k[j], a.k_gain, a.eps, a.rope, a.rope_rows, first + (slot - n0), i);
+    for (int j = 0; j < SLOTS; ++j) {
+      const uint32_t t = min(max(s0 + j, n0), n1 - 1) - n0;
+      const size_t row = row0 + t;
+      k_in[j].start(a.k, row * a.k_stride + (size_t)h * D, i);
+      v_in[j].start(a.v, row * a.v_stride + (size_t)h * D, i);
+      angles[j].start(a.rope, a.rope_rows, first + t, i);
+    }
+    gains.start(a.k_gain, i);
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+      k[j] = k_in[j].share();
+      v[j] = v_in[j].share();
+      norm_rotate<D>(k[j], a.k_gain, gains, a.eps, angles[j]);
+      if (s0 + j < n0 || s0 + j >= n1) continue;
+      const size_t row = row0 + (s0 + j - n0);
       if (a.k_out) store_share<D>(a.k_out, (row * a.kv_heads + h) * D, i, k[j]);
       if (a.v_out) store_share<D>(a.v_out, (row * a.kv_heads + h) * D, i, v[j]);
-    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      k_top = max(k_top, max(finite_bits(k[j].lo[e]), finite_bits(k[j].hi[e])));
-      v_top = max(v_top, max(finite_bits(v[j].lo[e]), finite_bits(v[j].hi[e])));
+      for (int e = 0; e < 4; ++e) {
+        k_top = max(k_top, max(finite_bits(k[j].lo[e]), finite_bits(k[j].hi[e])));
+        v_top = max(v_top, max(finite_bits(v[j].lo[e]), finite_bits(v[j].hi[e])));
+      }
     }
   }
   if (!a.codes || page >= a.width) return;
@@ -221,7 +269,28 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
       held[4 + e] |= (a1 >> 8 * e & 0xffu) << 8 * j;
     }
   }
-  const uint32_t s0 = SLOTS * group;
+  if (!ONE && n1 - n0 == kPageTokens) {
+    // a whole page of value codes leaves through LDS, 16 bytes a lane
+    constexpr int WORDS = kPageTokens / 4;  // of a column
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int column = 4 * i + e % 4 + e / 4 * (D / 2);
+      if constexpr (SLOTS == 4)
+        turned[column * WORDS + (group ^ (i & (WORDS - 1)))] = held[e];
+      else
+        ((uint16_t*)turned)[2 * (column * WORDS + (group / 2 ^ (i & (WORDS - 1)))) + group % 2] = (uint16_t)held[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int at = 4 * tid; at < D * WORDS; at += 4 * 256) {
+      const int column = at / WORDS, turn = column % (D / 2) / 4 & (WORDS - 1), word = at % WORDS;
+      v4u x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = turned[column * WORDS + ((word + j) ^ turn)];
+      *(v4u*)(vcodes + 4 * at) = x;
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     uint8_t* const p = vcodes + (size_t)(4 * i + e % 4 + e / 4 * (D / 2)) * kPageTokens + s0;
@@ -238,7 +307,12 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
   }
 }
 
-static uint32_t prepare_parts(const PrepareArgs& a) { return a.kv_heads + (a.heads + kPrepareHeads - 1) / kPrepareHeads; }
+// Workgroups of a unit: those of the key/value heads and of the queries.
+static uint32_t prepare_parts(const PrepareArgs& a) {
+  const uint32_t groups = 256 / (a.dim / 8);
+  if (!a.starts) return a.kv_heads + (a.heads + groups - 1) / groups;
+  return a.kv_heads + (a.heads + kPrepareHeads - 1) / kPrepareHeads * (kPageTokens / groups);
+}
 
 // Every unit has a row, and a sequence's pages hold 64 of its rows but for two.
 uint64_t prepare_qk_blocks(const PrepareArgs& a) {
@@ -246,14 +320,20 @@ uint64_t prepare_qk_blocks(const PrepareArgs& a) {
   return units * prepare_parts(a);
 }
 
-hipError_t launch_prepare_qk(hipStream_t st, const PrepareArgs& a) {
-  const uint32_t blocks = prepare_parts(a);
+template <int D, bool BF16IN>
+static void start_prepare_qk(hipStream_t st, const PrepareArgs& a) {
   const dim3 grid((uint32_t)prepare_qk_blocks(a));
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a, blocks); };
-  if (a.dim == 128)
-    a.bf16 ? go(prepare_qk_kernel<128, true>) : go(prepare_qk_kernel<128, false>);
+  if (a.starts)
+    hipLaunchKernelGGL((prepare_qk_kernel<D, BF16IN, false>), grid, dim3(256), 0, st, a, prepare_parts(a));
   else
-    a.bf16 ? go(prepare_qk_kernel<64, true>) : go(prepare_qk_kernel<64, false>);
+    hipLaunchKernelGGL((prepare_qk_kernel<D, BF16IN, true>), grid, dim3(256), 0, st, a, prepare_parts(a));
+}
+
+hipError_t launch_prepare_qk(hipStream_t st, const PrepareArgs& a) {
+  if (a.dim == 128)
+    a.bf16 ? start_prepare_qk<128, true>(st, a) : start_prepare_qk<128, false>(st, a);
+  else
+    a.bf16 ? start_prepare_qk<64, true>(st, a) : start_prepare_qk<64, false>(st, a);
   return hipGetLastError();
 }
 
