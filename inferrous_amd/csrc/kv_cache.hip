@@ -183,7 +183,16 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
     return;
   }
 
+  // the page and what its scales were, asked for before the rows
   const uint32_t h = part;
+  int32_t id = a.codes && page < a.width ? a.table[(size_t)seq * a.width + page] : -1;
+  if ((uint32_t)id >= a.pages) id = -1;
+  const size_t block = (size_t)max(id, 0) * a.kv_heads + h;
+  uint8_t* const codes = a.codes + block * page_head_bytes(D);
+  uint8_t* const vcodes = codes + kPageTokens * D;
+  float* const scales = a.scales + block * 2;
+  const bool added = n0 && id >= 0;  // to tokens that are there
+  const float k_was = added ? scales[0] : 0.f, v_was = added ? scales[1] : 0.f;
   Share k[SLOTS] = {}, v[SLOTS] = {};
   uint32_t k_top = 0, v_top = 0;
   const uint32_t s0 = SLOTS * group;
@@ -216,14 +225,7 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
       }
     }
   }
-  if (!a.codes || page >= a.width) return;
-  const int32_t id = a.table[(size_t)seq * a.width + page];
-  if (id < 0 || (uint32_t)id >= a.pages) return;
-  uint8_t* const codes = a.codes + ((size_t)id * a.kv_heads + h) * page_head_bytes(D);
-  uint8_t* const vcodes = codes + kPageTokens * D;
-  float* const scales = a.scales + ((size_t)id * a.kv_heads + h) * 2;
-  const float k_was = n0 ? scales[0] : 0.f, v_was = n0 ? scales[1] : 0.f;
-
+  if (id < 0) return;
   k_top = wave_max_u32(k_top);
   v_top = wave_max_u32(v_top);
   if ((tid & 63) == 0) red[0][tid >> 6] = k_top, red[1][tid >> 6] = v_top;
