@@ -616,7 +616,7 @@ int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
  * NaN and infinities become NaN codes.  Slots behind the last token are left as
  * they were.  A page may be in the table of one sequence that writes to it.
  * starts, past, table and scales 4-byte, everything else 16-byte aligned; strides
- * multiples of 8. */
+ * multiples of 8, at most 2^24. */
 #define W8A8_PAGE_TOKENS 64
 int w8a8_prepare_qk(void *stream, const void *q, size_t q_stride, const void *k,
                     size_t k_stride, const void *v, size_t v_stride, int dtype,

@@ -1169,8 +1169,11 @@ static int check_heads(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t hea
   return m > kMaxAttentionRows ? W8A8_ESHAPE : W8A8_OK;
 }
 
-// Rows of `values` values, `stride` from row to row.
-static bool good_stride(size_t stride, size_t values) { return stride >= values && stride % 8 == 0 && stride <= kU32Max; }
+// Rows of `values` values, `stride` from row to row: the offsets in a tile of 64 rows
+// fit 32 bits.
+static bool good_stride(size_t stride, size_t values) {
+  return stride >= values && stride % 8 == 0 && stride <= kMaxRowStride;
+}
 
 int w8a8_prepare_qk(void* stream, const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v,
                     size_t v_stride, int dtype, size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,

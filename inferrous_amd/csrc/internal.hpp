@@ -292,7 +292,7 @@ hipError_t launch_adapters_after(hipStream_t st, const AdapterArgs& a, const int
 // power-of-two scale of each.
 constexpr uint32_t kPageTokens = 64;
 __host__ __device__ constexpr size_t page_head_bytes(uint32_t head_dim) { return (size_t)2 * kPageTokens * head_dim; }
-constexpr uint32_t kMaxHeads = 1024, kMaxAttentionRows = 1u << 24, kMaxTableWidth = 1u << 24;
+constexpr uint32_t kMaxHeads = 1024, kMaxAttentionRows = 1u << 24, kMaxTableWidth = 1u << 24, kMaxRowStride = 1u << 24;
 
 // prepare_qk (kv_cache.hip): rows' heads normalised, rotated and appended.
 struct PrepareArgs {

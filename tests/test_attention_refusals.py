@@ -59,6 +59,13 @@ def test_attention_prefill(kw, status):
     assert prefill(**kw) == status
 
 
+@without_gpu
+@pytest.mark.parametrize("stride", ["qs", "ks", "vs"])
+def test_strides_keep_offsets_in_32_bits(stride):
+    for call in (prepare, prefill):
+        assert call(**{stride: 1 << 24}) == WELL and call(**{stride: (1 << 24) + 8}) == _lib.ESHAPE
+
+
 def decode(short=0, **kw):
     a = dict(q=A, m=3, h=32, kv=8, d=128, c=A, sc=A, pages=10, n=A, t=A, w=64, scale=0.1, out=A, dt=_lib.OUT_BF16, ws=A)
     a.update(kw)
