@@ -111,8 +111,11 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
     for (int s = 0; s < STEPS; ++s) q[s] = *(const v4u*)(p + 16 * s + 8 * half);
   }
 
-  const auto key_swizzle = [](int row) { return row & (CH - 1); };
-  const auto value_swizzle = [](int row) { return D == 128 ? (row & 7) * 2 : (row & 3) * 2; };
+  // 16-byte chunks of a row change places so that what one cycle of LDS serves, 256
+  // bytes in 64 banks, lies in as many banks: a chunk of 16 rows of keys, four chunks of
+  // four rows of values.
+  const auto key_swizzle = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+  const auto value_swizzle = [](int row) { return D == 128 ? (row & 3) * 4 : (row >> 1 & 1) * 4; };
   const uint16_t* const kbase = a.k + (size_t)r.lo * a.k_stride + (size_t)head * D;
   const uint16_t* const vbase = a.v + (size_t)r.lo * a.v_stride + (size_t)head * D;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
