@@ -27,7 +27,7 @@
 
 namespace w8a8 {
 
-constexpr int kTileKeys = 64, kPrefillWaves = 8;
+constexpr int kTileKeys = 64;
 
 // 16 keys of 32 columns of the values in LDS, as the first operand: lane l's
 // column is l % 32 and its keys 4 (l / 32) + {0..3, 8..11}.
@@ -73,9 +73,9 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t at, uint3
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(to) : "memory");
 }
 
-template <int D>
-__global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kernel(PrefillArgs a) {
-  constexpr int NW = kPrefillWaves, ROWS = 32 * NW, CH = D / 8, STEPS = D / 16, COLS = D / 32;
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(PrefillArgs a) {
+  constexpr int ROWS = 32 * NW, CH = D / 8, STEPS = D / 16, COLS = D / 32;
   constexpr int TILE = kTileKeys * D * 2;  // bytes of a tile of keys, or of values
   constexpr int LOADS = TILE / 1024 / NW;  // of a wave for one of them
   static_assert(LOADS * NW * 1024 == TILE, "whole loads");
@@ -434,18 +434,32 @@ __global__ __launch_bounds__(64 * kPrefillWaves, 2) void attention_prefill_kerne
     }
 }
 
-// Every tile has a row, and a sequence has at most one tile that is not full.
-uint64_t attention_prefill_blocks(const PrefillArgs& a) {
+// Workgroups of `waves` waves: each has a row, and all of a sequence's but its last
+// are full.
+static uint64_t prefill_blocks(const PrefillArgs& a, int waves) {
   const uint64_t rows = (uint64_t)a.m * (a.heads / a.kv_heads);
-  return std::min<uint64_t>(rows / (32 * kPrefillWaves) + a.seqs, rows) * a.kv_heads;
+  return std::min<uint64_t>((rows + (uint64_t)a.seqs * (32 * waves - 1)) / (32 * waves), rows) * a.kv_heads;
+}
+
+// Half the rows a workgroup where the compute units have no second workgroup of whole
+// ones to take: one wave a SIMD then ends sooner than two.  One sequence of 32/8 heads
+// of 128, 128 rows / 256 rows a workgroup, us: 200 tokens 11.3 / 12.5, 512 16.1 / 18.9,
+// 1024 25.9 / 31.0, 1400 33.7 / 40.1, 2048 54.1 / 57.3, 2300 72.4 / 65.4, 4096 176 / 139.
+static int prefill_waves(const PrefillArgs& a) { return prefill_blocks(a, 8) <= 256 ? 4 : 8; }
+
+uint64_t attention_prefill_blocks(const PrefillArgs& a) { return prefill_blocks(a, prefill_waves(a)); }
+
+template <int D, int NW>
+static void start_prefill(hipStream_t st, const PrefillArgs& a) {
+  hipLaunchKernelGGL((attention_prefill_kernel<D, NW>), dim3((uint32_t)prefill_blocks(a, NW)), dim3(64 * NW), 0, st, a);
 }
 
 hipError_t launch_attention_prefill(hipStream_t st, const PrefillArgs& a) {
-  const dim3 grid((uint32_t)attention_prefill_blocks(a)), block(64 * kPrefillWaves);
+  const bool small = prefill_waves(a) == 4;
   if (a.dim == 128)
-    hipLaunchKernelGGL(attention_prefill_kernel<128>, grid, block, 0, st, a);
+    small ? start_prefill<128, 4>(st, a) : start_prefill<128, 8>(st, a);
   else
-    hipLaunchKernelGGL(attention_prefill_kernel<64>, grid, block, 0, st, a);
+    small ? start_prefill<64, 4>(st, a) : start_prefill<64, 8>(st, a);
   return hipGetLastError();
 }
 

@@ -1,0 +1,76 @@
+"""Attention of prompts in workgroups of 128 and of 256 rows: which of the two runs
+depends on how many a batch can have, and empty sequences count as one.
+(Inputs, 64-bit forms and tolerances: test_gpu_attention.py.)"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from inferrous_amd import CudaContext, load
+from test_gpu_attention import F32, Prefill, bf16, close
+
+pytestmark = pytest.mark.gpu
+
+LAYOUTS = [(4, 1, 128), (2, 2, 64), (7, 1, 64), (8, 2, 128)]
+SIZES = pytest.mark.parametrize("empty", [0, 300])
+
+
+@pytest.fixture(scope="module")
+def env():
+    ctx = CudaContext(0)
+    return load(ctx), ctx.new_stream(), ctx
+
+
+@SIZES
+@pytest.mark.parametrize("heads, kv, dim", LAYOUTS)
+@pytest.mark.parametrize("rows", [[1], [63, 0, 64, 65], [257, 130], [1100, 5]])
+def test_prefill(env, heads, kv, dim, rows, empty):
+    Prefill(len(rows) + heads, [*rows, *[0] * empty], heads, kv, dim, lead=1, behind=3).check(env)
+
+
+@pytest.mark.parametrize("heads, kv, dim", [(32, 8, 128), (32, 32, 64)])
+def test_prefill_fills_the_card(env, heads, kv, dim):
+    Prefill(1, [2100], heads, kv, dim).check(env, starts=False)
+
+
+@SIZES
+@pytest.mark.parametrize("heads, kv, dim", LAYOUTS)
+@pytest.mark.parametrize("n", [64, 127, 128, 129, 192, 513, 1500])
+def test_every_key_counts_once(env, heads, kv, dim, n, empty):
+    c = Prefill(2, [n, 5, *[0] * empty], heads, kv, dim)
+    c.q[:] = 0
+    c.v = np.random.default_rng(n).integers(-8, 9, c.v.shape).astype(F32)
+    close(c.run(env), *c.want(exact=True))
+
+
+@SIZES
+@pytest.mark.parametrize("step", [30.0, -30.0, 9.0])
+def test_scores_far_apart(env, step, empty):
+    """The running maximum moves at every group of keys, or never again; what a
+    row does not see is far above what it does."""
+    c = Prefill(3, [500, *[0] * empty], 2, 1, 128)
+    c.q[:] = 0
+    c.k[:] = 0
+    c.q[..., 0] = 1.0
+    c.k[:, 0, 0] = bf16(np.arange(500) // 8 * step)
+    # groups of eight equal scores: each probability is 1 or at most e^-9, and a sum's weight beside it below 2^-9
+    got = c.run(env, scale=1.0)
+    want, err = c.want(scale=1.0)
+    close(got, want, err)
+
+
+@SIZES
+@pytest.mark.parametrize("heads, kv, dim", [(4, 1, 128), (2, 2, 64)])
+@pytest.mark.parametrize("n, at", [(100, 99), (300, 70), (300, 200), (700, 400), (64, 0)])
+def test_what_is_not_seen_does_not_count(env, heads, kv, dim, n, at, empty):
+    c = Prefill(4, [n, 40, *[0] * empty], heads, kv, dim)
+    clean = c.run(env)
+    for which, x in ((c.v, np.nan), (c.v, np.inf), (c.v, -np.inf), (c.k, np.nan), (c.k, np.inf)):
+        kept = which[at].copy()
+        which[at, 0, 3] = x
+        got = c.run(env)
+        assert np.array_equal(got[:at], clean[:at])
+        assert np.array_equal(got[n:], clean[n:])
+        if np.isnan(x) or which is c.v:
+            close(got, *c.want())
+        which[at] = kept
