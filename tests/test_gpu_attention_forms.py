@@ -74,3 +74,13 @@ def test_what_is_not_seen_does_not_count(env, heads, kv, dim, n, at, empty):
         if np.isnan(x) or which is c.v:
             close(got, *c.want())
         which[at] = kept
+
+
+@SIZES
+@pytest.mark.parametrize("n", [40, 100])
+def test_scores_of_minus_infinity_weigh_nothing(env, n, empty):
+    """The first n keys' scores overflow f32 downwards."""
+    c = Prefill(5, [n + 70, *[0] * empty], 4, 2, 64)
+    c.q[:, :, 0], c.k[:n, :, 0], c.k[n:, :, 0] = bf16(np.float32(3e38)), bf16(np.float32(-3e38)), 0
+    want, err = c.want()
+    close(c.run(env)[n:], want[n:], err[n:])
