@@ -34,6 +34,7 @@ struct DecodeSplit {
   uint32_t tiles;   // workgroups a key/value head's query heads take
   uint32_t chunk;   // pages of a workgroup
   uint32_t splits;  // workgroups of the widest sequence
+  uint32_t turn;    // rows that a turn of the compute units takes, 0: in the order they have
 };
 
 constexpr uint32_t kMaxSplits = 64;
@@ -50,6 +51,7 @@ static DecodeSplit decode_split(uint32_t m, uint32_t heads, uint32_t kv_heads, u
   const uint32_t splits = (uint32_t)std::min<uint64_t>(kMaxSplits, std::max<uint64_t>(1, 512 / units));
   d.chunk = ((width + splits - 1) / splits + kDecodeWaves - 1) / kDecodeWaves * kDecodeWaves;
   d.splits = (width + d.chunk - 1) / d.chunk;
+  d.turn = d.splits == 1 && m <= kWave ? std::max(1u, 256 / (kv_heads * d.tiles)) : 0;
   return d;
 }
 
@@ -95,6 +97,19 @@ struct PageCodes {
   float scale;  // of the keys in even lanes, of the values in odd ones
 };
 
+// The row that workgroup `place` of all takes: the rows by length, the longest first in
+// even turns of the compute units and the shortest first in odd ones.
+__device__ __forceinline__ uint32_t row_of_turn(const DecodeArgs& a, uint32_t place, uint32_t turn) {
+  const uint32_t lane = threadIdx.x & 63, n = place / turn, at = place % turn;
+  const uint32_t rank = n * turn + (n % 2 ? min(turn, a.m - n * turn) - 1 - at : at);
+  const uint32_t pages = lane < a.m ? ((uint32_t)max(a.lengths[lane], 0) + kPageTokens - 1) / kPageTokens : 0u;
+  const uint32_t key = min(pages, a.width) * 64 + (63 - lane);  // no two alike
+  uint32_t before = 0;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) before += (uint32_t)__builtin_amdgcn_readlane((int)key, i) > key;
+  return (uint32_t)__builtin_ctzll(__ballot(before == rank));
+}
+
 // partial: of sequences with more pages than a chunk, of each row, head and split its
 // unscaled sum o[D], then of each {m, l}.
 template <int D>
@@ -110,7 +125,9 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
   b /= a.kv_heads;
   const uint32_t tile = b % d.tiles;
   b /= d.tiles;
-  const uint32_t split = b % d.splits, row = b / d.splits;
+  const uint32_t split = b % d.splits;
+  uint32_t row = b / d.splits;
+  if (d.turn) row = row_of_turn(a, row, d.turn);
   const uint32_t head0 = h * group + tile * kDecodeHeads, live = min(kDecodeHeads, group - tile * kDecodeHeads);
 
   const int32_t* const table = a.table + (size_t)row * a.width;
