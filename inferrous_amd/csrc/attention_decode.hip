@@ -34,7 +34,7 @@ struct DecodeSplit {
   uint32_t tiles;   // workgroups a key/value head's query heads take
   uint32_t chunk;   // pages of a workgroup
   uint32_t splits;  // workgroups of the widest sequence
-  uint32_t turn;    // rows that a turn of the compute units takes, 0: in the order they have
+  uint32_t turn;    // units that a turn of the compute units takes, 0: in the order they have
 };
 
 constexpr uint32_t kMaxSplits = 64;
@@ -44,6 +44,14 @@ constexpr uint32_t join_splits(int waves) { return waves == 1 ? 16 : kMaxSplits;
 // Splits: two workgroups a CU where a wave keeps a page.  More, where the longest
 // sequences bound a large batch, gains less there than the join costs: 64 sequences
 // of up to 4096 tokens, 59 us alone, 60-65 us in 2 to 8 splits.
+//
+// Turns: workgroups that share a compute unit start together, so the order decides
+// which do.  Ranking the units takes each workgroup under a microsecond, paid back where
+// one has two pages a wave to read, up to 64 units (a lane each) or 256 whole rows.  32/8
+// heads of 128, in the rows' order / by pages, us: 8 sequences of up to 4096 tokens
+// 12.3 / 10.9, 16 17.7 / 13.9, 32 29.9 / 24.4, 64 53.8 / 47.0, 64 of up to 600
+// 10.8 / 10.1, 128 of up to 2000 52.4 / 47.8, 200 80.1 / 77.7.  More than 64 units of split
+// rows, 14/2 heads of 64: 5 of up to 65536 13.5 / 15.6, 100 of up to 4096 15.5 / 16.5.
 static DecodeSplit decode_split(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width) {
   DecodeSplit d;
   d.tiles = (heads / kv_heads + kDecodeHeads - 1) / kDecodeHeads;
@@ -51,7 +59,7 @@ static DecodeSplit decode_split(uint32_t m, uint32_t heads, uint32_t kv_heads, u
   const uint32_t splits = (uint32_t)std::min<uint64_t>(kMaxSplits, std::max<uint64_t>(1, 512 / units));
   d.chunk = ((width + splits - 1) / splits + kDecodeWaves - 1) / kDecodeWaves * kDecodeWaves;
   d.splits = (width + d.chunk - 1) / d.chunk;
-  d.turn = d.splits == 1 && m <= kWave ? std::max(1u, 256 / (kv_heads * d.tiles)) : 0;
+  d.turn = m > 1 && (m * d.splits <= 64 || (d.splits == 1 && m <= 256)) && d.chunk >= 8 ? std::max(1u, 256 / (kv_heads * d.tiles)) : 0;
   return d;
 }
 
@@ -97,17 +105,35 @@ struct PageCodes {
   float scale;  // of the keys in even lanes, of the values in odd ones
 };
 
-// The row that workgroup `place` of all takes: the rows by length, the longest first in
-// even turns of the compute units and the shortest first in odd ones.
-__device__ __forceinline__ uint32_t row_of_turn(const DecodeArgs& a, uint32_t place, uint32_t turn) {
-  const uint32_t lane = threadIdx.x & 63, n = place / turn, at = place % turn;
-  const uint32_t rank = n * turn + (n % 2 ? min(turn, a.m - n * turn) - 1 - at : at);
-  const uint32_t pages = lane < a.m ? ((uint32_t)max(a.lengths[lane], 0) + kPageTokens - 1) / kPageTokens : 0u;
-  const uint32_t key = min(pages, a.width) * 64 + (63 - lane);  // no two alike
-  uint32_t before = 0;
+// The unit (a row's split) that workgroup `place` of a key/value head takes: by their
+// pages, the most first in even turns of the compute units and the fewest first in odd ones.
+__device__ __forceinline__ uint32_t unit_of_turn(const DecodeArgs& a, const DecodeSplit& d, uint32_t place, uint32_t* keys) {
+  const uint32_t lane = threadIdx.x & 63, units = a.m * d.splits;
+  const uint32_t n = place / d.turn, at = place % d.turn;
+  const uint32_t rank = n * d.turn + (n % 2 ? min(d.turn, units - n * d.turn) - 1 - at : at);
+  const auto key = [&](uint32_t u) {  // no two alike
+    const uint32_t row = u / d.splits, first = u % d.splits * d.chunk;
+    const uint32_t pages = u < units ? min(((uint32_t)max(a.lengths[row], 0) + kPageTokens - 1) / kPageTokens, a.width) : 0u;
+    return (pages > first ? min(pages - first, d.chunk) : 0u) * 256 + (255 - u);
+  };
+  const auto before = [&](uint32_t mine, uint32_t others) {
+    uint32_t sum = 0;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) before += (uint32_t)__builtin_amdgcn_readlane((int)key, i) > key;
-  return (uint32_t)__builtin_ctzll(__ballot(before == rank));
+    for (int i = 0; i < 64; ++i) sum += (uint32_t)__builtin_amdgcn_readlane((int)others, i) > mine;
+    return sum;
+  };
+  if (units <= 64) {  // each wave for itself
+    const uint32_t k = key(lane);
+    return (uint32_t)__builtin_ctzll(__ballot(before(k, k) == rank));
+  }
+  const uint32_t k = key(threadIdx.x);
+  keys[threadIdx.x] = k;
+  __syncthreads();
+  uint32_t sum = 0;
+  for (uint32_t u = 0; u < units; u += 64) sum += before(k, keys[u + lane]);
+  if (sum == rank) keys[256] = threadIdx.x;
+  __syncthreads();
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)keys[256]);
 }
 
 // partial: of sequences with more pages than a chunk, of each row, head and split its
@@ -117,6 +143,7 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
   constexpr int HALVES = D / 64, TILES = D / 16;
   __shared__ float sh_m[4][16], sh_l[4][16];
   __shared__ float sh_o[4][16][D + 4];
+  __shared__ uint32_t keys[257];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t group = a.heads / a.kv_heads;
@@ -125,9 +152,8 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
   b /= a.kv_heads;
   const uint32_t tile = b % d.tiles;
   b /= d.tiles;
-  const uint32_t split = b % d.splits;
-  uint32_t row = b / d.splits;
-  if (d.turn) row = row_of_turn(a, row, d.turn);
+  if (d.turn) b = unit_of_turn(a, d, b, keys);
+  const uint32_t split = b % d.splits, row = b / d.splits;
   const uint32_t head0 = h * group + tile * kDecodeHeads, live = min(kDecodeHeads, group - tile * kDecodeHeads);
 
   const int32_t* const table = a.table + (size_t)row * a.width;

@@ -1,5 +1,6 @@
 """Attention of prompts in workgroups of 128 and of 256 rows: which of the two runs
-depends on how many a batch can have, and empty sequences count as one.
+depends on how many a batch can have, and empty sequences count as one.  Attention
+over the cache in the orders that its workgroups take rows and splits in.
 (Inputs, 64-bit forms and tolerances: test_gpu_attention.py.)"""
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, load
-from test_gpu_attention import F32, Prefill, bf16, close
+from test_gpu_attention import F32, PAGE, Decode, Prefill, bf16, close
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +85,31 @@ def test_scores_of_minus_infinity_weigh_nothing(env, n, empty):
     c.q[:, :, 0], c.k[:n, :, 0], c.k[n:, :, 0] = bf16(np.float32(3e38)), bf16(np.float32(-3e38)), 0
     want, err = c.want()
     close(c.run(env)[n:], want[n:], err[n:])
+
+
+@pytest.mark.parametrize("heads, kv, dim, m, most, width", [
+    (16, 8, 128, 64, 900, None), (16, 8, 128, 33, 1100, None), (8, 8, 64, 16, 2050, None), (6, 3, 64, 50, 700, 70),
+    (32, 8, 128, 8, 4096, None), (34, 2, 64, 20, 1500, None),          # ranked a lane each
+    (8, 8, 128, 65, 600, None), (8, 8, 64, 200, 600, 12), (5, 5, 128, 256, 520, None),  # by the workgroup
+    (8, 8, 64, 257, 600, None), (8, 8, 64, 64, 200, None), (2, 2, 64, 100, 2100, None)])  # in the order they have
+def test_decode_orders(env, heads, kv, dim, m, most, width):
+    """All kinds of lengths, many alike, none, negative ones and some beyond the table."""
+    rng = np.random.default_rng(m)
+    lengths = rng.integers(0, most + 1, m)
+    lengths[rng.integers(0, m, m // 4)] = most // 2
+    lengths[::7] = 0
+    lengths[1], lengths[-1] = most, 1
+    c = Decode(m, lengths.tolist(), heads, kv, dim, width=width)
+    c.lengths[0] = -5
+    if width is None:
+        c.lengths[1] = c.width * PAGE + 100
+        page = c.table[1, -1]   # its last page, seen to the end
+        c.cache.k[page], c.cache.v[page] = 0x30, 0x31
+    c.check(env)
+
+
+def test_decode_orders_one_length(env):
+    for n in (0, 640):
+        c = Decode(1, [640] * 40, 8, 8, 64)
+        c.lengths = [n] * 40
+        c.check(env)
