@@ -132,14 +132,14 @@ __device__ __forceinline__ void norm_rotate(Share& x, bool norm, const Gains<D>&
 constexpr uint32_t kPrepareHeads = 4;  // query heads that a group of lanes takes of one token
 
 // A unit is the rows that one sequence brings to one page.  Of a unit, one
-// workgroup takes a key/value head (its 64 x D keys and values: whole blocks of
-// the cache, so that their scale is one workgroup's).  The queries of GROUPS of its
+// workgroup takes a head's 64 x D keys or values (a whole block of the cache, so that
+// its scale is one workgroup's).  The queries of GROUPS of its
 // tokens and of kPrepareHeads heads are one workgroup's, too; if every sequence
 // brings one row (ONE), GROUPS heads of it are.  D / 8 lanes hold a head.
 template <int D, bool BF16IN, bool ONE>
 __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t blocks) {
   constexpr int LPH = D / 8, GROUPS = 256 / LPH, SLOTS = 64 / GROUPS;  // lanes of a head, heads in flight, tokens of a group
-  __shared__ uint32_t red[2][4];
+  __shared__ uint32_t red[4];
   __shared__ __align__(16) uint32_t turned[ONE ? 1 : D * kPageTokens / 4];  // the page's value codes
   const uint32_t unit = blockIdx.x / blocks, part = blockIdx.x % blocks;
   const int tid = threadIdx.x, i = tid % LPH, group = tid / LPH;
@@ -161,10 +161,10 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
   const uint32_t n0 = first - page * kPageTokens, n1 = last - page * kPageTokens;  // the unit's slots of the page
   const uint32_t row0 = lo + (first - past);
 
-  if (part >= a.kv_heads) {
+  if (part >= 2 * a.kv_heads) {
     constexpr uint32_t TIMES = ONE ? 1 : kPrepareHeads, HEADS = ONE ? GROUPS : kPrepareHeads;
-    const uint32_t sets = (a.heads + HEADS - 1) / HEADS, set = (part - a.kv_heads) % sets;
-    const uint32_t t = ONE ? 0u : (part - a.kv_heads) / sets * GROUPS + group, h0 = set * HEADS + (ONE ? group : 0u);
+    const uint32_t sets = (a.heads + HEADS - 1) / HEADS, set = (part - 2 * a.kv_heads) % sets;
+    const uint32_t t = ONE ? 0u : (part - 2 * a.kv_heads) / sets * GROUPS + group, h0 = set * HEADS + (ONE ? group : 0u);
     if (t >= n1 - n0 || h0 >= a.heads) return;
     const size_t row = row0 + t;
     Read<D, BF16IN> in[TIMES];
@@ -183,88 +183,93 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
     return;
   }
 
-  // the page and what its scales were, asked for before the rows
-  const uint32_t h = part;
+  // The keys of a head, or its values.  The page and what its scale was are asked for
+  // before the rows.
+  const bool keys = part < a.kv_heads;
+  const uint32_t h = keys ? part : part - a.kv_heads;
   int32_t id = a.codes && page < a.width ? a.table[(size_t)seq * a.width + page] : -1;
   if ((uint32_t)id >= a.pages) id = -1;
   const size_t block = (size_t)max(id, 0) * a.kv_heads + h;
-  uint8_t* const codes = a.codes + block * page_head_bytes(D);
-  uint8_t* const vcodes = codes + kPageTokens * D;
-  float* const scales = a.scales + block * 2;
-  const bool added = n0 && id >= 0;  // to tokens that are there
-  const float k_was = added ? scales[0] : 0.f, v_was = added ? scales[1] : 0.f;
-  Share k[SLOTS] = {}, v[SLOTS] = {};
-  uint32_t k_top = 0, v_top = 0;
+  uint8_t* const codes = a.codes + block * page_head_bytes(D) + (keys ? 0 : kPageTokens * D);
+  float* const scale = a.scales + block * 2 + (keys ? 0 : 1);
+  const float was = n0 && id >= 0 ? *scale : 0.f;  // of tokens that are there
+
+  Share x[SLOTS] = {};
+  uint32_t top = 0;
   const uint32_t s0 = SLOTS * group;
   if (s0 < n1 && s0 + SLOTS > n0) {  // the same for a head's lanes
-    Read<D, BF16IN> k_in[SLOTS], v_in[SLOTS];
-    Angles<D> angles[SLOTS];
-    Gains<D> gains;
+    const auto row_of = [&](int j) { return min(max(s0 + j, n0), n1 - 1) - n0; };
+    Read<D, BF16IN> in[SLOTS];
+    uint16_t* const out = keys ? a.k_out : a.v_out;
+    const void* const from = keys ? a.k : a.v;
+    const size_t stride = keys ? a.k_stride : a.v_stride;
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) {
-      const uint32_t t = min(max(s0 + j, n0), n1 - 1) - n0;
-      const size_t row = row0 + t;
-      k_in[j].start(a.k, row * a.k_stride + (size_t)h * D, i);
-      v_in[j].start(a.v, row * a.v_stride + (size_t)h * D, i);
-      angles[j].start(a.rope, a.rope_rows, first + t, i);
-    }
-    gains.start(a.k_gain, i);
+    for (int j = 0; j < SLOTS; ++j) in[j].start(from, (row0 + row_of(j)) * stride + (size_t)h * D, i);
+    if (keys) {
+      Angles<D> angles[SLOTS];
+      Gains<D> gains;
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) {
-      k[j] = k_in[j].share();
-      v[j] = v_in[j].share();
-      norm_rotate<D>(k[j], a.k_gain, gains, a.eps, angles[j]);
-      if (s0 + j < n0 || s0 + j >= n1) continue;
-      const size_t row = row0 + (s0 + j - n0);
-      if (a.k_out) store_share<D>(a.k_out, (row * a.kv_heads + h) * D, i, k[j]);
-      if (a.v_out) store_share<D>(a.v_out, (row * a.kv_heads + h) * D, i, v[j]);
+      for (int j = 0; j < SLOTS; ++j) angles[j].start(a.rope, a.rope_rows, first + row_of(j), i);
+      gains.start(a.k_gain, i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        k_top = max(k_top, max(finite_bits(k[j].lo[e]), finite_bits(k[j].hi[e])));
-        v_top = max(v_top, max(finite_bits(v[j].lo[e]), finite_bits(v[j].hi[e])));
+      for (int j = 0; j < SLOTS; ++j) {
+        x[j] = in[j].share();
+        norm_rotate<D>(x[j], a.k_gain, gains, a.eps, angles[j]);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < SLOTS; ++j) x[j] = in[j].share();
+    }
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+      if (s0 + j < n0 || s0 + j >= n1) continue;
+      if (out) store_share<D>(out, ((row0 + (s0 + j - n0)) * (size_t)a.kv_heads + h) * D, i, x[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(finite_bits(x[j].lo[e]), finite_bits(x[j].hi[e])));
     }
   }
   if (id < 0) return;
-  k_top = wave_max_u32(k_top);
-  v_top = wave_max_u32(v_top);
-  if ((tid & 63) == 0) red[0][tid >> 6] = k_top, red[1][tid >> 6] = v_top;
+  top = wave_max_u32(top);
+  if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
-  k_top = max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3]));
-  v_top = max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]));
-  const float k_s = fmaxf(page_scale(k_top), k_was), v_s = fmaxf(page_scale(v_top), v_was);
-  if (tid == 0) scales[0] = k_s, scales[1] = v_s;
+  top = max(max(red[0], red[1]), max(red[2], red[3]));
+  const float now = fmaxf(page_scale(top), was), r = pow2_inverse(now);
+  if (tid == 0) *scale = now;
 
   // a larger scale: the codes that are there move down
-  if (n0 && k_s > k_was) {
-    const float f = k_was * pow2_inverse(k_s);
-    for (uint32_t w = tid; w < n0 * (D / 4); w += 256) ((uint32_t*)codes)[w] = codes_times(((uint32_t*)codes)[w], f);
-  }
-  if (n0 && v_s > v_was) {
-    const float f = v_was * pow2_inverse(v_s);
-    for (uint32_t w = tid; w < D * (kPageTokens / 4); w += 256) {
-      const uint32_t slot = w % (kPageTokens / 4) * 4;
-      if (slot >= n0) continue;
-      const uint32_t keep = n0 - slot < 4 ? 0xffffffffu << 8 * (n0 - slot) : 0u;  // later slots' bytes
-      uint32_t* const p = (uint32_t*)vcodes + w;
-      *p = (codes_times(*p, f) & ~keep) | (*p & keep);
+  if (n0 && now > was) {
+    const float f = was * r;
+    if (keys) {
+      for (uint32_t w = tid; w < n0 * (D / 4); w += 256) ((uint32_t*)codes)[w] = codes_times(((uint32_t*)codes)[w], f);
+    } else {
+      for (uint32_t w = tid; w < D * (kPageTokens / 4); w += 256) {
+        const uint32_t slot = w % (kPageTokens / 4) * 4;
+        if (slot >= n0) continue;
+        const uint32_t keep = n0 - slot < 4 ? 0xffffffffu << 8 * (n0 - slot) : 0u;  // later slots' bytes
+        uint32_t* const p = (uint32_t*)codes + w;
+        *p = (codes_times(*p, f) & ~keep) | (*p & keep);
+      }
     }
+  }
+  if (keys) {
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) {
+      const uint32_t slot = s0 + j;
+      if (slot < n0 || slot >= n1) continue;
+      uint32_t* const p = (uint32_t*)(codes + slot * D) + i;
+      p[0] = codes_of(x[j].lo[0] * r, x[j].lo[1] * r, x[j].lo[2] * r, x[j].lo[3] * r);
+      p[D / 8] = codes_of(x[j].hi[0] * r, x[j].hi[1] * r, x[j].hi[2] * r, x[j].hi[3] * r);
+    }
+    return;
   }
   __syncthreads();  // a word of the values' codes may hold old tokens and new ones
 
-  const float k_r = pow2_inverse(k_s), v_r = pow2_inverse(v_s);
   uint32_t held[8] = {};  // of each of the lane's columns, its slots' value codes
 #pragma unroll
   for (int j = 0; j < SLOTS; ++j) {
-    const uint32_t slot = SLOTS * group + j;
-    const Share &x = k[j], &y = v[j];
-    if (slot >= n0 && slot < n1) {
-      uint32_t* const p = (uint32_t*)(codes + slot * D) + i;
-      p[0] = codes_of(x.lo[0] * k_r, x.lo[1] * k_r, x.lo[2] * k_r, x.lo[3] * k_r);
-      p[D / 8] = codes_of(x.hi[0] * k_r, x.hi[1] * k_r, x.hi[2] * k_r, x.hi[3] * k_r);
-    }
-    const uint32_t a0 = codes_of(y.lo[0] * v_r, y.lo[1] * v_r, y.lo[2] * v_r, y.lo[3] * v_r);
-    const uint32_t a1 = codes_of(y.hi[0] * v_r, y.hi[1] * v_r, y.hi[2] * v_r, y.hi[3] * v_r);
+    const Share& y = x[j];
+    const uint32_t a0 = codes_of(y.lo[0] * r, y.lo[1] * r, y.lo[2] * r, y.lo[3] * r);
+    const uint32_t a1 = codes_of(y.hi[0] * r, y.hi[1] * r, y.hi[2] * r, y.hi[3] * r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       held[e] |= (a0 >> 8 * e & 0xffu) << 8 * j;
@@ -289,13 +294,13 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
       v4u x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = turned[column * WORDS + ((word + j) ^ turn)];
-      *(v4u*)(vcodes + 4 * at) = x;
+      *(v4u*)(codes + 4 * at) = x;
     }
     return;
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    uint8_t* const p = vcodes + (size_t)(4 * i + e % 4 + e / 4 * (D / 2)) * kPageTokens + s0;
+    uint8_t* const p = codes + (size_t)(4 * i + e % 4 + e / 4 * (D / 2)) * kPageTokens + s0;
     if (s0 >= n0 && s0 + SLOTS <= n1) {
       if constexpr (SLOTS == 4)
         *(uint32_t*)p = held[e];
@@ -312,8 +317,8 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
 // Workgroups of a unit: those of the key/value heads and of the queries.
 static uint32_t prepare_parts(const PrepareArgs& a) {
   const uint32_t groups = 256 / (a.dim / 8);
-  if (!a.starts) return a.kv_heads + (a.heads + groups - 1) / groups;
-  return a.kv_heads + (a.heads + kPrepareHeads - 1) / kPrepareHeads * (kPageTokens / groups);
+  if (!a.starts) return 2 * a.kv_heads + (a.heads + groups - 1) / groups;
+  return 2 * a.kv_heads + (a.heads + kPrepareHeads - 1) / kPrepareHeads * (kPageTokens / groups);
 }
 
 // Every unit has a row, and a sequence's pages hold 64 of its rows but for two.
