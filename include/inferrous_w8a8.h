@@ -634,8 +634,8 @@ int w8a8_prepare_qk(void *stream, const void *q, size_t q_stride, const void *k,
  * q, k, v: BF16 rows as above (k and v as w8a8_prepare_qk leaves them, v also
  * straight from a projection); starts NULL: one sequence of m rows.  Products and
  * sums are held in f32, probabilities in BF16.  out: [m, heads, head_dim], F32
- * (holding BF16 values) or BF16.  scale: positive.  What a row does not see never
- * reaches it, whatever it holds. */
+ * (holding BF16 values) or BF16.  scale: positive, at most 2e38.  What a row does
+ * not see never reaches it, whatever it holds. */
 int w8a8_attention_prefill(void *stream, const uint16_t *q, size_t q_stride,
                            const uint16_t *k, size_t k_stride,
                            const uint16_t *v, size_t v_stride, size_t m,

@@ -1169,6 +1169,9 @@ static int check_heads(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t hea
   return m > kMaxAttentionRows ? W8A8_ESHAPE : W8A8_OK;
 }
 
+// The kernels take scale * log2 e.
+static constexpr float kMaxScale = 2e38f;
+
 // Rows of `values` values, `stride` from row to row: the offsets in a tile of 64 rows
 // fit 32 bits.
 static bool good_stride(size_t stride, size_t values) {
@@ -1234,7 +1237,7 @@ int w8a8_attention_prefill(void* stream, const uint16_t* q, size_t q_stride, con
                            uint32_t head_dim, const int32_t* starts, uint32_t n_seq, float scale, void* out,
                            int out_dtype) {
   if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
-  if (!(scale > 0.f) || scale > 3e38f) return W8A8_EARG;
+  if (!(scale > 0.f) || scale > kMaxScale) return W8A8_EARG;
   const int s = check_heads(m, heads, kv_heads, head_dim);
   if (s != W8A8_OK) return s;
   if (!good_stride(q_stride, (size_t)heads * head_dim) || !good_stride(k_stride, (size_t)kv_heads * head_dim) ||
@@ -1286,7 +1289,7 @@ int w8a8_attention_decode(void* stream, const uint16_t* q, size_t m, uint32_t he
                           const int32_t* lengths, const int32_t* table, uint32_t table_width, float scale, void* out,
                           int out_dtype, void* workspace, size_t workspace_bytes) {
   if (out_dtype != W8A8_OUT_F32 && out_dtype != W8A8_OUT_BF16) return W8A8_EARG;
-  if (!(scale > 0.f) || scale > 3e38f) return W8A8_EARG;
+  if (!(scale > 0.f) || scale > kMaxScale) return W8A8_EARG;
   const int s = check_decode_shape(m, heads, kv_heads, head_dim, table_width);
   if (s != W8A8_OK) return s;
   if (pages == 0 || pages > 0x7fffffffu) return W8A8_ESHAPE;

@@ -12,6 +12,8 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+// A maximum before the first score.  Finite, so that scores of -inf (f32 overflows) weigh nothing.
+constexpr float kNoScore = -3.402823466e38f;
 
 // Two f32 values as BF16, nearest even, NaN kept (v_cvt_pk_bf16_f32).
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {

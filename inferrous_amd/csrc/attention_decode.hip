@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
       q[s] = *(const v4u*)(a.q + ((size_t)row * a.heads + head0 + c) * D + 64 * (s / 2) + 16 * g + 8 * (s % 2));
   }
   const float to_log2 = a.scale * kLog2e;
-  float m = -__builtin_inff(), l = 0.f;
+  float m = kNoScore, l = 0.f;
   v4f o[TILES] = {};
 
   const auto attend = [&](PageCodes<D>& x, uint32_t page) {
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
     top = groups_max(top);
-    if (__ballot(top > m + 8.f || m == -__builtin_inff())) {
+    if (__ballot(top > m + 8.f || m == kNoScore)) {
       const float to = fmaxf(m, top);
       const float f = to == m ? 1.f : exp2_fast(m - to);
       m = to;

@@ -45,8 +45,6 @@
 namespace w8a8 {
 
 constexpr int kTileKeys = 64;
-// A maximum before the first score.  Finite, so that scores of -inf (f32 overflows) weigh nothing.
-constexpr float kNoScore = -3e38f;
 
 // 16 keys of 32 columns of the values in LDS, as the first operand: lane l's
 // column is l % 32 and its keys 4 (l / 32) + {0..3, 8..11}.

@@ -94,6 +94,12 @@ def test_a_workspace_for_the_largest_batch_serves_every_smaller_one(heads, kv, w
     assert need == sorted(need)
 
 
+@without_gpu
+def test_scale_times_log2_e_is_finite():
+    for call in (prefill, decode):
+        assert call(scale=2e38) == WELL and call(scale=2.4e38) == _lib.EARG
+
+
 def copy(**kw):
     a = dict(c=A, sc=A, layers=2, pages=10, kv=8, d=128, src=A, dst=A, n=3)
     a.update(kw)

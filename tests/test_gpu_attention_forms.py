@@ -113,3 +113,14 @@ def test_decode_orders_one_length(env):
         c = Decode(1, [640] * 40, 8, 8, 64)
         c.lengths = [n] * 40
         c.check(env)
+
+
+def test_decode_scores_of_minus_infinity_weigh_nothing(env):
+    """A page's scores overflow f32 downwards."""
+    c = Decode(2, [200, 130], 4, 2, 64)
+    c.q[:, :, 0] = bf16(np.float32(3e38))
+    c.cache.k[..., 0] = 0
+    for row, page in ((0, 0), (1, 1)):
+        at = c.table[row, page]
+        c.cache.k[at, :, :, 0], c.cache.s[at, :, 0] = 0xF0, 64.0
+    c.check(env)
