@@ -75,14 +75,26 @@ def _needs(buf: DeviceBuffer, dtype: np.dtype, need: int, what: str):
         raise ValueError(f"{what} has {len(buf)} elements, needs at least {need}")
 
 
+def _where(buf: DeviceBuffer | None, dtype: np.dtype, need: int, what: str):
+    """The address of a buffer that may be left out."""
+    if buf is None:
+        return None
+    if buf.dtype != dtype or len(buf) < need:
+        _needs(buf, dtype, need, what)
+    return buf.ptr
+
+
 def _table_width(table: DeviceBuffer | None, seqs: int) -> int:
     """Pages of a row of a page table of seqs rows."""
     if table is None:
         raise ValueError("a page table is required")
     _needs(table, _I32, seqs, "table")
-    if seqs and len(table) % seqs:
+    if not seqs:
+        return 0
+    width, rest = divmod(len(table), seqs)
+    if rest:
         raise ValueError("the table must hold one row of pages a sequence")
-    return len(table) // seqs if seqs else 0
+    return width
 
 
 class LoadedModule:
@@ -858,38 +870,37 @@ class LoadedModule:
         ``k_out`` / ``v_out`` (uint16 [M, kv_heads, head_dim]) and ``cache``
         with ``table`` (int32 [S, width]) are optional."""
         heads, kv_heads, dim = int(heads), int(kv_heads), int(head_dim)
-        width, kv_width = heads * dim, kv_heads * dim
-        if width <= 0 or kv_width <= 0 or len(q_out) % width:
+        width, kv_width, out_len = heads * dim, kv_heads * dim, len(q_out)
+        if width <= 0 or kv_width <= 0 or out_len % width:
             raise ValueError("prepare_qk: q_out must hold M rows of heads * head_dim")
-        m = len(q_out) // width
+        m = out_len // width
         seqs = m if starts is None else len(starts) - 1
         dtype = q.dtype
-        code = _OUT.get(dtype)
-        if dtype != _F32 and dtype != _U16:
+        if dtype == _U16:
+            code, size = _lib.OUT_BF16, 2
+        elif dtype == _F32:
+            code, size = _lib.OUT_F32, 4
+        else:
             raise TypeError(f"q dtype {dtype} not supported (float32/uint16)")
-        _needs(q_out, _U16, 0, "q_out")
-        if seqs < 0 or (starts is not None and starts.dtype != _I32):
+        if q_out.dtype != _U16:
+            _needs(q_out, _U16, 0, "q_out")
+        if starts is not None and (seqs < 0 or starts.dtype != _I32):
             raise TypeError("starts must be int32 [S + 1]")
         if (k is None) != (v is None):
             raise ValueError("k and v go together")
-        size = q.dtype.itemsize
+        qp = q.ptr
         if k is None:
-            stride = width + 2 * kv_width
-            _check_len(q, m * stride, "q")
-            strides = (stride, stride, stride)
-            kp, vp = q.ptr + width * size, q.ptr + (width + kv_width) * size
+            q_stride = k_stride = width + 2 * kv_width
+            _check_len(q, m * q_stride, "q")
+            kp = qp + width * size
+            vp = kp + kv_width * size
         else:
-            strides = (width, kv_width, kv_width)
+            q_stride, k_stride = width, kv_width
             _check_len(q, m * width, "q")
-            _needs(k, dtype, m * kv_width, "k")
-            _needs(v, dtype, m * kv_width, "v")
-            kp, vp = k.ptr, v.ptr
-        _needs(rope, _F32, dim, "rope")
-        for buf, dt, need, what in ((q_gain, _F32, dim, "q_gain"), (k_gain, _F32, dim, "k_gain"),
-                                    (past, _I32, seqs, "past"), (k_out, _U16, m * kv_width, "k_out"),
-                                    (v_out, _U16, m * kv_width, "v_out")):
-            if buf is not None:
-                _needs(buf, dt, need, what)
+            kp, vp = _where(k, dtype, m * kv_width, "k"), _where(v, dtype, m * kv_width, "v")
+        rope_len = len(rope)
+        if rope.dtype != _F32 or rope_len < dim:
+            _needs(rope, _F32, dim, "rope")
         codes = scales = table_ptr = None
         pages = columns = 0
         if cache is not None:
@@ -899,13 +910,15 @@ class LoadedModule:
             (codes, scales), pages, table_ptr = cache.layer(layer), cache.pages, table.ptr
         elif table is not None:
             raise ValueError("a table names the pages of a cache")
+        optional = (_where(q_gain, _F32, dim, "q_gain"), _where(k_gain, _F32, dim, "k_gain"),
+                    _where(past, _I32, seqs, "past"), _where(k_out, _U16, m * kv_width, "k_out"),
+                    _where(v_out, _U16, m * kv_width, "v_out"))
         if m == 0 or seqs == 0:
             return
-        ptr = lambda b: None if b is None else b.ptr  # noqa: E731
-        check(lib().w8a8_prepare_qk(_h(stream), q.ptr, strides[0], kp, strides[1], vp, strides[2], code, m, heads,
-                                    kv_heads, dim, ptr(q_gain), ptr(k_gain), eps, rope.ptr, len(rope) // dim,
-                                    ptr(starts), ptr(past), seqs, q_out.ptr, ptr(k_out), ptr(v_out), codes, scales,
-                                    pages, table_ptr, columns), "prepare_qk")
+        check(lib().w8a8_prepare_qk(
+            _h(stream), qp, q_stride, kp, k_stride, vp, k_stride, code, m, heads, kv_heads, dim, optional[0], optional[1],
+            eps, rope.ptr, rope_len // dim, None if starts is None else starts.ptr, optional[2], seqs, q_out.ptr,
+            optional[3], optional[4], codes, scales, pages, table_ptr, columns), "prepare_qk")
 
     def attention_prefill(self, stream, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer, heads: int, kv_heads: int,
                           head_dim: int, out: DeviceBuffer, starts: DeviceBuffer | None = None,
