@@ -11,6 +11,13 @@
 // A scale is a power of two, so that x / s is exact, a larger one later only
 // shifts the codes that are there (exact but for e4m3's subnormals), and the
 // readers' conversion to BF16 (v_cvt_scalef32_pk_bf16_fp8) applies it for free.
+//
+// Bytes bound both.  prepare_qk reads and writes each value once; everything of a page's
+// head is one workgroup's, so that the scale needs no second pass, and each lane asks
+// for all its rows before it uses the first.  4096 rows of five sequences, 32/8 heads of 128,
+// BF16: 26.9 us for 111 MB (4.1 TB/s; a large copy reaches 4.93); one row 4.2 us, a chain
+// of three dependent loads (the row's past, its page, the page's scale) and two barriers.
+// copy_pages: 200 pages of 36 layers 350 us (5.4 TB/s), 16 KiB a workgroup.
 #include <algorithm>
 #include <type_traits>
 
@@ -277,7 +284,8 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
     }
   }
   if (!ONE && n1 - n0 == kPageTokens) {
-    // a whole page of value codes leaves through LDS, 16 bytes a lane
+    // a whole page of value codes leaves through LDS, 16 bytes a lane: straight from the
+    // registers a store's lanes would write 4 bytes each of 64 lines
     constexpr int WORDS = kPageTokens / 4;  // of a column
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
