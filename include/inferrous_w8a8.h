@@ -614,7 +614,7 @@ int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
  * finite magnitude of its tokens, or the scale it had if past[i] lies inside the
  * page and that is larger; if it grows, the codes before past[i] are rounded to it.
  * NaN and infinities become NaN codes.  Slots behind the last token are left as
- * they were.  A page may be in the table of one sequence that writes to it.
+ * they were.  A page that rows of the call go to may be named once.
  * starts, past, table and scales 4-byte, everything else 16-byte aligned; strides
  * multiples of 8, at most 2^24. */
 #define W8A8_PAGE_TOKENS 64

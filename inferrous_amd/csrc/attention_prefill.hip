@@ -185,14 +185,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(Pref
   const auto key = [&](uint32_t t, int b, int i) {
     return read_row(lds0 + t % 3 * TILE + (key_at ^ (32 * i)) + 32 * b * (2 * D));
   };
-  // the largest of 32 keys' scores, for both of the row's lanes
+  // the largest of the lane's part of 32 keys' scores
   const auto top_of = [&](const v16f& x) {
     float tops[2] = {x[0], x[1]};
 #pragma unroll
     for (int i = 2; i < 16; ++i) tops[i % 2] = larger(tops[i % 2], x[i]);
     return larger(tops[0], tops[1]);
   };
-  // of both of the row's lanes, as a power of two
+  // of the row, both of its lanes', as a power of two
   const auto both = [&](float top) {
     const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
     return fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * to_log2;
