@@ -1272,7 +1272,7 @@ static int check_decode_shape(size_t m, uint32_t heads, uint32_t kv_heads, uint3
   const int s = check_heads(m, heads, kv_heads, head_dim);
   if (s != W8A8_OK) return s;
   if (table_width == 0 || table_width > kMaxTableWidth || m * table_width > 0x7fffffffu) return W8A8_ESHAPE;
-  return attention_decode_blocks((uint32_t)m, heads, kv_heads, table_width) > kMaxBlocks256 ? W8A8_ESHAPE : W8A8_OK;
+  return attention_decode_blocks((uint32_t)m, heads, kv_heads, head_dim, table_width) > kMaxBlocks256 ? W8A8_ESHAPE : W8A8_OK;
 }
 
 size_t w8a8_attention_decode_workspace_bytes(size_t m, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,

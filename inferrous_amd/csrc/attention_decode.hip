@@ -45,9 +45,14 @@ constexpr uint32_t kMaxSplits = 64;
 // Splits that a join of so many waves a head takes.
 constexpr uint32_t join_splits(int waves) { return waves == 1 ? 16 : kMaxSplits; }
 
-// Splits: two workgroups a CU where a wave keeps a page.  More, where the longest
-// sequences bound a large batch, gains less there than the join costs: 64 sequences
-// of up to 4096 tokens, 59 us alone, 60-65 us in 2 to 8 splits.
+// Splits: two workgroups a compute unit where a wave keeps a page, but none where a row's
+// pages are few, or not many and the splits two: a join costs its launch, about three
+// pages of a wave.  In splits / alone, us, 32/8 heads of 128 unless said: 1 row of 12
+// pages 8.0 / 6.9, of 16 8.1 / 8.2, of 24 8.0 / 10.8; 14/2 heads of 64, 1 row of 24
+// 7.9 / 6.2, of 48 8.0 / 9.8.  Two splits, rows of all lengths up to so many pages, or all
+// of so many: 24 rows, 16 10.4 / 9.2 and 14.6 / 10.9, 24 12.2 / 12.0 and 18.5 / 14.5, 64
+// 25.0 / 25.7 and 39.3 / 31.6; 32 rows, 64 24.4 / 27.4 and 47.7 / 43.2.  Four, 16 rows,
+// 64 13.8 / 21.4 and 26.3 / 26.9.  Three or four workgroups a compute unit: 10 to 70% slower.
 //
 // Turns: workgroups that share a compute unit start together, so the order decides
 // which do.  Ranking the units takes each workgroup under a microsecond, paid back where
@@ -56,11 +61,12 @@ constexpr uint32_t join_splits(int waves) { return waves == 1 ? 16 : kMaxSplits;
 // 12.3 / 10.9, 16 17.7 / 13.9, 32 29.9 / 24.4, 64 53.8 / 47.0, 64 of up to 600
 // 10.8 / 10.1, 128 of up to 2000 52.4 / 47.8, 200 80.1 / 77.7.  More than 64 units of split
 // rows, 14/2 heads of 64: 5 of up to 65536 13.5 / 15.6, 100 of up to 4096 15.5 / 16.5.
-static DecodeSplit decode_split(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width) {
+static DecodeSplit decode_split(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width) {
   DecodeSplit d;
   d.tiles = (heads / kv_heads + kDecodeHeads - 1) / kDecodeHeads;
   const uint64_t units = (uint64_t)m * kv_heads * d.tiles;
-  const uint32_t splits = (uint32_t)std::min<uint64_t>(kMaxSplits, std::max<uint64_t>(1, 512 / units));
+  const uint64_t most = std::min<uint64_t>(kMaxSplits, 512 / units);
+  const uint32_t splits = most < 2 || (uint64_t)width * dim <= (most == 2 ? 24 : 12) * 128 ? 1 : (uint32_t)most;
   d.chunk = ((width + splits - 1) / splits + kDecodeWaves - 1) / kDecodeWaves * kDecodeWaves;
   d.splits = (width + d.chunk - 1) / d.chunk;
   d.turn = m > 1 && (m * d.splits <= 64 || (d.splits == 1 && m <= 256)) && d.chunk >= 8 ? std::max(1u, 256 / (kv_heads * d.tiles)) : 0;
@@ -349,18 +355,18 @@ __global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a, Decod
 }
 
 size_t attention_decode_partial_bytes(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width) {
-  const DecodeSplit d = decode_split(m, heads, kv_heads, width);
+  const DecodeSplit d = decode_split(m, heads, kv_heads, dim, width);
   return d.splits > 1 ? (size_t)m * heads * d.splits * (dim + 2) * sizeof(float) : 0;
 }
 
-uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width) {
-  const DecodeSplit d = decode_split(std::max(1u, m), heads, kv_heads, width);
+uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width) {
+  const DecodeSplit d = decode_split(std::max(1u, m), heads, kv_heads, dim, width);
   return std::max((uint64_t)m * kv_heads * d.tiles * d.splits, (uint64_t)m * heads);
 }
 
 template <int D>
 static void launch_decode(hipStream_t st, const DecodeArgs& a, float* partial) {
-  const DecodeSplit d = decode_split(a.m, a.heads, a.kv_heads, a.width);
+  const DecodeSplit d = decode_split(a.m, a.heads, a.kv_heads, a.dim, a.width);
   const dim3 grid(a.m * a.kv_heads * d.tiles * d.splits), block(256);
   hipLaunchKernelGGL(attention_decode_kernel<D>, grid, block, 0, st, a, d, partial);
   if (d.splits == 1) return;

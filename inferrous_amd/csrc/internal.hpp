@@ -357,7 +357,7 @@ struct DecodeArgs {
 };
 // Bytes of the parts that a batch of exactly m rows leaves for a second launch to join (0: none).
 size_t attention_decode_partial_bytes(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width);
-uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t width);
+uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width);
 hipError_t launch_attention_decode(hipStream_t st, const DecodeArgs& a, void* workspace);
 
 hipError_t launch_synth_i8(hipStream_t st, int8_t* out, size_t n, uint64_t seed, uint64_t stream_id);
