@@ -29,6 +29,17 @@ __device__ __forceinline__ float as_bf16(float a) { return bf16_lo(pack_bf16(a, 
 // 2^x, x a finite exponent below 128 or -inf (v_exp_f32; results below 2^-126 are 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Division of an x below 2^24 by a d below 2^16: with e = inverse * d - 2^40 < d, x * e is
+// below 2^40.  (near: of an x below 2^11 by a d up to 2^10, the same with 2^21.)  The
+// kernels' code is fetched anew by each launch, and a division is about 40 instructions.
+struct Divisor {
+  uint32_t d, near_inverse;
+  uint64_t inverse;
+  explicit Divisor(uint32_t by) : d(by), near_inverse(((1u << 21) + by - 1) / by), inverse(((1ull << 40) + by - 1) / by) {}
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)(x * inverse >> 40); }
+  __device__ __forceinline__ uint32_t near(uint32_t x) const { return x * near_inverse >> 21; }
+};
+
 // Rows [lo, hi) of sequence i of a batch of m rows.  Whatever `starts` holds,
 // the range stays within the batch.
 struct RowRange {

@@ -40,6 +40,14 @@ struct DecodeSplit {
   uint32_t splits;  // workgroups of the widest sequence
   uint32_t turn;    // units that a turn of the compute units takes, 0: in the order they have
 };
+// Divisors of the launch's numbers.
+struct DecodeBy {
+  Divisor kv_heads, tiles, splits, turn, heads;
+  uint32_t group;
+  DecodeBy(const DecodeArgs& a, const DecodeSplit& d)
+      : kv_heads(a.kv_heads), tiles(d.tiles), splits(d.splits), turn(std::max(1u, d.turn)), heads(a.heads),
+        group(a.heads / a.kv_heads) {}
+};
 
 constexpr uint32_t kMaxSplits = 64;
 // Splits that a join of so many waves a head takes.
@@ -117,12 +125,12 @@ struct PageCodes {
 
 // The unit (a row's split) that workgroup `place` of a key/value head takes: by their
 // pages, the most first in even turns of the compute units and the fewest first in odd ones.
-__device__ __forceinline__ uint32_t unit_of_turn(const DecodeArgs& a, const DecodeSplit& d, uint32_t place, uint32_t* keys) {
+__device__ __forceinline__ uint32_t unit_of_turn(const DecodeArgs& a, const DecodeSplit& d, const DecodeBy& by, uint32_t place, uint32_t* keys) {
   const uint32_t lane = threadIdx.x & 63, units = a.m * d.splits;
-  const uint32_t n = place / d.turn, at = place % d.turn;
+  const uint32_t n = by.turn.of(place), at = place - n * d.turn;
   const uint32_t rank = n * d.turn + (n % 2 ? min(d.turn, units - n * d.turn) - 1 - at : at);
   const auto key = [&](uint32_t u) {  // no two alike
-    const uint32_t row = u / d.splits, first = u % d.splits * d.chunk;
+    const uint32_t row = by.splits.of(u), first = (u - row * d.splits) * d.chunk;
     const uint32_t pages = u < units ? min(((uint32_t)max(a.lengths[row], 0) + kPageTokens - 1) / kPageTokens, a.width) : 0u;
     return (pages > first ? min(pages - first, d.chunk) : 0u) * 256 + (255 - u);
   };
@@ -149,21 +157,18 @@ __device__ __forceinline__ uint32_t unit_of_turn(const DecodeArgs& a, const Deco
 // partial: of sequences with more pages than a chunk, of each row, head and split its
 // unscaled sum o[D], then of each {m, l}.
 template <int D>
-__global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, DecodeSplit d, float* partial) {
+__global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, DecodeSplit d, DecodeBy by, float* partial) {
   constexpr int HALVES = D / 64, TILES = D / 16;
   __shared__ float sh_m[4][16], sh_l[4][16];
   __shared__ float sh_o[4][16][D + 4];
   __shared__ uint32_t keys[257];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t group = a.heads / a.kv_heads;
-  uint32_t b = blockIdx.x;
-  const uint32_t h = b % a.kv_heads;
-  b /= a.kv_heads;
-  const uint32_t tile = b % d.tiles;
-  b /= d.tiles;
-  if (d.turn) b = unit_of_turn(a, d, b, keys);
-  const uint32_t split = b % d.splits, row = b / d.splits;
+  const uint32_t group = by.group, among = by.kv_heads.of(blockIdx.x), h = blockIdx.x - among * a.kv_heads;
+  uint32_t b = by.tiles.of(among);
+  const uint32_t tile = among - b * d.tiles;
+  if (d.turn) b = unit_of_turn(a, d, by, b, keys);
+  const uint32_t row = by.splits.of(b), split = b - row * d.splits;
   const uint32_t head0 = h * group + tile * kDecodeHeads, live = min(kDecodeHeads, group - tile * kDecodeHeads);
 
   const int32_t* const table = a.table + (size_t)row * a.width;
@@ -302,7 +307,7 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
 // A row's head, of WAVES waves: the splits' parts joined, each by the D / 4 threads
 // of a group, and the groups' results by the first.
 template <int D, int WAVES>
-__global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a, DecodeSplit d, const float* partial) {
+__global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a, DecodeSplit d, DecodeBy by, const float* partial) {
   constexpr uint32_t LANES = D / 4, GROUPS = 64 * WAVES / LANES, EACH = join_splits(WAVES) / GROUPS, HEADS = 4 / WAVES;
   __shared__ float sh_m[HEADS][GROUPS], sh_l[HEADS][GROUPS];
   __shared__ v4f sh_o[HEADS][GROUPS][LANES];
@@ -310,7 +315,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a, Decod
   const uint64_t at = (uint64_t)blockIdx.x * HEADS + mine;
   const bool real = at < (uint64_t)a.m * a.heads;
   const float* const ml = partial + (size_t)a.m * a.heads * d.splits * D;
-  const uint32_t len = real ? min((uint32_t)max(a.lengths[at / a.heads], 0), a.width * kPageTokens) : 0u;
+  const uint32_t len = real ? min((uint32_t)max(a.lengths[by.heads.of((uint32_t)at)], 0), a.width * kPageTokens) : 0u;
   uint32_t splits = ((len + kPageTokens - 1) / kPageTokens + d.chunk - 1) / d.chunk;
   if (splits == 1) splits = 0;  // the output is there
   float2 part[EACH];
@@ -367,13 +372,16 @@ uint64_t attention_decode_blocks(uint32_t m, uint32_t heads, uint32_t kv_heads, 
 template <int D>
 static void launch_decode(hipStream_t st, const DecodeArgs& a, float* partial) {
   const DecodeSplit d = decode_split(a.m, a.heads, a.kv_heads, a.dim, a.width);
+  const DecodeBy by(a, d);
   const dim3 grid(a.m * a.kv_heads * d.tiles * d.splits), block(256);
-  hipLaunchKernelGGL(attention_decode_kernel<D>, grid, block, 0, st, a, d, partial);
+  hipLaunchKernelGGL(attention_decode_kernel<D>, grid, block, 0, st, a, d, by, partial);
   if (d.splits == 1) return;
   if (d.splits <= join_splits(1))
-    hipLaunchKernelGGL((attention_join_kernel<D, 1>), dim3((a.m * a.heads + 3) / 4), block, 0, st, a, d, (const float*)partial);
+    hipLaunchKernelGGL((attention_join_kernel<D, 1>), dim3((a.m * a.heads + 3) / 4), block, 0, st, a, d, by,
+                       (const float*)partial);
   else
-    hipLaunchKernelGGL((attention_join_kernel<D, 4>), dim3(a.m * a.heads), block, 0, st, a, d, (const float*)partial);
+    hipLaunchKernelGGL((attention_join_kernel<D, 4>), dim3(a.m * a.heads), block, 0, st, a, d, by,
+                       (const float*)partial);
 }
 
 hipError_t launch_attention_decode(hipStream_t st, const DecodeArgs& a, void* workspace) {

@@ -92,7 +92,7 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t at, uint3
 }
 
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(PrefillArgs a) {
+__global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(PrefillArgs a, Divisor kv, Divisor members) {
   constexpr int ROWS = 32 * NW, CH = D / 8, STEPS = D / 16, COLS = D / 32;
   constexpr int TILE = kTileKeys * D * 2;  // bytes of a tile of keys, or of values
   constexpr int LOADS = TILE / 1024 / NW;  // of a wave for one of them
@@ -100,23 +100,25 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(Pref
   __shared__ __align__(1024) uint8_t lds[6 * TILE];  // three tiles of keys, then of values
   const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+  const uint32_t unit = kv.of(blockIdx.x), head = blockIdx.x - unit * kv.d, group = members.d;
   uint32_t seq, tile;
   const auto count = [&](uint32_t s) {
     const RowRange r = rows_of(a.starts, s, a.m);
     return (uint32_t)(((uint64_t)(r.hi - r.lo) * group + ROWS - 1) / ROWS);
   };
-  if (!find_unit(blockIdx.x / a.kv_heads, a.seqs, count, &seq, &tile)) return;
+  if (!find_unit(unit, a.seqs, count, &seq, &tile)) return;
   tile = count(seq) - 1 - tile;  // the longest first
   const RowRange r = rows_of(a.starts, seq, a.m);
   const uint32_t len = r.hi - r.lo;
 
   // the lane's row: a query and a head
   const uint64_t rows = (uint64_t)len * group, first = (uint64_t)tile * ROWS;
-  const uint32_t first_query = (uint32_t)(first / group), first_member = (uint32_t)(first % group);
-  const auto query_of = [&](uint32_t row) { return min(first_query + (first_member + row) / group, len - 1); };
+  const uint32_t turns = members.of(tile), left = (tile - turns * group) * ROWS;  // of whole tiles of queries; below 2^18
+  const uint32_t first_query = turns * ROWS + members.of(left), first_member = left - members.of(left) * group;
+  const auto queries_on = [&](uint32_t row) { return members.near(first_member + row); };
+  const auto query_of = [&](uint32_t row) { return min(first_query + queries_on(row), len - 1); };
   const bool mine = first + 32 * wave + col < rows;
-  const uint32_t query = query_of(32 * wave + col), member = (first_member + 32 * wave + col) % group;
+  const uint32_t query = query_of(32 * wave + col), member = first_member + 32 * wave + col - queries_on(32 * wave + col) * group;
   const uint32_t last_query = query_of(ROWS - 1), wave_first = query_of(32 * wave), wave_last = query_of(32 * wave + 31);
   const uint32_t tiles = last_query / kTileKeys + 1;    // of the workgroup
   const uint32_t own = wave_last / kTileKeys + 1;       // with a key that a row of the wave sees
@@ -403,7 +405,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(Pref
           for (int i = 0; i < 16; ++i)
             if (32 * b + 8 * (i / 4) + i % 4 > seen) s[b][i] = -__builtin_inff();
       }
-      const float to = raised(both(larger(top_of(s[0]), top_of(s[1])))), f = factor(to);
+      const float to = raised(both(larger(top_of(s[0]), top_of(s[1])))), f = t ? factor(to) : 1.f;
       m = to;
       l = __builtin_fmaf(l, f, soften(s[0], p) + soften(s[1], p + 2));
 #pragma unroll
@@ -432,10 +434,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_prefill_kernel(Pref
 #pragma unroll
     for (int j = 0; j < 32 / (64 / CH); ++j) {
       const uint32_t row = j * (64 / CH) + lane / CH;
-      const uint32_t to = first_member + 32 * wave + row;
+      const uint32_t on = queries_on(32 * wave + row), of = first_member + 32 * wave + row - on * group;
       const v4u x = read_row(part + row * (2 * D) + ((lane % CH) ^ key_swizzle(row)) * 16);
       if (first + 32 * wave + row < rows)
-        *(v4u*)((uint16_t*)a.out + ((size_t)(r.lo + first_query + to / group) * a.heads + head * group + to % group) * D +
+        *(v4u*)((uint16_t*)a.out + ((size_t)(r.lo + first_query + on) * a.heads + head * group + of) * D +
                 lane % CH * 8) = x;
     }
     return;
@@ -469,7 +471,8 @@ uint64_t attention_prefill_blocks(const PrefillArgs& a) { return prefill_blocks(
 
 template <int D, int NW>
 static void start_prefill(hipStream_t st, const PrefillArgs& a) {
-  hipLaunchKernelGGL((attention_prefill_kernel<D, NW>), dim3((uint32_t)prefill_blocks(a, NW)), dim3(64 * NW), 0, st, a);
+  hipLaunchKernelGGL((attention_prefill_kernel<D, NW>), dim3((uint32_t)prefill_blocks(a, NW)), dim3(64 * NW), 0, st, a, Divisor(a.kv_heads),
+                     Divisor(a.heads / a.kv_heads));
 }
 
 hipError_t launch_attention_prefill(hipStream_t st, const PrefillArgs& a) {

@@ -144,11 +144,11 @@ constexpr uint32_t kPrepareHeads = 4;  // query heads that a group of lanes take
 // tokens and of kPrepareHeads heads are one workgroup's, too; if every sequence
 // brings one row (ONE), GROUPS heads of it are.  D / 8 lanes hold a head.
 template <int D, bool BF16IN, bool ONE>
-__global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t blocks) {
+__global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, Divisor parts, Divisor sets) {
   constexpr int LPH = D / 8, GROUPS = 256 / LPH, SLOTS = 64 / GROUPS;  // lanes of a head, heads in flight, tokens of a group
   __shared__ uint32_t red[4];
   __shared__ __align__(16) uint32_t turned[ONE ? 1 : D * kPageTokens / 4];  // the page's value codes
-  const uint32_t unit = blockIdx.x / blocks, part = blockIdx.x % blocks;
+  const uint32_t unit = parts.of(blockIdx.x), part = blockIdx.x - unit * parts.d;
   const int tid = threadIdx.x, i = tid % LPH, group = tid / LPH;
   uint32_t seq = unit, index = 0, lo = unit, n = 1;
   if constexpr (!ONE) {
@@ -170,8 +170,8 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
 
   if (part >= 2 * a.kv_heads) {
     constexpr uint32_t TIMES = ONE ? 1 : kPrepareHeads, HEADS = ONE ? GROUPS : kPrepareHeads;
-    const uint32_t sets = (a.heads + HEADS - 1) / HEADS, set = (part - 2 * a.kv_heads) % sets;
-    const uint32_t t = ONE ? 0u : (part - 2 * a.kv_heads) / sets * GROUPS + group, h0 = set * HEADS + (ONE ? group : 0u);
+    const uint32_t part_q = part - 2 * a.kv_heads, tokens = sets.of(part_q), set = part_q - tokens * sets.d;
+    const uint32_t t = ONE ? 0u : tokens * GROUPS + group, h0 = set * HEADS + (ONE ? group : 0u);
     if (t >= n1 - n0 || h0 >= a.heads) return;
     const size_t row = row0 + t;
     Read<D, BF16IN> in[TIMES];
@@ -322,11 +322,14 @@ __global__ __launch_bounds__(256) void prepare_qk_kernel(PrepareArgs a, uint32_t
   }
 }
 
-// Workgroups of a unit: those of the key/value heads and of the queries.
+// Workgroups of a unit: those of the key/value heads, and sets of query heads (of whole
+// rows, or of the tokens of one after another).
+static uint32_t prepare_sets(const PrepareArgs& a) {
+  const uint32_t heads = a.starts ? kPrepareHeads : 256 / (a.dim / 8);
+  return (a.heads + heads - 1) / heads;
+}
 static uint32_t prepare_parts(const PrepareArgs& a) {
-  const uint32_t groups = 256 / (a.dim / 8);
-  if (!a.starts) return 2 * a.kv_heads + (a.heads + groups - 1) / groups;
-  return 2 * a.kv_heads + (a.heads + kPrepareHeads - 1) / kPrepareHeads * (kPageTokens / groups);
+  return 2 * a.kv_heads + prepare_sets(a) * (a.starts ? kPageTokens * (a.dim / 8) / 256 : 1);
 }
 
 // Every unit has a row, and a sequence's pages hold 64 of its rows but for two.
@@ -338,10 +341,11 @@ uint64_t prepare_qk_blocks(const PrepareArgs& a) {
 template <int D, bool BF16IN>
 static void start_prepare_qk(hipStream_t st, const PrepareArgs& a) {
   const dim3 grid((uint32_t)prepare_qk_blocks(a));
+  const Divisor parts(prepare_parts(a)), sets(prepare_sets(a));
   if (a.starts)
-    hipLaunchKernelGGL((prepare_qk_kernel<D, BF16IN, false>), grid, dim3(256), 0, st, a, prepare_parts(a));
+    hipLaunchKernelGGL((prepare_qk_kernel<D, BF16IN, false>), grid, dim3(256), 0, st, a, parts, sets);
   else
-    hipLaunchKernelGGL((prepare_qk_kernel<D, BF16IN, true>), grid, dim3(256), 0, st, a, prepare_parts(a));
+    hipLaunchKernelGGL((prepare_qk_kernel<D, BF16IN, true>), grid, dim3(256), 0, st, a, parts, sets);
 }
 
 hipError_t launch_prepare_qk(hipStream_t st, const PrepareArgs& a) {
