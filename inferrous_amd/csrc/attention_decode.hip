@@ -22,9 +22,9 @@
 // rescaled a few times, not once a page.  A probability is rounded to BF16, and the
 // sum that divides is that of the rounded ones.
 //
-// 64 sequences of up to 4096 tokens, 32/8 heads of 128: 261 MB in 49.5 us (5.3 TB/s; a
-// plain read of the same pages, a page a wave, 45 us).  One of 4001 tokens: 5.1 us and
-// 3.2 for the join, both mostly latency.
+// 64 sequences of up to 4096 tokens, 32/8 heads of 128: 261 MB in 49.1 us (5.3 TB/s; a
+// plain read of the same pages, a page a wave, 45 us).  One of 4001 tokens: 5.0 us and
+// 3.6 for the join, both mostly latency.
 #include <algorithm>
 
 #include "attention.hpp"

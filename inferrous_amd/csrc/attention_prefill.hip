@@ -32,8 +32,8 @@
 // every 32 keys.  A probability is rounded to BF16, and the sum that divides is that of
 // the rounded ones.
 //
-// 32/8 heads of 128: one prompt of 4096 tokens 137 us (1000 TFLOP/s), one of 16384
-// 1960 us (1122 TFLOP/s, where a library product of 8192^3 reaches 1371).  The matrix
+// 32/8 heads of 128: one prompt of 4096 tokens 136 us (1010 TFLOP/s), one of 16384
+// 1942 us (1134 TFLOP/s, where a library product of 8192^3 reaches 1371).  The matrix
 // cores are busy in 58% of the cycles, and the clock is down to 1.95 of 2.4 GHz: each
 // part of the loop that is left out (exponentials, reads of LDS, loads) gives its power
 // back as clock, 5 to 12%, so that none of them is what the others wait for.  Waves that
@@ -463,8 +463,9 @@ static uint64_t prefill_blocks(const PrefillArgs& a, int waves) {
 
 // Half the rows a workgroup where the compute units have no second workgroup of whole
 // ones to take: one wave a SIMD then ends sooner than two.  One sequence of 32/8 heads
-// of 128, 128 rows / 256 rows a workgroup, us: 200 tokens 11.3 / 12.5, 512 16.1 / 18.9,
-// 1024 25.9 / 31.0, 1400 33.7 / 40.1, 2048 54.1 / 57.3, 2300 72.4 / 65.4, 4096 176 / 139.
+// of 128, 128 rows / 256 rows a workgroup, us: 37 tokens 7.0 / 7.5, 200 10.5 / 12.1, 512
+// 15.3 / 18.4, 1024 25.4 / 30.6, 1400 32.8 / 39.9, 2048 52.9 / 56.3, 2300 69.3 / 64.8,
+// 4096 170 / 137.
 static int prefill_waves(const PrefillArgs& a) { return prefill_blocks(a, 8) <= 256 ? 4 : 8; }
 
 uint64_t attention_prefill_blocks(const PrefillArgs& a) { return prefill_blocks(a, prefill_waves(a)); }
