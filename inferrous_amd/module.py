@@ -970,14 +970,17 @@ class LoadedModule:
         ``reserve_workspace(attention_decode_workspace_bytes(...))`` before
         capturing a graph."""
         heads, dim, kv_heads = int(heads), cache.head_dim, cache.kv_heads
-        width, dtype = heads * dim, out.dtype
-        if width <= 0 or len(out) % width:
+        width, out_len, dtype = heads * dim, len(out), out.dtype
+        if width <= 0 or out_len % width:
             raise ValueError("attention_decode: out must hold M rows of heads * head_dim")
-        m = len(out) // width
-        if dtype != _F32 and dtype != _U16:
+        m = out_len // width
+        if dtype == _U16:
+            code = _lib.OUT_BF16
+        elif dtype == _F32:
+            code = _lib.OUT_F32
+        else:
             raise TypeError(f"out dtype {dtype} not supported (float32/uint16)")
-        _needs(q, _U16, m * width, "q")
-        _needs(lengths, _I32, m, "lengths")
+        qp, lp = _where(q, _U16, m * width, "q"), _where(lengths, _I32, m, "lengths")
         columns = _table_width(table, m)
         codes, scales = cache.layer(layer)
         if m == 0:
@@ -986,9 +989,9 @@ class LoadedModule:
             raise ValueError("the query heads must be a multiple of the cache's heads")
         wp, wb = self._routed_workspace(stream, "w8a8_attention_decode_workspace_bytes", m, heads, kv_heads, dim,
                                         columns, none_if_zero=True)
-        check(lib().w8a8_attention_decode(_h(stream), q.ptr, m, heads, kv_heads, dim, codes, scales, cache.pages,
-                                          lengths.ptr, table.ptr, columns, dim ** -0.5 if scale is None else scale,
-                                          out.ptr, _OUT[dtype], wp, wb), "attention_decode")
+        check(lib().w8a8_attention_decode(_h(stream), qp, m, heads, kv_heads, dim, codes, scales, cache.pages, lp,
+                                          table.ptr, columns, dim ** -0.5 if scale is None else scale, out.ptr, code,
+                                          wp, wb), "attention_decode")
 
     def copy_pages(self, stream, cache: KvCache, src: DeviceBuffer, dst: DeviceBuffer) -> None:
         """Pages ``src`` to ``dst`` (int32, one length) of every layer of a
