@@ -84,16 +84,26 @@ def _where(buf: DeviceBuffer | None, dtype: np.dtype, need: int, what: str):
     return buf.ptr
 
 
-def _table_width(table: DeviceBuffer | None, seqs: int) -> int:
-    """Pages of a row of a page table of seqs rows."""
+def _table_width(table: DeviceBuffer | None, seqs: int, width: int | None, beside: DeviceBuffer | None) -> int:
+    """Pages of a row of a page table: ``width``, or what a table of exactly seqs
+    rows has.  beside: a buffer of a number for each sequence; one for more of them
+    speaks for a table of as many rows."""
     if table is None:
         raise ValueError("a page table is required")
+    if width is not None:
+        if width < 1:
+            raise ValueError("table_width must be positive")
+        _needs(table, _I32, seqs * width, "table")
+        return width
     _needs(table, _I32, seqs, "table")
     if not seqs:
         return 0
     width, rest = divmod(len(table), seqs)
     if rest:
-        raise ValueError("the table must hold one row of pages a sequence")
+        raise ValueError("the table must hold one row of pages a sequence, or table_width must say how many a row has")
+    if beside is not None and len(beside) > seqs and len(table) % len(beside) == 0:
+        raise ValueError(f"the table may be for {seqs} sequences or for {len(beside)}: table_width must say "
+                         "how many pages a row has")
     return width
 
 
@@ -857,7 +867,7 @@ class LoadedModule:
                    starts: DeviceBuffer | None = None, past: DeviceBuffer | None = None,
                    k_out: DeviceBuffer | None = None, v_out: DeviceBuffer | None = None,
                    cache: KvCache | None = None, table: DeviceBuffer | None = None, layer: int = 0,
-                   eps: float = 1e-6) -> None:
+                   eps: float = 1e-6, table_width: int | None = None) -> None:
         """Query and key heads normalised and rotated, keys and values into the
         cache (w8a8_prepare_qk; `prepare_qk` with the caches of
         src/kernels.rs:1290-1488).  ``q`` is a qkv projection's rows [M, (heads
@@ -868,7 +878,9 @@ class LoadedModule:
         norm.  ``starts`` (int32 [S + 1]): the sequences' rows, None for one
         row each; ``past`` (int32 [S]): their tokens so far, None for none.
         ``k_out`` / ``v_out`` (uint16 [M, kv_heads, head_dim]) and ``cache``
-        with ``table`` (int32 [S, width]) are optional."""
+        with ``table`` (int32 [S, width]) are optional.  ``table_width`` is the
+        width, for a table that has more rows than S; without it the table
+        is taken to be exactly S rows."""
         heads, kv_heads, dim = int(heads), int(kv_heads), int(head_dim)
         width, kv_width, out_len = heads * dim, kv_heads * dim, len(q_out)
         if width <= 0 or kv_width <= 0 or out_len % width:
@@ -906,7 +918,7 @@ class LoadedModule:
         if cache is not None:
             if cache.kv_heads != kv_heads or cache.head_dim != dim:
                 raise ValueError("the cache has other heads")
-            columns = _table_width(table, seqs)
+            columns = _table_width(table, seqs, table_width, past)
             (codes, scales), pages, table_ptr = cache.layer(layer), cache.pages, table.ptr
         elif table is not None:
             raise ValueError("a table names the pages of a cache")
@@ -960,12 +972,15 @@ class LoadedModule:
         return lib().w8a8_attention_decode_workspace_bytes(max_rows, heads, kv_heads, head_dim, table_width)
 
     def attention_decode(self, stream, q: DeviceBuffer, cache: KvCache, lengths: DeviceBuffer, table: DeviceBuffer,
-                         heads: int, out: DeviceBuffer, layer: int = 0, scale: float | None = None) -> None:
+                         heads: int, out: DeviceBuffer, layer: int = 0, scale: float | None = None,
+                         table_width: int | None = None) -> None:
         """One query row of each sequence over the cache (w8a8_attention_decode;
         `attention` of src/kernels.rs:1489-2161): ``q`` (uint16 BF16 [M,
         heads, head_dim]) over the first ``lengths`` (int32 [M]) tokens of the
         pages that ``table`` (int32 [M, width]) names, into ``out`` (float32 or
-        uint16, as q).  ``scale``: head_dim ** -0.5 by default.  The scratch
+        uint16, as q).  ``scale``: head_dim ** -0.5 by default.
+        ``table_width`` is the table's width, for one that has more rows than
+        M; without it the table is taken to be exactly M rows.  The scratch
         space is the stream's workspace;
         ``reserve_workspace(attention_decode_workspace_bytes(...))`` before
         capturing a graph."""
@@ -981,7 +996,7 @@ class LoadedModule:
         else:
             raise TypeError(f"out dtype {dtype} not supported (float32/uint16)")
         qp, lp = _where(q, _U16, m * width, "q"), _where(lengths, _I32, m, "lengths")
-        columns = _table_width(table, m)
+        columns = _table_width(table, m, table_width, lengths)
         codes, scales = cache.layer(layer)
         if m == 0:
             return
