@@ -635,7 +635,8 @@ int w8a8_prepare_qk(void *stream, const void *q, size_t q_stride, const void *k,
  * straight from a projection); starts NULL: one sequence of m rows.  Products and
  * sums are held in f32, probabilities in BF16.  out: [m, heads, head_dim], F32
  * (holding BF16 values) or BF16.  scale: positive, at most 2e38.  What a row does
- * not see never reaches it, whatever it holds. */
+ * not see never reaches it, whatever it holds.  Scores are f32: one that overflows to
+ * -inf weighs nothing, a row of nothing else, or with one of +inf, is NaN. */
 int w8a8_attention_prefill(void *stream, const uint16_t *q, size_t q_stride,
                            const uint16_t *k, size_t k_stride,
                            const uint16_t *v, size_t v_stride, size_t m,
@@ -646,8 +647,9 @@ int w8a8_attention_prefill(void *stream, const uint16_t *q, size_t q_stride,
 
 /* One query row of each of m sequences over the cache: q[m, heads, head_dim]
  * (BF16), row i over the first lengths[i] tokens of its sequence (cut to what
- * table[i] can name; 0 or less: out is 0).  Rows of one sequence (draft tokens)
- * may repeat its pages with lengths of their own.  out, scale: as above.  The
+ * table[i] can name).  A row that sees no token (a length of 0 or less, or no page of
+ * its own) is 0.  Rows of one sequence (draft tokens) may repeat its pages with
+ * lengths of their own.  out, scale: as above.  The
  * workspace (256-byte aligned) is written before it is read; calls sharing one must
  * not overlap.  w8a8_attention_decode_workspace_bytes does not fall with m: a
  * buffer for the largest batch serves every smaller one (with the same

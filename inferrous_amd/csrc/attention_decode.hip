@@ -116,6 +116,10 @@ __device__ __forceinline__ float groups_sum(float v) {
   return across_groups(v, [](float a, float b) { return a + b; });
 }
 
+// What divides a row's sum o by l: a row that saw no token (its maximum is -inf, below any
+// that a score leaves) is 0, one whose scores are all -inf is 0 / 0 as its softmax is.
+__device__ __forceinline__ float weight(float m, float l) { return m == -__builtin_inff() ? 0.f : 1.f / l; }
+
 // A page's codes as the two products take them.
 template <int D>
 struct PageCodes {
@@ -263,6 +267,7 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
       o[t] = mfma16(widen(x.v[t].z, x.v[t].w, vs), w[1], o[t]);
     }
   };
+  bool seen = false;  // a page with a token that counts
   for (uint32_t n = 0; p < end; p += kDecodeWaves, ++n) {
     if (n == 64) ids = ids_from(p), n = 0;
     const int32_t id = __builtin_amdgcn_readlane(ids, (int)n);
@@ -270,7 +275,9 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
     PageCodes<D> x;
     load(x, id);
     attend(x, p);
+    seen = true;
   }
+  if (!seen) m = -__builtin_inff();
   l = groups_sum(l);
   if (g == 0) sh_m[wave][c] = m, sh_l[wave][c] = l;
 #pragma unroll
@@ -299,7 +306,7 @@ __global__ __launch_bounds__(256, 3) void attention_decode_kernel(DecodeArgs a, 
     for (int j = 0; j < D / 64; ++j) *(v4f*)(partial + (at * d.splits + split) * D + 64 * j + 4 * part) = oo[j];
     return;
   }
-  const float r = ll == 0.f ? 0.f : 1.f / ll;
+  const float r = weight(mm, ll);
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) store4(a, at * D + 64 * j + 4 * part, oo[j] * r);
 }
@@ -356,7 +363,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a, Decod
     l += sh_l[mine][e] * f;
     o += sh_o[mine][e][i] * f;
   }
-  store4(a, at * D + 4 * i, o * (l == 0.f ? 0.f : 1.f / l));
+  store4(a, at * D + 4 * i, o * weight(m, l));
 }
 
 size_t attention_decode_partial_bytes(uint32_t m, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t width) {
