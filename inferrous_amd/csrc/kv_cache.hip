@@ -120,11 +120,23 @@ struct Gains {
 template <int D>
 __device__ __forceinline__ void norm_rotate(Share& x, bool norm, const Gains<D>& g, float eps, const Angles<D>& r) {
   if (norm) {
-    float ss = 0.f;
+    const auto mean = [&](float e) {
+      float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x.lo[j], x.lo[j], __builtin_fmaf(x.hi[j], x.hi[j], ss));
-    // v_rsq_f32: one unit of the last place
-    const float inv = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<D>(ss), 1.0f / D, eps));
+      for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x.lo[j], x.lo[j], __builtin_fmaf(x.hi[j], x.hi[j], ss));
+      return __builtin_fmaf(head_sum<D>(ss), 1.0f / D, e);
+    };
+    float v = mean(eps);
+    // squares that lose bits below f32's normal numbers (v_rsq_f32 takes those for zeros) or
+    // overflow: n is that of x times a power of two
+    constexpr uint32_t LEAST = 0x0d800000u;  // 2^-100
+    if (__ballot(__float_as_uint(v) - LEAST >= kInfBits - LEAST)) {
+      const float by = v < __uint_as_float(LEAST) ? 0x1p100f : v == __builtin_inff() ? 0x1p-70f : 1.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.lo[j] *= by, x.hi[j] *= by;
+      v = mean(eps * by * by);
+    }
+    const float inv = __builtin_amdgcn_rsqf(v);  // one unit of the last place
 #pragma unroll
     for (int j = 0; j < 4; ++j) x.lo[j] = x.lo[j] * inv * g.a[j], x.hi[j] = x.hi[j] * inv * g.b[j];
   }

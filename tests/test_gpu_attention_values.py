@@ -1,4 +1,5 @@
-"""Attention at the ends of f32: scores that overflow, and rows that see nothing.
+"""Attention at the ends of f32: scores that overflow, rows that see nothing, and
+heads whose squares leave f32.
 (Inputs, 64-bit forms and tolerances: test_gpu_attention.py.)"""
 from __future__ import annotations
 
@@ -6,7 +7,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, load
-from test_gpu_attention import PAGE, Decode, Prefill, bf16, close
+from test_gpu_attention import F32, PAGE, Decode, Prefill, bf16, bf16_bits, close, dev, from_bits, rope_table
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +96,46 @@ def test_a_score_that_overflows_upwards(env, n):
     assert np.isnan(got[at:p.rows[0], 1]).all()
     got[at:p.rows[0], 1] = 0
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [np.uint16, np.float32])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("power, eps", [(0, 0.0), (-55, 0.0), (-64, 0.0), (-70, 0.0), (-100, 0.0), (-125, 0.0), (40, 0.0),
+                                        (66, 0.0), (100, 0.0), (120, 1e-6), (-70, 2.0 ** -140), (-60, 2.0 ** -118),
+                                        (-60, 1e-6), (-125, 1e-38), (0, 1e30), (30, 1e18), (0, 3e38), (100, 3e38)])
+def test_heads_of_any_size_are_normalised(env, dim, dtype, packed, power, eps):
+    """The squares' mean of finite heads may lie anywhere, below f32's normal numbers and above its largest."""
+    mod, s, _ = env
+    rng = np.random.default_rng(dim)
+    heads, kv, m = 6, 2, 5
+    x = np.ldexp(bf16(rng.standard_normal((m, heads + 2 * kv, dim))), power).astype(F32)
+    x[1] = 0
+    x[1, :, 3] = np.ldexp(F32(1.5), power)
+    if dtype == np.uint16:
+        x = bf16(x)   # subnormal ones have fewer bits
+    gain, rope = [(1 + 0.3 * rng.standard_normal(dim)).astype(F32) for _ in range(2)], rope_table(m, dim)
+    q, k = (dev(s, np.zeros(m * n * dim, np.uint16)) for n in (heads, kv))
+    kw = dict(starts=dev(s, np.array([0, m], np.int32))) if packed else dict(past=dev(s, np.arange(m, dtype=np.int32)))
+    mod.prepare_qk(s, dev(s, bf16_bits(x) if dtype == np.uint16 else x), heads, kv, dim, dev(s, rope), q,
+                   q_gain=dev(s, gain[0]), k_gain=dev(s, gain[1]), k_out=k, eps=eps, **kw)
+    for out, part, g in ((q, x[:, :heads], gain[0]), (k, x[:, heads:heads + kv], gain[1])):
+        n = part.astype(np.float64)
+        n = n / np.sqrt((n ** 2).mean(2, keepdims=True) + float(F32(eps))) * g.astype(np.float64)
+        c, t, a, b = (z.astype(np.float64) for z in (rope[:, None, :dim // 2], rope[:, None, dim // 2:],
+                                                     n[..., :dim // 2], n[..., dim // 2:]))
+        want = np.concatenate([a * c - b * t, b * c + a * t], 2)
+        size = np.concatenate([abs(a * c) + abs(b * t), abs(b * c) + abs(a * t)], 2)
+        # below 2^-126 bf16's steps no longer shrink
+        close(from_bits(out.to_host_vec(s)).reshape(want.shape), want, 2.0 ** -19 * size + 2.0 ** -134)
+
+
+def test_a_head_of_zeros_without_eps(env):
+    """0 / 0, as the formula has it; with any eps it is 0."""
+    mod, s, _ = env
+    x, rope, gain = dev(s, np.zeros(2 * 3 * 64, F32)), dev(s, rope_table(2, 64)), dev(s, np.ones(64, F32))
+    out = dev(s, np.ones(2 * 64, np.uint16))
+    for eps in (0.0, 1e-45, 1e-6):
+        mod.prepare_qk(s, x, 1, 1, 64, rope, out, q_gain=gain, eps=eps)
+        got = from_bits(out.to_host_vec(s))
+        assert np.isnan(got).all() if eps == 0 else np.all(got == 0)
