@@ -602,10 +602,11 @@ int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
  *   n = x / sqrt(mean(x^2) + eps) * gain     (gain NULL: n = x)
  *   (a cos - b sin, b cos + a sin)           (a, b: n's halves; cos and sin:
  *                                             the halves of rope[position])
- * in f32 (also where the squares leave it), rounded once, to q_out[m, heads, head_dim] and, where not NULL,
- * k_out[m, kv_heads, head_dim]; v_out (or NULL) is v as BF16.  q, k and v (F32 or
- * BF16, dtype) are rows of heads * head_dim values with q_stride, k_stride and
- * v_stride values from row to row: a qkv projection's output, or three.
+ * in f32 (heads whose squares leave it, too), rounded once, to q_out[m, heads,
+ * head_dim] and, where not NULL, k_out[m, kv_heads, head_dim]; v_out (or NULL) is v
+ * as BF16.  q, k and v (F32 or BF16, dtype) are rows of heads * head_dim values with
+ * q_stride, k_stride and v_stride values from row to row: a qkv projection's output,
+ * or three.
  * Position: past[i] (NULL: 0) plus the row's place in sequence i.  starts NULL:
  * one row a sequence, n_seq == m.  A position not below rope_rows gives NaN.
  * With codes (then scales and table too) the f32 keys and the values are also
