@@ -85,10 +85,10 @@ __device__ __forceinline__ void meet() {
 }
 // 16 bytes a lane from `base` + `at` to LDS, at `to` + 16 * lane (base and to are the
 // same in every lane).  In assembly: the compiler would make every later read of
-// LDS wait for it.  (m0 is the compiler's only within one of its own instructions'
-// expansions; this kernel has none that use it.)
+// LDS wait for it.  (m0 takes the LDS address; the warning is that it is reserved.)
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t at, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(to) : "memory", "m0");
 }
 
 template <int D, int NW>
