@@ -258,6 +258,7 @@ __device__ __forceinline__ void issue_row_values(float* dst, const float* src) {
   const uint32_t lds = (uint32_t)(uintptr_t)(void __attribute__((address_space(3)))*)dst;
   asm volatile(
       "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"  // a load to LDS reads m0 a wait state after its write
       "global_load_lds_dword %0, off"
       :
       : "v"(src), "s"(lds)

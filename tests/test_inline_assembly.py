@@ -48,3 +48,11 @@ def test_a_register_by_name_is_declared(file, line, code, clobbers):
     for c in code:
         written = NAMED.match(c.split(None, 1)[1].split(",")[0].strip()) if " " in c else None
         assert not written or written[1] in clobbers, f"{file}:{line}: {c} writes {written[1]}"
+
+
+@pytest.mark.parametrize("file, line, code, clobbers", ALL)
+def test_m0_is_written_a_wait_state_before_a_load_to_lds(file, line, code, clobbers):
+    """A load to LDS may follow a write of m0, its LDS address, after one other instruction."""
+    for before, after in zip(code, code[1:]):
+        if re.match(r"s_\w+\s+m0\b", before):
+            assert not re.search(r"_lds_", after), f"{file}:{line}: {before}; {after}"
