@@ -650,10 +650,10 @@ int w8a8_attention_prefill(void *stream, const uint16_t *q, size_t q_stride,
  * (BF16), row i over the first lengths[i] tokens of its sequence (cut to what
  * table[i] can name).  A row that sees no token (a length of 0 or less, or no page of
  * its own) is 0.  Rows of one sequence (draft tokens) may repeat its pages with
- * lengths of their own.  out, scale: as above.  The
- * workspace (256-byte aligned) is written before it is read; calls sharing one must
- * not overlap.  w8a8_attention_decode_workspace_bytes does not fall with m: a
- * buffer for the largest batch serves every smaller one (with the same
+ * lengths of their own.  out, scale: as above; probabilities are held in 16 bits
+ * or more.  The workspace (256-byte aligned) is written before it is read; calls
+ * sharing one must not overlap.  w8a8_attention_decode_workspace_bytes does not fall
+ * with m: a buffer for the largest batch serves every smaller one (with the same
  * table_width). */
 size_t w8a8_attention_decode_workspace_bytes(size_t m, uint32_t heads,
                                              uint32_t kv_heads,

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from inferrous_amd import CudaContext, load
-from test_gpu_attention import F32, PAGE, Decode, Prefill, bf16, bf16_bits, close, dev, from_bits, rope_table
+from test_gpu_attention import F32, PAGE, Decode, Prefill, bf16, bf16_bits, close, dev, e4m3, from_bits, rope_table
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +139,24 @@ def test_a_head_of_zeros_without_eps(env):
         mod.prepare_qk(s, x, 1, 1, 64, rope, out, q_gain=gain, eps=eps)
         got = from_bits(out.to_host_vec(s))
         assert np.isnan(got).all() if eps == 0 else np.all(got == 0)
+
+
+@pytest.mark.parametrize("heads, kv, dim", [(7, 1, 128), (14, 2, 64)])
+@pytest.mark.parametrize("lengths", [[64], [500], [130, 500, 63], [4000, 2500]])
+def test_decode_weights_have_more_bits_than_bf16(env, heads, kv, dim, lengths):
+    """Two kinds of tokens whose values almost cancel: what is left shows the weights'
+    roundings, which all tokens of a kind share.
+
+    A weight in two BF16 parts is off by 2^-16, its exponent (below 2^3 here) by 2^-21 and
+    v_exp_f32 by 2^-23; a sum has at most 512 terms in a chain (a wave's tokens, then the
+    waves' and the splits' parts), so 2^-15. Numerator and denominator: 2^-13 of sum p |v|."""
+    c = Decode(len(lengths) + sum(lengths), lengths, heads, kv, dim)
+    c.cache.s[:] = 1
+    c.q[:] = 0
+    c.q[:, :, 0] = bf16(np.linspace(0.1, 2.2, heads))
+    c.cache.k[:], c.cache.v[:] = 0, e4m3(-np.arange(dim) / dim)   # by column
+    c.cache.k[:, :, ::2, 0], c.cache.v[:, :, ::2] = e4m3(-1.0), e4m3(1.0)
+    want, err = c.want(scale=1.0)
+    size = err / (2.0 ** -7 + 2.0 ** -9)
+    assert np.all((np.abs(want) / size).min(2) < 2.0 ** -5)   # some column nearly cancels
+    close(c.run(env, scale=1.0), want, 2.0 ** -13 * size)
