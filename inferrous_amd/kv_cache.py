@@ -63,7 +63,12 @@ class PagePool:
 
     Full pages may be shared by forked sequences; a page that a sequence still
     writes to (its last, while it is not full) is its own: ``extend`` copies a shared
-    one first.  Nothing changes where a call raises."""
+    one first.  Nothing changes where a call raises.
+
+    The pairs that ``extend`` and ``compact`` return are copied before any sequence's
+    rows are written.  Those of several calls of ``extend`` may be one copy; before a
+    ``fork``, ``free``, ``shorten`` or ``compact`` they are made, since these can let a
+    page that is copied to be copied from, or to again."""
 
     def __init__(self, pages: int):
         if pages < 1:
@@ -122,6 +127,18 @@ class PagePool:
         for page in held:
             self._users[page] += 1
         return new
+
+    def shorten(self, seq: int, tokens: int) -> None:
+        """The sequence keeps its first ``tokens`` tokens (drafts that were not taken
+        are gone); pages behind them that nobody else holds are free again."""
+        held, have = self._of[seq], self._tokens[seq]
+        if not 0 <= tokens <= have:
+            raise ValueError(f"a sequence of {have} tokens cannot keep {tokens}")
+        keep = -(-tokens // PAGE_TOKENS)
+        for page in reversed(held[keep:]):
+            self._drop(page)
+        del held[keep:]
+        self._tokens[seq] = tokens
 
     def free(self, seq: int) -> None:
         """The sequence ends; pages that nobody else holds are free again."""
