@@ -130,7 +130,7 @@ __device__ __forceinline__ void norm_rotate(Share& x, bool norm, const Gains<D>&
     // squares that lose bits below f32's normal numbers (v_rsq_f32 takes those for zeros) or
     // overflow: n is that of x times a power of two
     constexpr uint32_t LEAST = 0x0d800000u;  // 2^-100
-    if (__ballot(__float_as_uint(v) - LEAST >= kInfBits - LEAST)) {
+    if (__builtin_expect(__ballot(__float_as_uint(v) - LEAST >= kInfBits - LEAST) != 0, 0)) {
       const float by = v < __uint_as_float(LEAST) ? 0x1p100f : v == __builtin_inff() ? 0x1p-70f : 1.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) x.lo[j] *= by, x.hi[j] *= by;
