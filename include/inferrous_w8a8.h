@@ -585,6 +585,9 @@ int w8a8_linear_adapters(void *stream, const int8_t *q, const float *asc,
  *
  * Heads: `heads` query heads share `kv_heads` key/value heads, heads / kv_heads
  * neighbours each; head_dim is 64 or 128.
+ * Limits, beyond which W8A8_ESHAPE: 1024 heads; 2^24 rows, sequences and pages of a
+ * table's row; 2^31 - 1 pages and, in decode, m * table_width; 2^24 - 1 workgroups of
+ * a launch (2^23 - 1 of prompts).
  *
  * Batches: rows of n_seq sequences one after another; sequence i has rows
  * starts[i] .. starts[i + 1] - 1 (int32 [n_seq + 1], not decreasing; cut to [0,

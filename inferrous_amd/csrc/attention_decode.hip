@@ -26,8 +26,8 @@
 // bound (64 sequences of up to 4096 tokens) and 3% where a row's chain does (5 of up to
 // 65536, 14/2 heads of 64).
 //
-// 64 sequences of up to 4096 tokens, 32/8 heads of 128: 261 MB in 49.1 us (5.3 TB/s; a
-// plain read of the same pages, a page a wave, 45 us).  One of 4001 tokens: 5.0 us and
+// 64 sequences of up to 4096 tokens, 32/8 heads of 128: 261 MB in 49.4 us (5.3 TB/s; a
+// plain read of the same pages, a page a wave, 45 us).  One of 4001 tokens: 5.1 us and
 // 3.6 for the join, both mostly latency.
 #include <algorithm>
 
@@ -65,6 +65,9 @@ constexpr uint32_t join_splits(int waves) { return waves == 1 ? 16 : kMaxSplits;
 // of so many: 24 rows, 16 10.4 / 9.2 and 14.6 / 10.9, 24 12.2 / 12.0 and 18.5 / 14.5, 64
 // 25.0 / 25.7 and 39.3 / 31.6; 32 rows, 64 24.4 / 27.4 and 47.7 / 43.2.  Four, 16 rows,
 // 64 13.8 / 21.4 and 26.3 / 26.9.  Three or four workgroups a compute unit: 10 to 70% slower.
+// (All with a table as wide as the longest row.  The pages of a workgroup follow from the
+// width alone, so a wider table leaves shorter rows to fewer workgroups: one row of 63 pages
+// 7.8 at a width of 63, 9.6 at 512, 17.4 at 2048, eight of them 16.9, 28.2 and 28.3.)
 //
 // Turns: workgroups that share a compute unit start together, so the order decides
 // which do.  Ranking the units takes each workgroup under a microsecond, paid back where

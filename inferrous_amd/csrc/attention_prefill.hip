@@ -29,11 +29,15 @@
 //
 // The running maximum moves when the scores exceed it by more than 8 (in powers of two):
 // probabilities stay below 2^8, and the sums are rescaled a few times, not once for
-// every 32 keys.  A probability is rounded to BF16, and the sum that divides is that of
-// the rounded ones.
+// every 32 keys.  A probability is rounded to BF16, which the second product takes
+// at its rate (in two parts it would be half as many products again, and power bounds
+// already), and the sum that divides is that of the rounded ones: against 64 bits the
+// outputs are off by 0.0017, where their own rounding alone gives 0.0016.
 //
-// 32/8 heads of 128: one prompt of 4096 tokens 136 us (1010 TFLOP/s), one of 16384
-// 1942 us (1134 TFLOP/s, where a library product of 8192^3 reaches 1371).  The matrix
+// 32/8 heads of 128: one prompt of 4096 tokens 133 to 145 us (by the card; 136: 1010
+// TFLOP/s), one of 16384 1942 us (1134 TFLOP/s, where a library product of 8192^3 reaches
+// 1371); heads of 64, twice the exponentials for the same products: 92 and 1254 us (743
+// and 877 TFLOP/s).  The matrix
 // cores are busy in 58% of the cycles, and the clock is down to 1.95 of 2.4 GHz: each
 // part of the loop that is left out (exponentials, reads of LDS, loads) gives its power
 // back as clock, 5 to 12%, so that none of them is what the others wait for.  Waves that
@@ -465,7 +469,8 @@ static uint64_t prefill_blocks(const PrefillArgs& a, int waves) {
 // ones to take: one wave a SIMD then ends sooner than two.  One sequence of 32/8 heads
 // of 128, 128 rows / 256 rows a workgroup, us: 37 tokens 7.0 / 7.5, 200 10.5 / 12.1, 512
 // 15.3 / 18.4, 1024 25.4 / 30.6, 1400 32.8 / 39.9, 2048 52.9 / 56.3, 2300 69.3 / 64.8,
-// 4096 170 / 137.
+// 4096 170 / 137.  (The bound counts a part of a workgroup for every sequence, so a batch
+// of many short prompts gets 256 rows: 64 of 32 tokens, which fill half of them, 18.7.)
 static int prefill_waves(const PrefillArgs& a) { return prefill_blocks(a, 8) <= 256 ? 4 : 8; }
 
 uint64_t attention_prefill_blocks(const PrefillArgs& a) { return prefill_blocks(a, prefill_waves(a)); }

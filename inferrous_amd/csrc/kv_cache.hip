@@ -15,7 +15,7 @@
 // Bytes bound both.  prepare_qk reads and writes each value once; everything of a page's
 // head is one workgroup's, so that the scale needs no second pass, and each lane asks
 // for all its rows before it uses the first.  4096 rows of five sequences, 32/8 heads of 128,
-// BF16: 26.6 us for 111 MB (4.2 TB/s; a large copy reaches 4.93); one row 4.2 us, a chain
+// BF16: 26.9 us for 111 MB (4.1 TB/s; a large copy reaches 4.93); one row 4.2 to 5 us, a chain
 // of three dependent loads (the row's past, its page, the page's scale) and two barriers.
 // copy_pages: 200 pages of 36 layers 350 us (5.4 TB/s), 16 KiB a workgroup.
 #include <algorithm>
